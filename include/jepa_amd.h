@@ -163,6 +163,73 @@ int jepa_amd_gemm_step_probe(int device, int mode, int waves_per_simd, int iters
 /* Copy of n float32 values between device buffers (a plain copy kernel, for counter calibration). */
 int jepa_amd_copy(int device, const float * src_dev, float * dst_dev, int64_t n, int reps, double * ms);
 
+/* ---- 4-bit paged key/value cache -------------------------------------------------------------------
+ * Keys and values that stay on the device between calls, for predictors and decoders that run step by step (the reference
+ * keeps an f16 / f32 one per context, jepa_ac_context_*). One cache is n_pages * jepa_amd_cache_page_bytes() bytes of
+ * device memory that the caller allocates (one for each layer; 16-byte aligned; it need not be cleared); a page holds
+ * page_size tokens of every K/V head as ggml q4_0 blocks along the head, 4.5 bits a value. A sequence's tokens lie in the
+ * pages of its row of a block table: token t in page table[t / page_size]. A step is
+ *     jepa_amd_cache_plan        once: which pages and slots the step's rows get
+ *     jepa_amd_cache_store       for each layer: the rows' keys and values into their slots
+ *     jepa_amd_cache_attention   for each layer: the rows' queries over their sequences
+ * The calls queue their work on `stream` (a hipStream_t of `device`; NULL: the null stream), allocate nothing, do not wait
+ * and can be captured into a HIP graph. All pointers but `shape` are device pointers. Rows are packed one after the other,
+ * sequence by sequence, each row its heads one after the other; types are 0 f32, 1 f16, 30 bf16; strides are in elements;
+ * row pointers and strides are multiples of 16 bytes. Outputs must not overlap inputs or each other unless stated. */
+typedef struct {
+    int32_t n_head;      /* query heads, a multiple of n_kv_head; head h reads K/V head h / (n_head / n_kv_head) */
+    int32_t n_kv_head;
+    int32_t head_dim;    /* 32, 64, 96 or 128 */
+    int32_t page_size;   /* tokens of a page: 16, 32, 64, 128 or 256 */
+    int64_t n_pages;     /* pages of the cache, below 2^31 */
+} jepa_amd_cache_shape;
+
+/* Bytes of one page, or -1 on a shape that is not supported (n_head and n_pages do not matter but are checked). */
+int64_t jepa_amd_cache_page_bytes(const jepa_amd_cache_shape * shape);
+
+/* One step's bookkeeping for n_seq sequences (up to 4096), n_rows packed rows and tables of table_width pages.
+ *   len [n_seq]          tokens that each sequence has in the cache
+ *   n_new [n_seq]        tokens that come to it in this step; below zero, that many are dropped from its end
+ *   table [n_seq][table_width]   in and out: pages for the new tokens are written in, dropped pages' entries set to -1
+ *   ring [n_pages], free_in [2]  the free pages: free_in[1] of them from ring[free_in[0]] on, around the end. Pages are
+ *                        taken at the front in sequence order; dropped pages are put behind the last, in sequence and table
+ *                        order, and not taken again in the same step. A caller starts with ring = 0 .. n_pages - 1 and (0, n_pages).
+ *   free_out [2]         the ring's front and count afterwards (may be free_in)
+ *   kv_len [n_seq]       tokens of each sequence afterwards (may be len)
+ *   row_start [n_seq + 1]  where its rows begin: the sums of the positive n_new, at most n_rows
+ *   slot [n_rows]        the cache slot of each row, page * page_size + place; -1 for a row of a refused sequence and behind the last
+ *   refused [n_seq]      1 where the step could not be done for a sequence: its lengths do not fit a table row, its rows end
+ *                        past n_rows, or the free pages end before it (then every later one that needs a page is refused
+ *                        too). It keeps its len and pages. */
+int jepa_amd_cache_plan(int device, const jepa_amd_cache_shape * shape, int64_t n_seq, int64_t n_rows, const int32_t * len,
+                        const int32_t * n_new, int32_t * table, int64_t table_width, int32_t * ring, const int32_t * free_in,
+                        int32_t * free_out, int32_t * kv_len, int32_t * row_start, int64_t * slot, int32_t * refused, void * stream);
+
+/* Keys and values of n_rows rows ([n_kv_head * head_dim], k_stride / v_stride apart) quantized into their slots, ggml's
+ * q4_0 bit for bit (as jepa_amd_quantize_rows). Rows whose slot is negative or past the cache are skipped; no slot may be given
+ * twice. Values beyond +-65504 are held there; a head of a row with a NaN or an infinity in its K or V is stored as K NaN and V
+ * zero, so that a query which reads the token comes out NaN. */
+int jepa_amd_cache_store(int device, const jepa_amd_cache_shape * shape, void * cache, int type, const void * k, int64_t k_stride,
+                         const void * v, int64_t v_stride, int64_t n_rows, const int64_t * slot, void * stream);
+
+/* The values that n_rows slots hold, rounded to `type`; rows whose slot is negative or past the cache come out zero. */
+int jepa_amd_cache_read(int device, const jepa_amd_cache_shape * shape, const void * cache, const int64_t * slot, int64_t n_rows, int type,
+                        void * k, int64_t k_stride, void * v, int64_t v_stride, void * stream);
+
+/* out = softmax(scale * q K^T) V for each row and head over its sequence's cached tokens. Row j of the r rows of a sequence of
+ * kv_len tokens stands at position kv_len - r + j, so the step's own tokens are stored first. causal_block 0: every row reads
+ * all kv_len tokens; 1: those up to its own position; T: those of its own and earlier blocks of T positions (frames).
+ * q and out hold rows of n_head * head_dim values of `type`; keys and values enter as they are held, sums and the softmax
+ * are f32, and f32 rows are computed to f32 accuracy. Tokens whose page is not one of the cache's are not read; a row that
+ * reads nothing comes out zero; rows behind the last sequence (row_start[n_seq] on) are left as they are.
+ * `work` is jepa_amd_cache_work_bytes() bytes of device memory (16-byte aligned) with nothing kept in it between calls: calls
+ * that may overlap on the device (on two streams, in two graphs) need one each. */
+int64_t jepa_amd_cache_work_bytes(const jepa_amd_cache_shape * shape, int64_t n_seq, int64_t n_rows, int64_t table_width);
+int jepa_amd_cache_attention(int device, const jepa_amd_cache_shape * shape, const void * cache, int type, const void * q, int64_t q_stride,
+                             int64_t n_seq, int64_t n_rows, const int32_t * row_start, const int32_t * kv_len, const int32_t * table,
+                             int64_t table_width, float scale, int64_t causal_block, void * out, int64_t out_stride, void * work,
+                             int64_t work_bytes, void * stream);
+
 /* Force the MFMA GEMM onto workgroup tile `index` for later launches whose n_out it divides; -1
  * restores the automatic choice. Process-wide (tests and tuning). Tiles (weight rows x tokens):
  * 0: 256x128, 1: 192x128, 2: 128x128, 3: 128x128 (other wave shape), 4: 64x128, 5: 128x64, 6: 256x64,

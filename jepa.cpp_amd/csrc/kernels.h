@@ -125,6 +125,39 @@ void launch_prefix_rows(float * x, const float * cls, const float * reg, int n_r
 // quantizers; n a multiple of the block size. Returns false for another type or a ragged n.
 bool launch_quantize_rows(int dst_type, const float * x, int64_t n, void * y, hipStream_t s);
 
+// The 4-bit paged K/V cache (cache_dev.h has its layout). Each returns its launches' own status and allocates nothing.
+struct cache_shape { int n_head = 0, n_kv_head = 0, hd = 0, page_size = 0; int64_t n_pages = 0; };
+
+// one step's bookkeeping: len / come (tokens cached; to add, or to drop when negative) per sequence, the block table
+// [n_seq][width] and the ring of free pages updated in place, the ring's (head, count) from free_in to free_out,
+// kv_len / refused per sequence, row_start [n_seq + 1], and the slot of each of n_rows packed rows (-1: none)
+struct cache_plan_args {
+    int n_seq = 0, width = 0, page_size = 0;
+    int64_t n_rows = 0, n_pages = 0;
+    const int32_t * len = nullptr, * come = nullptr, * free_in = nullptr;
+    int32_t * table = nullptr, * ring = nullptr, * free_out = nullptr, * kv_len = nullptr, * row_start = nullptr, * refused = nullptr;
+    int64_t * slot = nullptr;
+};
+hipError_t launch_cache_plan(const cache_plan_args & a, hipStream_t s);
+// rows of K and V (type T_F32 / T_F16 / T_BF16, head-major, ld elements apart) quantized into their slots, and back
+hipError_t launch_cache_store(const cache_shape & c, void * cache, int type, const void * k, int64_t ldk, const void * v, int64_t ldv,
+                              int64_t n_rows, const int64_t * slot, hipStream_t s);
+hipError_t launch_cache_read(const cache_shape & c, const void * cache, const int64_t * slot, int64_t n_rows, int type, void * k,
+                             int64_t ldk, void * v, int64_t ldv, hipStream_t s);
+// attention of packed rows over the cache; `work` holds cache_attention_work_bytes
+struct cache_attn_args {
+    const unsigned char * cache = nullptr;
+    const void * q = nullptr;
+    void * out = nullptr;
+    int64_t ldq = 0, ldo = 0, n_rows = 0, n_pages = 0, block = 0;
+    const int32_t * row_start = nullptr, * kv_len = nullptr, * table = nullptr;
+    int n_seq = 0, width = 0, n_head = 0, n_kv_head = 0, page_size = 0;
+    float scale = 0;
+    float * work = nullptr;
+};
+int64_t cache_attention_work_bytes(const cache_shape & c, int64_t n_seq, int64_t n_rows, int64_t width);
+hipError_t launch_cache_attention(const cache_shape & c, int type, const cache_attn_args & a, hipStream_t s);
+
 // weight expansion at load: raw ggml blocks (device) -> dev_linear operand arrays (int8: q4_0 rows
 // go to the int8 layout of q8_0 whatever their length, for a linear whose parts mix the two)
 void launch_repack(int gtype, const void * raw, int64_t n_out, int64_t n_in, void * w, void * wd,

@@ -38,6 +38,11 @@ class PreprocessParams(C.Structure):
                 ("resample", C.c_int), ("resize_mode", C.c_int), ("rescale", C.c_float), ("fused_norm", C.c_bool)]
 
 
+class CacheShape(C.Structure):
+    """The shape of a 4-bit paged key/value cache (jepa_amd_cache_shape)."""
+    _fields_ = [("n_head", C.c_int32), ("n_kv_head", C.c_int32), ("head_dim", C.c_int32), ("page_size", C.c_int32), ("n_pages", C.c_int64)]
+
+
 _lib = None
 
 
@@ -122,6 +127,13 @@ def lib() -> C.CDLL:
         "jepa_amd_matmul": (C.c_int, [C.c_int, C.c_int, vp, i64, i64, vp, vp, i64, vp, C.c_int, C.POINTER(C.c_double)]),
         "jepa_amd_matmul_gelu": (C.c_int, [C.c_int, C.c_int, vp, i64, i64, vp, vp, i64, C.c_int, vp, C.c_int, C.POINTER(C.c_double)]),
         "jepa_amd_attention": (C.c_int, [C.c_int, vp, i64, i64, C.c_int, C.c_int, vp, vp, C.c_int, i64, C.c_int, vp]),
+        "jepa_amd_cache_page_bytes": (i64, [C.POINTER(CacheShape)]),
+        "jepa_amd_cache_work_bytes": (i64, [C.POINTER(CacheShape), i64, i64, i64]),
+        "jepa_amd_cache_plan": (C.c_int, [C.c_int, C.POINTER(CacheShape), i64, i64, vp, vp, vp, i64, vp, vp, vp, vp, vp, vp, vp, vp]),
+        "jepa_amd_cache_store": (C.c_int, [C.c_int, C.POINTER(CacheShape), vp, C.c_int, vp, i64, vp, i64, i64, vp, vp]),
+        "jepa_amd_cache_read": (C.c_int, [C.c_int, C.POINTER(CacheShape), vp, vp, i64, C.c_int, vp, i64, vp, i64, vp]),
+        "jepa_amd_cache_attention": (C.c_int, [C.c_int, C.POINTER(CacheShape), vp, C.c_int, vp, i64, i64, i64, vp, vp, vp, i64, C.c_float, i64,
+                                               vp, i64, vp, i64, vp]),
         "jepa_amd_mfma_probe": (C.c_int, [C.c_int, vp, vp, vp]),
         "jepa_amd_copy": (C.c_int, [C.c_int, vp, vp, i64, C.c_int, C.POINTER(C.c_double)]),
         "jepa_amd_gemm_step_probe": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int, C.POINTER(C.c_double)]),
