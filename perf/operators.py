@@ -345,12 +345,15 @@ def _shape(s, lib):
 def _own_plan(s):
     lib = _lib()
     n, rows, dev = s["n_seq"], s["rows"], s["table"].device
+    # the call works in place: on copies, so that a pass can be made again
+    both = torch.cat((s["table"].flatten(), s["ring"]))
+    table, ring = both[:s["table"].numel()].view_as(s["table"]), both[s["table"].numel():]
     kv_len, row_start, free = (torch.empty(m, dtype=torch.int32, device=dev) for m in (n, n + 1, 2))
     slot, refused = torch.empty(rows, dtype=torch.int64, device=dev), torch.empty(n, dtype=torch.int32, device=dev)
-    lib.check(lib.lib().jepa_amd_cache_plan(dev.index, _shape(s, lib), n, rows, s["len"].data_ptr(), s["new"].data_ptr(), s["table"].data_ptr(), s["width"],
-                                            s["ring"].data_ptr(), s["free"].data_ptr(), free.data_ptr(), kv_len.data_ptr(), row_start.data_ptr(), slot.data_ptr(),
+    lib.check(lib.lib().jepa_amd_cache_plan(dev.index, _shape(s, lib), n, rows, s["len"].data_ptr(), s["new"].data_ptr(), table.data_ptr(), s["width"],
+                                            ring.data_ptr(), s["free"].data_ptr(), free.data_ptr(), kv_len.data_ptr(), row_start.data_ptr(), slot.data_ptr(),
                                             refused.data_ptr(), torch.cuda.current_stream().cuda_stream), "jepa_amd_cache_plan")
-    return dict(table=s["table"], ring=s["ring"], free=free, kv_len=kv_len, row_start=row_start, slot=slot, refused=refused)
+    return dict(table=table, ring=ring, free=free, kv_len=kv_len, row_start=row_start, slot=slot, refused=refused)
 
 
 def _own_store(s):
