@@ -187,7 +187,7 @@ typedef struct {
 /* Bytes of one page, or -1 on a shape that is not supported (n_head and n_pages do not matter but are checked). */
 int64_t jepa_amd_cache_page_bytes(const jepa_amd_cache_shape * shape);
 
-/* One step's bookkeeping for n_seq sequences (up to 4096), n_rows packed rows and tables of table_width pages.
+/* One step's bookkeeping for n_seq sequences (up to 4096), n_rows packed rows and tables of table_width pages (2^30 tokens at most).
  *   len [n_seq]          tokens that each sequence has in the cache
  *   n_new [n_seq]        tokens that come to it in this step; below zero, that many are dropped from its end
  *   table [n_seq][table_width]   in and out: pages for the new tokens are written in, dropped pages' entries set to -1

@@ -10,6 +10,7 @@
 namespace {
 
 constexpr int64_t I31 = 0x7fffffff;
+constexpr int64_t MAX_TOKENS = 1 << 30;      // of a table row: positions and the steps past them stay in 32 bits
 
 // the shape, checked; who: the entry point for the message
 bool shape_of(const char * who, const jepa_amd_cache_shape * s, cache_shape & c) {
@@ -27,8 +28,8 @@ bool shape_of(const char * who, const jepa_amd_cache_shape * s, cache_shape & c)
 }
 
 bool sizes_ok(const char * who, const cache_shape & c, int64_t n_seq, int64_t n_rows, int64_t width) {
-    if (n_seq < 0 || n_seq > CACHE_MAX_SEQ || n_rows < 0 || n_rows >= I31 || width < 1 || width > I31 / c.page_size) {
-        jepa_log("jepa: %s: %lld sequences, %lld rows, tables of %lld pages not supported (up to %d sequences; rows and tokens of a table below 2^31)\n",
+    if (n_seq < 0 || n_seq > CACHE_MAX_SEQ || n_rows < 0 || n_rows >= I31 || width < 1 || width > MAX_TOKENS / c.page_size) {
+        jepa_log("jepa: %s: %lld sequences, %lld rows, tables of %lld pages not supported (up to %d sequences, 2^31 rows, 2^30 tokens of a table row)\n",
                  who, (long long) n_seq, (long long) n_rows, (long long) width, CACHE_MAX_SEQ);
         return false;
     }
@@ -48,9 +49,16 @@ bool rows_ok(const char * who, const char * what, int type, const void * p, int6
     return true;
 }
 
-bool grid_ok(const char * who, int64_t n_blocks) {
-    if (n_blocks <= I31) return true;
-    jepa_log("jepa: %s: too many rows for one call\n", who);
+// heads of rows that one launch takes (its threads are below 2^32, 16 of them for a head at most)
+bool grid_ok(const char * who, int64_t n) {
+    if (n < (int64_t) 1 << 27) return true;
+    jepa_log("jepa: %s: %lld heads of rows in one call (below 2^27)\n", who, (long long) n);
+    return false;
+}
+
+bool cache_ok(const char * who, const void * cache) {
+    if (cache && (uintptr_t) cache % 16 == 0) return true;
+    jepa_log("jepa: %s: the cache must be 16-byte aligned device memory\n", who);
     return false;
 }
 
@@ -112,7 +120,7 @@ extern "C" int jepa_amd_cache_store(int device, const jepa_amd_cache_shape * sha
     cache_shape c;
     if (!shape_of(who, shape, c) || !sizes_ok(who, c, 0, n_rows, 1)) return -1;
     const int64_t width = (int64_t) c.n_kv_head * c.hd;
-    if (!rows_ok(who, "cache", T_F32, cache, 4, 4, 1) || !rows_ok(who, "k", type, k, k_stride, width, n_rows) ||
+    if (!cache_ok(who, cache) || !rows_ok(who, "k", type, k, k_stride, width, n_rows) ||
         !rows_ok(who, "v", type, v, v_stride, width, n_rows) || (n_rows && !all(who, {slot})) || !grid_ok(who, n_rows * c.n_kv_head))
         return -1;
     return on_device(who, device, [&] {
@@ -126,7 +134,7 @@ extern "C" int jepa_amd_cache_read(int device, const jepa_amd_cache_shape * shap
     cache_shape c;
     if (!shape_of(who, shape, c) || !sizes_ok(who, c, 0, n_rows, 1)) return -1;
     const int64_t width = (int64_t) c.n_kv_head * c.hd;
-    if (!rows_ok(who, "cache", T_F32, cache, 4, 4, 1) || !rows_ok(who, "k", type, k, k_stride, width, n_rows) ||
+    if (!cache_ok(who, cache) || !rows_ok(who, "k", type, k, k_stride, width, n_rows) ||
         !rows_ok(who, "v", type, v, v_stride, width, n_rows) || (n_rows && !all(who, {slot})) || !grid_ok(who, n_rows * c.n_kv_head))
         return -1;
     return on_device(who, device, [&] {
@@ -142,7 +150,7 @@ extern "C" int jepa_amd_cache_attention(int device, const jepa_amd_cache_shape *
     cache_shape c;
     if (!shape_of(who, shape, c) || !sizes_ok(who, c, n_seq, n_rows, table_width)) return -1;
     const int64_t width = (int64_t) c.n_head * c.hd;
-    if (!rows_ok(who, "cache", T_F32, cache, 4, 4, 1) || !rows_ok(who, "q", type, q, q_stride, width, n_rows) ||
+    if (!cache_ok(who, cache) || !rows_ok(who, "q", type, q, q_stride, width, n_rows) ||
         !rows_ok(who, "out", type, out, out_stride, width, n_rows) || !grid_ok(who, n_rows * c.n_head))
         return -1;
     if (!std::isfinite(scale) || causal_block < 0) {

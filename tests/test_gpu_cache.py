@@ -9,6 +9,11 @@ Attention's tolerance, for one row and head with out = sum_j p_j v_j and A = sum
                                  value and an exact key, times a scale: off by at most (head_dim / 8 + 8) 2^-22 S,
                                  S = max_j scale |q|max |k_j|_1; the weights follow by the factor e^x ~ 1 + x on both sides
                                  of the fraction (twice), and their own 2^-21 and the sums' sqrt(n) 2^-24 come on top.
+  small weights                  a weight enters the product with V as p_j d_j in f16 (the scale d_j of its block of V, the value
+                                 at most 8 d_j), moved by a power of two that brings the largest p_j max d to 2^6 or more: f16's
+                                 smallest step, half of it 2^-25, is 2^-31 of that largest one. Divided by the sum of the p_j, which
+                                 is no less than the largest p_j, and times a code of at most 8 that is an error of at most
+                                 2^-31 * 2 max|v| (the power of two above max d is under 2 max d) for each of the n keys.
 """
 import ctypes as C
 
@@ -308,7 +313,7 @@ def reference(p, q, start, total, table, block, scale, kind):
             S = abs(scale) * x.abs().amax(-1, keepdim=True) * (k1.max() if n else 0.0)
             f32 = 2 * (hd / 8 + 8) * 2.0 ** -22 * S + 2.0 ** -20 + (n ** 0.5) * 2.0 ** -24
             out[a:b, h] = y
-            tol[a:b, h] = eps * y.abs() + tiny + (f32 + (2.0 ** -12 if kind != "f32" else 0.0)) * A * (1 + eps)
+            tol[a:b, h] = eps * y.abs() + tiny + n * 2.0 ** -30 * (v[:, h // group].abs().max() if n else 0.0) + (f32 + (2.0 ** -12 if kind != "f32" else 0.0)) * A * (1 + eps)
     return out.reshape(q.shape), tol.reshape(q.shape)
 
 
