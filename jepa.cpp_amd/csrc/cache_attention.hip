@@ -30,8 +30,10 @@
 #include "cache_dev.h"
 #include "common.h"
 #include "kernels.h"
+#include "lds_dma.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace {
 
@@ -49,15 +51,16 @@ constexpr int PIECE = 4 * TILE;      // pieces are multiples of this: one step o
 constexpr int UNITS = 1024;          // units that a call is split into where its columns alone are fewer
 
 // the 8 codes of a word less 8, in the order of its elements (nibbles 0 4 1 5 2 6 3 7), exact in f16: a nibble or'ed into the low
-// mantissa bits of 1024 is 1024 + c, into the next four 1024 + 16 c
-__device__ __forceinline__ half8_t codes8(uint32_t w) {
+// mantissa bits of 1024 is 1024 + c, into the next four 1024 + 16 c. `k1024` is the pair of f16 1024 in a vector register (an
+// instruction reads one scalar register: with the mask in it, and + or are one v_and_or_b32).
+__device__ __forceinline__ half8_t codes8(uint32_t w, uint32_t k1024) {
     const half2_t off = {(_Float16) -1032.0f, (_Float16) -1032.0f}, off16 = {(_Float16) -72.0f, (_Float16) -72.0f};
     const half2_t sixteenth = {(_Float16) 0.0625f, (_Float16) 0.0625f};
     const uint32_t u = w >> 8;
-    const half2_t a = __builtin_bit_cast(half2_t, (w & 0x000f000fu) | 0x64006400u) + off;
-    const half2_t b = __builtin_elementwise_fma(__builtin_bit_cast(half2_t, (w & 0x00f000f0u) | 0x64006400u), sixteenth, off16);
-    const half2_t c = __builtin_bit_cast(half2_t, (u & 0x000f000fu) | 0x64006400u) + off;
-    const half2_t d = __builtin_elementwise_fma(__builtin_bit_cast(half2_t, (u & 0x00f000f0u) | 0x64006400u), sixteenth, off16);
+    const half2_t a = __builtin_bit_cast(half2_t, (w & 0x000f000fu) | k1024) + off;
+    const half2_t b = __builtin_elementwise_fma(__builtin_bit_cast(half2_t, (w & 0x00f000f0u) | k1024), sixteenth, off16);
+    const half2_t c = __builtin_bit_cast(half2_t, (u & 0x000f000fu) | k1024) + off;
+    const half2_t d = __builtin_elementwise_fma(__builtin_bit_cast(half2_t, (u & 0x00f000f0u) | k1024), sixteenth, off16);
     return half8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
@@ -83,6 +86,17 @@ __device__ __forceinline__ uint32_t wave_umax(uint32_t x) {
     x = max((uint32_t) r[0], (uint32_t) r[1]);
     r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
     return (uint32_t) __builtin_amdgcn_readfirstlane((int) max((uint32_t) r[0], (uint32_t) r[1]));
+}
+// N words per lane of a buffer
+template <int N>
+__device__ __forceinline__ void load_words(uint32_t * x, brsrc r, int at, int off) {
+    typedef uint32_t uint2_t __attribute__((ext_vector_type(2)));
+    typedef uint32_t uint3_t __attribute__((ext_vector_type(3)));
+    typedef uint32_t uint4_t __attribute__((ext_vector_type(4)));
+    if constexpr (N == 1) x[0] = __builtin_amdgcn_raw_buffer_load_b32(r, at, off, 0);
+    if constexpr (N == 2) { const uint2_t v = __builtin_amdgcn_raw_buffer_load_b64(r, at, off, 0); x[0] = v[0]; x[1] = v[1]; }
+    if constexpr (N == 3) { const uint3_t v = __builtin_amdgcn_raw_buffer_load_b96(r, at, off, 0); x[0] = v[0]; x[1] = v[1]; x[2] = v[2]; }
+    if constexpr (N == 4) { const uint4_t v = __builtin_amdgcn_raw_buffer_load_b128(r, at, off, 0); x[0] = v[0]; x[1] = v[1]; x[2] = v[2]; x[3] = v[3]; }
 }
 __device__ __forceinline__ void wave_order() {      // LDS accesses of the wave's lanes before and after stay in this order
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -193,7 +207,7 @@ template <int HD, int CT, int KW> constexpr int group_lds() {
 }
 
 template <typename T, int HD, int CT, int KW>
-__global__ __launch_bounds__(NT) void k_cache_attention(cache_attn_args a) {
+__global__ __launch_bounds__(NT, CT == 1 ? 3 : 2) void k_cache_attention(cache_attn_args a) {
     constexpr int NB = HD / 32, ND = HD / 16, TERMS = sizeof(T) == 4 ? 2 : 1, WC = 16 * CT, C = KW == 4 ? WC : 4 * WC;
     __shared__ __attribute__((aligned(16))) unsigned char lds[group_lds<HD, CT, KW>()];
     unit u;
@@ -256,43 +270,46 @@ __global__ __launch_bounds__(NT) void k_cache_attention(cache_attn_args a) {
     const int last_strip = (kend - 1) / 16, strips_of_page = a.page_size / 16, page_shift = __builtin_ctz(strips_of_page);
     const int32_t * table = a.table + (int64_t) seq * a.width;
     auto load_pages = [&](int32_t key) { return table[min(key / 16 + (lane & 3), last_strip) >> page_shift]; };
-    uint32_t kn[4][NB], vn[4][NB], sn[4], bad = 0, bad_n = 0;
-    auto load_tile = [&](int32_t key, int pages) {
+    uint32_t kn[4][NB], vn[4][NB], sn[4], bad_n = 0;      // the tile's codes and scales, in flight
+    int pages = 0;                                         // page numbers of the next one, in lanes 0 to 3
+    // a strip as a buffer resource (no bytes past the end of this wave's keys: such loads give 0 without a memory access)
+    auto strip_of = [&](int32_t key, int pages, int t, uint32_t & bad) {
+        const int strip = min(key / 16 + t, last_strip);
+        int64_t page = __builtin_amdgcn_readlane(pages, t);
+        if (page < 0 || page >= a.n_pages) { page = 0; bad |= 1u << t; }
+        return make_brsrc(a.cache + ((page * a.n_kv_head + kvh) * strips_of_page + (strip & (strips_of_page - 1))) * (18 * HD), key < kend ? 18 * HD : 0);
+    };
+    auto load_v = [&](int32_t key, int pages) {
         bad_n = 0;
 #pragma unroll
         for (int t = 0; t < 4; t++) {
-            const int strip = min(key / 16 + t, last_strip);
-            int64_t page = __builtin_amdgcn_readlane(pages, t);
-            if (page < 0 || page >= a.n_pages) { page = 0; bad_n |= 1u << t; }
-            const unsigned char * s = a.cache + ((page * a.n_kv_head + kvh) * strips_of_page + (strip & (strips_of_page - 1))) * (18 * HD);
-            const uint32_t * kp = (const uint32_t *) (s + lane * (4 * NB)), * vp = (const uint32_t *) (s + 8 * HD + lane * (4 * NB));
-#pragma unroll
-            for (int b = 0; b < NB; b++) { kn[t][b] = kp[b]; vn[t][b] = vp[b]; }
-            sn[t] = lane < HD / 2 ? *(const uint32_t *) (s + 16 * HD + lane * 4) : 0u;
+            const brsrc s = strip_of(key, pages, t, bad_n);
+            load_words<NB>(vn[t], s, lane * (4 * NB), 8 * HD);
+            load_words<1>(&sn[t], s, 16 * HD + lane * 4, 0);      // (0 past the strip's scales, from lane HD / 2 on)
         }
+    };
+    auto load_k = [&](int32_t key, int pages) {
+        uint32_t bad = 0;
+#pragma unroll
+        for (int t = 0; t < 4; t++) load_words<NB>(kn[t], strip_of(key, pages, t, bad), lane * (4 * NB), 0);
     };
     unsigned char * const mine = lds + wv * wave_lds<HD>();
     unsigned char * const scales = mine + ND * 528;
     // where this lane's V words go, [dimension tile][64 keys][8 bytes], and the row that it names for the transposed read
     const int e = (l15 & 3) * 2 + ((l15 & 7) >> 2);
     const int tr_at = (((l15 >> 3) * 2 + (e >> 2)) * 16 + g * 4 + (e & 3)) * 8;
-    int pages = 0;
-    if (k0 < kend) {
-        pages = load_pages(k0);
-        load_tile(k0, pages);
-        pages = load_pages(k0 + STEP);
-    }
-    for (; k0 < kend; k0 += STEP) {
-        uint32_t kw[4][NB];
-        wave_order();
-        // keys past the end, and pages that are none: scales 0, so that what lies there does not matter
-        const bool whole = k0 + TILE <= lim_lo && bad_n == 0;
-        bad = bad_n;
+    uint32_t k1024 = 0x64006400u;
+    asm volatile("" : "+v"(k1024));
+    // one tile: MASKED where it passes some column's last key, the end, or has a page that is none
+    auto tile = [&](auto masked) {
+        constexpr bool MASKED = decltype(masked)::value;
+        const uint32_t bad = bad_n;
         uint32_t dmax = 0;
+        wave_order();
 #pragma unroll
         for (int t = 0; t < 4; t++) {
             uint32_t sc = sn[t];
-            if (!whole) {
+            if constexpr (MASKED) {      // scales of tokens that nobody reads are 0: what lies there does not matter
                 const int d = lane % (HD / 4);
                 const int32_t key = k0 + t * 16 + d / (2 * NB) * 4 + (d & 1) * 2;
                 if (key >= kend || (bad >> t & 1)) sc = 0;
@@ -304,13 +321,9 @@ __global__ __launch_bounds__(NT) void k_cache_attention(cache_attn_args a) {
             for (int b = 0; b < NB; b++) {
                 const int w = (lane & 3) * NB + b;
                 *(uint32_t *) (mine + (w >> 1) * 528 + (t * 16 + (lane >> 2)) * 8 + (w & 1) * 4) = vn[t][b];
-                kw[t][b] = kn[t][b];
             }
         }
-        if (k0 + STEP < kend) {
-            load_tile(k0 + STEP, pages);
-            pages = load_pages(k0 + 2 * STEP);
-        }
+        load_v(k0 + STEP, pages);
         const float dexp = (float) ((int) (wave_umax(dmax) >> 10) - 14);      // every |dv| of the tile is below 2^dexp
         wave_order();
 
@@ -321,21 +334,24 @@ __global__ __launch_bounds__(NT) void k_cache_attention(cache_attn_args a) {
             const half4_t * dk = (const half4_t *) (scales + t * 2 * HD + g * (8 * NB));
 #pragma unroll
             for (int b = 0; b < NB; b++) {
-                const half8_t kc = codes8(kw[t][b]);
+                const half8_t kc = codes8(kn[t][b], k1024);
                 const half4_t d = dk[b];
 #pragma unroll
                 for (int ct = 0; ct < CT; ct++) {
                     float4_t x = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc, q[ct][b][0], float4_t{0, 0, 0, 0}, 0, 0, 0);
                     if constexpr (TERMS == 2) x = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc, q[ct][b][1], x, 0, 0, 0);
 #pragma unroll
-                    for (int r = 0; r < 4; r++) s[ct][t][r] = b == 0 ? (float) d[r] * x[r] : __builtin_fmaf((float) d[r], x[r], s[ct][t][r]);
+                    for (int r = 0; r < 4; r++) s[ct][t][r] = __builtin_fmaf((float) d[r], x[r], b == 0 ? 0.0f : s[ct][t][r]);
                 }
             }
+            __builtin_amdgcn_sched_barrier(0);
         }
+        load_k(k0 + STEP, pages);
+        pages = load_pages(k0 + 2 * STEP);
         // weights
 #pragma unroll
         for (int ct = 0; ct < CT; ct++) {
-            if (!whole) {
+            if constexpr (MASKED) {
 #pragma unroll
                 for (int t = 0; t < 4; t++)
 #pragma unroll
@@ -365,14 +381,14 @@ __global__ __launch_bounds__(NT) void k_cache_attention(cache_attn_args a) {
                 for (int r = 0; r < 4; r++) {
                     const float x = s[ct][t][r];
                     float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x, c[ct], -m));
-                    if (!whole && x == -INFINITY) p = 0.0f;
+                    if constexpr (MASKED) p = x == -INFINITY ? 0.0f : p;
                     s[ct][t][r] = p;
                 }
                 sum += s[ct][t];
             }
             l[ct] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         }
-        // O^T += V^T P'^T, block by block of the head
+        // O^T += V^T P'^T, block by block of the head (the fma with 0 is one v_fma_mix from and to f16)
 #pragma unroll
         for (int b = 0; b < NB; b++) {
             half8_t p[CT][2][TERMS];
@@ -382,14 +398,17 @@ __global__ __launch_bounds__(NT) void k_cache_attention(cache_attn_args a) {
                 const half4_t d1 = *(const half4_t *) (scales + (2 * h + 1) * 2 * HD + HD + g * (8 * NB) + b * 8);
 #pragma unroll
                 for (int ct = 0; ct < CT; ct++) {
-                    float8_t x;
 #pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        x[r] = s[ct][2 * h][r] * (float) d0[r];
-                        x[r + 4] = s[ct][2 * h + 1][r] * (float) d1[r];
+                    for (int r = 0; r < 8; r++) {
+                        const float w = s[ct][2 * h + (r >> 2)][r & 3], d = (float) (r < 4 ? d0[r & 3] : d1[r & 3]);
+                        if constexpr (TERMS == 1) {
+                            p[ct][h][0][r] = (_Float16) __builtin_fmaf(w, d, 0.0f);
+                        } else {
+                            const float x = __builtin_fmaf(w, d, 0.0f);
+                            p[ct][h][0][r] = (_Float16) x;
+                            p[ct][h][1][r] = (_Float16) (x - (float) p[ct][h][0][r]);
+                        }
                     }
-                    p[ct][h][0] = __builtin_convertvector(x, half8_t);
-                    if constexpr (TERMS == 2) p[ct][h][1] = __builtin_convertvector(x - __builtin_convertvector(p[ct][h][0], float8_t), half8_t);
                 }
             }
 #pragma unroll
@@ -398,7 +417,7 @@ __global__ __launch_bounds__(NT) void k_cache_attention(cache_attn_args a) {
                 const int2_t w = __builtin_amdgcn_ds_read_tr4_b64_v2i32((__attribute__((address_space(3))) int2_t *) (mine + d * 528 + tr_at));
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    const half8_t vc = codes8((uint32_t) w[h]);
+                    const half8_t vc = codes8((uint32_t) w[h], k1024);
 #pragma unroll
                     for (int ct = 0; ct < CT; ct++) {
                         o[ct][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vc, p[ct][h][0], o[ct][d], 0, 0, 0);
@@ -406,8 +425,17 @@ __global__ __launch_bounds__(NT) void k_cache_attention(cache_attn_args a) {
                     }
                 }
             }
+            __builtin_amdgcn_sched_barrier(0);
         }
+    };
+    if (k0 < kend) {
+        pages = load_pages(k0);
+        load_v(k0, pages);
+        load_k(k0, pages);
+        pages = load_pages(k0 + STEP);
     }
+    for (; k0 + TILE <= min(lim_lo, kend) && bad_n == 0; k0 += STEP) tile(std::false_type{});
+    for (; k0 < kend; k0 += STEP) tile(std::true_type{});
 #pragma unroll
     for (int ct = 0; ct < CT; ct++) l[ct] = col_sum(l[ct]);
 
