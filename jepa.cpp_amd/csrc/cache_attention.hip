@@ -48,7 +48,10 @@ constexpr float LOG2E = 1.4426950408889634f;
 constexpr int NT = 256;              // threads of a workgroup
 constexpr int TILE = 64;             // keys of a wave's step
 constexpr int PIECE = 4 * TILE;      // pieces are multiples of this: one step of each of four waves
-constexpr int UNITS = 1024;          // units that a call is split into where its columns alone are fewer
+
+// Units that a call is split into where its columns alone are fewer: the workgroups that the chip holds at once (256 CUs; 512 registers
+// a SIMD lane over the kernel's count), so that pieces of equal length end together.
+constexpr int units_of(int hd, int ct) { return 256 * (ct > 1 ? 2 : hd > 64 ? 3 : 4); }
 
 // the 8 codes of a word less 8, in the order of its elements (nibbles 0 4 1 5 2 6 3 7), exact in f16: a nibble or'ed into the low
 // mantissa bits of 1024 is 1024 + c, into the next four 1024 + 16 c. `k1024` is the pair of f16 1024 in a vector register (an
@@ -115,41 +118,91 @@ __device__ __forceinline__ seq_view view_of(const cache_attn_args & a, int i) {
     return v;
 }
 
-struct unit { int seq, tile, piece, pieces; int32_t length; int64_t part; };      // part: the first piece's place in `work`
+// A piece of a column tile: keys [piece, piece + 1) * length of sequence v; part: the first piece's place in `work`
+struct unit { seq_view v; int seq, tile, piece, pieces; int32_t length; int64_t part; };
 
-__device__ __forceinline__ uint64_t wave_sum64(uint64_t x) {
-    for (int o = 32; o; o >>= 1) x += __shfl_xor((unsigned long long) x, o, 64);
+// Column tiles and pieces of a sequence where the call's keys (over all column tiles and K/V heads) are `keys`: the number of pieces
+// that comes nearest to keys / UNITS each
+template <int C, int UNITS>
+struct seq_cut {
+    uint64_t tiles, pieces;
+    __device__ seq_cut(const seq_view & v, int group, uint64_t keys) {
+        tiles = (uint64_t) (((int64_t) v.rows * group + C - 1) / C);
+        const uint64_t length = max(keys / UNITS, (uint64_t) PIECE);
+        pieces = max(((uint32_t) v.len + length / 2) / length, (uint64_t) 1);
+    }
+};
+
+template <typename X>
+__device__ __forceinline__ X wave_sum(X x) {
+    for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o, 64);
     return x;
 }
 
-// Unit x of the call (x-th column tile if TILES), for column tiles of C. Every thread gets it; false past the last.
-template <int C, bool TILES>
+__device__ __forceinline__ int32_t uniform(int32_t x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ unit uniform(const unit & f) {
+    unit u;
+    u.v = {uniform(f.v.row0), uniform(f.v.rows), uniform(f.v.len)};
+    u.seq = uniform(f.seq);
+    u.tile = uniform(f.tile);
+    u.piece = uniform(f.piece);
+    u.pieces = uniform(f.pieces);
+    u.length = uniform(f.length);
+    u.part = (int64_t) ((uint64_t) (uint32_t) uniform((int32_t) (f.part >> 32)) << 32 | (uint32_t) uniform((int32_t) f.part));
+    return u;
+}
+
+// Unit x of the call (x-th column tile if TILES), for column tiles of C. Every thread gets it, in scalar registers; false past the last.
+template <int C, int UNITS, bool TILES>
 __device__ __forceinline__ bool find_unit(const cache_attn_args & a, uint32_t x, unit & u) {
-    __shared__ uint64_t sums[3][NT / 64];
+    typedef unsigned long long u64;
+    __shared__ u64 sums[3][NT / 64];
     __shared__ unit found;
     const int tid = (int) threadIdx.x, lane = tid & 63, wv = tid >> 6, group = a.n_head / a.n_kv_head;
     const int per = (a.n_seq + NT - 1) / NT, i0 = min(tid * per, a.n_seq), i1 = min(i0 + per, a.n_seq);
-    uint64_t keys = 0;
+    seq_view first = {};
+    u64 keys = 0;
     for (int i = i0; i < i1; i++) {
         const seq_view v = view_of(a, i);
-        keys += (uint64_t) (((int64_t) v.rows * group + C - 1) / C) * (uint32_t) v.len;
+        if (i == i0) first = v;
+        keys += (u64) (((int64_t) v.rows * group + C - 1) / C) * (uint32_t) v.len;
     }
-    keys = wave_sum64(keys);
-    if (tid == 0) found.seq = -1;
-    if (lane == 0) sums[0][wv] = keys;
-    __syncthreads();
-    keys = (sums[0][0] + sums[0][1] + sums[0][2] + sums[0][3]) * (uint32_t) a.n_kv_head;
-    const int32_t length = (int32_t) min<uint64_t>((keys / UNITS + PIECE) / PIECE * PIECE, 0x7fffff00u);
-    uint64_t mine = 0, parts = 0;
+    if (a.n_seq > 1) {
+        keys = wave_sum(keys);
+        if (lane == 0) sums[0][wv] = keys;
+        if (tid == 0) found.seq = -1;
+        __syncthreads();
+        keys = sums[0][0] + sums[0][1] + sums[0][2] + sums[0][3];
+    } else {      // one sequence: every thread has it
+        first = view_of(a, 0);
+        keys = (u64) (((int64_t) first.rows * group + C - 1) / C) * (uint32_t) first.len;
+    }
+    keys *= (uint32_t) a.n_kv_head;
+    auto set = [&](unit & f, const seq_view & v, int i, const seq_cut<C, UNITS> & cut, u64 at, u64 part) {
+        f.v = v;
+        f.seq = i;
+        f.tile = (int) (cut.tiles - 1 - (TILES ? at : at / cut.pieces));      // a prompt's last rows read the most keys: they go first
+        f.piece = TILES ? 0 : (int) (at % cut.pieces);
+        f.pieces = (int) cut.pieces;
+        f.length = (int32_t) (((uint32_t) v.len + cut.pieces * PIECE - 1) / (cut.pieces * PIECE) * PIECE);
+        f.part = (int64_t) (part + (u64) f.tile * cut.pieces);
+    };
+    if (a.n_seq == 1) {
+        const seq_cut<C, UNITS> cut(first, group, keys);
+        if (x >= (TILES ? cut.tiles : cut.tiles * cut.pieces)) return false;
+        set(u, first, 0, cut, x, 0);
+        u = uniform(u);
+        return true;
+    }
+    u64 mine = 0, parts = 0;
     for (int i = i0; i < i1; i++) {
-        const seq_view v = view_of(a, i);
-        const uint64_t tiles = (uint64_t) (((int64_t) v.rows * group + C - 1) / C), pieces = max((v.len + (int64_t) length - 1) / length, (int64_t) 1);
-        mine += TILES ? tiles : tiles * pieces;
-        parts += pieces > 1 ? tiles * pieces : 0;
+        const seq_cut<C, UNITS> cut(i == i0 ? first : view_of(a, i), group, keys);
+        mine += TILES ? cut.tiles : cut.tiles * cut.pieces;
+        parts += cut.pieces > 1 ? cut.tiles * cut.pieces : 0;
     }
-    uint64_t before = mine, parts_before = parts;
+    u64 before = mine, parts_before = parts;
     for (int o = 1; o < 64; o <<= 1) {
-        const uint64_t y = __shfl_up((unsigned long long) before, o, 64), z = __shfl_up((unsigned long long) parts_before, o, 64);
+        const u64 y = __shfl_up(before, o, 64), z = __shfl_up(parts_before, o, 64);
         if (lane >= o) { before += y; parts_before += z; }
     }
     if (lane == 63) { sums[1][wv] = before; sums[2][wv] = parts_before; }
@@ -158,28 +211,21 @@ __device__ __forceinline__ bool find_unit(const cache_attn_args & a, uint32_t x,
     before -= mine;
     parts_before -= parts;
     if (x >= before && x < before + mine) {
-        uint64_t at = x - before;
+        u64 at = x - before;
         for (int i = i0; i < i1; i++) {
-            const seq_view v = view_of(a, i);
-            const uint64_t tiles = (uint64_t) (((int64_t) v.rows * group + C - 1) / C), pieces = max((v.len + (int64_t) length - 1) / length, (int64_t) 1);
-            const uint64_t n = TILES ? tiles : tiles * pieces;
+            const seq_view v = i == i0 ? first : view_of(a, i);
+            const seq_cut<C, UNITS> cut(v, group, keys);
+            const u64 n = TILES ? cut.tiles : cut.tiles * cut.pieces;
             if (at < n) {
-                // a prompt's last rows read the most keys: they go first
-                found.tile = (int) (tiles - 1 - (TILES ? at : at / pieces));
-                found.piece = TILES ? 0 : (int) (at % pieces);
-                found.pieces = (int) pieces;
-                found.length = length;
-                found.part = (int64_t) (parts_before + (uint64_t) found.tile * pieces);
-                found.seq = i;
+                set(found, v, i, cut, at, parts_before);
                 break;
             }
             at -= n;
-            parts_before += pieces > 1 ? n : 0;
-            if (TILES && pieces > 1) parts_before += tiles * pieces - n;
+            parts_before += cut.pieces > 1 ? cut.tiles * cut.pieces : 0;
         }
     }
     __syncthreads();
-    u = found;
+    u = uniform(found);
     return u.seq >= 0;
 }
 
@@ -200,78 +246,135 @@ __device__ __forceinline__ void store4(T * p, float4_t x) {
     *(vec *) p = __builtin_convertvector(x, vec);
 }
 
+// The column's query row to f16: scaled by a power of two to a largest value in [1, 2), one term or two; c: what a product of it with a
+// key is multiplied by to be an exponent of 2 (never negative: the row carries the scale's sign)
+template <typename T, int HD, int TERMS>
+__device__ __forceinline__ void load_query(const cache_attn_args & a, const seq_view & sv, int kvh, int group, int32_t col, int g, half8_t (*q)[TERMS], float & c) {
+    constexpr int NB = HD / 32;
+    typedef T vec __attribute__((ext_vector_type(8)));
+    const T * p = (const T *) a.q + (sv.row0 + (int64_t) (col / group)) * a.ldq + ((int64_t) kvh * group + col % group) * HD + g * 8;
+    float8_t x[NB];
+    float top = 0.0f;
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+        x[b] = __builtin_convertvector(*(const vec *) (p + b * 32), float8_t);
+        for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(x[b][j]));
+    }
+    const uint32_t ex = __float_as_uint(col_max(top)) >> 23;
+    float f = ex < 254 ? __uint_as_float((254 - ex) << 23) : 0x1p-127f;
+    c = fabsf(a.scale) * LOG2E * (ex ? __uint_as_float(ex << 23) : 0x1p-127f);
+    if (ex == 0) f = 0x1p127f;                  // (below f32's normal range: 2^127 will do)
+    if (ex == 255) f = __builtin_nanf("");      // an infinity in the row: all of it NaN
+    if (a.scale < 0.0f) f = -f;
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+        x[b] *= f;
+        q[b][0] = __builtin_convertvector(x[b], half8_t);
+        if constexpr (TERMS == 2) q[b][1] = __builtin_convertvector(x[b] - __builtin_convertvector(q[b][0], float8_t), half8_t);
+    }
+}
+
+// One column's scores of a tile, s[t][r] of key + 16 t + r, to weights; its maximum, sum and accumulators follow
+template <bool MASKED, int ND>
+__device__ __forceinline__ void softmax_step(float4_t * s, int32_t key, int32_t lim, uint32_t hidden, float c, float dexp, float & mu, float & l, float4_t * o) {
+    if constexpr (MASKED) {
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+                if (key + t * 16 + r >= lim || (hidden >> t & 1)) s[t][r] = -INFINITY;
+    }
+    float top = s[0][0];
+#pragma unroll
+    for (int t = 0; t < 4; t++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) top = fmaxf(top, s[t][r]);
+    const float want = col_max(top) * c + dexp;
+    const bool move = want - mu > 14.0f;
+    if (__any(move)) {
+        const float to = move ? want - 6.0f : mu;
+        const float f = move ? __builtin_amdgcn_exp2f(mu - to) : 1.0f;
+        mu = to;
+        l *= f;
+#pragma unroll
+        for (int d = 0; d < ND; d++) o[d] *= f;
+    }
+    const float m = mu == -INFINITY ? 0.0f : mu;
+    float4_t sum = {0, 0, 0, 0};
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const float x = s[t][r];
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x, c, -m));
+            s[t][r] = MASKED && x == -INFINITY ? 0.0f : p;
+        }
+        sum += s[t];
+    }
+    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+}
+
+// The B operand of the product with V, 32 keys of strips 2 h and 2 h + 1: weights times the keys' scales of one block (4 of them at d + t *
+// stride for strip t). The fma with 0 is one v_fma_mix from and to f16.
+template <int TERMS>
+__device__ __forceinline__ void weights_times_scales(const float4_t * s, int h, const unsigned char * d, int stride, half8_t * p) {
+    const half4_t d0 = *(const half4_t *) (d + 2 * h * stride), d1 = *(const half4_t *) (d + (2 * h + 1) * stride);
+#pragma unroll
+    for (int r = 0; r < 8; r++) {
+        const float w = s[2 * h + (r >> 2)][r & 3], e = (float) (r < 4 ? d0[r & 3] : d1[r & 3]);
+        if constexpr (TERMS == 1) {
+            p[0][r] = (_Float16) __builtin_fmaf(w, e, 0.0f);
+        } else {
+            const float x = __builtin_fmaf(w, e, 0.0f);
+            p[0][r] = (_Float16) x;
+            p[1][r] = (_Float16) (x - (float) p[0][r]);
+        }
+    }
+}
+
+// 16 dimensions x 32 keys of V as the A operand, from rows of f16 VS bytes apart: lane i of 16 names row i / 4, its 4 values i % 4
+template <int VS>
+__device__ __forceinline__ half8_t read_v(const unsigned char * at, int h) {
+    typedef short short4_t __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) short4_t * lds4;
+    const half4_t x = __builtin_bit_cast(half4_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4) (at + (2 * h) * 16 * VS)));
+    const half4_t y = __builtin_bit_cast(half4_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4) (at + (2 * h + 1) * 16 * VS)));
+    return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
 template <int HD> constexpr int wave_lds() { return HD / 16 * 528 + 8 * HD; }      // V codes of a tile, then its scales
-template <int HD, int CT, int KW> constexpr int group_lds() {
-    const int loop = 4 * wave_lds<HD>(), join = KW == 4 ? 4 * 16 * CT * (HD + 4) * 4 + 4 * 16 * CT * 8 : 0;
+template <int HD, int CT> constexpr int group_lds() {
+    const int loop = 4 * wave_lds<HD>(), join = 4 * 16 * CT * (HD + 4) * 4 + 4 * 16 * CT * 8;
     return loop > join ? loop : join;
 }
 
-template <typename T, int HD, int CT, int KW>
+template <typename T, int HD, int CT>
 __global__ __launch_bounds__(NT, CT == 1 ? 3 : 2) void k_cache_attention(cache_attn_args a) {
-    constexpr int NB = HD / 32, ND = HD / 16, TERMS = sizeof(T) == 4 ? 2 : 1, WC = 16 * CT, C = KW == 4 ? WC : 4 * WC;
-    __shared__ __attribute__((aligned(16))) unsigned char lds[group_lds<HD, CT, KW>()];
+    constexpr int NB = HD / 32, ND = HD / 16, UNITS = units_of(HD, CT), TERMS = sizeof(T) == 4 ? 2 : 1, C = 16 * CT;
+    __shared__ __attribute__((aligned(16))) unsigned char lds[group_lds<HD, CT>()];
     unit u;
     const int kvh = (int) (blockIdx.x % (unsigned) a.n_kv_head);
-    if (!find_unit<C, false>(a, blockIdx.x / (unsigned) a.n_kv_head, u)) return;
+    if (!find_unit<C, UNITS, false>(a, blockIdx.x / (unsigned) a.n_kv_head, u)) return;
     if (u.pieces > 1 && u.part + u.piece >= a.parts) return;      // (row_start that overlaps itself: more pieces than rows can have)
-    const int tid = (int) threadIdx.x, lane = tid & 63, l15 = lane & 15, g = lane >> 4, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int seq = __builtin_amdgcn_readfirstlane(u.seq), group = a.n_head / a.n_kv_head;
-    const seq_view sv = view_of(a, seq);
-    const int32_t n_cols = __builtin_amdgcn_readfirstlane((int32_t) min<int64_t>((int64_t) sv.rows * group, 0x7fffffff));
-    const int32_t col0 = u.tile * C + (KW == 4 ? 0 : wv * WC);
+    const int tid = (int) threadIdx.x, lane = tid & 63, l15 = lane & 15, g = lane >> 4, wv = uniform(tid >> 6);
+    const int seq = u.seq, group = a.n_head / a.n_kv_head;
+    const seq_view sv = u.v;
+    const int32_t n_cols = (int32_t) min<int64_t>((int64_t) sv.rows * group, 0x7fffffff);
+    const int32_t col0 = u.tile * C;
     auto visible = [&](int32_t col) { return cache_visible((int64_t) sv.len - sv.rows + col / group, sv.len, a.block); };
 
-    // the wave's columns: their queries, and the keys that the first and the last of them read
-    int32_t lim[CT];
-    float c[CT];
-    half8_t q[CT][NB][TERMS];
-    const bool has = col0 < n_cols;
-    const int32_t lim_lo = has ? visible(col0) : 0, lim_hi = has ? visible(min(col0 + WC, n_cols) - 1) : 0;
-#pragma unroll
-    for (int ct = 0; ct < CT; ct++) {
-        const int32_t col = min(col0 + ct * 16 + l15, n_cols - 1);
-        lim[ct] = visible(col);
-        const T * p = (const T *) a.q + (sv.row0 + (int64_t) (col / group)) * a.ldq + ((int64_t) kvh * group + col % group) * HD + g * 8;
-        float8_t x[NB];
-        typedef T vec __attribute__((ext_vector_type(8)));
-        float top = 0.0f;
-#pragma unroll
-        for (int b = 0; b < NB; b++) {
-            x[b] = __builtin_convertvector(*(const vec *) (p + b * 32), float8_t);
-            for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(x[b][j]));
-        }
-        const uint32_t ex = __float_as_uint(col_max(top)) >> 23;
-        float f = ex < 254 ? __uint_as_float((254 - ex) << 23) : 0x1p-127f;      // (an f32 below its normal range: 2^127 will do)
-        c[ct] = fabsf(a.scale) * LOG2E * (ex ? __uint_as_float(ex << 23) : 0x1p-127f);
-        if (ex == 0) f = 0x1p127f;
-        if (ex == 255) f = __builtin_nanf("");      // an infinity in the row: all of it NaN
-        if (a.scale < 0.0f) f = -f;
-#pragma unroll
-        for (int b = 0; b < NB; b++) {
-            x[b] *= f;
-            q[ct][b][0] = __builtin_convertvector(x[b], half8_t);
-            if constexpr (TERMS == 2) q[ct][b][1] = __builtin_convertvector(x[b] - __builtin_convertvector(q[ct][b][0], float8_t), half8_t);
-        }
-    }
-
-    float4_t o[CT][ND];
-    float mu[CT], l[CT];      // mu: -inf before the first key
-#pragma unroll
-    for (int ct = 0; ct < CT; ct++) {
-        mu[ct] = -INFINITY;
-        l[ct] = 0.0f;
-        for (int d = 0; d < ND; d++) o[ct][d] = float4_t{0, 0, 0, 0};
-    }
+    // the keys that the first and the last of the wave's columns read
+    const int32_t lim_lo = visible(col0), lim_hi = visible(min(col0 + C, n_cols) - 1);
 
     // this wave's tiles of the unit's keys
-    constexpr int STEP = KW * TILE;
+    constexpr int STEP = 4 * TILE;
     const int32_t kend = (int32_t) min<int64_t>((int64_t) (u.piece + 1) * u.length, lim_hi);
-    int32_t k0 = __builtin_amdgcn_readfirstlane((int32_t) min<int64_t>((int64_t) u.piece * u.length + (KW == 4 ? wv * TILE : 0), 0x7fffff00));
+    int32_t k0 = ((int32_t) min<int64_t>((int64_t) u.piece * u.length + wv * TILE, 0x7fffff00));
     const int last_strip = (kend - 1) / 16, strips_of_page = a.page_size / 16, page_shift = __builtin_ctz(strips_of_page);
     const int32_t * table = a.table + (int64_t) seq * a.width;
     auto load_pages = [&](int32_t key) { return table[min(key / 16 + (lane & 3), last_strip) >> page_shift]; };
     uint32_t kn[4][NB], vn[4][NB], sn[4], bad_n = 0;      // the tile's codes and scales, in flight
-    int pages = 0;                                         // page numbers of the next one, in lanes 0 to 3
+    int pages = k0 < kend ? load_pages(k0) : 0;            // page numbers of the next one, in lanes 0 to 3
     // a strip as a buffer resource (no bytes past the end of this wave's keys: such loads give 0 without a memory access)
     auto strip_of = [&](int32_t key, int pages, int t, uint32_t & bad) {
         const int strip = min(key / 16 + t, last_strip);
@@ -298,6 +401,27 @@ __global__ __launch_bounds__(NT, CT == 1 ? 3 : 2) void k_cache_attention(cache_a
     // where this lane's V words go, [dimension tile][64 keys][8 bytes], and the row that it names for the transposed read
     const int e = (l15 & 3) * 2 + ((l15 & 7) >> 2);
     const int tr_at = (((l15 >> 3) * 2 + (e >> 2)) * 16 + g * 4 + (e & 3)) * 8;
+    if (k0 < kend) {
+        load_v(k0, pages);
+        load_k(k0, pages);
+        pages = load_pages(k0 + STEP);
+    }
+    int32_t lim[CT];
+    float c[CT];
+    half8_t q[CT][NB][TERMS];
+#pragma unroll
+    for (int ct = 0; ct < CT; ct++) load_query<T, HD, TERMS>(a, sv, kvh, group, min(col0 + ct * 16 + l15, n_cols - 1), g, q[ct], c[ct]);
+#pragma unroll
+    for (int ct = 0; ct < CT; ct++) lim[ct] = visible(min(col0 + ct * 16 + l15, n_cols - 1));
+    float4_t o[CT][ND];
+    float mu[CT], l[CT];      // mu: -inf before the first key
+#pragma unroll
+    for (int ct = 0; ct < CT; ct++) {
+        mu[ct] = -INFINITY;
+        l[ct] = 0.0f;
+        for (int d = 0; d < ND; d++) o[ct][d] = float4_t{0, 0, 0, 0};
+    }
+
     uint32_t k1024 = 0x64006400u;
     asm volatile("" : "+v"(k1024));
     // one tile: MASKED where it passes some column's last key, the end, or has a page that is none
@@ -348,69 +472,16 @@ __global__ __launch_bounds__(NT, CT == 1 ? 3 : 2) void k_cache_attention(cache_a
         }
         load_k(k0 + STEP, pages);
         pages = load_pages(k0 + 2 * STEP);
-        // weights
 #pragma unroll
-        for (int ct = 0; ct < CT; ct++) {
-            if constexpr (MASKED) {
-#pragma unroll
-                for (int t = 0; t < 4; t++)
-#pragma unroll
-                    for (int r = 0; r < 4; r++)
-                        if (k0 + t * 16 + g * 4 + r >= lim[ct] || (bad >> t & 1)) s[ct][t][r] = -INFINITY;
-            }
-            float top = s[ct][0][0];
-#pragma unroll
-            for (int t = 0; t < 4; t++)
-#pragma unroll
-                for (int r = 0; r < 4; r++) top = fmaxf(top, s[ct][t][r]);
-            const float want = col_max(top) * c[ct] + dexp;
-            const bool move = want - mu[ct] > 14.0f;
-            if (__any(move)) {
-                const float to = move ? want - 6.0f : mu[ct];
-                const float f = move ? __builtin_amdgcn_exp2f(mu[ct] - to) : 1.0f;
-                mu[ct] = to;
-                l[ct] *= f;
-#pragma unroll
-                for (int d = 0; d < ND; d++) o[ct][d] *= f;
-            }
-            const float m = mu[ct] == -INFINITY ? 0.0f : mu[ct];
-            float4_t sum = {0, 0, 0, 0};
-#pragma unroll
-            for (int t = 0; t < 4; t++) {
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const float x = s[ct][t][r];
-                    float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x, c[ct], -m));
-                    if constexpr (MASKED) p = x == -INFINITY ? 0.0f : p;
-                    s[ct][t][r] = p;
-                }
-                sum += s[ct][t];
-            }
-            l[ct] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        }
-        // O^T += V^T P'^T, block by block of the head (the fma with 0 is one v_fma_mix from and to f16)
+        for (int ct = 0; ct < CT; ct++) softmax_step<MASKED, ND>(s[ct], k0 + g * 4, lim[ct], bad, c[ct], dexp, mu[ct], l[ct], o[ct]);
+        // O^T += V^T P'^T, block by block of the head
 #pragma unroll
         for (int b = 0; b < NB; b++) {
             half8_t p[CT][2][TERMS];
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const half4_t d0 = *(const half4_t *) (scales + 2 * h * 2 * HD + HD + g * (8 * NB) + b * 8);
-                const half4_t d1 = *(const half4_t *) (scales + (2 * h + 1) * 2 * HD + HD + g * (8 * NB) + b * 8);
+            for (int h = 0; h < 2; h++)
 #pragma unroll
-                for (int ct = 0; ct < CT; ct++) {
-#pragma unroll
-                    for (int r = 0; r < 8; r++) {
-                        const float w = s[ct][2 * h + (r >> 2)][r & 3], d = (float) (r < 4 ? d0[r & 3] : d1[r & 3]);
-                        if constexpr (TERMS == 1) {
-                            p[ct][h][0][r] = (_Float16) __builtin_fmaf(w, d, 0.0f);
-                        } else {
-                            const float x = __builtin_fmaf(w, d, 0.0f);
-                            p[ct][h][0][r] = (_Float16) x;
-                            p[ct][h][1][r] = (_Float16) (x - (float) p[ct][h][0][r]);
-                        }
-                    }
-                }
-            }
+                for (int ct = 0; ct < CT; ct++) weights_times_scales<TERMS>(s[ct], h, scales + HD + g * (8 * NB) + b * 8, 2 * HD, p[ct][h]);
 #pragma unroll
             for (int dd = 0; dd < 2; dd++) {
                 const int d = 2 * b + dd;
@@ -428,12 +499,6 @@ __global__ __launch_bounds__(NT, CT == 1 ? 3 : 2) void k_cache_attention(cache_a
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    if (k0 < kend) {
-        pages = load_pages(k0);
-        load_v(k0, pages);
-        load_k(k0, pages);
-        pages = load_pages(k0 + STEP);
-    }
     for (; k0 + TILE <= min(lim_lo, kend) && bad_n == 0; k0 += STEP) tile(std::false_type{});
     for (; k0 < kend; k0 += STEP) tile(std::true_type{});
 #pragma unroll
@@ -441,78 +506,299 @@ __global__ __launch_bounds__(NT, CT == 1 ? 3 : 2) void k_cache_attention(cache_a
 
     const parts_view<HD, C> part(a, u.part + u.piece, kvh);
     auto out_at = [&](int32_t col) { return (T *) a.out + (sv.row0 + (int64_t) (col / group)) * a.ldo + ((int64_t) kvh * group + col % group) * HD; };
-    if constexpr (KW == 1) {
+    // the four waves' sums at the largest of their maxima
+    float * const stat = (float *) (lds + 4 * C * (HD + 4) * 4), * const sum = (float *) lds;
+    __syncthreads();      // the loop's LDS is read out
+    if (g == 0)
+        for (int ct = 0; ct < CT; ct++) { stat[(wv * C + ct * 16 + l15) * 2] = mu[ct]; stat[(wv * C + ct * 16 + l15) * 2 + 1] = l[ct]; }
 #pragma unroll
-        for (int ct = 0; ct < CT; ct++) {
-            const int32_t at = wv * WC + ct * 16 + l15, col = u.tile * C + at;
-            if (col >= n_cols) continue;
-            if (u.pieces > 1) {
-                if (g == 0) { part.s[2 * at] = mu[ct]; part.s[2 * at + 1] = l[ct]; }
-                for (int d = 0; d < ND; d++) *(float4_t *) (part.o + (int64_t) at * HD + d * 16 + g * 4) = o[ct][d];
-            } else {
-                const float inv = l[ct] == 0.0f ? 0.0f : 1.0f / l[ct];
-                T * p = out_at(col);
-                for (int d = 0; d < ND; d++) store4(p + d * 16 + g * 4, o[ct][d] * inv);
-            }
+    for (int ct = 0; ct < CT; ct++)
+        for (int d = 0; d < ND; d++) *(float4_t *) (sum + (wv * C + ct * 16 + l15) * (HD + 4) + d * 16 + g * 4) = o[ct][d];
+    __syncthreads();
+    for (int i = tid; i < C * (HD / 4); i += NT) {
+        const int at = i / (HD / 4), n = i % (HD / 4) * 4;
+        const int32_t col = col0 + at;
+        if (col >= n_cols) break;
+        float top = -INFINITY, all = 0.0f;
+        for (int w = 0; w < 4; w++) top = fmaxf(top, stat[(w * C + at) * 2]);
+        const float m = top == -INFINITY ? 0.0f : top;
+        float4_t x = {0, 0, 0, 0};
+        for (int w = 0; w < 4; w++) {
+            const float f = __builtin_amdgcn_exp2f(stat[(w * C + at) * 2] - m);
+            all += stat[(w * C + at) * 2 + 1] * f;
+            x += *(const float4_t *) (sum + (w * C + at) * (HD + 4) + n) * f;
         }
-    } else {
-        // the four waves' sums at the largest of their maxima
-        float * const stat = (float *) (lds + 4 * WC * (HD + 4) * 4), * const sum = (float *) lds;
-        __syncthreads();      // the loop's LDS is read out
-        if (g == 0)
-            for (int ct = 0; ct < CT; ct++) { stat[(wv * WC + ct * 16 + l15) * 2] = mu[ct]; stat[(wv * WC + ct * 16 + l15) * 2 + 1] = l[ct]; }
-#pragma unroll
-        for (int ct = 0; ct < CT; ct++)
-            for (int d = 0; d < ND; d++) *(float4_t *) (sum + (wv * WC + ct * 16 + l15) * (HD + 4) + d * 16 + g * 4) = o[ct][d];
-        __syncthreads();
-        for (int i = tid; i < WC * (HD / 4); i += NT) {
-            const int at = i / (HD / 4), n = i % (HD / 4) * 4;
-            const int32_t col = col0 + at;
-            if (col >= n_cols) break;
-            float top = -INFINITY, all = 0.0f;
-            for (int w = 0; w < 4; w++) top = fmaxf(top, stat[(w * WC + at) * 2]);
-            const float m = top == -INFINITY ? 0.0f : top;
-            float4_t x = {0, 0, 0, 0};
-            for (int w = 0; w < 4; w++) {
-                const float f = __builtin_amdgcn_exp2f(stat[(w * WC + at) * 2] - m);
-                all += stat[(w * WC + at) * 2 + 1] * f;
-                x += *(const float4_t *) (sum + (w * WC + at) * (HD + 4) + n) * f;
-            }
-            if (u.pieces > 1) {
-                if (n == 0) { part.s[2 * at] = top; part.s[2 * at + 1] = all; }
-                *(float4_t *) (part.o + (int64_t) at * HD + n) = x;
-            } else {
-                store4(out_at(col) + n, x * (all == 0.0f ? 0.0f : 1.0f / all));
-            }
+        if (u.pieces > 1) {
+            if (n == 0) { part.s[2 * at] = top; part.s[2 * at + 1] = all; }
+            *(float4_t *) (part.o + (int64_t) at * HD + n) = x;
+        } else {
+            store4(out_at(col) + n, x * (all == 0.0f ? 0.0f : 1.0f / all));
         }
     }
 }
 
-// the pieces of a column tile added in their order
-template <typename T, int HD, int C>
-__global__ __launch_bounds__(NT) void k_cache_join(cache_attn_args a) {
+// Prompts: many columns for each key, so what a key costs is paid once a workgroup. Its four waves have 16 CT columns each; a
+// tile's codes are turned into f16 once, by all four (a strip each), into double-buffered LDS, K as rows for the A operand and V as
+// rows that ds_read_b64_tr_b16 turns around. One barrier a tile; the next tile's codes are in flight meanwhile.
+// For bf16 rows the scales go in with the codes (K and V rounded to f16, 2^-12 relative, against bf16's half step of 2^-9): no
+// work per score is left but the softmax. f16 and f32 rows keep codes exact and scales in 32 bits as above.
+template <typename T, int HD, int CT>
+__global__ __launch_bounds__(NT, 2) void k_cache_prompt(cache_attn_args a) {
+    constexpr bool SCALED = std::is_same<T, __bf16>::value;
+    constexpr int NB = HD / 32, ND = HD / 16, UNITS = units_of(HD, 2), TERMS = sizeof(T) == 4 ? 2 : 1, WC = 16 * CT, C = 4 * WC;
+    constexpr int KS = 2 * HD + 16, VS = 2 * HD + 32, SCALES = TILE * (KS + VS), BUF = SCALES + (SCALED ? 0 : 8 * HD);
+    __shared__ __attribute__((aligned(16))) unsigned char lds[2 * BUF];
+    __shared__ uint32_t tile_dmax[2][4], tile_bad[2][4];
     unit u;
     const int kvh = (int) (blockIdx.x % (unsigned) a.n_kv_head);
-    if (!find_unit<C, true>(a, blockIdx.x / (unsigned) a.n_kv_head, u) || u.pieces < 2 || u.part + u.pieces > a.parts) return;
-    const seq_view sv = view_of(a, u.seq);
-    const int group = a.n_head / a.n_kv_head;
-    const int64_t n_cols = (int64_t) sv.rows * group, col0 = (int64_t) u.tile * C;
-    for (int i = (int) threadIdx.x; i < C * (HD / 4); i += NT) {
-        const int at = i / (HD / 4), n = i % (HD / 4) * 4;
-        const int64_t col = col0 + at;
-        if (col >= n_cols) break;
-        float top = -INFINITY, all = 0.0f;
-        for (int k = 0; k < u.pieces; k++) top = fmaxf(top, parts_view<HD, C>(a, u.part + k, kvh).s[2 * at]);
-        const float m = top == -INFINITY ? 0.0f : top;
-        float4_t x = {0, 0, 0, 0};
-        for (int k = 0; k < u.pieces; k++) {
-            const parts_view<HD, C> p(a, u.part + k, kvh);
-            const float f = __builtin_amdgcn_exp2f(p.s[2 * at] - m);
-            all += p.s[2 * at + 1] * f;
-            x += *(const float4_t *) (p.o + (int64_t) at * HD + n) * f;
+    if (!find_unit<C, UNITS, false>(a, blockIdx.x / (unsigned) a.n_kv_head, u)) return;
+    if (u.pieces > 1 && u.part + u.piece >= a.parts) return;
+    const int tid = (int) threadIdx.x, lane = tid & 63, l15 = lane & 15, g = lane >> 4, wv = uniform(tid >> 6);
+    const int seq = u.seq, group = a.n_head / a.n_kv_head;
+    const seq_view sv = u.v;
+    const int32_t n_cols = (int32_t) min<int64_t>((int64_t) sv.rows * group, 0x7fffffff);
+    const int32_t first = u.tile * C, col0 = first + wv * WC;
+    auto visible = [&](int32_t col) { return cache_visible((int64_t) sv.len - sv.rows + col / group, sv.len, a.block); };
+    const bool has = col0 < n_cols;
+    const int32_t lim_lo = has ? visible(col0) : 0, lim_hi = has ? visible(min(col0 + WC, n_cols) - 1) : 0;
+    const int32_t kend = (int32_t) min<int64_t>((int64_t) (u.piece + 1) * u.length, visible(min(first + C, n_cols) - 1));      // the workgroup's
+    int32_t k0 = ((int32_t) min<int64_t>((int64_t) u.piece * u.length, 0x7fffff00));
+
+    // this wave's strip of a tile: codes and scales on their way to LDS
+    const int last_strip = (kend - 1) / 16, strips_of_page = a.page_size / 16, page_shift = __builtin_ctz(strips_of_page);
+    const int32_t * table = a.table + (int64_t) seq * a.width;
+    auto load_page = [&](int32_t key) { return table[min(key / 16 + wv, last_strip) >> page_shift]; };
+    uint32_t kx[NB], vx[NB], sx[SCALED ? NB + 2 : 1], bad = 0;
+    int32_t page_n = k0 < kend ? load_page(k0) : 0;
+    const int vb0 = (lane & 3) * NB >> 2, vb1 = ((lane & 3) * NB + NB - 1) >> 2;      // blocks of the lane's first and last V word
+    auto load = [&](int32_t key) {
+        const int strip = min(key / 16 + wv, last_strip);
+        int64_t page = __builtin_amdgcn_readfirstlane(page_n);
+        bad = page < 0 || page >= a.n_pages;
+        if (bad) page = 0;
+        const brsrc s = make_brsrc(a.cache + ((page * a.n_kv_head + kvh) * strips_of_page + (strip & (strips_of_page - 1))) * (18 * HD), key < kend ? 18 * HD : 0);
+        load_words<NB>(kx, s, lane * (4 * NB), 0);
+        load_words<NB>(vx, s, lane * (4 * NB), 8 * HD);
+        if constexpr (SCALED) {
+#pragma unroll
+            for (int b = 0; b < NB; b++) sx[b] = __builtin_amdgcn_raw_buffer_load_b16(s, cache_k_scale(l15, b, HD), 0, 0);
+            sx[NB] = __builtin_amdgcn_raw_buffer_load_b16(s, cache_v_scale(lane >> 2, vb0, HD), 0, 0);
+            sx[NB + 1] = NB == 3 ? (uint32_t) __builtin_amdgcn_raw_buffer_load_b16(s, cache_v_scale(lane >> 2, vb1, HD), 0, 0) : sx[NB];
+        } else {
+            load_words<1>(sx, s, 16 * HD + lane * 4, 0);      // (0 past the strip's scales, from lane HD / 2 on)
         }
-        T * out = (T *) a.out + (sv.row0 + col / group) * a.ldo + ((int64_t) kvh * group + col % group) * HD;
-        store4(out + n, x * (all == 0.0f ? 0.0f : 1.0f / all));
+        page_n = load_page(key + TILE);
+    };
+    uint32_t k1024 = 0x64006400u;
+    asm volatile("" : "+v"(k1024));
+    auto scale2 = [](half8_t x, uint32_t d) {
+        const _Float16 h = __builtin_bit_cast(_Float16, (uint16_t) d);
+        return x * half8_t{h, h, h, h, h, h, h, h};
+    };
+    auto stage = [&](int32_t key, int buf) {      // the strip that load(key) brought
+        unsigned char * const l = lds + buf * BUF;
+        const bool k_ok = key + wv * 16 + l15 < kend && !bad, v_ok = key + wv * 16 + (lane >> 2) < kend && !bad;
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            half8_t x = codes8(kx[b], k1024);
+            if constexpr (SCALED) x = scale2(x, k_ok ? sx[b] : 0u);
+            *(half8_t *) (l + (wv * 16 + l15) * KS + b * 64 + g * 16) = x;
+        }
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            const int w = (lane & 3) * NB + b;
+            half8_t x = codes8(vx[b], k1024);
+            x = half8_t{x[0], x[2], x[4], x[6], x[1], x[3], x[5], x[7]};      // dims in order
+            if constexpr (SCALED) x = scale2(x, !v_ok ? 0u : w >> 2 == vb0 ? sx[NB] : sx[NB + 1]);
+            *(half8_t *) (l + TILE * KS + (wv * 16 + (lane >> 2)) * VS + w * 16) = x;
+        }
+        uint32_t dmax = 0;
+        if constexpr (!SCALED) {
+            const int d = lane % (HD / 4);
+            const int32_t at = key + wv * 16 + d / (2 * NB) * 4 + (d & 1) * 2;
+            const uint32_t sc = at >= kend || bad ? 0u : at + 1 >= kend ? sx[0] & 0xffffu : sx[0];
+            if (lane < HD / 2) *(uint32_t *) (l + SCALES + wv * 2 * HD + lane * 4) = sc;
+            dmax = wave_umax(lane >= HD / 4 ? max(sc & 0x7fffu, sc >> 16 & 0x7fffu) : 0u);
+        }
+        if (lane == 0) {
+            tile_dmax[buf][wv] = dmax;
+            tile_bad[buf][wv] = bad;
+        }
+    };
+
+    float c[CT];
+    half8_t q[CT][NB][TERMS];
+    int32_t lim[CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ct++) load_query<T, HD, TERMS>(a, sv, kvh, group, min(col0 + ct * 16 + l15, n_cols - 1), g, q[ct], c[ct]);
+#pragma unroll
+    for (int ct = 0; ct < CT; ct++) lim[ct] = visible(min(col0 + ct * 16 + l15, n_cols - 1));
+    float4_t o[CT][ND];
+    float mu[CT], l[CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ct++) {
+        mu[ct] = -INFINITY;
+        l[ct] = 0.0f;
+        for (int d = 0; d < ND; d++) o[ct][d] = float4_t{0, 0, 0, 0};
+    }
+
+    int buf = 0;
+    const int tr_at = TILE * KS + (g * 4 + (l15 >> 2)) * VS + (lane & 3) * 8;
+    auto tile = [&](auto masked) {
+        constexpr bool MASKED = decltype(masked)::value;
+        const unsigned char * const m = lds + buf * BUF, * const scales = m + SCALES;
+        uint32_t hidden = 0;
+        if constexpr (MASKED) hidden = tile_bad[buf][0] | tile_bad[buf][1] << 1 | tile_bad[buf][2] << 2 | tile_bad[buf][3] << 3;
+        float dexp = 0.0f;
+        if constexpr (!SCALED) dexp = (float) ((int) (max(max(tile_dmax[buf][0], tile_dmax[buf][1]), max(tile_dmax[buf][2], tile_dmax[buf][3])) >> 10) - 14);
+        float4_t s[CT][4];
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+#pragma unroll
+            for (int ct = 0; ct < CT; ct++) s[ct][t] = float4_t{0, 0, 0, 0};
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                const half8_t kc = *(const half8_t *) (m + (t * 16 + l15) * KS + b * 64 + g * 16);
+                if constexpr (SCALED) {
+#pragma unroll
+                    for (int ct = 0; ct < CT; ct++) s[ct][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc, q[ct][b][0], s[ct][t], 0, 0, 0);
+                } else {
+                    const half4_t d = *(const half4_t *) (scales + t * 2 * HD + g * (8 * NB) + b * 8);
+#pragma unroll
+                    for (int ct = 0; ct < CT; ct++) {
+                        float4_t x = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc, q[ct][b][0], float4_t{0, 0, 0, 0}, 0, 0, 0);
+                        if constexpr (TERMS == 2) x = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc, q[ct][b][1], x, 0, 0, 0);
+#pragma unroll
+                        for (int r = 0; r < 4; r++) s[ct][t][r] = __builtin_fmaf((float) d[r], x[r], s[ct][t][r]);
+                    }
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int ct = 0; ct < CT; ct++) softmax_step<MASKED, ND>(s[ct], k0 + g * 4, lim[ct], hidden, c[ct], dexp, mu[ct], l[ct], o[ct]);
+        if constexpr (SCALED) {
+            half8_t p[CT][2];
+#pragma unroll
+            for (int ct = 0; ct < CT; ct++)
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int r = 0; r < 8; r++) p[ct][h][r] = (_Float16) s[ct][2 * h + (r >> 2)][r & 3];
+#pragma unroll
+            for (int d = 0; d < ND; d++) {
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const half8_t v = read_v<VS>(m + tr_at + d * 32, h);
+#pragma unroll
+                    for (int ct = 0; ct < CT; ct++) o[ct][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[ct][h], o[ct][d], 0, 0, 0);
+                }
+                if (d & 1) __builtin_amdgcn_sched_barrier(0);
+            }
+        } else {
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                half8_t p[CT][2][TERMS];
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int ct = 0; ct < CT; ct++) weights_times_scales<TERMS>(s[ct], h, scales + HD + g * (8 * NB) + b * 8, 2 * HD, p[ct][h]);
+#pragma unroll
+                for (int dd = 0; dd < 2; dd++) {
+                    const int d = 2 * b + dd;
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const half8_t v = read_v<VS>(m + tr_at + d * 32, h);
+#pragma unroll
+                        for (int ct = 0; ct < CT; ct++)
+#pragma unroll
+                            for (int k = 0; k < TERMS; k++) o[ct][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[ct][h][k], o[ct][d], 0, 0, 0);
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+    };
+    if (k0 < kend) {
+        load(k0);
+        stage(k0, 0);
+        load(k0 + TILE);
+    }
+    __syncthreads();
+    auto step = [&](auto masked) {
+        if (k0 + TILE < kend) stage(k0 + TILE, buf ^ 1);
+        load(k0 + 2 * TILE);
+        if (k0 < lim_hi) tile(masked);
+        __syncthreads();
+        buf ^= 1;
+    };
+    auto no_bad = [&] { return (tile_bad[buf][0] | tile_bad[buf][1] | tile_bad[buf][2] | tile_bad[buf][3]) == 0; };
+    for (; k0 + TILE <= min(lim_lo, kend) && no_bad(); k0 += TILE) step(std::false_type{});
+    for (; k0 < kend; k0 += TILE) step(std::true_type{});
+
+    const parts_view<HD, C> part(a, u.part + u.piece, kvh);
+#pragma unroll
+    for (int ct = 0; ct < CT; ct++) {
+        const float sum = col_sum(l[ct]);
+        const int32_t at = wv * WC + ct * 16 + l15, col = first + at;
+        if (col >= n_cols) continue;
+        if (u.pieces > 1) {
+            if (g == 0) { part.s[2 * at] = mu[ct]; part.s[2 * at + 1] = sum; }
+            for (int d = 0; d < ND; d++) *(float4_t *) (part.o + (int64_t) at * HD + d * 16 + g * 4) = o[ct][d];
+        } else {
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            T * p = (T *) a.out + (sv.row0 + (int64_t) (col / group)) * a.ldo + ((int64_t) kvh * group + col % group) * HD;
+            for (int d = 0; d < ND; d++) store4(p + d * 16 + g * 4, o[ct][d] * inv);
+        }
+    }
+}
+
+// The pieces of a column tile added in a fixed order: a column at a time, HD / 4 threads across its values, the others across its
+// pieces. `split` workgroups share a tile's columns.
+template <typename T, int HD, int C, int UNITS>
+__global__ __launch_bounds__(NT) void k_cache_join(cache_attn_args a, int split) {
+    constexpr int W = HD / 4, PG = NT / W;      // threads across a column, pieces at once
+    __shared__ float top4[NT / 64], sum[PG];
+    __shared__ __attribute__((aligned(16))) float acc[PG][HD];
+    unit u;
+    const unsigned id = blockIdx.x / (unsigned) a.n_kv_head;
+    const int kvh = (int) (blockIdx.x % (unsigned) a.n_kv_head);
+    if (!find_unit<C, UNITS, true>(a, id / (unsigned) split, u) || u.pieces < 2 || u.part + u.pieces > a.parts) return;
+    const int tid = (int) threadIdx.x, pg = tid / W, n = tid % W * 4, group = a.n_head / a.n_kv_head;
+    const int64_t n_cols = (int64_t) u.v.rows * group, col0 = (int64_t) u.tile * C;
+    for (int at = (int) (id % (unsigned) split); at < C && col0 + at < n_cols; at += split) {
+        float top = -INFINITY;
+        for (int k = tid; k < u.pieces; k += NT) top = fmaxf(top, parts_view<HD, C>(a, u.part + k, kvh).s[2 * at]);
+        for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+        if (tid % 64 == 0) top4[tid / 64] = top;
+        __syncthreads();
+        top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3]));
+        const float m = top == -INFINITY ? 0.0f : top;
+        float all = 0.0f;
+        float4_t x = {0, 0, 0, 0};
+        if (pg < PG)
+#pragma unroll 4
+            for (int k = pg; k < u.pieces; k += PG) {
+                const parts_view<HD, C> p(a, u.part + k, kvh);
+                const float f = __builtin_amdgcn_exp2f(p.s[2 * at] - m);
+                all += p.s[2 * at + 1] * f;
+                x += *(const float4_t *) (p.o + (int64_t) at * HD + n) * f;
+            }
+        if (pg < PG) {
+            *(float4_t *) &acc[pg][n] = x;
+            if (n == 0) sum[pg] = all;
+        }
+        __syncthreads();
+        if (tid < W) {
+            for (int k = 1; k < PG; k++) {
+                all += sum[k];
+                x += *(const float4_t *) &acc[k][n];
+            }
+            const int64_t col = col0 + at;
+            T * out = (T *) a.out + (u.v.row0 + col / group) * a.ldo + ((int64_t) kvh * group + col % group) * HD;
+            store4(out + n, x * (all == 0.0f ? 0.0f : 1.0f / all));
+        }
+        __syncthreads();
     }
 }
 
@@ -526,32 +812,36 @@ int columns_of(const cache_shape & c, int64_t n_seq, int64_t n_rows) {
 int64_t tiles_bound(const cache_shape & c, int64_t n_seq, int64_t n_rows) {
     return n_rows * (c.n_head / c.n_kv_head) / columns_of(c, n_seq, n_rows) + n_seq;
 }
-// Pieces are at least keys * kv heads / UNITS long, keys summed over column tiles: all of them without rounding up are UNITS / kv
-// heads at most, and rounding up doubles that at most where there are two or more of a tile, as there must be to have parts.
+// A tile's pieces are keys of its sequence / length rounded, length at least UNITS-th of the keys of all tiles and K/V heads: without
+// the rounding all are UNITS / K/V heads at most, and where there are two or more (1.5 before rounding) it adds a third at most.
 int64_t parts_bound(const cache_shape & c, int64_t n_seq, int64_t n_rows, int64_t width) {
-    const int64_t most = (width * c.page_size + PIECE - 1) / PIECE;
+    const int64_t most = (width * c.page_size + PIECE / 2) / PIECE, units = units_of(c.hd, columns_of(c, n_seq, n_rows) > 16 ? 2 : 1);
     if (most < 2) return 0;
-    return std::min(tiles_bound(c, n_seq, n_rows) * most, 2 * (int64_t) ((UNITS + c.n_kv_head - 1) / c.n_kv_head));
+    return std::min(tiles_bound(c, n_seq, n_rows) * most, (4 * units / 3 + c.n_kv_head - 1) / c.n_kv_head + 1);
 }
 
-template <typename T, int HD, int CT, int KW>
-hipError_t attend(const cache_shape & c, const cache_attn_args & a, hipStream_t s) {
-    constexpr int C = KW == 4 ? 16 * CT : 64 * CT;
+template <typename T, int HD, int CT, int C>
+hipError_t attend(const cache_shape & c, const cache_attn_args & a, hipStream_t s, const void * kernel) {
     cache_attn_args args = a;
     void * p[] = {&args};
     const int64_t tiles = tiles_bound(c, a.n_seq, a.n_rows), parts = parts_bound(c, a.n_seq, a.n_rows, a.width);
     args.parts = parts;
     const int64_t blocks = (tiles + parts) * c.n_kv_head;
     if (blocks >= 1 << 24) return hipErrorInvalidConfiguration;      // threads of a launch are below 2^32
-    const hipError_t e = hipLaunchKernel((const void *) k_cache_attention<T, HD, CT, KW>, dim3((unsigned) blocks), dim3(NT), p, 0, s);
+    const hipError_t e = hipLaunchKernel(kernel, dim3((unsigned) blocks), dim3(NT), p, 0, s);
     if (e != hipSuccess || !parts) return e;
-    return hipLaunchKernel((const void *) k_cache_join<T, HD, C>, dim3((unsigned) (tiles * c.n_kv_head)), dim3(NT), p, 0, s);
+    // few tiles: up to a workgroup for each column; many are hardly split
+    int split = (int) std::min<int64_t>(C, std::max<int64_t>(1, 2048 / (tiles * c.n_kv_head)));
+    void * pj[] = {&args, &split};
+    return hipLaunchKernel((const void *) k_cache_join<T, HD, C, units_of(HD, CT)>, dim3((unsigned) (tiles * c.n_kv_head * split)), dim3(NT), pj, 0, s);
 }
 
 template <typename T, int HD>
 hipError_t by_columns(const cache_shape & c, const cache_attn_args & a, hipStream_t s) {
     const int cols = columns_of(c, a.n_seq, a.n_rows);
-    return cols == 16 ? attend<T, HD, 1, 4>(c, a, s) : cols == 32 ? attend<T, HD, 2, 4>(c, a, s) : attend<T, HD, 2, 1>(c, a, s);
+    return cols == 16 ? attend<T, HD, 1, 16>(c, a, s, (const void *) k_cache_attention<T, HD, 1>)
+         : cols == 32 ? attend<T, HD, 2, 32>(c, a, s, (const void *) k_cache_attention<T, HD, 2>)
+                      : attend<T, HD, 2, 128>(c, a, s, (const void *) k_cache_prompt<T, HD, 2>);
 }
 
 template <typename T>

@@ -9,6 +9,9 @@ Attention's tolerance, for one row and head with out = sum_j p_j v_j and A = sum
                                  value and an exact key, times a scale: off by at most (head_dim / 8 + 8) 2^-22 S,
                                  S = max_j scale |q|max |k_j|_1; the weights follow by the factor e^x ~ 1 + x on both sides
                                  of the fraction (twice), and their own 2^-21 and the sums' sqrt(n) 2^-24 come on top.
+  bf16 rows, keys and values     where many rows share them the cached values are rounded to f16, 2^-12 relative: a score is off by at
+                                 most 2^-12 S1, S1 = max_j scale sum_n |q_n| |k_jn|, on both sides of the fraction, and the sum over
+                                 V by 2^-12 A
   small weights                  a weight enters the product with V as p_j d_j in f16 (the scale d_j of its block of V, the value
                                  at most 8 d_j), moved by a power of two that brings the largest p_j max d to 2^6 or more: f16's
                                  smallest step, half of it 2^-25, is 2^-31 of that largest one. Divided by the sum of the p_j, which
@@ -311,7 +314,10 @@ def reference(p, q, start, total, table, block, scale, kind):
             A = w @ v[:, h // group].abs()
             k1 = torch.nan_to_num(k[:, h // group]).abs().sum(-1)
             S = abs(scale) * x.abs().amax(-1, keepdim=True) * (k1.max() if n else 0.0)
-            f32 = 2 * (hd / 8 + 8) * 2.0 ** -22 * S + 2.0 ** -20 + (n ** 0.5) * 2.0 ** -24
+            low = 0.0
+            if kind == "bf16" and n:
+                low = 2.0 ** -12 * (1 + 2 * abs(scale) * (x.abs() @ torch.nan_to_num(k[:, h // group]).abs().T).amax(-1, keepdim=True))
+            f32 = low + 2 * (hd / 8 + 8) * 2.0 ** -22 * S + 2.0 ** -20 + (n ** 0.5) * 2.0 ** -24
             out[a:b, h] = y
             tol[a:b, h] = eps * y.abs() + tiny + n * 2.0 ** -30 * (v[:, h // group].abs().max() if n else 0.0) + (f32 + (2.0 ** -12 if kind != "f32" else 0.0)) * A * (1 + eps)
     return out.reshape(q.shape), tol.reshape(q.shape)
