@@ -165,7 +165,7 @@ extern "C" int jepa_amd_cache_attention(int device, const jepa_amd_cache_shape *
     }
     cache_attn_args a;
     a.cache = (const unsigned char *) cache; a.q = q; a.out = out; a.ldq = q_stride; a.ldo = out_stride; a.n_rows = n_rows; a.n_pages = c.n_pages;
-    a.block = causal_block; a.row_start = row_start; a.kv_len = kv_len; a.table = table; a.n_seq = (int) n_seq; a.width = (int) table_width;
+    a.block = cache_block_of(causal_block); a.row_start = row_start; a.kv_len = kv_len; a.table = table; a.n_seq = (int) n_seq; a.width = (int) table_width;
     a.n_head = c.n_head; a.n_kv_head = c.n_kv_head; a.page_size = c.page_size; a.scale = scale; a.work = (float *) work;
     return on_device(who, device, [&] { return n_rows && n_seq ? launch_cache_attention(c, type, a, (hipStream_t) stream) : hipSuccess; });
 }

@@ -122,102 +122,100 @@ __device__ __forceinline__ seq_view view_of(const cache_attn_args & a, int i) {
 struct unit { seq_view v; int seq, tile, piece, pieces; int32_t length; int64_t part; };
 
 // Column tiles and pieces of a sequence where the call's keys (over all column tiles and K/V heads) are `keys`: the number of pieces
-// that comes nearest to keys / UNITS each
-template <int C, int UNITS>
+// that comes nearest to keys / UNITS each. A float sum will do: every workgroup adds the same numbers in the same order.
+template <int C>
 struct seq_cut {
-    uint64_t tiles, pieces;
-    __device__ seq_cut(const seq_view & v, int group, uint64_t keys) {
-        tiles = (uint64_t) (((int64_t) v.rows * group + C - 1) / C);
-        const uint64_t length = max(keys / UNITS, (uint64_t) PIECE);
-        pieces = max(((uint32_t) v.len + length / 2) / length, (uint64_t) 1);
+    uint32_t tiles, pieces;
+    __device__ seq_cut(const seq_view & v, int group, uint32_t length) {
+        tiles = ((uint32_t) v.rows * (uint32_t) group + C - 1) / C;      // (rows * heads are below 2^27)
+        pieces = max(((uint32_t) v.len + length / 2) / length, 1u);
     }
 };
-
-template <typename X>
-__device__ __forceinline__ X wave_sum(X x) {
-    for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o, 64);
-    return x;
+template <int C> __device__ __forceinline__ float keys_of(const seq_view & v, int group) {
+    return (float) (((uint32_t) v.rows * (uint32_t) group + C - 1) / C) * (float) v.len;
+}
+template <int UNITS> __device__ __forceinline__ uint32_t piece_length(const cache_attn_args & a, float keys) {
+    return (uint32_t) min(max(keys * (float) a.n_kv_head * (1.0f / UNITS), (float) PIECE), 0x1p30f);
 }
 
 __device__ __forceinline__ int32_t uniform(int32_t x) { return __builtin_amdgcn_readfirstlane(x); }
-__device__ __forceinline__ unit uniform(const unit & f) {
-    unit u;
-    u.v = {uniform(f.v.row0), uniform(f.v.rows), uniform(f.v.len)};
-    u.seq = uniform(f.seq);
-    u.tile = uniform(f.tile);
-    u.piece = uniform(f.piece);
-    u.pieces = uniform(f.pieces);
-    u.length = uniform(f.length);
-    u.part = (int64_t) ((uint64_t) (uint32_t) uniform((int32_t) (f.part >> 32)) << 32 | (uint32_t) uniform((int32_t) f.part));
-    return u;
+// sums over the lanes up to this one, and over all of them, in the VALU: within rows of 16 lanes, then across rows
+template <typename X>
+__device__ __forceinline__ X wave_scan(X x) {
+    static_assert(sizeof(X) == 4, "one register");
+#define DPP(ctrl, rows) __builtin_bit_cast(X, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), ctrl, rows, 0xf, true))
+    x += DPP(0x111, 0xf);      // row_shr 1, 2, 4, 8
+    x += DPP(0x112, 0xf);
+    x += DPP(0x114, 0xf);
+    x += DPP(0x118, 0xf);
+    x += DPP(0x142, 0xa);      // row_bcast 15, 31
+    x += DPP(0x143, 0xc);
+#undef DPP
+    return x;
 }
+template <typename X>
+__device__ __forceinline__ X wave_add(X x) { return __builtin_bit_cast(X, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wave_scan(x)), 63)); }
 
 // Unit x of the call (x-th column tile if TILES), for column tiles of C. Every thread gets it, in scalar registers; false past the last.
+// Up to 64 sequences each wave finds it by itself, a sequence a lane; more are dealt to the workgroup's threads.
 template <int C, int UNITS, bool TILES>
 __device__ __forceinline__ bool find_unit(const cache_attn_args & a, uint32_t x, unit & u) {
-    typedef unsigned long long u64;
-    __shared__ u64 sums[3][NT / 64];
-    __shared__ unit found;
     const int tid = (int) threadIdx.x, lane = tid & 63, wv = tid >> 6, group = a.n_head / a.n_kv_head;
-    const int per = (a.n_seq + NT - 1) / NT, i0 = min(tid * per, a.n_seq), i1 = min(i0 + per, a.n_seq);
-    seq_view first = {};
-    u64 keys = 0;
-    for (int i = i0; i < i1; i++) {
-        const seq_view v = view_of(a, i);
-        if (i == i0) first = v;
-        keys += (u64) (((int64_t) v.rows * group + C - 1) / C) * (uint32_t) v.len;
-    }
-    if (a.n_seq > 1) {
-        keys = wave_sum(keys);
-        if (lane == 0) sums[0][wv] = keys;
-        if (tid == 0) found.seq = -1;
-        __syncthreads();
-        keys = sums[0][0] + sums[0][1] + sums[0][2] + sums[0][3];
-    } else {      // one sequence: every thread has it
-        first = view_of(a, 0);
-        keys = (u64) (((int64_t) first.rows * group + C - 1) / C) * (uint32_t) first.len;
-    }
-    keys *= (uint32_t) a.n_kv_head;
-    auto set = [&](unit & f, const seq_view & v, int i, const seq_cut<C, UNITS> & cut, u64 at, u64 part) {
+    auto set = [&](unit & f, const seq_view & v, int i, uint32_t tiles, uint32_t pieces, uint32_t at, uint32_t part) {
         f.v = v;
         f.seq = i;
-        f.tile = (int) (cut.tiles - 1 - (TILES ? at : at / cut.pieces));      // a prompt's last rows read the most keys: they go first
-        f.piece = TILES ? 0 : (int) (at % cut.pieces);
-        f.pieces = (int) cut.pieces;
-        f.length = (int32_t) (((uint32_t) v.len + cut.pieces * PIECE - 1) / (cut.pieces * PIECE) * PIECE);
-        f.part = (int64_t) (part + (u64) f.tile * cut.pieces);
+        f.tile = (int) (tiles - 1 - (TILES ? at : at / pieces));      // a prompt's last rows read the most keys: they go first
+        f.piece = TILES ? 0 : (int) (at % pieces);
+        f.pieces = (int) pieces;
+        f.length = (int32_t) (((uint32_t) v.len + pieces * PIECE - 1) / (pieces * PIECE) * PIECE);
+        f.part = (int64_t) part + (int64_t) f.tile * (int64_t) pieces;
     };
-    if (a.n_seq == 1) {
-        const seq_cut<C, UNITS> cut(first, group, keys);
-        if (x >= (TILES ? cut.tiles : cut.tiles * cut.pieces)) return false;
-        set(u, first, 0, cut, x, 0);
-        u = uniform(u);
+    if (a.n_seq <= 64) {
+        seq_view v = {};
+        if (lane < a.n_seq) v = view_of(a, lane);
+        const uint32_t length = piece_length<UNITS>(a, wave_add(keys_of<C>(v, group)));
+        const seq_cut<C> cut(v, group, length);
+        const uint32_t n = TILES ? cut.tiles : cut.tiles * cut.pieces, parts = cut.pieces > 1 ? cut.tiles * cut.pieces : 0u;
+        const uint32_t upto = wave_scan(n), parts_upto = wave_scan(parts);
+        const uint64_t mine = __ballot(x >= upto - n && x < upto);
+        if (!mine) return false;
+        const int i = __builtin_ctzll(mine);
+        auto of = [&](uint32_t y) { return (uint32_t) __builtin_amdgcn_readlane((int) y, i); };
+        set(u, {(int32_t) of((uint32_t) v.row0), (int32_t) of((uint32_t) v.rows), (int32_t) of((uint32_t) v.len)}, i, of(cut.tiles), of(cut.pieces),
+            x - of(upto - n), of(parts_upto - parts));
         return true;
     }
-    u64 mine = 0, parts = 0;
+    __shared__ float keys4[NT / 64];
+    __shared__ uint32_t sums[2][NT / 64];
+    __shared__ struct { seq_view v; int seq; uint32_t tiles, pieces, at, part; } found;
+    const int per = (a.n_seq + NT - 1) / NT, i0 = min(tid * per, a.n_seq), i1 = min(i0 + per, a.n_seq);
+    float keys = 0.0f;
+    for (int i = i0; i < i1; i++) keys += keys_of<C>(view_of(a, i), group);
+    keys = wave_add(keys);
+    if (lane == 0) keys4[wv] = keys;
+    if (tid == 0) found.seq = -1;
+    __syncthreads();
+    const uint32_t length = piece_length<UNITS>(a, (keys4[0] + keys4[1]) + (keys4[2] + keys4[3]));
+    uint32_t mine = 0, parts = 0;
     for (int i = i0; i < i1; i++) {
-        const seq_cut<C, UNITS> cut(i == i0 ? first : view_of(a, i), group, keys);
+        const seq_cut<C> cut(view_of(a, i), group, length);
         mine += TILES ? cut.tiles : cut.tiles * cut.pieces;
         parts += cut.pieces > 1 ? cut.tiles * cut.pieces : 0;
     }
-    u64 before = mine, parts_before = parts;
-    for (int o = 1; o < 64; o <<= 1) {
-        const u64 y = __shfl_up(before, o, 64), z = __shfl_up(parts_before, o, 64);
-        if (lane >= o) { before += y; parts_before += z; }
-    }
-    if (lane == 63) { sums[1][wv] = before; sums[2][wv] = parts_before; }
+    uint32_t before = wave_scan(mine), parts_before = wave_scan(parts);
+    if (lane == 63) { sums[0][wv] = before; sums[1][wv] = parts_before; }
     __syncthreads();
-    for (int w = 0; w < wv; w++) { before += sums[1][w]; parts_before += sums[2][w]; }
+    for (int w = 0; w < wv; w++) { before += sums[0][w]; parts_before += sums[1][w]; }
     before -= mine;
     parts_before -= parts;
     if (x >= before && x < before + mine) {
-        u64 at = x - before;
+        uint32_t at = x - before;
         for (int i = i0; i < i1; i++) {
-            const seq_view v = i == i0 ? first : view_of(a, i);
-            const seq_cut<C, UNITS> cut(v, group, keys);
-            const u64 n = TILES ? cut.tiles : cut.tiles * cut.pieces;
+            const seq_view v = view_of(a, i);
+            const seq_cut<C> cut(v, group, length);
+            const uint32_t n = TILES ? cut.tiles : cut.tiles * cut.pieces;
             if (at < n) {
-                set(found, v, i, cut, at, parts_before);
+                found = {v, i, cut.tiles, cut.pieces, at, parts_before};
                 break;
             }
             at -= n;
@@ -225,8 +223,10 @@ __device__ __forceinline__ bool find_unit(const cache_attn_args & a, uint32_t x,
         }
     }
     __syncthreads();
-    u = uniform(found);
-    return u.seq >= 0;
+    if (found.seq < 0) return false;
+    set(u, {uniform(found.v.row0), uniform(found.v.rows), uniform(found.v.len)}, uniform(found.seq), (uint32_t) uniform((int) found.tiles),
+        (uint32_t) uniform((int) found.pieces), (uint32_t) uniform((int) found.at), (uint32_t) uniform((int) found.part));
+    return true;
 }
 
 // the parts of `work`: sums [part][kv head][C][hd], then (maximum, sum) [part][kv head][C][2]
@@ -252,7 +252,7 @@ template <typename T, int HD, int TERMS>
 __device__ __forceinline__ void load_query(const cache_attn_args & a, const seq_view & sv, int kvh, int group, int32_t col, int g, half8_t (*q)[TERMS], float & c) {
     constexpr int NB = HD / 32;
     typedef T vec __attribute__((ext_vector_type(8)));
-    const T * p = (const T *) a.q + (sv.row0 + (int64_t) (col / group)) * a.ldq + ((int64_t) kvh * group + col % group) * HD + g * 8;
+    const T * p = (const T *) a.q + (sv.row0 + (int64_t) ((uint32_t) col / (uint32_t) group)) * a.ldq + ((int64_t) kvh * group + (uint32_t) col % (uint32_t) group) * HD + g * 8;
     float8_t x[NB];
     float top = 0.0f;
 #pragma unroll
@@ -359,9 +359,9 @@ __global__ __launch_bounds__(NT, CT == 1 ? 3 : 2) void k_cache_attention(cache_a
     const int tid = (int) threadIdx.x, lane = tid & 63, l15 = lane & 15, g = lane >> 4, wv = uniform(tid >> 6);
     const int seq = u.seq, group = a.n_head / a.n_kv_head;
     const seq_view sv = u.v;
-    const int32_t n_cols = (int32_t) min<int64_t>((int64_t) sv.rows * group, 0x7fffffff);
+    const int32_t n_cols = sv.rows * group;      // (below 2^27)
     const int32_t col0 = u.tile * C;
-    auto visible = [&](int32_t col) { return cache_visible((int64_t) sv.len - sv.rows + col / group, sv.len, a.block); };
+    auto visible = [&](int32_t col) { return cache_visible(sv.len - sv.rows + (int32_t) ((uint32_t) col / (uint32_t) group), sv.len, a.block); };
 
     // the keys that the first and the last of the wave's columns read
     const int32_t lim_lo = visible(col0), lim_hi = visible(min(col0 + C, n_cols) - 1);
@@ -402,9 +402,10 @@ __global__ __launch_bounds__(NT, CT == 1 ? 3 : 2) void k_cache_attention(cache_a
     const int e = (l15 & 3) * 2 + ((l15 & 7) >> 2);
     const int tr_at = (((l15 >> 3) * 2 + (e >> 2)) * 16 + g * 4 + (e & 3)) * 8;
     if (k0 < kend) {
+        const int pages_after = load_pages(k0 + STEP);
         load_v(k0, pages);
         load_k(k0, pages);
-        pages = load_pages(k0 + STEP);
+        pages = pages_after;
     }
     int32_t lim[CT];
     float c[CT];
@@ -447,6 +448,8 @@ __global__ __launch_bounds__(NT, CT == 1 ? 3 : 2) void k_cache_attention(cache_a
                 *(uint32_t *) (mine + (w >> 1) * 528 + (t * 16 + (lane >> 2)) * 8 + (w & 1) * 4) = vn[t][b];
             }
         }
+        // in the order of their use: a wait for one load is a wait for all before it
+        const int pages_after = load_pages(k0 + 2 * STEP);
         load_v(k0 + STEP, pages);
         const float dexp = (float) ((int) (wave_umax(dmax) >> 10) - 14);      // every |dv| of the tile is below 2^dexp
         wave_order();
@@ -468,10 +471,10 @@ __global__ __launch_bounds__(NT, CT == 1 ? 3 : 2) void k_cache_attention(cache_a
                     for (int r = 0; r < 4; r++) s[ct][t][r] = __builtin_fmaf((float) d[r], x[r], b == 0 ? 0.0f : s[ct][t][r]);
                 }
             }
-            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_sched_barrier(0x100);
         }
         load_k(k0 + STEP, pages);
-        pages = load_pages(k0 + 2 * STEP);
+        pages = pages_after;
 #pragma unroll
         for (int ct = 0; ct < CT; ct++) softmax_step<MASKED, ND>(s[ct], k0 + g * 4, lim[ct], bad, c[ct], dexp, mu[ct], l[ct], o[ct]);
         // O^T += V^T P'^T, block by block of the head
@@ -496,7 +499,7 @@ __global__ __launch_bounds__(NT, CT == 1 ? 3 : 2) void k_cache_attention(cache_a
                     }
                 }
             }
-            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_sched_barrier(0x100);
         }
     };
     for (; k0 + TILE <= min(lim_lo, kend) && bad_n == 0; k0 += STEP) tile(std::false_type{});
@@ -505,7 +508,7 @@ __global__ __launch_bounds__(NT, CT == 1 ? 3 : 2) void k_cache_attention(cache_a
     for (int ct = 0; ct < CT; ct++) l[ct] = col_sum(l[ct]);
 
     const parts_view<HD, C> part(a, u.part + u.piece, kvh);
-    auto out_at = [&](int32_t col) { return (T *) a.out + (sv.row0 + (int64_t) (col / group)) * a.ldo + ((int64_t) kvh * group + col % group) * HD; };
+    auto out_at = [&](int32_t col) { return (T *) a.out + (sv.row0 + (int64_t) ((uint32_t) col / (uint32_t) group)) * a.ldo + ((int64_t) kvh * group + (uint32_t) col % (uint32_t) group) * HD; };
     // the four waves' sums at the largest of their maxima
     float * const stat = (float *) (lds + 4 * C * (HD + 4) * 4), * const sum = (float *) lds;
     __syncthreads();      // the loop's LDS is read out
@@ -556,9 +559,9 @@ __global__ __launch_bounds__(NT, 2) void k_cache_prompt(cache_attn_args a) {
     const int tid = (int) threadIdx.x, lane = tid & 63, l15 = lane & 15, g = lane >> 4, wv = uniform(tid >> 6);
     const int seq = u.seq, group = a.n_head / a.n_kv_head;
     const seq_view sv = u.v;
-    const int32_t n_cols = (int32_t) min<int64_t>((int64_t) sv.rows * group, 0x7fffffff);
+    const int32_t n_cols = sv.rows * group;      // (below 2^27)
     const int32_t first = u.tile * C, col0 = first + wv * WC;
-    auto visible = [&](int32_t col) { return cache_visible((int64_t) sv.len - sv.rows + col / group, sv.len, a.block); };
+    auto visible = [&](int32_t col) { return cache_visible(sv.len - sv.rows + (int32_t) ((uint32_t) col / (uint32_t) group), sv.len, a.block); };
     const bool has = col0 < n_cols;
     const int32_t lim_lo = has ? visible(col0) : 0, lim_hi = has ? visible(min(col0 + WC, n_cols) - 1) : 0;
     const int32_t kend = (int32_t) min<int64_t>((int64_t) (u.piece + 1) * u.length, visible(min(first + C, n_cols) - 1));      // the workgroup's
@@ -673,7 +676,7 @@ __global__ __launch_bounds__(NT, 2) void k_cache_prompt(cache_attn_args a) {
                     }
                 }
             }
-            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_sched_barrier(0x100);
         }
 #pragma unroll
         for (int ct = 0; ct < CT; ct++) softmax_step<MASKED, ND>(s[ct], k0 + g * 4, lim[ct], hidden, c[ct], dexp, mu[ct], l[ct], o[ct]);
@@ -693,7 +696,7 @@ __global__ __launch_bounds__(NT, 2) void k_cache_prompt(cache_attn_args a) {
 #pragma unroll
                     for (int ct = 0; ct < CT; ct++) o[ct][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[ct][h], o[ct][d], 0, 0, 0);
                 }
-                if (d & 1) __builtin_amdgcn_sched_barrier(0);
+                if (d & 1) __builtin_amdgcn_sched_barrier(0x100);
             }
         } else {
 #pragma unroll
@@ -715,7 +718,7 @@ __global__ __launch_bounds__(NT, 2) void k_cache_prompt(cache_attn_args a) {
                             for (int k = 0; k < TERMS; k++) o[ct][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[ct][h][k], o[ct][d], 0, 0, 0);
                     }
                 }
-                __builtin_amdgcn_sched_barrier(0);
+                __builtin_amdgcn_sched_barrier(0x100);
             }
         }
     };
@@ -747,28 +750,59 @@ __global__ __launch_bounds__(NT, 2) void k_cache_prompt(cache_attn_args a) {
             for (int d = 0; d < ND; d++) *(float4_t *) (part.o + (int64_t) at * HD + d * 16 + g * 4) = o[ct][d];
         } else {
             const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-            T * p = (T *) a.out + (sv.row0 + (int64_t) (col / group)) * a.ldo + ((int64_t) kvh * group + col % group) * HD;
+            T * p = (T *) a.out + (sv.row0 + (int64_t) ((uint32_t) col / (uint32_t) group)) * a.ldo + ((int64_t) kvh * group + (uint32_t) col % (uint32_t) group) * HD;
             for (int d = 0; d < ND; d++) store4(p + d * 16 + g * 4, o[ct][d] * inv);
         }
     }
 }
 
-// The pieces of a column tile added in a fixed order: a column at a time, HD / 4 threads across its values, the others across its
-// pieces. `split` workgroups share a tile's columns.
+// The pieces of a column tile added in a fixed order, HD / 4 threads across a column's values: few pieces by those threads alone, a
+// column each; many by all threads, a column at a time. `split` workgroups share a tile's columns.
 template <typename T, int HD, int C, int UNITS>
 __global__ __launch_bounds__(NT) void k_cache_join(cache_attn_args a, int split) {
-    constexpr int W = HD / 4, PG = NT / W;      // threads across a column, pieces at once
+    constexpr int W = HD / 4, PG = NT / W;      // threads across a column, columns or pieces at once
     __shared__ float top4[NT / 64], sum[PG];
     __shared__ __attribute__((aligned(16))) float acc[PG][HD];
     unit u;
     const unsigned id = blockIdx.x / (unsigned) a.n_kv_head;
     const int kvh = (int) (blockIdx.x % (unsigned) a.n_kv_head);
     if (!find_unit<C, UNITS, true>(a, id / (unsigned) split, u) || u.pieces < 2 || u.part + u.pieces > a.parts) return;
-    const int tid = (int) threadIdx.x, pg = tid / W, n = tid % W * 4, group = a.n_head / a.n_kv_head;
-    const int64_t n_cols = (int64_t) u.v.rows * group, col0 = (int64_t) u.tile * C;
-    for (int at = (int) (id % (unsigned) split); at < C && col0 + at < n_cols; at += split) {
+    const int tid = (int) threadIdx.x, pg = tid / W, n = tid % W * 4, group = a.n_head / a.n_kv_head, mine = (int) (id % (unsigned) split);
+    const int32_t n_cols = u.v.rows * group, col0 = u.tile * C;
+    const parts_view<HD, C> p0(a, u.part, kvh), p1(a, u.part + 1, kvh);
+    const int64_t next = p1.o - p0.o;      // from a piece to the next
+    auto write = [&](int32_t col, float4_t x, float all) {
+        T * out = (T *) a.out + (u.v.row0 + (int64_t) ((uint32_t) col / (uint32_t) group)) * a.ldo + ((int64_t) kvh * group + (uint32_t) col % (uint32_t) group) * HD;
+        store4(out + n, x * (all == 0.0f ? 0.0f : 1.0f / all));
+    };
+    if (u.pieces <= 8) {
+        for (int at = mine + split * pg; at < C && col0 + at < n_cols && pg < PG; at += split * PG) {
+            float mu[8], l[8], top = -INFINITY, all = 0.0f;
+            float4_t y[8], x = {0, 0, 0, 0};
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const int64_t o = min(k, u.pieces - 1) * next;
+                mu[k] = p0.s[o + 2 * at];
+                l[k] = p0.s[o + 2 * at + 1];
+                y[k] = *(const float4_t *) (p0.o + o + (int64_t) at * HD + n);
+            }
+#pragma unroll
+            for (int k = 0; k < 8; k++) top = fmaxf(top, mu[k]);
+            const float m = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                if (k >= u.pieces) break;
+                const float f = __builtin_amdgcn_exp2f(mu[k] - m);
+                all += l[k] * f;
+                x += y[k] * f;
+            }
+            write(col0 + at, x, all);
+        }
+        return;
+    }
+    for (int at = mine; at < C && col0 + at < n_cols; at += split) {
         float top = -INFINITY;
-        for (int k = tid; k < u.pieces; k += NT) top = fmaxf(top, parts_view<HD, C>(a, u.part + k, kvh).s[2 * at]);
+        for (int k = tid; k < u.pieces; k += NT) top = fmaxf(top, p0.s[k * next + 2 * at]);
         for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
         if (tid % 64 == 0) top4[tid / 64] = top;
         __syncthreads();
@@ -776,15 +810,13 @@ __global__ __launch_bounds__(NT) void k_cache_join(cache_attn_args a, int split)
         const float m = top == -INFINITY ? 0.0f : top;
         float all = 0.0f;
         float4_t x = {0, 0, 0, 0};
-        if (pg < PG)
+        if (pg < PG) {
 #pragma unroll 4
             for (int k = pg; k < u.pieces; k += PG) {
-                const parts_view<HD, C> p(a, u.part + k, kvh);
-                const float f = __builtin_amdgcn_exp2f(p.s[2 * at] - m);
-                all += p.s[2 * at + 1] * f;
-                x += *(const float4_t *) (p.o + (int64_t) at * HD + n) * f;
+                const float f = __builtin_amdgcn_exp2f(p0.s[k * next + 2 * at] - m);
+                all += p0.s[k * next + 2 * at + 1] * f;
+                x += *(const float4_t *) (p0.o + k * next + (int64_t) at * HD + n) * f;
             }
-        if (pg < PG) {
             *(float4_t *) &acc[pg][n] = x;
             if (n == 0) sum[pg] = all;
         }
@@ -794,9 +826,7 @@ __global__ __launch_bounds__(NT) void k_cache_join(cache_attn_args a, int split)
                 all += sum[k];
                 x += *(const float4_t *) &acc[k][n];
             }
-            const int64_t col = col0 + at;
-            T * out = (T *) a.out + (u.v.row0 + col / group) * a.ldo + ((int64_t) kvh * group + col % group) * HD;
-            store4(out + n, x * (all == 0.0f ? 0.0f : 1.0f / all));
+            write(col0 + at, x, all);
         }
         __syncthreads();
     }
@@ -830,8 +860,8 @@ hipError_t attend(const cache_shape & c, const cache_attn_args & a, hipStream_t 
     if (blocks >= 1 << 24) return hipErrorInvalidConfiguration;      // threads of a launch are below 2^32
     const hipError_t e = hipLaunchKernel(kernel, dim3((unsigned) blocks), dim3(NT), p, 0, s);
     if (e != hipSuccess || !parts) return e;
-    // few tiles: up to a workgroup for each column; many are hardly split
-    int split = (int) std::min<int64_t>(C, std::max<int64_t>(1, 2048 / (tiles * c.n_kv_head)));
+    // few tiles are split into many pieces: up to a workgroup for each column; many hardly
+    int split = (int) std::min<int64_t>(C, std::max<int64_t>(1, 512 / (tiles * c.n_kv_head)));
     void * pj[] = {&args, &split};
     return hipLaunchKernel((const void *) k_cache_join<T, HD, C, units_of(HD, CT)>, dim3((unsigned) (tiles * c.n_kv_head * split)), dim3(NT), pj, 0, s);
 }

@@ -66,10 +66,12 @@ CACHE_HD int cache_find(const uint32_t * ends, int n, uint32_t x) {
     return lo;
 }
 // keys that the row at position pos of a sequence of len tokens reads: block 0 all, else those of its own and earlier
-// blocks of `block` positions (1: causal)
-CACHE_HD int32_t cache_visible(int64_t pos, int32_t len, int64_t block) {
+// blocks of `block` positions (1: causal). block is at most 2^30 (cache_block_of), as is len.
+CACHE_HD int32_t cache_visible(int32_t pos, int32_t len, int32_t block) {
     if (block == 0) return len;
     if (pos < 0) return 0;
-    const int64_t end = (pos / block + 1) * block;
-    return (int32_t) (end < len ? end : len);
+    const uint32_t end = block == 1 ? (uint32_t) pos + 1 : ((uint32_t) pos / (uint32_t) block + 1) * (uint32_t) block;
+    return end < (uint32_t) len ? (int32_t) end : len;
 }
+// a caller's block in 32 bits: 2^30 positions are all that a sequence has
+CACHE_HD int32_t cache_block_of(int64_t block) { return block < 1 << 30 ? (int32_t) block : 1 << 30; }

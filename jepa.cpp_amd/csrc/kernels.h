@@ -149,9 +149,9 @@ struct cache_attn_args {
     const unsigned char * cache = nullptr;
     const void * q = nullptr;
     void * out = nullptr;
-    int64_t ldq = 0, ldo = 0, n_rows = 0, n_pages = 0, block = 0;
+    int64_t ldq = 0, ldo = 0, n_rows = 0, n_pages = 0;
     const int32_t * row_start = nullptr, * kv_len = nullptr, * table = nullptr;
-    int n_seq = 0, width = 0, n_head = 0, n_kv_head = 0, page_size = 0;
+    int n_seq = 0, width = 0, n_head = 0, n_kv_head = 0, page_size = 0, block = 0;
     float scale = 0;
     float * work = nullptr;
     int64_t parts = 0;      // set by the launcher: partial results that `work` holds

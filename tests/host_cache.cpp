@@ -66,7 +66,9 @@ static int views() {
     CHECK(cache_find(e, 4, 0) == 1 && cache_find(e, 4, 2) == 1 && cache_find(e, 4, 3) == 3 && cache_find(e, 4, 6) == 3 && cache_find(e, 4, 7) == 4);
     CHECK(cache_find(e, 0, 0) == 0);
     CHECK(cache_visible(0, 10, 0) == 10 && cache_visible(3, 10, 1) == 4 && cache_visible(-1, 10, 1) == 0 && cache_visible(-1, 10, 0) == 10);
-    CHECK(cache_visible(5, 10, 4) == 8 && cache_visible(9, 10, 4) == 10 && cache_visible(0, 10, (int64_t) 1 << 40) == 10);
+    CHECK(cache_visible(5, 10, 4) == 8 && cache_visible(9, 10, 4) == 10 && cache_visible(0, 10, cache_block_of((int64_t) 1 << 40)) == 10);
+    CHECK(cache_visible(0x3fffffff, 0x40000000, 0x40000000) == 0x40000000 && cache_visible(0x3ffffffe, 0x40000000, 1) == 0x3fffffff && cache_visible(0x3fffffff, 0x40000000, 3) == 0x40000000);
+    CHECK(cache_block_of(0) == 0 && cache_block_of(1) == 1 && cache_block_of(1 << 30) == 1 << 30);
     return 0;
 }
 
