@@ -49,9 +49,10 @@ constexpr int NT = 256;              // threads of a workgroup
 constexpr int TILE = 64;             // keys of a wave's step
 constexpr int PIECE = 4 * TILE;      // pieces are multiples of this: one step of each of four waves
 
-// Units that a call is split into where its columns alone are fewer: the workgroups that the chip holds at once (256 CUs; 512 registers
-// a SIMD lane over the kernel's count), so that pieces of equal length end together.
-constexpr int units_of(int hd, int ct) { return 256 * (ct > 1 ? 2 : hd > 64 ? 3 : 4); }
+// Workgroups that the chip holds at once (256 CUs; 512 registers of a SIMD lane over the kernel's): calls whose column tiles alone are
+// fewer are split into about as many units, or up to twice as many where that ends more evenly.
+constexpr int slots_of(int hd, int c) { return 256 * (c == 128 ? 2 : c == 64 || hd > 64 ? 3 : 4); }
+constexpr float UNIT_KEYS = 768.0f;      // what a unit costs beside its keys, in keys
 
 // the 8 codes of a word less 8, in the order of its elements (nibbles 0 4 1 5 2 6 3 7), exact in f16: a nibble or'ed into the low
 // mantissa bits of 1024 is 1024 + c, into the next four 1024 + 16 c. `k1024` is the pair of f16 1024 in a vector register (an
@@ -121,22 +122,15 @@ __device__ __forceinline__ seq_view view_of(const cache_attn_args & a, int i) {
 // A piece of a column tile: keys [piece, piece + 1) * length of sequence v; part: the first piece's place in `work`
 struct unit { seq_view v; int seq, tile, piece, pieces; int32_t length; int64_t part; };
 
-// Column tiles and pieces of a sequence where the call's keys (over all column tiles and K/V heads) are `keys`: the number of pieces
-// that comes nearest to keys / UNITS each. A float sum will do: every workgroup adds the same numbers in the same order.
-template <int C>
-struct seq_cut {
-    uint32_t tiles, pieces;
-    __device__ seq_cut(const seq_view & v, int group, uint32_t length) {
-        tiles = ((uint32_t) v.rows * (uint32_t) group + C - 1) / C;      // (rows * heads are below 2^27)
-        pieces = max(((uint32_t) v.len + length / 2) / length, 1u);
-    }
-};
-template <int C> __device__ __forceinline__ float keys_of(const seq_view & v, int group) {
-    return (float) (((uint32_t) v.rows * (uint32_t) group + C - 1) / C) * (float) v.len;
+// Column tiles of a sequence, and its pieces where pieces are to be about 1 / inv keys (the nearest number of equal ones)
+template <int C> __device__ __forceinline__ uint32_t tiles_of(const seq_view & v, int group) {
+    return ((uint32_t) v.rows * (uint32_t) group + C - 1) / C;      // (rows * heads are below 2^27)
 }
-template <int UNITS> __device__ __forceinline__ uint32_t piece_length(const cache_attn_args & a, float keys) {
-    return (uint32_t) min(max(keys * (float) a.n_kv_head * (1.0f / UNITS), (float) PIECE), 0x1p30f);
-}
+__device__ __forceinline__ float pieces_of(const seq_view & v, float inv) { return fmaxf(floorf(__builtin_fmaf((float) v.len, inv, 0.5f)), 1.0f); }
+// the inverse length of `units` equal pieces of `keys` keys (over all sequences, column tiles and K/V heads). Float sums and
+// reciprocals will do: every workgroup makes the same ones of the same numbers.
+__device__ __forceinline__ float piece_inv(float keys, float units) { return __builtin_amdgcn_rcpf(fmaxf(keys * (1.0f / units), (float) PIECE)); }
+constexpr float MOST_UNITS = 1.9f;      // that a call is split into, in slots
 
 __device__ __forceinline__ int32_t uniform(int32_t x) { return __builtin_amdgcn_readfirstlane(x); }
 // sums over the lanes up to this one, and over all of them, in the VALU: within rows of 16 lanes, then across rows
@@ -153,12 +147,24 @@ __device__ __forceinline__ X wave_scan(X x) {
 #undef DPP
     return x;
 }
+__device__ __forceinline__ float wave_max(float x) {      // (of values that are not negative)
+#define DPP(ctrl, rows) __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), ctrl, rows, 0xf, true))
+    x = fmaxf(x, DPP(0x111, 0xf));
+    x = fmaxf(x, DPP(0x112, 0xf));
+    x = fmaxf(x, DPP(0x114, 0xf));
+    x = fmaxf(x, DPP(0x118, 0xf));
+    x = fmaxf(x, DPP(0x142, 0xa));
+    x = fmaxf(x, DPP(0x143, 0xc));
+#undef DPP
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
+}
 template <typename X>
 __device__ __forceinline__ X wave_add(X x) { return __builtin_bit_cast(X, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wave_scan(x)), 63)); }
 
 // Unit x of the call (x-th column tile if TILES), for column tiles of C. Every thread gets it, in scalar registers; false past the last.
-// Up to 64 sequences each wave finds it by itself, a sequence a lane; more are dealt to the workgroup's threads.
-template <int C, int UNITS, bool TILES>
+// Up to 64 sequences each wave finds it by itself, a sequence a lane, and weighs a few piece lengths against each other; more are
+// dealt to the workgroup's threads.
+template <int C, int SLOTS, bool TILES>
 __device__ __forceinline__ bool find_unit(const cache_attn_args & a, uint32_t x, unit & u) {
     const int tid = (int) threadIdx.x, lane = tid & 63, wv = tid >> 6, group = a.n_head / a.n_kv_head;
     auto set = [&](unit & f, const seq_view & v, int i, uint32_t tiles, uint32_t pieces, uint32_t at, uint32_t part) {
@@ -173,15 +179,26 @@ __device__ __forceinline__ bool find_unit(const cache_attn_args & a, uint32_t x,
     if (a.n_seq <= 64) {
         seq_view v = {};
         if (lane < a.n_seq) v = view_of(a, lane);
-        const uint32_t length = piece_length<UNITS>(a, wave_add(keys_of<C>(v, group)));
-        const seq_cut<C> cut(v, group, length);
-        const uint32_t n = TILES ? cut.tiles : cut.tiles * cut.pieces, parts = cut.pieces > 1 ? cut.tiles * cut.pieces : 0u;
+        const uint32_t tiles = tiles_of<C>(v, group);
+        const float heads = (float) a.n_kv_head, keys = wave_add((float) tiles * (float) v.len) * heads;
+        float inv = 0.0f, least = INFINITY;
+#pragma unroll
+        for (int i = 0; i < 3; i++) {
+            // so many units for each slot: the time of all, and of the longest while the last round is not full
+            constexpr float SHARE[3] = {1.0f, 0.93f, MOST_UNITS};
+            const float x1 = piece_inv(keys, SHARE[i] * SLOTS), n = pieces_of(v, x1);
+            const float units = wave_add((float) tiles * n) * heads, rounds = units * (1.0f / SLOTS);
+            const float longest = wave_max(tiles ? (float) v.len * __builtin_amdgcn_rcpf(n) : 0.0f) + UNIT_KEYS;
+            const float time = fmaxf(__builtin_fmaf(units, UNIT_KEYS, keys) * (1.0f / SLOTS) + longest * (ceilf(rounds) - rounds), longest);
+            if (time < least) { least = time; inv = x1; }
+        }
+        const uint32_t pieces = (uint32_t) pieces_of(v, inv), n = TILES ? tiles : tiles * pieces, parts = pieces > 1 ? tiles * pieces : 0u;
         const uint32_t upto = wave_scan(n), parts_upto = wave_scan(parts);
         const uint64_t mine = __ballot(x >= upto - n && x < upto);
         if (!mine) return false;
         const int i = __builtin_ctzll(mine);
         auto of = [&](uint32_t y) { return (uint32_t) __builtin_amdgcn_readlane((int) y, i); };
-        set(u, {(int32_t) of((uint32_t) v.row0), (int32_t) of((uint32_t) v.rows), (int32_t) of((uint32_t) v.len)}, i, of(cut.tiles), of(cut.pieces),
+        set(u, {(int32_t) of((uint32_t) v.row0), (int32_t) of((uint32_t) v.rows), (int32_t) of((uint32_t) v.len)}, i, of(tiles), of(pieces),
             x - of(upto - n), of(parts_upto - parts));
         return true;
     }
@@ -190,17 +207,21 @@ __device__ __forceinline__ bool find_unit(const cache_attn_args & a, uint32_t x,
     __shared__ struct { seq_view v; int seq; uint32_t tiles, pieces, at, part; } found;
     const int per = (a.n_seq + NT - 1) / NT, i0 = min(tid * per, a.n_seq), i1 = min(i0 + per, a.n_seq);
     float keys = 0.0f;
-    for (int i = i0; i < i1; i++) keys += keys_of<C>(view_of(a, i), group);
+    for (int i = i0; i < i1; i++) {
+        const seq_view v = view_of(a, i);
+        keys += (float) tiles_of<C>(v, group) * (float) v.len;
+    }
     keys = wave_add(keys);
     if (lane == 0) keys4[wv] = keys;
     if (tid == 0) found.seq = -1;
     __syncthreads();
-    const uint32_t length = piece_length<UNITS>(a, (keys4[0] + keys4[1]) + (keys4[2] + keys4[3]));
+    const float inv = piece_inv(((keys4[0] + keys4[1]) + (keys4[2] + keys4[3])) * (float) a.n_kv_head, MOST_UNITS * SLOTS);
     uint32_t mine = 0, parts = 0;
     for (int i = i0; i < i1; i++) {
-        const seq_cut<C> cut(view_of(a, i), group, length);
-        mine += TILES ? cut.tiles : cut.tiles * cut.pieces;
-        parts += cut.pieces > 1 ? cut.tiles * cut.pieces : 0;
+        const seq_view v = view_of(a, i);
+        const uint32_t tiles = tiles_of<C>(v, group), pieces = (uint32_t) pieces_of(v, inv);
+        mine += TILES ? tiles : tiles * pieces;
+        parts += pieces > 1 ? tiles * pieces : 0;
     }
     uint32_t before = wave_scan(mine), parts_before = wave_scan(parts);
     if (lane == 63) { sums[0][wv] = before; sums[1][wv] = parts_before; }
@@ -212,14 +233,13 @@ __device__ __forceinline__ bool find_unit(const cache_attn_args & a, uint32_t x,
         uint32_t at = x - before;
         for (int i = i0; i < i1; i++) {
             const seq_view v = view_of(a, i);
-            const seq_cut<C> cut(v, group, length);
-            const uint32_t n = TILES ? cut.tiles : cut.tiles * cut.pieces;
+            const uint32_t tiles = tiles_of<C>(v, group), pieces = (uint32_t) pieces_of(v, inv), n = TILES ? tiles : tiles * pieces;
             if (at < n) {
-                found = {v, i, cut.tiles, cut.pieces, at, parts_before};
+                found = {v, i, tiles, pieces, at, parts_before};
                 break;
             }
             at -= n;
-            parts_before += cut.pieces > 1 ? cut.tiles * cut.pieces : 0;
+            parts_before += pieces > 1 ? tiles * pieces : 0;
         }
     }
     __syncthreads();
@@ -343,18 +363,18 @@ __device__ __forceinline__ half8_t read_v(const unsigned char * at, int h) {
 }
 
 template <int HD> constexpr int wave_lds() { return HD / 16 * 528 + 8 * HD; }      // V codes of a tile, then its scales
-template <int HD, int CT> constexpr int group_lds() {
-    const int loop = 4 * wave_lds<HD>(), join = 4 * 16 * CT * (HD + 4) * 4 + 4 * 16 * CT * 8;
+template <int HD> constexpr int group_lds() {
+    const int loop = 4 * wave_lds<HD>(), join = 4 * 16 * (HD + 4) * 4 + 4 * 16 * 8;
     return loop > join ? loop : join;
 }
 
-template <typename T, int HD, int CT>
-__global__ __launch_bounds__(NT, CT == 1 ? 3 : 2) void k_cache_attention(cache_attn_args a) {
-    constexpr int NB = HD / 32, ND = HD / 16, UNITS = units_of(HD, CT), TERMS = sizeof(T) == 4 ? 2 : 1, C = 16 * CT;
-    __shared__ __attribute__((aligned(16))) unsigned char lds[group_lds<HD, CT>()];
+template <typename T, int HD>
+__global__ __launch_bounds__(NT, 3) void k_cache_attention(cache_attn_args a) {
+    constexpr int NB = HD / 32, ND = HD / 16, TERMS = sizeof(T) == 4 ? 2 : 1, C = 16;
+    __shared__ __attribute__((aligned(16))) unsigned char lds[group_lds<HD>()];
     unit u;
     const int kvh = (int) (blockIdx.x % (unsigned) a.n_kv_head);
-    if (!find_unit<C, UNITS, false>(a, blockIdx.x / (unsigned) a.n_kv_head, u)) return;
+    if (!find_unit<C, slots_of(HD, C), false>(a, blockIdx.x / (unsigned) a.n_kv_head, u)) return;
     if (u.pieces > 1 && u.part + u.piece >= a.parts) return;      // (row_start that overlaps itself: more pieces than rows can have)
     const int tid = (int) threadIdx.x, lane = tid & 63, l15 = lane & 15, g = lane >> 4, wv = uniform(tid >> 6);
     const int seq = u.seq, group = a.n_head / a.n_kv_head;
@@ -382,19 +402,19 @@ __global__ __launch_bounds__(NT, CT == 1 ? 3 : 2) void k_cache_attention(cache_a
         if (page < 0 || page >= a.n_pages) { page = 0; bad |= 1u << t; }
         return make_brsrc(a.cache + ((page * a.n_kv_head + kvh) * strips_of_page + (strip & (strips_of_page - 1))) * (18 * HD), key < kend ? 18 * HD : 0);
     };
+    brsrc strips[4];
     auto load_v = [&](int32_t key, int pages) {
         bad_n = 0;
 #pragma unroll
         for (int t = 0; t < 4; t++) {
-            const brsrc s = strip_of(key, pages, t, bad_n);
-            load_words<NB>(vn[t], s, lane * (4 * NB), 8 * HD);
-            load_words<1>(&sn[t], s, 16 * HD + lane * 4, 0);      // (0 past the strip's scales, from lane HD / 2 on)
+            strips[t] = strip_of(key, pages, t, bad_n);
+            load_words<NB>(vn[t], strips[t], lane * (4 * NB), 8 * HD);
+            load_words<1>(&sn[t], strips[t], 16 * HD + lane * 4, 0);      // (0 past the strip's scales, from lane HD / 2 on)
         }
     };
-    auto load_k = [&](int32_t key, int pages) {
-        uint32_t bad = 0;
+    auto load_k = [&] {      // of the tile whose load_v came last
 #pragma unroll
-        for (int t = 0; t < 4; t++) load_words<NB>(kn[t], strip_of(key, pages, t, bad), lane * (4 * NB), 0);
+        for (int t = 0; t < 4; t++) load_words<NB>(kn[t], strips[t], lane * (4 * NB), 0);
     };
     unsigned char * const mine = lds + wv * wave_lds<HD>();
     unsigned char * const scales = mine + ND * 528;
@@ -404,24 +424,16 @@ __global__ __launch_bounds__(NT, CT == 1 ? 3 : 2) void k_cache_attention(cache_a
     if (k0 < kend) {
         const int pages_after = load_pages(k0 + STEP);
         load_v(k0, pages);
-        load_k(k0, pages);
+        load_k();
         pages = pages_after;
     }
-    int32_t lim[CT];
-    float c[CT];
-    half8_t q[CT][NB][TERMS];
-#pragma unroll
-    for (int ct = 0; ct < CT; ct++) load_query<T, HD, TERMS>(a, sv, kvh, group, min(col0 + ct * 16 + l15, n_cols - 1), g, q[ct], c[ct]);
-#pragma unroll
-    for (int ct = 0; ct < CT; ct++) lim[ct] = visible(min(col0 + ct * 16 + l15, n_cols - 1));
-    float4_t o[CT][ND];
-    float mu[CT], l[CT];      // mu: -inf before the first key
-#pragma unroll
-    for (int ct = 0; ct < CT; ct++) {
-        mu[ct] = -INFINITY;
-        l[ct] = 0.0f;
-        for (int d = 0; d < ND; d++) o[ct][d] = float4_t{0, 0, 0, 0};
-    }
+    const int32_t col = min(col0 + l15, n_cols - 1), lim = visible(col);
+    float c;
+    half8_t q[NB][TERMS];
+    load_query<T, HD, TERMS>(a, sv, kvh, group, col, g, q, c);
+    float4_t o[ND];
+    float mu = -INFINITY, l = 0.0f;      // mu: -inf before the first key
+    for (int d = 0; d < ND; d++) o[d] = float4_t{0, 0, 0, 0};
 
     uint32_t k1024 = 0x64006400u;
     asm volatile("" : "+v"(k1024));
@@ -455,7 +467,7 @@ __global__ __launch_bounds__(NT, CT == 1 ? 3 : 2) void k_cache_attention(cache_a
         wave_order();
 
         // scores
-        float4_t s[CT][4];
+        float4_t s[4];
 #pragma unroll
         for (int t = 0; t < 4; t++) {
             const half4_t * dk = (const half4_t *) (scales + t * 2 * HD + g * (8 * NB));
@@ -463,28 +475,22 @@ __global__ __launch_bounds__(NT, CT == 1 ? 3 : 2) void k_cache_attention(cache_a
             for (int b = 0; b < NB; b++) {
                 const half8_t kc = codes8(kn[t][b], k1024);
                 const half4_t d = dk[b];
+                float4_t x = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc, q[b][0], float4_t{0, 0, 0, 0}, 0, 0, 0);
+                if constexpr (TERMS == 2) x = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc, q[b][1], x, 0, 0, 0);
 #pragma unroll
-                for (int ct = 0; ct < CT; ct++) {
-                    float4_t x = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc, q[ct][b][0], float4_t{0, 0, 0, 0}, 0, 0, 0);
-                    if constexpr (TERMS == 2) x = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc, q[ct][b][1], x, 0, 0, 0);
-#pragma unroll
-                    for (int r = 0; r < 4; r++) s[ct][t][r] = __builtin_fmaf((float) d[r], x[r], b == 0 ? 0.0f : s[ct][t][r]);
-                }
+                for (int r = 0; r < 4; r++) s[t][r] = __builtin_fmaf((float) d[r], x[r], b == 0 ? 0.0f : s[t][r]);
             }
             __builtin_amdgcn_sched_barrier(0x100);
         }
-        load_k(k0 + STEP, pages);
+        load_k();
         pages = pages_after;
-#pragma unroll
-        for (int ct = 0; ct < CT; ct++) softmax_step<MASKED, ND>(s[ct], k0 + g * 4, lim[ct], bad, c[ct], dexp, mu[ct], l[ct], o[ct]);
+        softmax_step<MASKED, ND>(s, k0 + g * 4, lim, bad, c, dexp, mu, l, o);
         // O^T += V^T P'^T, block by block of the head
 #pragma unroll
         for (int b = 0; b < NB; b++) {
-            half8_t p[CT][2][TERMS];
+            half8_t p[2][TERMS];
 #pragma unroll
-            for (int h = 0; h < 2; h++)
-#pragma unroll
-                for (int ct = 0; ct < CT; ct++) weights_times_scales<TERMS>(s[ct], h, scales + HD + g * (8 * NB) + b * 8, 2 * HD, p[ct][h]);
+            for (int h = 0; h < 2; h++) weights_times_scales<TERMS>(s, h, scales + HD + g * (8 * NB) + b * 8, 2 * HD, p[h]);
 #pragma unroll
             for (int dd = 0; dd < 2; dd++) {
                 const int d = 2 * b + dd;
@@ -493,10 +499,7 @@ __global__ __launch_bounds__(NT, CT == 1 ? 3 : 2) void k_cache_attention(cache_a
                 for (int h = 0; h < 2; h++) {
                     const half8_t vc = codes8((uint32_t) w[h], k1024);
 #pragma unroll
-                    for (int ct = 0; ct < CT; ct++) {
-                        o[ct][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vc, p[ct][h][0], o[ct][d], 0, 0, 0);
-                        if constexpr (TERMS == 2) o[ct][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vc, p[ct][h][1], o[ct][d], 0, 0, 0);
-                    }
+                    for (int k = 0; k < TERMS; k++) o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vc, p[h][k], o[d], 0, 0, 0);
                 }
             }
             __builtin_amdgcn_sched_barrier(0x100);
@@ -504,24 +507,23 @@ __global__ __launch_bounds__(NT, CT == 1 ? 3 : 2) void k_cache_attention(cache_a
     };
     for (; k0 + TILE <= min(lim_lo, kend) && bad_n == 0; k0 += STEP) tile(std::false_type{});
     for (; k0 < kend; k0 += STEP) tile(std::true_type{});
-#pragma unroll
-    for (int ct = 0; ct < CT; ct++) l[ct] = col_sum(l[ct]);
+    l = col_sum(l);
 
     const parts_view<HD, C> part(a, u.part + u.piece, kvh);
     auto out_at = [&](int32_t col) { return (T *) a.out + (sv.row0 + (int64_t) ((uint32_t) col / (uint32_t) group)) * a.ldo + ((int64_t) kvh * group + (uint32_t) col % (uint32_t) group) * HD; };
     // the four waves' sums at the largest of their maxima
     float * const stat = (float *) (lds + 4 * C * (HD + 4) * 4), * const sum = (float *) lds;
     __syncthreads();      // the loop's LDS is read out
-    if (g == 0)
-        for (int ct = 0; ct < CT; ct++) { stat[(wv * C + ct * 16 + l15) * 2] = mu[ct]; stat[(wv * C + ct * 16 + l15) * 2 + 1] = l[ct]; }
+    if (g == 0) {
+        stat[(wv * C + l15) * 2] = mu;
+        stat[(wv * C + l15) * 2 + 1] = l;
+    }
 #pragma unroll
-    for (int ct = 0; ct < CT; ct++)
-        for (int d = 0; d < ND; d++) *(float4_t *) (sum + (wv * C + ct * 16 + l15) * (HD + 4) + d * 16 + g * 4) = o[ct][d];
+    for (int d = 0; d < ND; d++) *(float4_t *) (sum + (wv * C + l15) * (HD + 4) + d * 16 + g * 4) = o[d];
     __syncthreads();
     for (int i = tid; i < C * (HD / 4); i += NT) {
         const int at = i / (HD / 4), n = i % (HD / 4) * 4;
-        const int32_t col = col0 + at;
-        if (col >= n_cols) break;
+        if (col0 + at >= n_cols) break;
         float top = -INFINITY, all = 0.0f;
         for (int w = 0; w < 4; w++) top = fmaxf(top, stat[(w * C + at) * 2]);
         const float m = top == -INFINITY ? 0.0f : top;
@@ -535,7 +537,7 @@ __global__ __launch_bounds__(NT, CT == 1 ? 3 : 2) void k_cache_attention(cache_a
             if (n == 0) { part.s[2 * at] = top; part.s[2 * at + 1] = all; }
             *(float4_t *) (part.o + (int64_t) at * HD + n) = x;
         } else {
-            store4(out_at(col) + n, x * (all == 0.0f ? 0.0f : 1.0f / all));
+            store4(out_at(col0 + at) + n, x * (all == 0.0f ? 0.0f : 1.0f / all));
         }
     }
 }
@@ -546,15 +548,15 @@ __global__ __launch_bounds__(NT, CT == 1 ? 3 : 2) void k_cache_attention(cache_a
 // For bf16 rows the scales go in with the codes (K and V rounded to f16, 2^-12 relative, against bf16's half step of 2^-9): no
 // work per score is left but the softmax. f16 and f32 rows keep codes exact and scales in 32 bits as above.
 template <typename T, int HD, int CT>
-__global__ __launch_bounds__(NT, 2) void k_cache_prompt(cache_attn_args a) {
+__global__ __launch_bounds__(NT, CT == 1 ? 3 : 2) void k_cache_prompt(cache_attn_args a) {
     constexpr bool SCALED = std::is_same<T, __bf16>::value;
-    constexpr int NB = HD / 32, ND = HD / 16, UNITS = units_of(HD, 2), TERMS = sizeof(T) == 4 ? 2 : 1, WC = 16 * CT, C = 4 * WC;
+    constexpr int NB = HD / 32, ND = HD / 16, TERMS = sizeof(T) == 4 ? 2 : 1, WC = 16 * CT, C = 4 * WC;
     constexpr int KS = 2 * HD + 16, VS = 2 * HD + 32, SCALES = TILE * (KS + VS), BUF = SCALES + (SCALED ? 0 : 8 * HD);
     __shared__ __attribute__((aligned(16))) unsigned char lds[2 * BUF];
     __shared__ uint32_t tile_dmax[2][4], tile_bad[2][4];
     unit u;
     const int kvh = (int) (blockIdx.x % (unsigned) a.n_kv_head);
-    if (!find_unit<C, UNITS, false>(a, blockIdx.x / (unsigned) a.n_kv_head, u)) return;
+    if (!find_unit<C, slots_of(HD, C), false>(a, blockIdx.x / (unsigned) a.n_kv_head, u)) return;
     if (u.pieces > 1 && u.part + u.piece >= a.parts) return;
     const int tid = (int) threadIdx.x, lane = tid & 63, l15 = lane & 15, g = lane >> 4, wv = uniform(tid >> 6);
     const int seq = u.seq, group = a.n_head / a.n_kv_head;
@@ -758,7 +760,7 @@ __global__ __launch_bounds__(NT, 2) void k_cache_prompt(cache_attn_args a) {
 
 // The pieces of a column tile added in a fixed order, HD / 4 threads across a column's values: few pieces by those threads alone, a
 // column each; many by all threads, a column at a time. `split` workgroups share a tile's columns.
-template <typename T, int HD, int C, int UNITS>
+template <typename T, int HD, int C>
 __global__ __launch_bounds__(NT) void k_cache_join(cache_attn_args a, int split) {
     constexpr int W = HD / 4, PG = NT / W;      // threads across a column, columns or pieces at once
     __shared__ float top4[NT / 64], sum[PG];
@@ -766,7 +768,7 @@ __global__ __launch_bounds__(NT) void k_cache_join(cache_attn_args a, int split)
     unit u;
     const unsigned id = blockIdx.x / (unsigned) a.n_kv_head;
     const int kvh = (int) (blockIdx.x % (unsigned) a.n_kv_head);
-    if (!find_unit<C, UNITS, true>(a, id / (unsigned) split, u) || u.pieces < 2 || u.part + u.pieces > a.parts) return;
+    if (!find_unit<C, slots_of(HD, C), true>(a, id / (unsigned) split, u) || u.pieces < 2 || u.part + u.pieces > a.parts) return;
     const int tid = (int) threadIdx.x, pg = tid / W, n = tid % W * 4, group = a.n_head / a.n_kv_head, mine = (int) (id % (unsigned) split);
     const int32_t n_cols = u.v.rows * group, col0 = u.tile * C;
     const parts_view<HD, C> p0(a, u.part, kvh), p1(a, u.part + 1, kvh);
@@ -832,29 +834,29 @@ __global__ __launch_bounds__(NT) void k_cache_join(cache_attn_args a, int split)
     }
 }
 
-// Column tiles of 16, 32 or 128: by the columns that a sequence of the call has on average
-int columns_of(const cache_shape & c, int64_t n_seq, int64_t n_rows) {
+// Column tiles: 16 (the four waves split the keys) where a sequence of the call has few columns on average, else the four waves'
+// own 16 or 32 each. Measured
+int columns_of(const cache_shape & c, int type, int64_t n_seq, int64_t n_rows) {
     const int64_t cols = n_rows * (c.n_head / c.n_kv_head);
-    return cols <= 16 * n_seq ? 16 : cols <= 64 * n_seq ? 32 : 128;
+    return cols <= 64 * n_seq ? 16 : type == T_F32 ? 64 : 128;
 }
 
 // bounds on the column tiles of all sequences, and on the pieces that the ones split into several have
-int64_t tiles_bound(const cache_shape & c, int64_t n_seq, int64_t n_rows) {
-    return n_rows * (c.n_head / c.n_kv_head) / columns_of(c, n_seq, n_rows) + n_seq;
-}
-// A tile's pieces are keys of its sequence / length rounded, length at least UNITS-th of the keys of all tiles and K/V heads: without
-// the rounding all are UNITS / K/V heads at most, and where there are two or more (1.5 before rounding) it adds a third at most.
-int64_t parts_bound(const cache_shape & c, int64_t n_seq, int64_t n_rows, int64_t width) {
-    const int64_t most = (width * c.page_size + PIECE / 2) / PIECE, units = units_of(c.hd, columns_of(c, n_seq, n_rows) > 16 ? 2 : 1);
+int64_t tiles_bound(const cache_shape & c, int C, int64_t n_seq, int64_t n_rows) { return n_rows * (c.n_head / c.n_kv_head) / C + n_seq; }
+// A tile's pieces are keys of its sequence / length rounded, length at least the keys of all tiles and K/V heads over MOST_UNITS
+// slots: without the rounding all are that / K/V heads at most, and where there are two or more (1.5 before rounding) it adds a third
+// at most. (A half is counted: the device's sums are floats.)
+int64_t parts_bound(const cache_shape & c, int C, int64_t n_seq, int64_t n_rows, int64_t width) {
+    const int64_t most = (width * c.page_size + PIECE / 2) / PIECE, units = (int64_t) (1.5f * MOST_UNITS * slots_of(c.hd, C));
     if (most < 2) return 0;
-    return std::min(tiles_bound(c, n_seq, n_rows) * most, (4 * units / 3 + c.n_kv_head - 1) / c.n_kv_head + 1);
+    return std::min(tiles_bound(c, C, n_seq, n_rows) * most, (units + c.n_kv_head - 1) / c.n_kv_head);
 }
 
-template <typename T, int HD, int CT, int C>
+template <typename T, int HD, int C>
 hipError_t attend(const cache_shape & c, const cache_attn_args & a, hipStream_t s, const void * kernel) {
     cache_attn_args args = a;
     void * p[] = {&args};
-    const int64_t tiles = tiles_bound(c, a.n_seq, a.n_rows), parts = parts_bound(c, a.n_seq, a.n_rows, a.width);
+    const int64_t tiles = tiles_bound(c, C, a.n_seq, a.n_rows), parts = parts_bound(c, C, a.n_seq, a.n_rows, a.width);
     args.parts = parts;
     const int64_t blocks = (tiles + parts) * c.n_kv_head;
     if (blocks >= 1 << 24) return hipErrorInvalidConfiguration;      // threads of a launch are below 2^32
@@ -863,28 +865,35 @@ hipError_t attend(const cache_shape & c, const cache_attn_args & a, hipStream_t 
     // few tiles are split into many pieces: up to a workgroup for each column; many hardly
     int split = (int) std::min<int64_t>(C, std::max<int64_t>(1, 512 / (tiles * c.n_kv_head)));
     void * pj[] = {&args, &split};
-    return hipLaunchKernel((const void *) k_cache_join<T, HD, C, units_of(HD, CT)>, dim3((unsigned) (tiles * c.n_kv_head * split)), dim3(NT), pj, 0, s);
+    return hipLaunchKernel((const void *) k_cache_join<T, HD, C>, dim3((unsigned) (tiles * c.n_kv_head * split)), dim3(NT), pj, 0, s);
 }
 
 template <typename T, int HD>
-hipError_t by_columns(const cache_shape & c, const cache_attn_args & a, hipStream_t s) {
-    const int cols = columns_of(c, a.n_seq, a.n_rows);
-    return cols == 16 ? attend<T, HD, 1, 16>(c, a, s, (const void *) k_cache_attention<T, HD, 1>)
-         : cols == 32 ? attend<T, HD, 2, 32>(c, a, s, (const void *) k_cache_attention<T, HD, 2>)
-                      : attend<T, HD, 2, 128>(c, a, s, (const void *) k_cache_prompt<T, HD, 2>);
+hipError_t by_columns(const cache_shape & c, int type, const cache_attn_args & a, hipStream_t s) {
+    constexpr int CT = sizeof(T) == 4 ? 1 : 2;
+    return columns_of(c, type, a.n_seq, a.n_rows) == 16 ? attend<T, HD, 16>(c, a, s, (const void *) k_cache_attention<T, HD>)
+                                                        : attend<T, HD, 64 * CT>(c, a, s, (const void *) k_cache_prompt<T, HD, CT>);
 }
 
 template <typename T>
-hipError_t by_head(const cache_shape & c, const cache_attn_args & a, hipStream_t s) {
-    return c.hd == 32 ? by_columns<T, 32>(c, a, s) : c.hd == 64 ? by_columns<T, 64>(c, a, s) : c.hd == 96 ? by_columns<T, 96>(c, a, s) : by_columns<T, 128>(c, a, s);
+hipError_t by_head(const cache_shape & c, int type, const cache_attn_args & a, hipStream_t s) {
+    return c.hd == 32   ? by_columns<T, 32>(c, type, a, s)
+           : c.hd == 64 ? by_columns<T, 64>(c, type, a, s)
+           : c.hd == 96 ? by_columns<T, 96>(c, type, a, s)
+                        : by_columns<T, 128>(c, type, a, s);
 }
 
 }  // namespace
 
 int64_t cache_attention_work_bytes(const cache_shape & c, int64_t n_seq, int64_t n_rows, int64_t width) {
-    return std::max<int64_t>(16, parts_bound(c, n_seq, n_rows, width) * c.n_kv_head * columns_of(c, n_seq, n_rows) * (c.hd + 2) * 4);
+    int64_t most = 16;
+    for (int type : {(int) T_F32, (int) T_F16}) {      // (the call may come with either)
+        const int C = columns_of(c, type, n_seq, n_rows);
+        most = std::max(most, parts_bound(c, C, n_seq, n_rows, width) * c.n_kv_head * C * (c.hd + 2) * 4);
+    }
+    return most;
 }
 
 hipError_t launch_cache_attention(const cache_shape & c, int type, const cache_attn_args & a, hipStream_t s) {
-    return type == T_F32 ? by_head<float>(c, a, s) : type == T_F16 ? by_head<_Float16>(c, a, s) : by_head<__bf16>(c, a, s);
+    return type == T_F32 ? by_head<float>(c, type, a, s) : type == T_F16 ? by_head<_Float16>(c, type, a, s) : by_head<__bf16>(c, type, a, s);
 }
