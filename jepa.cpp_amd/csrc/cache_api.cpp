@@ -49,7 +49,7 @@ bool rows_ok(const char * who, const char * what, int type, const void * p, int6
     return true;
 }
 
-// heads of rows that one launch takes (its threads are below 2^32, 16 of them for a head at most)
+// heads of rows that one launch takes (its threads are below 2^32, 16 of them for a head of a row, or 64 for one of a few rows)
 bool grid_ok(const char * who, int64_t n) {
     if (n < (int64_t) 1 << 27) return true;
     jepa_log("jepa: %s: %lld heads of rows in one call (below 2^27)\n", who, (long long) n);

@@ -52,7 +52,9 @@ constexpr int PIECE = 4 * TILE;      // pieces are multiples of this: one step o
 // Workgroups that the chip holds at once (256 CUs; 512 registers of a SIMD lane over the kernel's): calls whose column tiles alone are
 // fewer are split into about as many units, or up to twice as many where that ends more evenly.
 constexpr int slots_of(int hd, int c) { return 256 * (c == 128 ? 2 : c == 64 || hd > 64 ? 3 : 4); }
-constexpr float UNIT_KEYS = 768.0f;      // what a unit costs beside its keys, in keys
+// What a unit costs beside its keys, in keys; and how many units a call is split into at most, in slots
+constexpr float unit_keys(int c) { return c == 16 ? 768.0f : 192.0f; }
+constexpr float most_units(int c) { return c == 64 ? 2.9f : 1.9f; }
 
 // the 8 codes of a word less 8, in the order of its elements (nibbles 0 4 1 5 2 6 3 7), exact in f16: a nibble or'ed into the low
 // mantissa bits of 1024 is 1024 + c, into the next four 1024 + 16 c. `k1024` is the pair of f16 1024 in a vector register (an
@@ -130,7 +132,6 @@ __device__ __forceinline__ float pieces_of(const seq_view & v, float inv) { retu
 // the inverse length of `units` equal pieces of `keys` keys (over all sequences, column tiles and K/V heads). Float sums and
 // reciprocals will do: every workgroup makes the same ones of the same numbers.
 __device__ __forceinline__ float piece_inv(float keys, float units) { return __builtin_amdgcn_rcpf(fmaxf(keys * (1.0f / units), (float) PIECE)); }
-constexpr float MOST_UNITS = 1.9f;      // that a call is split into, in slots
 
 __device__ __forceinline__ int32_t uniform(int32_t x) { return __builtin_amdgcn_readfirstlane(x); }
 // sums over the lanes up to this one, and over all of them, in the VALU: within rows of 16 lanes, then across rows
@@ -185,11 +186,11 @@ __device__ __forceinline__ bool find_unit(const cache_attn_args & a, uint32_t x,
 #pragma unroll
         for (int i = 0; i < 3; i++) {
             // so many units for each slot: the time of all, and of the longest while the last round is not full
-            constexpr float SHARE[3] = {1.0f, 0.93f, MOST_UNITS};
+            constexpr float SHARE[3] = {1.0f, 0.93f, most_units(C)};
             const float x1 = piece_inv(keys, SHARE[i] * SLOTS), n = pieces_of(v, x1);
             const float units = wave_add((float) tiles * n) * heads, rounds = units * (1.0f / SLOTS);
-            const float longest = wave_max(tiles ? (float) v.len * __builtin_amdgcn_rcpf(n) : 0.0f) + UNIT_KEYS;
-            const float time = fmaxf(__builtin_fmaf(units, UNIT_KEYS, keys) * (1.0f / SLOTS) + longest * (ceilf(rounds) - rounds), longest);
+            const float longest = wave_max(tiles ? (float) v.len * __builtin_amdgcn_rcpf(n) : 0.0f) + unit_keys(C);
+            const float time = fmaxf(__builtin_fmaf(units, unit_keys(C), keys) * (1.0f / SLOTS) + longest * (ceilf(rounds) - rounds), longest);
             if (time < least) { least = time; inv = x1; }
         }
         const uint32_t pieces = (uint32_t) pieces_of(v, inv), n = TILES ? tiles : tiles * pieces, parts = pieces > 1 ? tiles * pieces : 0u;
@@ -215,7 +216,7 @@ __device__ __forceinline__ bool find_unit(const cache_attn_args & a, uint32_t x,
     if (lane == 0) keys4[wv] = keys;
     if (tid == 0) found.seq = -1;
     __syncthreads();
-    const float inv = piece_inv(((keys4[0] + keys4[1]) + (keys4[2] + keys4[3])) * (float) a.n_kv_head, MOST_UNITS * SLOTS);
+    const float inv = piece_inv(((keys4[0] + keys4[1]) + (keys4[2] + keys4[3])) * (float) a.n_kv_head, most_units(C) * SLOTS);
     uint32_t mine = 0, parts = 0;
     for (int i = i0; i < i1; i++) {
         const seq_view v = view_of(a, i);
@@ -345,9 +346,10 @@ __device__ __forceinline__ void weights_times_scales(const float4_t * s, int h, 
         if constexpr (TERMS == 1) {
             p[0][r] = (_Float16) __builtin_fmaf(w, e, 0.0f);
         } else {
-            const float x = __builtin_fmaf(w, e, 0.0f);
+            float x = __builtin_fmaf(w, e, 0.0f);
+            asm("" : "+v"(x));      // (once, not again inside each conversion)
             p[0][r] = (_Float16) x;
-            p[1][r] = (_Float16) (x - (float) p[0][r]);
+            p[1][r] = (_Float16) __builtin_fmaf((float) p[0][r], -1.0f, x);
         }
     }
 }
@@ -843,11 +845,11 @@ int columns_of(const cache_shape & c, int type, int64_t n_seq, int64_t n_rows) {
 
 // bounds on the column tiles of all sequences, and on the pieces that the ones split into several have
 int64_t tiles_bound(const cache_shape & c, int C, int64_t n_seq, int64_t n_rows) { return n_rows * (c.n_head / c.n_kv_head) / C + n_seq; }
-// A tile's pieces are keys of its sequence / length rounded, length at least the keys of all tiles and K/V heads over MOST_UNITS
+// A tile's pieces are keys of its sequence / length rounded, length at least the keys of all tiles and K/V heads over most_units
 // slots: without the rounding all are that / K/V heads at most, and where there are two or more (1.5 before rounding) it adds a third
 // at most. (A half is counted: the device's sums are floats.)
 int64_t parts_bound(const cache_shape & c, int C, int64_t n_seq, int64_t n_rows, int64_t width) {
-    const int64_t most = (width * c.page_size + PIECE / 2) / PIECE, units = (int64_t) (1.5f * MOST_UNITS * slots_of(c.hd, C));
+    const int64_t most = (width * c.page_size + PIECE / 2) / PIECE, units = (int64_t) (1.5f * most_units(C) * slots_of(c.hd, C));
     if (most < 2) return 0;
     return std::min(tiles_bound(c, C, n_seq, n_rows) * most, (units + c.n_kv_head - 1) / c.n_kv_head);
 }

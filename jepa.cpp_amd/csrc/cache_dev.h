@@ -45,10 +45,11 @@ CACHE_HD cache_seq_step cache_step_of(int32_t have, int32_t come, int32_t width,
     cache_seq_step s;
     const int64_t cap = (int64_t) width * page_size;
     const int64_t keep = (int64_t) have + come > 0 ? (int64_t) have + come : 0;
+    const int shift = __builtin_ctz((unsigned) page_size);
     s.rows = come > 0 ? (uint32_t) come : 0u;
     s.bad = have < 0 || have > cap || keep > cap;
-    s.held = s.bad ? 0 : (int32_t) ((have + (int64_t) page_size - 1) / page_size);
-    const int32_t kept = s.bad ? 0 : (int32_t) ((keep + page_size - 1) / page_size);
+    s.held = s.bad ? 0 : (int32_t) ((have + (int64_t) page_size - 1) >> shift);
+    const int32_t kept = s.bad ? 0 : (int32_t) ((keep + page_size - 1) >> shift);
     s.need = kept > s.held ? (uint32_t) (kept - s.held) : 0u;
     s.give = kept < s.held ? (uint32_t) (s.held - kept) : 0u;
     s.len = s.bad ? (int32_t) (have < 0 ? 0 : have > cap ? cap : have) : (int32_t) keep;

@@ -7,7 +7,8 @@
 // that reads the key comes out NaN, as it would from the values, and no NaN can reach one that does not.
 //
 // Memory-bound. One thread takes 8 values of K and V (a 32-bit word of codes each), four threads a block (its maximum
-// by two shuffles).
+// by two shuffles). A workgroup has up to 16 consecutive rows of one head: of a prompt that is a whole strip, which leaves its
+// L2 as whole lines (rows of all heads in a workgroup spread a strip over the L2s of all XCDs).
 #include "cache_dev.h"
 #include "common.h"
 #include "kernels.h"
@@ -60,19 +61,17 @@ __device__ __forceinline__ uint16_t quantize8(float8 x, int lane, int code[8], b
 }
 
 // lanes of a row of one head: hd / 8 threads work, the next power of two is the group
-template <int HD> struct group { static constexpr int work = HD / 8, size = HD == 96 ? 16 : HD / 8; };
+template <int HD> struct group { static constexpr int work = HD / 8, size = HD == 96 ? 16 : HD / 8, rows = 256 / size; };
 
 template <typename T, int HD>
 __global__ __launch_bounds__(256) void k_cache_store(unsigned char * __restrict__ cache, const T * __restrict__ k, int64_t ldk,
                                                      const T * __restrict__ v, int64_t ldv, int64_t n_rows, const int64_t * __restrict__ slots,
-                                                     int n_kv_head, int page_size, int64_t n_pages) {
-    constexpr int GS = group<HD>::size, GW = group<HD>::work;
-    const int tid = (int) threadIdx.x, lane = tid & 63, t = tid % GS;
-    const int64_t item = (int64_t) blockIdx.x * (256 / GS) + tid / GS;
-    const int64_t row = item / n_kv_head;
-    const int head = (int) (item % n_kv_head);
+                                                     int n_kv_head, int page_shift, int64_t n_slots) {
+    constexpr int GS = group<HD>::size, GW = group<HD>::work, ROWS = group<HD>::rows;
+    const int tid = (int) threadIdx.x, lane = tid & 63, t = tid % GS, head = (int) (blockIdx.x % (unsigned) n_kv_head);
+    const int64_t row = (int64_t) (blockIdx.x / (unsigned) n_kv_head) * ROWS + tid / GS;
     const int64_t slot = row < n_rows ? slots[row] : -1;
-    const bool live = slot >= 0 && slot < n_pages * page_size && t < GW;
+    const bool live = slot >= 0 && slot < n_slots && t < GW;
     float8 xk = {}, xv = {};
     if (live) {
         xk = load8(k + row * ldk + (int64_t) head * HD + 8 * t);
@@ -93,8 +92,8 @@ __global__ __launch_bounds__(256) void k_cache_store(unsigned char * __restrict_
         wk |= (uint32_t) ck[j] << (4 * ((j & 1) * 4 + (j >> 1)));
         wv |= (uint32_t) cv[j] << (4 * j);
     }
-    const int in_page = (int) (slot % page_size), token = in_page % CACHE_STRIP, b = t / 4, g = t % 4;
-    unsigned char * strip = cache + cache_strip_at(slot / page_size, head, in_page, n_kv_head, page_size, HD);
+    const int in_page = (int) slot & ((1 << page_shift) - 1), token = in_page % CACHE_STRIP, b = t / 4, g = t % 4;
+    unsigned char * strip = cache + cache_strip_at(slot >> page_shift, head, in_page, n_kv_head, 1 << page_shift, HD);
     *(uint32_t *) (strip + cache_k_word(token, g, b, HD)) = wk;
     *(uint32_t *) (strip + cache_v_word(token, t, HD)) = wv;
     if (g == 0) {
@@ -107,17 +106,16 @@ __global__ __launch_bounds__(256) void k_cache_store(unsigned char * __restrict_
 template <typename T, int HD>
 __global__ __launch_bounds__(256) void k_cache_read(const unsigned char * __restrict__ cache, const int64_t * __restrict__ slots, int64_t n_rows,
                                                     T * __restrict__ k, int64_t ldk, T * __restrict__ v, int64_t ldv, int n_kv_head,
-                                                    int page_size, int64_t n_pages) {
-    const int64_t item = (int64_t) blockIdx.x * 256 + threadIdx.x;
-    const int t = (int) (item % (HD / 8));
-    const int64_t row = item / (HD / 8) / n_kv_head;
-    const int head = (int) (item / (HD / 8) % n_kv_head);
-    if (row >= n_rows) return;
+                                                    int page_shift, int64_t n_slots) {
+    constexpr int GS = group<HD>::size, GW = group<HD>::work, ROWS = group<HD>::rows;
+    const int tid = (int) threadIdx.x, t = tid % GS, head = (int) (blockIdx.x % (unsigned) n_kv_head);
+    const int64_t row = (int64_t) (blockIdx.x / (unsigned) n_kv_head) * ROWS + tid / GS;
+    if (row >= n_rows || t >= GW) return;
     const int64_t slot = slots[row];
     float8 xk = {}, xv = {};
-    if (slot >= 0 && slot < n_pages * page_size) {
-        const int in_page = (int) (slot % page_size), token = in_page % CACHE_STRIP, b = t / 4, g = t % 4;
-        const unsigned char * strip = cache + cache_strip_at(slot / page_size, head, in_page, n_kv_head, page_size, HD);
+    if (slot >= 0 && slot < n_slots) {
+        const int in_page = (int) slot & ((1 << page_shift) - 1), token = in_page % CACHE_STRIP, b = t / 4, g = t % 4;
+        const unsigned char * strip = cache + cache_strip_at(slot >> page_shift, head, in_page, n_kv_head, 1 << page_shift, HD);
         const uint32_t wk = *(const uint32_t *) (strip + cache_k_word(token, g, b, HD)), wv = *(const uint32_t *) (strip + cache_v_word(token, t, HD));
         const float dk = h2f(*(const uint16_t *) (strip + cache_k_scale(token, b, HD))), dv = h2f(*(const uint16_t *) (strip + cache_v_scale(token, b, HD)));
 #pragma unroll
@@ -132,19 +130,20 @@ __global__ __launch_bounds__(256) void k_cache_read(const unsigned char * __rest
 
 template <typename T, int HD>
 hipError_t store(const cache_shape & c, void * cache, const void * k, int64_t ldk, const void * v, int64_t ldv, int64_t n_rows, const int64_t * slot, hipStream_t s) {
-    int n_kv_head = c.n_kv_head, page_size = c.page_size;
-    int64_t n_pages = c.n_pages;
-    const int64_t per = 256 / group<HD>::size;
-    void * p[] = {&cache, &k, &ldk, &v, &ldv, &n_rows, &slot, &n_kv_head, &page_size, &n_pages};
-    return hipLaunchKernel((const void *) k_cache_store<T, HD>, dim3((unsigned) ((n_rows * n_kv_head + per - 1) / per)), dim3(256), p, 0, s);
+    int n_kv_head = c.n_kv_head, page_shift = __builtin_ctz((unsigned) c.page_size);
+    int64_t n_slots = c.n_pages * c.page_size;
+    const int64_t per = group<HD>::rows;
+    void * p[] = {&cache, &k, &ldk, &v, &ldv, &n_rows, &slot, &n_kv_head, &page_shift, &n_slots};
+    return hipLaunchKernel((const void *) k_cache_store<T, HD>, dim3((unsigned) ((n_rows + per - 1) / per * n_kv_head)), dim3(256), p, 0, s);
 }
 
 template <typename T, int HD>
 hipError_t read(const cache_shape & c, const void * cache, const int64_t * slot, int64_t n_rows, void * k, int64_t ldk, void * v, int64_t ldv, hipStream_t s) {
-    int n_kv_head = c.n_kv_head, page_size = c.page_size;
-    int64_t n_pages = c.n_pages;
-    void * p[] = {&cache, &slot, &n_rows, &k, &ldk, &v, &ldv, &n_kv_head, &page_size, &n_pages};
-    return hipLaunchKernel((const void *) k_cache_read<T, HD>, dim3((unsigned) ((n_rows * n_kv_head * (HD / 8) + 255) / 256)), dim3(256), p, 0, s);
+    int n_kv_head = c.n_kv_head, page_shift = __builtin_ctz((unsigned) c.page_size);
+    int64_t n_slots = c.n_pages * c.page_size;
+    const int64_t per = group<HD>::rows;
+    void * p[] = {&cache, &slot, &n_rows, &k, &ldk, &v, &ldv, &n_kv_head, &page_shift, &n_slots};
+    return hipLaunchKernel((const void *) k_cache_read<T, HD>, dim3((unsigned) ((n_rows + per - 1) / per * n_kv_head)), dim3(256), p, 0, s);
 }
 
 }  // namespace
