@@ -48,13 +48,16 @@ constexpr float LOG2E = 1.4426950408889634f;
 constexpr int NT = 256;              // threads of a workgroup
 constexpr int TILE = 64;             // keys of a wave's step
 constexpr int PIECE = 4 * TILE;      // pieces are multiples of this: one step of each of four waves
+constexpr int piece_min(int c) { return c == 16 ? PIECE : 2 * PIECE; }      // many columns' sums are more to write and to join
 
-// Workgroups that the chip holds at once (256 CUs; 512 registers of a SIMD lane over the kernel's): calls whose column tiles alone are
-// fewer are split into about as many units, or up to twice as many where that ends more evenly.
-constexpr int slots_of(int hd, int c) { return 256 * (c == 128 ? 2 : c == 64 || hd > 64 ? 3 : 4); }
+// Workgroups that a CU holds, by its registers (512 of a SIMD lane) and LDS, of the kernel for column tiles of c; and the chip (256
+// CUs). Calls whose column tiles alone are fewer are split into about as many units, or up to twice as many where that ends more
+// evenly: of 64 requests of 200 to 8000 tokens, as many units as slots took 73 us, twice as many 67.
+template <typename T> constexpr int groups_of(int hd, int c) { return c == 128 ? 2 : c == 64 ? (sizeof(T) == 4 && hd == 128 ? 3 : 4) : hd > 64 ? 3 : 4; }
+template <typename T> constexpr int slots_of(int hd, int c) { return 256 * groups_of<T>(hd, c); }
 // What a unit costs beside its keys, in keys; and how many units a call is split into at most, in slots
-constexpr float unit_keys(int c) { return c == 16 ? 768.0f : 192.0f; }
-constexpr float most_units(int c) { return c == 64 ? 2.9f : 1.9f; }
+constexpr float UNIT_KEYS = 768.0f;
+constexpr float MOST_UNITS = 1.9f;
 
 // the 8 codes of a word less 8, in the order of its elements (nibbles 0 4 1 5 2 6 3 7), exact in f16: a nibble or'ed into the low
 // mantissa bits of 1024 is 1024 + c, into the next four 1024 + 16 c. `k1024` is the pair of f16 1024 in a vector register (an
@@ -131,7 +134,9 @@ template <int C> __device__ __forceinline__ uint32_t tiles_of(const seq_view & v
 __device__ __forceinline__ float pieces_of(const seq_view & v, float inv) { return fmaxf(floorf(__builtin_fmaf((float) v.len, inv, 0.5f)), 1.0f); }
 // the inverse length of `units` equal pieces of `keys` keys (over all sequences, column tiles and K/V heads). Float sums and
 // reciprocals will do: every workgroup makes the same ones of the same numbers.
-__device__ __forceinline__ float piece_inv(float keys, float units) { return __builtin_amdgcn_rcpf(fmaxf(keys * (1.0f / units), (float) PIECE)); }
+template <int C> __device__ __forceinline__ float piece_inv(float keys, float units) {
+    return __builtin_amdgcn_rcpf(fmaxf(keys * (1.0f / units), (float) piece_min(C)));
+}
 
 __device__ __forceinline__ int32_t uniform(int32_t x) { return __builtin_amdgcn_readfirstlane(x); }
 // sums over the lanes up to this one, and over all of them, in the VALU: within rows of 16 lanes, then across rows
@@ -186,11 +191,11 @@ __device__ __forceinline__ bool find_unit(const cache_attn_args & a, uint32_t x,
 #pragma unroll
         for (int i = 0; i < 3; i++) {
             // so many units for each slot: the time of all, and of the longest while the last round is not full
-            constexpr float SHARE[3] = {1.0f, 0.93f, most_units(C)};
-            const float x1 = piece_inv(keys, SHARE[i] * SLOTS), n = pieces_of(v, x1);
+            constexpr float SHARE[3] = {1.0f, 0.93f, MOST_UNITS};
+            const float x1 = piece_inv<C>(keys, SHARE[i] * SLOTS), n = pieces_of(v, x1);
             const float units = wave_add((float) tiles * n) * heads, rounds = units * (1.0f / SLOTS);
-            const float longest = wave_max(tiles ? (float) v.len * __builtin_amdgcn_rcpf(n) : 0.0f) + unit_keys(C);
-            const float time = fmaxf(__builtin_fmaf(units, unit_keys(C), keys) * (1.0f / SLOTS) + longest * (ceilf(rounds) - rounds), longest);
+            const float longest = wave_max(tiles ? (float) v.len * __builtin_amdgcn_rcpf(n) : 0.0f) + UNIT_KEYS;
+            const float time = fmaxf(__builtin_fmaf(units, UNIT_KEYS, keys) * (1.0f / SLOTS) + longest * (ceilf(rounds) - rounds), longest);
             if (time < least) { least = time; inv = x1; }
         }
         const uint32_t pieces = (uint32_t) pieces_of(v, inv), n = TILES ? tiles : tiles * pieces, parts = pieces > 1 ? tiles * pieces : 0u;
@@ -216,7 +221,7 @@ __device__ __forceinline__ bool find_unit(const cache_attn_args & a, uint32_t x,
     if (lane == 0) keys4[wv] = keys;
     if (tid == 0) found.seq = -1;
     __syncthreads();
-    const float inv = piece_inv(((keys4[0] + keys4[1]) + (keys4[2] + keys4[3])) * (float) a.n_kv_head, most_units(C) * SLOTS);
+    const float inv = piece_inv<C>(((keys4[0] + keys4[1]) + (keys4[2] + keys4[3])) * (float) a.n_kv_head, MOST_UNITS * SLOTS);
     uint32_t mine = 0, parts = 0;
     for (int i = i0; i < i1; i++) {
         const seq_view v = view_of(a, i);
@@ -336,21 +341,15 @@ __device__ __forceinline__ void softmax_step(float4_t * s, int32_t key, int32_t 
 }
 
 // The B operand of the product with V, 32 keys of strips 2 h and 2 h + 1: weights times the keys' scales of one block (4 of them at d + t *
-// stride for strip t). The fma with 0 is one v_fma_mix from and to f16.
+// stride for strip t). The fmas are one v_fma_mix each, from and to f16.
 template <int TERMS>
 __device__ __forceinline__ void weights_times_scales(const float4_t * s, int h, const unsigned char * d, int stride, half8_t * p) {
     const half4_t d0 = *(const half4_t *) (d + 2 * h * stride), d1 = *(const half4_t *) (d + (2 * h + 1) * stride);
 #pragma unroll
     for (int r = 0; r < 8; r++) {
         const float w = s[2 * h + (r >> 2)][r & 3], e = (float) (r < 4 ? d0[r & 3] : d1[r & 3]);
-        if constexpr (TERMS == 1) {
-            p[0][r] = (_Float16) __builtin_fmaf(w, e, 0.0f);
-        } else {
-            float x = __builtin_fmaf(w, e, 0.0f);
-            asm("" : "+v"(x));      // (once, not again inside each conversion)
-            p[0][r] = (_Float16) x;
-            p[1][r] = (_Float16) __builtin_fmaf((float) p[0][r], -1.0f, x);
-        }
+        p[0][r] = (_Float16) __builtin_fmaf(w, e, 0.0f);
+        if constexpr (TERMS == 2) p[1][r] = (_Float16) __builtin_fmaf(w, e, -(float) p[0][r]);
     }
 }
 
@@ -371,12 +370,12 @@ template <int HD> constexpr int group_lds() {
 }
 
 template <typename T, int HD>
-__global__ __launch_bounds__(NT, 3) void k_cache_attention(cache_attn_args a) {
+__global__ __launch_bounds__(NT, groups_of<T>(HD, 16)) void k_cache_attention(cache_attn_args a) {
     constexpr int NB = HD / 32, ND = HD / 16, TERMS = sizeof(T) == 4 ? 2 : 1, C = 16;
     __shared__ __attribute__((aligned(16))) unsigned char lds[group_lds<HD>()];
     unit u;
     const int kvh = (int) (blockIdx.x % (unsigned) a.n_kv_head);
-    if (!find_unit<C, slots_of(HD, C), false>(a, blockIdx.x / (unsigned) a.n_kv_head, u)) return;
+    if (!find_unit<C, slots_of<T>(HD, C), false>(a, blockIdx.x / (unsigned) a.n_kv_head, u)) return;
     if (u.pieces > 1 && u.part + u.piece >= a.parts) return;      // (row_start that overlaps itself: more pieces than rows can have)
     const int tid = (int) threadIdx.x, lane = tid & 63, l15 = lane & 15, g = lane >> 4, wv = uniform(tid >> 6);
     const int seq = u.seq, group = a.n_head / a.n_kv_head;
@@ -544,21 +543,28 @@ __global__ __launch_bounds__(NT, 3) void k_cache_attention(cache_attn_args a) {
     }
 }
 
-// Prompts: many columns for each key, so what a key costs is paid once a workgroup. Its four waves have 16 CT columns each; a
-// tile's codes are turned into f16 once, by all four (a strip each), into double-buffered LDS, K as rows for the A operand and V as
-// rows that ds_read_b64_tr_b16 turns around. One barrier a tile; the next tile's codes are in flight meanwhile.
+// Prompts: many columns for each key, so what a key costs is paid once a workgroup. Its four waves have 16 or 32 columns each; a
+// tile's codes are turned into f16 once, by all four (a strip each), into LDS, K as rows for the A operand and V as rows that
+// ds_read_b64_tr_b16 turns around. The next tile's codes are in flight meanwhile.
 // For bf16 rows the scales go in with the codes (K and V rounded to f16, 2^-12 relative, against bf16's half step of 2^-9): no
-// work per score is left but the softmax. f16 and f32 rows keep codes exact and scales in 32 bits as above.
-template <typename T, int HD, int CT>
-__global__ __launch_bounds__(NT, CT == 1 ? 3 : 2) void k_cache_prompt(cache_attn_args a) {
-    constexpr bool SCALED = std::is_same<T, __bf16>::value;
-    constexpr int NB = HD / 32, ND = HD / 16, TERMS = sizeof(T) == 4 ? 2 : 1, WC = 16 * CT, C = 4 * WC;
+// work per score is left but the softmax, and two column tiles a wave with two LDS buffers (one barrier a tile, two
+// workgroups a CU) are best: 17.6k prompt rows of 32 x 128 take 0.84 ms, one column tile 1.04.
+// f16 and f32 rows keep codes exact and scales in 32 bits as above, twice the work per score; what hides its latencies best is four
+// workgroups a CU, of one column tile a wave and one buffer: 2000 f16 rows over 16000 tokens take 0.97 ms, two column tiles 1.14.
+template <typename T> struct prompt {
+    static constexpr bool scaled = std::is_same<T, __bf16>::value;
+    static constexpr int tiles = scaled ? 2 : 1, bufs = scaled ? 2 : 1, columns = 64 * tiles;
+};
+template <typename T, int HD>
+__global__ __launch_bounds__(NT, groups_of<T>(HD, prompt<T>::columns)) void k_cache_prompt(cache_attn_args a) {
+    constexpr bool SCALED = prompt<T>::scaled;
+    constexpr int CT = prompt<T>::tiles, BUFS = prompt<T>::bufs, NB = HD / 32, ND = HD / 16, TERMS = sizeof(T) == 4 ? 2 : 1, WC = 16 * CT, C = 4 * WC;
     constexpr int KS = 2 * HD + 16, VS = 2 * HD + 32, SCALES = TILE * (KS + VS), BUF = SCALES + (SCALED ? 0 : 8 * HD);
-    __shared__ __attribute__((aligned(16))) unsigned char lds[2 * BUF];
-    __shared__ uint32_t tile_dmax[2][4], tile_bad[2][4];
+    __shared__ __attribute__((aligned(16))) unsigned char lds[BUFS * BUF];
+    __shared__ uint32_t tile_dmax[BUFS][4], tile_bad[BUFS][4];
     unit u;
     const int kvh = (int) (blockIdx.x % (unsigned) a.n_kv_head);
-    if (!find_unit<C, slots_of(HD, C), false>(a, blockIdx.x / (unsigned) a.n_kv_head, u)) return;
+    if (!find_unit<C, slots_of<T>(HD, C), false>(a, blockIdx.x / (unsigned) a.n_kv_head, u)) return;
     if (u.pieces > 1 && u.part + u.piece >= a.parts) return;
     const int tid = (int) threadIdx.x, lane = tid & 63, l15 = lane & 15, g = lane >> 4, wv = uniform(tid >> 6);
     const int seq = u.seq, group = a.n_head / a.n_kv_head;
@@ -733,11 +739,18 @@ __global__ __launch_bounds__(NT, CT == 1 ? 3 : 2) void k_cache_prompt(cache_attn
     }
     __syncthreads();
     auto step = [&](auto masked) {
-        if (k0 + TILE < kend) stage(k0 + TILE, buf ^ 1);
-        load(k0 + 2 * TILE);
-        if (k0 < lim_hi) tile(masked);
+        if constexpr (BUFS == 2) {
+            if (k0 + TILE < kend) stage(k0 + TILE, buf ^ 1);
+            load(k0 + 2 * TILE);
+            if (k0 < lim_hi) tile(masked);
+            buf ^= 1;
+        } else {
+            if (k0 < lim_hi) tile(masked);
+            __syncthreads();
+            if (k0 + TILE < kend) stage(k0 + TILE, 0);
+            load(k0 + 2 * TILE);
+        }
         __syncthreads();
-        buf ^= 1;
     };
     auto no_bad = [&] { return (tile_bad[buf][0] | tile_bad[buf][1] | tile_bad[buf][2] | tile_bad[buf][3]) == 0; };
     for (; k0 + TILE <= min(lim_lo, kend) && no_bad(); k0 += TILE) step(std::false_type{});
@@ -770,7 +783,7 @@ __global__ __launch_bounds__(NT) void k_cache_join(cache_attn_args a, int split)
     unit u;
     const unsigned id = blockIdx.x / (unsigned) a.n_kv_head;
     const int kvh = (int) (blockIdx.x % (unsigned) a.n_kv_head);
-    if (!find_unit<C, slots_of(HD, C), true>(a, id / (unsigned) split, u) || u.pieces < 2 || u.part + u.pieces > a.parts) return;
+    if (!find_unit<C, slots_of<T>(HD, C), true>(a, id / (unsigned) split, u) || u.pieces < 2 || u.part + u.pieces > a.parts) return;
     const int tid = (int) threadIdx.x, pg = tid / W, n = tid % W * 4, group = a.n_head / a.n_kv_head, mine = (int) (id % (unsigned) split);
     const int32_t n_cols = u.v.rows * group, col0 = u.tile * C;
     const parts_view<HD, C> p0(a, u.part, kvh), p1(a, u.part + 1, kvh);
@@ -836,29 +849,34 @@ __global__ __launch_bounds__(NT) void k_cache_join(cache_attn_args a, int split)
     }
 }
 
-// Column tiles: 16 (the four waves split the keys) where a sequence of the call has few columns on average, else the four waves'
-// own 16 or 32 each. Measured
-int columns_of(const cache_shape & c, int type, int64_t n_seq, int64_t n_rows) {
-    const int64_t cols = n_rows * (c.n_head / c.n_kv_head);
-    return cols <= 64 * n_seq ? 16 : type == T_F32 ? 64 : 128;
+// Column tiles: 16 (the four waves split the keys) where a sequence of the call has few columns on average, else the prompts'.
+// Measured, us of a call of 16 sequences of 1500 tokens, 8 K/V heads of 128, 16 against the prompts' tiles: 96 columns bf16 37 / 41, f16
+// 37 / 57, f32 45 / 54; 128 columns 46 / 46, 46 / 57, 57 / 57; 192 columns 66 / 62, 66 / 71, 82 / 86; 256 columns 85 / 63, 85 / 85,
+// 106 / 116; 512 columns 160 / 79, 160 / 122, 198 / 164.
+template <typename T> int columns_of(const cache_shape & c, int64_t n_seq, int64_t n_rows) {
+    return n_rows * (c.n_head / c.n_kv_head) <= (prompt<T>::scaled ? 128 : 256) * n_seq ? 16 : prompt<T>::columns;
 }
 
 // bounds on the column tiles of all sequences, and on the pieces that the ones split into several have
 int64_t tiles_bound(const cache_shape & c, int C, int64_t n_seq, int64_t n_rows) { return n_rows * (c.n_head / c.n_kv_head) / C + n_seq; }
-// A tile's pieces are keys of its sequence / length rounded, length at least the keys of all tiles and K/V heads over most_units
+// A tile's pieces are keys of its sequence / length rounded, length at least the keys of all tiles and K/V heads over MOST_UNITS
 // slots: without the rounding all are that / K/V heads at most, and where there are two or more (1.5 before rounding) it adds a third
 // at most. (A half is counted: the device's sums are floats.)
-int64_t parts_bound(const cache_shape & c, int C, int64_t n_seq, int64_t n_rows, int64_t width) {
-    const int64_t most = (width * c.page_size + PIECE / 2) / PIECE, units = (int64_t) (1.5f * most_units(C) * slots_of(c.hd, C));
+template <typename T> int64_t parts_bound(const cache_shape & c, int C, int64_t n_seq, int64_t n_rows, int64_t width) {
+    const int64_t most = (width * c.page_size + piece_min(C) / 2) / piece_min(C), units = (int64_t) (1.5f * MOST_UNITS * slots_of<T>(c.hd, C));
     if (most < 2) return 0;
     return std::min(tiles_bound(c, C, n_seq, n_rows) * most, (units + c.n_kv_head - 1) / c.n_kv_head);
+}
+template <typename T> int64_t work_bytes(const cache_shape & c, int64_t n_seq, int64_t n_rows, int64_t width) {
+    const int C = columns_of<T>(c, n_seq, n_rows);
+    return parts_bound<T>(c, C, n_seq, n_rows, width) * c.n_kv_head * C * (c.hd + 2) * 4;
 }
 
 template <typename T, int HD, int C>
 hipError_t attend(const cache_shape & c, const cache_attn_args & a, hipStream_t s, const void * kernel) {
     cache_attn_args args = a;
     void * p[] = {&args};
-    const int64_t tiles = tiles_bound(c, C, a.n_seq, a.n_rows), parts = parts_bound(c, C, a.n_seq, a.n_rows, a.width);
+    const int64_t tiles = tiles_bound(c, C, a.n_seq, a.n_rows), parts = parts_bound<T>(c, C, a.n_seq, a.n_rows, a.width);
     args.parts = parts;
     const int64_t blocks = (tiles + parts) * c.n_kv_head;
     if (blocks >= 1 << 24) return hipErrorInvalidConfiguration;      // threads of a launch are below 2^32
@@ -871,31 +889,23 @@ hipError_t attend(const cache_shape & c, const cache_attn_args & a, hipStream_t 
 }
 
 template <typename T, int HD>
-hipError_t by_columns(const cache_shape & c, int type, const cache_attn_args & a, hipStream_t s) {
-    constexpr int CT = sizeof(T) == 4 ? 1 : 2;
-    return columns_of(c, type, a.n_seq, a.n_rows) == 16 ? attend<T, HD, 16>(c, a, s, (const void *) k_cache_attention<T, HD>)
-                                                        : attend<T, HD, 64 * CT>(c, a, s, (const void *) k_cache_prompt<T, HD, CT>);
+hipError_t by_columns(const cache_shape & c, const cache_attn_args & a, hipStream_t s) {
+    return columns_of<T>(c, a.n_seq, a.n_rows) == 16 ? attend<T, HD, 16>(c, a, s, (const void *) k_cache_attention<T, HD>)
+                                                     : attend<T, HD, prompt<T>::columns>(c, a, s, (const void *) k_cache_prompt<T, HD>);
 }
 
 template <typename T>
-hipError_t by_head(const cache_shape & c, int type, const cache_attn_args & a, hipStream_t s) {
-    return c.hd == 32   ? by_columns<T, 32>(c, type, a, s)
-           : c.hd == 64 ? by_columns<T, 64>(c, type, a, s)
-           : c.hd == 96 ? by_columns<T, 96>(c, type, a, s)
-                        : by_columns<T, 128>(c, type, a, s);
+hipError_t by_head(const cache_shape & c, const cache_attn_args & a, hipStream_t s) {
+    return c.hd == 32 ? by_columns<T, 32>(c, a, s) : c.hd == 64 ? by_columns<T, 64>(c, a, s) : c.hd == 96 ? by_columns<T, 96>(c, a, s) : by_columns<T, 128>(c, a, s);
 }
 
 }  // namespace
 
-int64_t cache_attention_work_bytes(const cache_shape & c, int64_t n_seq, int64_t n_rows, int64_t width) {
-    int64_t most = 16;
-    for (int type : {(int) T_F32, (int) T_F16}) {      // (the call may come with either)
-        const int C = columns_of(c, type, n_seq, n_rows);
-        most = std::max(most, parts_bound(c, C, n_seq, n_rows, width) * c.n_kv_head * C * (c.hd + 2) * 4);
-    }
-    return most;
+int64_t cache_attention_work_bytes(const cache_shape & c, int64_t n_seq, int64_t n_rows, int64_t width) {      // (rows of any type)
+    return std::max(std::max<int64_t>(16, work_bytes<float>(c, n_seq, n_rows, width)),
+                    std::max(work_bytes<_Float16>(c, n_seq, n_rows, width), work_bytes<__bf16>(c, n_seq, n_rows, width)));
 }
 
 hipError_t launch_cache_attention(const cache_shape & c, int type, const cache_attn_args & a, hipStream_t s) {
-    return type == T_F32 ? by_head<float>(c, type, a, s) : type == T_F16 ? by_head<_Float16>(c, type, a, s) : by_head<__bf16>(c, type, a, s);
+    return type == T_F32 ? by_head<float>(c, a, s) : type == T_F16 ? by_head<_Float16>(c, a, s) : by_head<__bf16>(c, a, s);
 }
