@@ -38,25 +38,28 @@ __device__ __forceinline__ uint16_t f2h(float f) {
 }
 __device__ __forceinline__ float h2f(uint16_t h) { return (float) __builtin_bit_cast(_Float16, h); }
 
-// codes of 8 of a block's 32 values (this thread's, of four neighbouring lanes) and the block's f16 scale
-__device__ __forceinline__ uint16_t quantize8(float8 x, int lane, int code[8], bool & finite) {
-    float amax = 0.0f, mx = 0.0f;
-    finite = true;
+// Codes of 8 of a block's 32 values (this thread's, of the four of a quad) and the block's f16 scale. Magnitudes are compared as their
+// bits, held at f16's largest (a value beyond it gets the end code of its side as it would if it were held there itself).
+__device__ __forceinline__ uint16_t quantize8(float8 x, int lane, uint32_t code[8], bool & finite) {
+    constexpr uint32_t F16_MAX = 0x477fe000;      // 65504
+    uint32_t most = 0, from = 0;
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-        finite = finite && fabsf(x[j]) <= 3.402823466e38f;
-        x[j] = fminf(fmaxf(x[j], -65504.0f), 65504.0f);
-        if (amax < fabsf(x[j])) { amax = fabsf(x[j]); mx = x[j]; }
-    }
+    for (int j = 0; j < 8; j++) most = max(most, __float_as_uint(x[j]) & 0x7fffffffu);
+    finite = most < 0x7f800000u;
+    most = min(most, F16_MAX);
 #pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {      // the first of equal magnitudes wins, so the lower lane's
-        const float oa = __shfl_xor(amax, o, 64), om = __shfl_xor(mx, o, 64);
-        if (oa > amax || (oa == amax && (lane & o))) { amax = oa; mx = om; }
-    }
-    const float d = mx / -8.0f;
+    for (int j = 7; j >= 0; j--)      // the first of equal magnitudes gives the sign
+        if (min(__float_as_uint(x[j]) & 0x7fffffffu, F16_MAX) == most) from = __float_as_uint(x[j]);
+    auto join = [&](uint32_t m, uint32_t f, bool second) {
+        if (m > most || (m == most && second)) { most = m; from = f; }
+    };
+    // quad_perm 1 0 3 2, then 2 3 0 1: of equal magnitudes the lower lane's is the first
+    join((uint32_t) __builtin_amdgcn_update_dpp(0, (int) most, 0xb1, 0xf, 0xf, true), (uint32_t) __builtin_amdgcn_update_dpp(0, (int) from, 0xb1, 0xf, 0xf, true), lane & 1);
+    join((uint32_t) __builtin_amdgcn_update_dpp(0, (int) most, 0x4e, 0xf, 0xf, true), (uint32_t) __builtin_amdgcn_update_dpp(0, (int) from, 0x4e, 0xf, 0xf, true), lane & 2);
+    const float d = __uint_as_float(most | (from & 0x80000000u)) / -8.0f;
     const float id = d != 0.0f ? 1.0f / d : 0.0f;
 #pragma unroll
-    for (int j = 0; j < 8; j++) code[j] = (int) fminf(fmaxf(x[j] * id + 8.5f, 0.0f), 15.0f);      // (an overflowing id: in range all the same)
+    for (int j = 0; j < 8; j++) code[j] = (uint32_t) __builtin_amdgcn_fmed3f(x[j] * id + 8.5f, 0.0f, 15.0f);      // (an overflowing id: in range all the same)
     return f2h(d);
 }
 
@@ -70,18 +73,18 @@ __global__ __launch_bounds__(256) void k_cache_store(unsigned char * __restrict_
     constexpr int GS = group<HD>::size, GW = group<HD>::work, ROWS = group<HD>::rows;
     const int tid = (int) threadIdx.x, lane = tid & 63, t = tid % GS, head = (int) (blockIdx.x % (unsigned) n_kv_head);
     const int64_t row = (int64_t) (blockIdx.x / (unsigned) n_kv_head) * ROWS + tid / GS;
-    const int64_t slot = row < n_rows ? slots[row] : -1;
-    const bool live = slot >= 0 && slot < n_slots && t < GW;
+    const bool has = row < n_rows && t < GW;
+    const int64_t slot = has ? slots[row] : -1;
     float8 xk = {}, xv = {};
-    if (live) {
+    if (has) {      // (whatever its slot: the loads do not wait for it)
         xk = load8(k + row * ldk + (int64_t) head * HD + 8 * t);
         xv = load8(v + row * ldv + (int64_t) head * HD + 8 * t);
     }
-    int ck[8], cv[8];
+    uint32_t ck[8], cv[8];
     bool fk, fv;
     uint16_t dk = quantize8(xk, lane, ck, fk), dv = quantize8(xv, lane, cv, fv);
     const uint64_t odd = __ballot(!(fk && fv)) >> (lane & ~(GS - 1));
-    if (!live) return;
+    if (slot < 0 || slot >= n_slots) return;
     if (odd & ((1ull << GS) - 1)) {
         dk = 0x7e00; dv = 0;
         for (int j = 0; j < 8; j++) ck[j] = cv[j] = 8;
@@ -89,8 +92,8 @@ __global__ __launch_bounds__(256) void k_cache_store(unsigned char * __restrict_
     uint32_t wk = 0, wv = 0;
 #pragma unroll
     for (int j = 0; j < 8; j++) {
-        wk |= (uint32_t) ck[j] << (4 * ((j & 1) * 4 + (j >> 1)));
-        wv |= (uint32_t) cv[j] << (4 * j);
+        wk |= ck[j] << (4 * ((j & 1) * 4 + (j >> 1)));
+        wv |= cv[j] << (4 * j);
     }
     const int in_page = (int) slot & ((1 << page_shift) - 1), token = in_page % CACHE_STRIP, b = t / 4, g = t % 4;
     unsigned char * strip = cache + cache_strip_at(slot >> page_shift, head, in_page, n_kv_head, 1 << page_shift, HD);
