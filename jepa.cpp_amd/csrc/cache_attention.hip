@@ -10,8 +10,8 @@
 //   - the MFMA's depth (32) is one q4_0 block: its sum times dk, in f32, added over the blocks of a head;
 //   - q is scaled by a power of two to a largest value in [1, 2) (exact) and taken as one f16 (f16 and bf16 rows: below
 //     2^-14 of the row's largest value they lose bits, 2^-25 of it at most) or as the sum of two (f32 rows: 22 bits);
-//   - dv goes into the weights: P'_jb = p_j dv_jb in f32, rounded to one f16 (16-bit rows: 2^-12 relative, half a step of
-//     f16, under the output's own rounding) or the sum of two (f32 rows). V itself then holds no NaN whatever a
+//   - dv goes into the weights: P'_jb = p_j dv_jb in f32, rounded to one f16 (16-bit rows: half a step of f16, 2^-11
+//     relative at most, as the output's own rounding is or finer, and averaged over the keys) or the sum of two (f32 rows). V itself then holds no NaN whatever a
 //     masked token contains. mu is the running maximum of the scores plus the exponent of the tile's largest dv, less 6, and moves
 //     when a tile passes it by more than 2^8: so P' is below 2^14, f16's range, however small or large the values are.
 // Scores, maxima, sums and accumulators are f32.
@@ -546,7 +546,7 @@ __global__ __launch_bounds__(NT, groups_of<T>(HD, 16)) void k_cache_attention(ca
 // Prompts: many columns for each key, so what a key costs is paid once a workgroup. Its four waves have 16 or 32 columns each; a
 // tile's codes are turned into f16 once, by all four (a strip each), into LDS, K as rows for the A operand and V as rows that
 // ds_read_b64_tr_b16 turns around. The next tile's codes are in flight meanwhile.
-// For bf16 rows the scales go in with the codes (K and V rounded to f16, 2^-12 relative, against bf16's half step of 2^-9): no
+// For bf16 rows the scales go in with the codes (K and V rounded to f16, 2^-11 relative, against bf16's half step of 2^-8): no
 // work per score is left but the softmax, and two column tiles a wave with two LDS buffers (one barrier a tile, two
 // workgroups a CU) are best: 17.6k prompt rows of 32 x 128 take 0.84 ms, one column tile 1.04.
 // f16 and f32 rows keep codes exact and scales in 32 bits as above, twice the work per score; what hides its latencies best is four

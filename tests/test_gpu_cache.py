@@ -4,14 +4,14 @@ cache holds, and the calls together as a step-by-step program makes them, eager 
 
 Attention's tolerance, for one row and head with out = sum_j p_j v_j and A = sum_j p_j |v_j| (both in 64 bits):
   the output's own rounding      eps_T / 2 |out| (half a step of its type), and half its smallest step
-  16-bit types, weights in f16   2^-12 A (half a step of f16, relative to each weight)
+  16-bit types, weights in f16   2^-11 A (half a step of f16, eps / 2, relative to each weight)
   the 32-bit arithmetic          every score is a sum of head_dim products of a query held to 2^-22 of its row's largest
                                  value and an exact key, times a scale: off by at most (head_dim / 8 + 8) 2^-22 S,
                                  S = max_j scale |q|max |k_j|_1; the weights follow by the factor e^x ~ 1 + x on both sides
                                  of the fraction (twice), and their own 2^-21 and the sums' sqrt(n) 2^-24 come on top.
-  bf16 rows, keys and values     where many rows share them the cached values are rounded to f16, 2^-12 relative: a score is off by at
-                                 most 2^-12 S1, S1 = max_j scale sum_n |q_n| |k_jn|, on both sides of the fraction, and the sum over
-                                 V by 2^-12 A
+  bf16 rows, keys and values     where many rows share them the cached values are rounded to f16, 2^-11 relative: a score is off by at
+                                 most 2^-11 S1, S1 = max_j scale sum_n |q_n| |k_jn|, on both sides of the fraction, and the sum over
+                                 V by 2^-11 A
   small weights                  a weight enters the product with V as p_j d_j in f16 (the scale d_j of its block of V, the value
                                  at most 8 d_j), moved by a power of two that brings the largest p_j max d to 2^6 or more: f16's
                                  smallest step, half of it 2^-25, is 2^-31 of that largest one. Divided by the sum of the p_j, which
@@ -123,6 +123,7 @@ def pool(rng, lens, page, width, spare, extra=0):
 @pytest.mark.parametrize("n,hi,most,page,spare,slack", [
     (1, 0, 1, 16, 1, 0), (1, 5, 40, 16, 3, 0), (3, 100, 20, 32, 9, 7), (64, 300, 1, 64, 64, 0), (65, 50, 33, 16, 60, 0), (200, 40, 100, 16, 500, -300),
     (1025, 30, 3, 16, 300, 5), (4096, 20, 2, 256, 2000, 0), (7, 400, 9000, 256, 200, 0), (5, 0, 20000, 16, 4000, -1), (2, 17, 0, 16, 0, 4),
+    (2500, 40, 9, 16, 1500, 0), (4096, 100, 40, 32, 5000, 9), (1, 0, 4, 16, 1, 0), (1, 15, 4097, 128, 40, 0), (300, 200, 4, 128, 100, -9),
 ])
 def test_plan(jlib, n, hi, most, page, spare, slack, alias):
     rng = np.random.default_rng(n * 7 + page)
@@ -316,10 +317,10 @@ def reference(p, q, start, total, table, block, scale, kind):
             S = abs(scale) * x.abs().amax(-1, keepdim=True) * (k1.max() if n else 0.0)
             low = 0.0
             if kind == "bf16" and n:
-                low = 2.0 ** -12 * (1 + 2 * abs(scale) * (x.abs() @ torch.nan_to_num(k[:, h // group]).abs().T).amax(-1, keepdim=True))
+                low = 2.0 ** -11 * (1 + 2 * abs(scale) * (x.abs() @ torch.nan_to_num(k[:, h // group]).abs().T).amax(-1, keepdim=True))
             f32 = low + 2 * (hd / 8 + 8) * 2.0 ** -22 * S + 2.0 ** -20 + (n ** 0.5) * 2.0 ** -24
             out[a:b, h] = y
-            tol[a:b, h] = eps * y.abs() + tiny + n * 2.0 ** -30 * (v[:, h // group].abs().max() if n else 0.0) + (f32 + (2.0 ** -12 if kind != "f32" else 0.0)) * A * (1 + eps)
+            tol[a:b, h] = eps * y.abs() + tiny + n * 2.0 ** -30 * (v[:, h // group].abs().max() if n else 0.0) + (f32 + (2.0 ** -11 if kind != "f32" else 0.0)) * A * (1 + eps)
     return out.reshape(q.shape), tol.reshape(q.shape)
 
 
@@ -393,7 +394,8 @@ def test_attention_ragged_rows(jlib, kind, hd, kvh, group, page, block):
 
 
 @pytest.mark.parametrize("kind", list(TYPES))
-@pytest.mark.parametrize("rows,length,kvh,group,hd", [(300, 300, 2, 4, 64), (513, 900, 1, 8, 128), (258, 1032, 4, 1, 64), (64, 64, 1, 1, 32), (1000, 1000, 1, 3, 96)])
+@pytest.mark.parametrize("rows,length,kvh,group,hd", [(300, 300, 2, 4, 64), (513, 900, 1, 8, 128), (258, 1032, 4, 1, 64), (64, 64, 1, 1, 32), (1000, 1000, 1, 3, 96),
+                                                        (200, 5000, 2, 4, 128), (130, 3000, 1, 8, 96), (300, 2500, 2, 1, 32), (257, 1900, 3, 2, 64)])
 def test_attention_prompt(jlib, kind, rows, length, kvh, group, hd):
     rng = np.random.default_rng(rows)
     lens, start = [length, 20], [0, rows, rows + 20]
@@ -504,6 +506,44 @@ def test_attention_strides_and_neighbours(jlib):
         want, tol = reference(p, q.contiguous(), start, lens, table, 1, 0.125, kind)
         assert ((out[:, 512:768].double() - want).abs() <= tol).all()
         assert (out[:, :512] == 7).all() and (out[:, 768:] == 7).all()
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("rows", [1, 40])
+def test_attention_many_sequences_and_a_long_one(jlib, kind, rows):
+    """More sequences than a wave has lanes, some split into pieces."""
+    rng = np.random.default_rng(14)
+    lens = rng.integers(1, 200, 70).tolist()
+    lens[3], lens[66], lens[69] = 9000, 2100, 700
+    p, table = filled(jlib, rng, 8, 1, 64, 64, lens)
+    n = [0 if i % 9 == 5 else min(rows, lens[i]) for i in range(70)]
+    start = [0] + np.cumsum(n).tolist()
+    check(p, queries(rng, start[-1] + 1, 512, kind), start, lens, table, kind)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("scale", [0.0, -0.125, 1.0, 1e-30])
+def test_attention_scales(jlib, kind, scale):
+    rng = np.random.default_rng(15)
+    lens, start = [300, 40], [0, 90, 130]
+    p, table = filled(jlib, rng, 4, 1, 64, 16, lens, k_scale=0.3)
+    q = queries(rng, 130, 256, kind)
+    check(p, q, start, lens, table, kind, 1, scale)
+    check(p, q, [0, 2, 5], lens, table, kind, 7, scale)
+
+
+def test_attention_row_starts_that_overlap(jlib):
+    """row_start that runs backwards: sequences claim the same rows. Which one a row comes from is not said, but every row is written by
+    one of them or left, and nothing beside the rows is touched."""
+    rng = np.random.default_rng(16)
+    lens = [3000, 2900, 2800, 2700]
+    p, table = filled(jlib, rng, 4, 2, 64, 64, lens)
+    for kind in TYPES:
+        out = torch.full((40, 256), 7.0, dtype=TYPES[kind][0], device="cuda")
+        for start in ([0, 12, 3, 12, 2], [12, 0, 12, 0, 12], [-5, 40, -40, 12, 12], [2147483647, -2147483648, 12, 1, 9]):
+            p.attend(queries(rng, 12, 256, kind), ints(start), ints(lens), ints(table), kind, 1, out=out[:12])
+            torch.cuda.synchronize()
+            assert (out[12:] == 7).all() and not torch.isnan(out).any()
 
 
 def test_attention_many_sequences(jlib):
