@@ -26,7 +26,8 @@
 // Work. A unit is (sequence, tile of columns, piece of its keys, K/V head). The piece length is the same for all sequences
 // of a call and chosen on the device from the sum of their lengths, so that long sequences are split and short ones are not and
 // the chip is filled evenly by ragged batches; the host knows only a bound on the units, and workgroups past the last one
-// leave. Pieces of a column tile write their sums to `work` and k_cache_join adds them in order.
+// leave. Pieces of a column tile write their sums to `work`; the last one to arrive adds them in their order, so the result does not
+// depend on which that is, and nothing waits for another workgroup.
 #include "cache_dev.h"
 #include "common.h"
 #include "kernels.h"
@@ -43,6 +44,9 @@ typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
 typedef float float4_t __attribute__((ext_vector_type(4)));
 typedef float float8_t __attribute__((ext_vector_type(8)));
 typedef int int2_t __attribute__((ext_vector_type(2)));
+typedef uint32_t word2_t __attribute__((ext_vector_type(2)));
+typedef uint32_t word3_t __attribute__((ext_vector_type(3)));
+typedef uint32_t word4_t __attribute__((ext_vector_type(4)));
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int NT = 256;              // threads of a workgroup
@@ -99,13 +103,10 @@ __device__ __forceinline__ uint32_t wave_umax(uint32_t x) {
 // N words per lane of a buffer
 template <int N>
 __device__ __forceinline__ void load_words(uint32_t * x, brsrc r, int at, int off) {
-    typedef uint32_t uint2_t __attribute__((ext_vector_type(2)));
-    typedef uint32_t uint3_t __attribute__((ext_vector_type(3)));
-    typedef uint32_t uint4_t __attribute__((ext_vector_type(4)));
     if constexpr (N == 1) x[0] = __builtin_amdgcn_raw_buffer_load_b32(r, at, off, 0);
-    if constexpr (N == 2) { const uint2_t v = __builtin_amdgcn_raw_buffer_load_b64(r, at, off, 0); x[0] = v[0]; x[1] = v[1]; }
-    if constexpr (N == 3) { const uint3_t v = __builtin_amdgcn_raw_buffer_load_b96(r, at, off, 0); x[0] = v[0]; x[1] = v[1]; x[2] = v[2]; }
-    if constexpr (N == 4) { const uint4_t v = __builtin_amdgcn_raw_buffer_load_b128(r, at, off, 0); x[0] = v[0]; x[1] = v[1]; x[2] = v[2]; x[3] = v[3]; }
+    if constexpr (N == 2) { const word2_t v = __builtin_amdgcn_raw_buffer_load_b64(r, at, off, 0); x[0] = v[0]; x[1] = v[1]; }
+    if constexpr (N == 3) { const word3_t v = __builtin_amdgcn_raw_buffer_load_b96(r, at, off, 0); x[0] = v[0]; x[1] = v[1]; x[2] = v[2]; }
+    if constexpr (N == 4) { const word4_t v = __builtin_amdgcn_raw_buffer_load_b128(r, at, off, 0); x[0] = v[0]; x[1] = v[1]; x[2] = v[2]; x[3] = v[3]; }
 }
 __device__ __forceinline__ void wave_order() {      // LDS accesses of the wave's lanes before and after stay in this order
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -167,17 +168,17 @@ __device__ __forceinline__ float wave_max(float x) {      // (of values that are
 template <typename X>
 __device__ __forceinline__ X wave_add(X x) { return __builtin_bit_cast(X, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wave_scan(x)), 63)); }
 
-// Unit x of the call (x-th column tile if TILES), for column tiles of C. Every thread gets it, in scalar registers; false past the last.
+// Unit x of the call, for column tiles of C. Every thread gets it, in scalar registers; false past the last.
 // Up to 64 sequences each wave finds it by itself, a sequence a lane, and weighs a few piece lengths against each other; more are
 // dealt to the workgroup's threads.
-template <int C, int SLOTS, bool TILES>
+template <int C, int SLOTS>
 __device__ __forceinline__ bool find_unit(const cache_attn_args & a, uint32_t x, unit & u) {
     const int tid = (int) threadIdx.x, lane = tid & 63, wv = tid >> 6, group = a.n_head / a.n_kv_head;
     auto set = [&](unit & f, const seq_view & v, int i, uint32_t tiles, uint32_t pieces, uint32_t at, uint32_t part) {
         f.v = v;
         f.seq = i;
-        f.tile = (int) (tiles - 1 - (TILES ? at : at / pieces));      // a prompt's last rows read the most keys: they go first
-        f.piece = TILES ? 0 : (int) (at % pieces);
+        f.tile = (int) (tiles - 1 - at / pieces);      // a prompt's last rows read the most keys: they go first
+        f.piece = (int) (at % pieces);
         f.pieces = (int) pieces;
         f.length = (int32_t) (((uint32_t) v.len + pieces * PIECE - 1) / (pieces * PIECE) * PIECE);
         f.part = (int64_t) part + (int64_t) f.tile * (int64_t) pieces;
@@ -198,7 +199,7 @@ __device__ __forceinline__ bool find_unit(const cache_attn_args & a, uint32_t x,
             const float time = fmaxf(__builtin_fmaf(units, UNIT_KEYS, keys) * (1.0f / SLOTS) + longest * (ceilf(rounds) - rounds), longest);
             if (time < least) { least = time; inv = x1; }
         }
-        const uint32_t pieces = (uint32_t) pieces_of(v, inv), n = TILES ? tiles : tiles * pieces, parts = pieces > 1 ? tiles * pieces : 0u;
+        const uint32_t pieces = (uint32_t) pieces_of(v, inv), n = tiles * pieces, parts = pieces > 1 ? tiles * pieces : 0u;
         const uint32_t upto = wave_scan(n), parts_upto = wave_scan(parts);
         const uint64_t mine = __ballot(x >= upto - n && x < upto);
         if (!mine) return false;
@@ -226,7 +227,7 @@ __device__ __forceinline__ bool find_unit(const cache_attn_args & a, uint32_t x,
     for (int i = i0; i < i1; i++) {
         const seq_view v = view_of(a, i);
         const uint32_t tiles = tiles_of<C>(v, group), pieces = (uint32_t) pieces_of(v, inv);
-        mine += TILES ? tiles : tiles * pieces;
+        mine += tiles * pieces;
         parts += pieces > 1 ? tiles * pieces : 0;
     }
     uint32_t before = wave_scan(mine), parts_before = wave_scan(parts);
@@ -239,7 +240,7 @@ __device__ __forceinline__ bool find_unit(const cache_attn_args & a, uint32_t x,
         uint32_t at = x - before;
         for (int i = i0; i < i1; i++) {
             const seq_view v = view_of(a, i);
-            const uint32_t tiles = tiles_of<C>(v, group), pieces = (uint32_t) pieces_of(v, inv), n = TILES ? tiles : tiles * pieces;
+            const uint32_t tiles = tiles_of<C>(v, group), pieces = (uint32_t) pieces_of(v, inv), n = tiles * pieces;
             if (at < n) {
                 found = {v, i, tiles, pieces, at, parts_before};
                 break;
@@ -255,21 +256,96 @@ __device__ __forceinline__ bool find_unit(const cache_attn_args & a, uint32_t x,
     return true;
 }
 
-// the parts of `work`: sums [part][kv head][C][hd], then (maximum, sum) [part][kv head][C][2]
-template <int HD, int C>
-struct parts_view {
-    float * o, * s;
-    __device__ parts_view(const cache_attn_args & a, int64_t part, int kvh) {
-        const int64_t p = (part * a.n_kv_head + kvh) * C;
-        o = a.work + p * (HD + 2);
-        s = o + (int64_t) C * HD;
-    }
-};
-
 template <typename T>
 __device__ __forceinline__ void store4(T * p, float4_t x) {
     typedef T vec __attribute__((ext_vector_type(4)));
     *(vec *) p = __builtin_convertvector(x, vec);
+}
+
+// `work`: a counter for each column tile of several pieces and K/V head (at the place of its first part), then the parts, [part][kv head]:
+// sums [C][hd], (maximum, sum) [C][2]. The parts bypass the L2s of the XCDs (cache policy sc1, what agent-scope atomics use): once a
+// wave's stores have completed they are visible to every XCD, and no L2 is written back or invalidated.
+constexpr int64_t COUNTERS = 8192;
+template <int HD, int C>
+struct parts_view {
+    static constexpr int SC1 = 16, PART = C * (HD + 2) * 4;      // bytes
+    const brsrc r;
+    const uint32_t at, step;      // this tile's first part, from one to the next
+    __device__ parts_view(const cache_attn_args & a, int64_t part, int kvh)
+        : r(make_brsrc(a.work + 2 * COUNTERS, a.parts * a.n_kv_head * PART)), at((uint32_t) (part * a.n_kv_head + kvh) * PART), step((uint32_t) a.n_kv_head * PART) {}
+    __device__ void put(int piece, int col, int n, float4_t x) const {
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(word4_t, x), r, at + piece * step + (uint32_t) (col * HD + n) * 4, 0, SC1);
+    }
+    __device__ void put_stat(int piece, int col, float mu, float l) const {
+        __builtin_amdgcn_raw_buffer_store_b64(word2_t{__float_as_uint(mu), __float_as_uint(l)}, r, at + piece * step + (uint32_t) (C * HD * 4 + col * 8), 0, SC1);
+    }
+    __device__ float4_t get(int piece, int col, int n) const {
+        return __builtin_bit_cast(float4_t, __builtin_amdgcn_raw_buffer_load_b128(r, at + piece * step + (uint32_t) (col * HD + n) * 4, 0, SC1));
+    }
+    __device__ void get_stat(int piece, int col, float & mu, float & l) const {
+        const word2_t x = __builtin_amdgcn_raw_buffer_load_b64(r, at + piece * step + (uint32_t) (C * HD * 4 + col * 8), 0, SC1);
+        mu = __uint_as_float(x[0]);
+        l = __uint_as_float(x[1]);
+    }
+};
+
+// Whether this workgroup's piece, whose part it has stored, is the last of its tile's. The counter is 0 between calls; what is no
+// counter (a work space not used before holds anything) is told by its upper 40 bits, and made one by whoever comes first. Every
+// wait ends: each workgroup adds to a word that is no counter once, so one of the exchanges succeeds.
+__device__ __forceinline__ bool last_to_arrive(const cache_attn_args & a, const unit & u, int kvh) {
+    typedef unsigned long long u64;
+    constexpr u64 TAG = 0x6a65706163ull;
+    __shared__ int last;
+    __builtin_amdgcn_s_waitcnt(0x0f70);      // vmcnt(0): this wave's part has been written
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        u64 * counter = (u64 *) a.work + u.part * a.n_kv_head + kvh, was;
+        while ((was = atomicAdd(counter, 1ull)) >> 24 != TAG) {
+            u64 now;
+            while ((now = __hip_atomic_load(counter, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) >> 24 != TAG) atomicCAS(counter, now, TAG << 24);
+        }
+        last = (int) (was & 0xffffff) + 1 == u.pieces;
+        if (last) __hip_atomic_store(counter, TAG << 24, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    return last;
+}
+
+// The pieces of a column tile added in their order, HD / 4 threads a column, 8 pieces in flight
+template <typename T, int HD, int C>
+__device__ __forceinline__ void join_pieces(const cache_attn_args & a, const unit & u, int kvh, const parts_view<HD, C> & part) {
+    constexpr int W = HD / 4, PG = NT / W, AT_ONCE = 8;
+    const int tid = (int) threadIdx.x, n = tid % W * 4, group = a.n_head / a.n_kv_head;
+    const int32_t n_cols = u.v.rows * group, col0 = u.tile * C;
+    for (int at = tid / W; at < C && col0 + at < n_cols && tid < PG * W; at += PG) {
+        float top = -INFINITY, all = 0.0f;
+        float4_t x = {0, 0, 0, 0};
+        for (int k0 = 0; k0 < u.pieces; k0 += AT_ONCE) {
+            float mu[AT_ONCE], l[AT_ONCE], to = top;
+            float4_t y[AT_ONCE];
+#pragma unroll
+            for (int k = 0; k < AT_ONCE; k++) {
+                const int piece = min(k0 + k, u.pieces - 1);
+                part.get_stat(piece, at, mu[k], l[k]);
+                y[k] = part.get(piece, at, n);
+            }
+#pragma unroll
+            for (int k = 0; k < AT_ONCE; k++) to = fmaxf(to, mu[k]);
+            const float m = to == -INFINITY ? 0.0f : to, back = __builtin_amdgcn_exp2f(top - m);
+            all *= back;
+            x *= back;
+#pragma unroll
+            for (int k = 0; k < AT_ONCE; k++) {
+                const float f = k0 + k < u.pieces ? __builtin_amdgcn_exp2f(mu[k] - m) : 0.0f;
+                all += l[k] * f;
+                x += y[k] * f;
+            }
+            top = to;
+        }
+        const uint32_t col = (uint32_t) (col0 + at);
+        T * out = (T *) a.out + (u.v.row0 + (int64_t) (col / (uint32_t) group)) * a.ldo + ((int64_t) kvh * group + col % (uint32_t) group) * HD;
+        store4(out + n, x * (all == 0.0f ? 0.0f : 1.0f / all));
+    }
 }
 
 // The column's query row to f16: scaled by a power of two to a largest value in [1, 2), one term or two; c: what a product of it with a
@@ -375,8 +451,8 @@ __global__ __launch_bounds__(NT, groups_of<T>(HD, 16)) void k_cache_attention(ca
     __shared__ __attribute__((aligned(16))) unsigned char lds[group_lds<HD>()];
     unit u;
     const int kvh = (int) (blockIdx.x % (unsigned) a.n_kv_head);
-    if (!find_unit<C, slots_of<T>(HD, C), false>(a, blockIdx.x / (unsigned) a.n_kv_head, u)) return;
-    if (u.pieces > 1 && u.part + u.piece >= a.parts) return;      // (row_start that overlaps itself: more pieces than rows can have)
+    if (!find_unit<C, slots_of<T>(HD, C)>(a, blockIdx.x / (unsigned) a.n_kv_head, u)) return;
+    if (u.pieces > 1 && u.part + u.pieces > a.parts) return;      // (row_start that overlaps itself: more pieces than rows can have)
     const int tid = (int) threadIdx.x, lane = tid & 63, l15 = lane & 15, g = lane >> 4, wv = uniform(tid >> 6);
     const int seq = u.seq, group = a.n_head / a.n_kv_head;
     const seq_view sv = u.v;
@@ -510,7 +586,7 @@ __global__ __launch_bounds__(NT, groups_of<T>(HD, 16)) void k_cache_attention(ca
     for (; k0 < kend; k0 += STEP) tile(std::true_type{});
     l = col_sum(l);
 
-    const parts_view<HD, C> part(a, u.part + u.piece, kvh);
+    const parts_view<HD, C> part(a, u.part, kvh);
     auto out_at = [&](int32_t col) { return (T *) a.out + (sv.row0 + (int64_t) ((uint32_t) col / (uint32_t) group)) * a.ldo + ((int64_t) kvh * group + (uint32_t) col % (uint32_t) group) * HD; };
     // the four waves' sums at the largest of their maxima
     float * const stat = (float *) (lds + 4 * C * (HD + 4) * 4), * const sum = (float *) lds;
@@ -535,12 +611,13 @@ __global__ __launch_bounds__(NT, groups_of<T>(HD, 16)) void k_cache_attention(ca
             x += *(const float4_t *) (sum + (w * C + at) * (HD + 4) + n) * f;
         }
         if (u.pieces > 1) {
-            if (n == 0) { part.s[2 * at] = top; part.s[2 * at + 1] = all; }
-            *(float4_t *) (part.o + (int64_t) at * HD + n) = x;
+            if (n == 0) part.put_stat(u.piece, at, top, all);
+            part.put(u.piece, at, n, x);
         } else {
             store4(out_at(col0 + at) + n, x * (all == 0.0f ? 0.0f : 1.0f / all));
         }
     }
+    if (u.pieces > 1 && last_to_arrive(a, u, kvh)) join_pieces<T>(a, u, kvh, part);
 }
 
 // Prompts: many columns for each key, so what a key costs is paid once a workgroup. Its four waves have 16 or 32 columns each; a
@@ -564,8 +641,8 @@ __global__ __launch_bounds__(NT, groups_of<T>(HD, prompt<T>::columns)) void k_ca
     __shared__ uint32_t tile_dmax[BUFS][4], tile_bad[BUFS][4];
     unit u;
     const int kvh = (int) (blockIdx.x % (unsigned) a.n_kv_head);
-    if (!find_unit<C, slots_of<T>(HD, C), false>(a, blockIdx.x / (unsigned) a.n_kv_head, u)) return;
-    if (u.pieces > 1 && u.part + u.piece >= a.parts) return;
+    if (!find_unit<C, slots_of<T>(HD, C)>(a, blockIdx.x / (unsigned) a.n_kv_head, u)) return;
+    if (u.pieces > 1 && u.part + u.pieces > a.parts) return;
     const int tid = (int) threadIdx.x, lane = tid & 63, l15 = lane & 15, g = lane >> 4, wv = uniform(tid >> 6);
     const int seq = u.seq, group = a.n_head / a.n_kv_head;
     const seq_view sv = u.v;
@@ -756,97 +833,28 @@ __global__ __launch_bounds__(NT, groups_of<T>(HD, prompt<T>::columns)) void k_ca
     for (; k0 + TILE <= min(lim_lo, kend) && no_bad(); k0 += TILE) step(std::false_type{});
     for (; k0 < kend; k0 += TILE) step(std::true_type{});
 
-    const parts_view<HD, C> part(a, u.part + u.piece, kvh);
 #pragma unroll
-    for (int ct = 0; ct < CT; ct++) {
-        const float sum = col_sum(l[ct]);
-        const int32_t at = wv * WC + ct * 16 + l15, col = first + at;
-        if (col >= n_cols) continue;
-        if (u.pieces > 1) {
-            if (g == 0) { part.s[2 * at] = mu[ct]; part.s[2 * at + 1] = sum; }
-            for (int d = 0; d < ND; d++) *(float4_t *) (part.o + (int64_t) at * HD + d * 16 + g * 4) = o[ct][d];
-        } else {
-            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    for (int ct = 0; ct < CT; ct++) l[ct] = col_sum(l[ct]);
+    if (u.pieces == 1) {
+#pragma unroll
+        for (int ct = 0; ct < CT; ct++) {
+            const int32_t col = col0 + ct * 16 + l15;
+            if (col >= n_cols) continue;
+            const float inv = l[ct] == 0.0f ? 0.0f : 1.0f / l[ct];
             T * p = (T *) a.out + (sv.row0 + (int64_t) ((uint32_t) col / (uint32_t) group)) * a.ldo + ((int64_t) kvh * group + (uint32_t) col % (uint32_t) group) * HD;
             for (int d = 0; d < ND; d++) store4(p + d * 16 + g * 4, o[ct][d] * inv);
         }
-    }
-}
-
-// The pieces of a column tile added in a fixed order, HD / 4 threads across a column's values: few pieces by those threads alone, a
-// column each; many by all threads, a column at a time. `split` workgroups share a tile's columns.
-template <typename T, int HD, int C>
-__global__ __launch_bounds__(NT) void k_cache_join(cache_attn_args a, int split) {
-    constexpr int W = HD / 4, PG = NT / W;      // threads across a column, columns or pieces at once
-    __shared__ float top4[NT / 64], sum[PG];
-    __shared__ __attribute__((aligned(16))) float acc[PG][HD];
-    unit u;
-    const unsigned id = blockIdx.x / (unsigned) a.n_kv_head;
-    const int kvh = (int) (blockIdx.x % (unsigned) a.n_kv_head);
-    if (!find_unit<C, slots_of<T>(HD, C), true>(a, id / (unsigned) split, u) || u.pieces < 2 || u.part + u.pieces > a.parts) return;
-    const int tid = (int) threadIdx.x, pg = tid / W, n = tid % W * 4, group = a.n_head / a.n_kv_head, mine = (int) (id % (unsigned) split);
-    const int32_t n_cols = u.v.rows * group, col0 = u.tile * C;
-    const parts_view<HD, C> p0(a, u.part, kvh), p1(a, u.part + 1, kvh);
-    const int64_t next = p1.o - p0.o;      // from a piece to the next
-    auto write = [&](int32_t col, float4_t x, float all) {
-        T * out = (T *) a.out + (u.v.row0 + (int64_t) ((uint32_t) col / (uint32_t) group)) * a.ldo + ((int64_t) kvh * group + (uint32_t) col % (uint32_t) group) * HD;
-        store4(out + n, x * (all == 0.0f ? 0.0f : 1.0f / all));
-    };
-    if (u.pieces <= 8) {
-        for (int at = mine + split * pg; at < C && col0 + at < n_cols && pg < PG; at += split * PG) {
-            float mu[8], l[8], top = -INFINITY, all = 0.0f;
-            float4_t y[8], x = {0, 0, 0, 0};
-#pragma unroll
-            for (int k = 0; k < 8; k++) {
-                const int64_t o = min(k, u.pieces - 1) * next;
-                mu[k] = p0.s[o + 2 * at];
-                l[k] = p0.s[o + 2 * at + 1];
-                y[k] = *(const float4_t *) (p0.o + o + (int64_t) at * HD + n);
-            }
-#pragma unroll
-            for (int k = 0; k < 8; k++) top = fmaxf(top, mu[k]);
-            const float m = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-            for (int k = 0; k < 8; k++) {
-                if (k >= u.pieces) break;
-                const float f = __builtin_amdgcn_exp2f(mu[k] - m);
-                all += l[k] * f;
-                x += y[k] * f;
-            }
-            write(col0 + at, x, all);
-        }
         return;
     }
-    for (int at = mine; at < C && col0 + at < n_cols; at += split) {
-        float top = -INFINITY;
-        for (int k = tid; k < u.pieces; k += NT) top = fmaxf(top, p0.s[k * next + 2 * at]);
-        for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-        if (tid % 64 == 0) top4[tid / 64] = top;
-        __syncthreads();
-        top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3]));
-        const float m = top == -INFINITY ? 0.0f : top;
-        float all = 0.0f;
-        float4_t x = {0, 0, 0, 0};
-        if (pg < PG) {
-#pragma unroll 4
-            for (int k = pg; k < u.pieces; k += PG) {
-                const float f = __builtin_amdgcn_exp2f(p0.s[k * next + 2 * at] - m);
-                all += p0.s[k * next + 2 * at + 1] * f;
-                x += *(const float4_t *) (p0.o + k * next + (int64_t) at * HD + n) * f;
-            }
-            *(float4_t *) &acc[pg][n] = x;
-            if (n == 0) sum[pg] = all;
-        }
-        __syncthreads();
-        if (tid < W) {
-            for (int k = 1; k < PG; k++) {
-                all += sum[k];
-                x += *(const float4_t *) &acc[k][n];
-            }
-            write(col0 + at, x, all);
-        }
-        __syncthreads();
+    const parts_view<HD, C> part(a, u.part, kvh);
+#pragma unroll
+    for (int ct = 0; ct < CT; ct++) {
+        const int32_t at = wv * WC + ct * 16 + l15;
+        if (first + at >= n_cols) continue;
+        if (g == 0) part.put_stat(u.piece, at, mu[ct], l[ct]);
+        for (int d = 0; d < ND; d++) part.put(u.piece, at, d * 16 + g * 4, o[ct][d]);
     }
+    if (last_to_arrive(a, u, kvh)) join_pieces<T>(a, u, kvh, part);
 }
 
 // Column tiles: 16 (the four waves split the keys) where a sequence of the call has few columns on average, else the prompts'.
@@ -865,11 +873,12 @@ int64_t tiles_bound(const cache_shape & c, int C, int64_t n_seq, int64_t n_rows)
 template <typename T> int64_t parts_bound(const cache_shape & c, int C, int64_t n_seq, int64_t n_rows, int64_t width) {
     const int64_t most = (width * c.page_size + piece_min(C) / 2) / piece_min(C), units = (int64_t) (1.5f * MOST_UNITS * slots_of<T>(c.hd, C));
     if (most < 2) return 0;
+    static_assert(1.5f * MOST_UNITS * 1024 + 4096 <= COUNTERS, "a counter for each part: units and a round-up to K/V heads, of which there are 4096 at most");
     return std::min(tiles_bound(c, C, n_seq, n_rows) * most, (units + c.n_kv_head - 1) / c.n_kv_head);
 }
 template <typename T> int64_t work_bytes(const cache_shape & c, int64_t n_seq, int64_t n_rows, int64_t width) {
     const int C = columns_of<T>(c, n_seq, n_rows);
-    return parts_bound<T>(c, C, n_seq, n_rows, width) * c.n_kv_head * C * (c.hd + 2) * 4;
+    return COUNTERS * 8 + parts_bound<T>(c, C, n_seq, n_rows, width) * c.n_kv_head * C * (c.hd + 2) * 4;
 }
 
 template <typename T, int HD, int C>
@@ -880,12 +889,7 @@ hipError_t attend(const cache_shape & c, const cache_attn_args & a, hipStream_t 
     args.parts = parts;
     const int64_t blocks = (tiles + parts) * c.n_kv_head;
     if (blocks >= 1 << 24) return hipErrorInvalidConfiguration;      // threads of a launch are below 2^32
-    const hipError_t e = hipLaunchKernel(kernel, dim3((unsigned) blocks), dim3(NT), p, 0, s);
-    if (e != hipSuccess || !parts) return e;
-    // few tiles are split into many pieces: up to a workgroup for each column; many hardly
-    int split = (int) std::min<int64_t>(C, std::max<int64_t>(1, 512 / (tiles * c.n_kv_head)));
-    void * pj[] = {&args, &split};
-    return hipLaunchKernel((const void *) k_cache_join<T, HD, C>, dim3((unsigned) (tiles * c.n_kv_head * split)), dim3(NT), pj, 0, s);
+    return hipLaunchKernel(kernel, dim3((unsigned) blocks), dim3(NT), p, 0, s);
 }
 
 template <typename T, int HD>
@@ -902,8 +906,7 @@ hipError_t by_head(const cache_shape & c, const cache_attn_args & a, hipStream_t
 }  // namespace
 
 int64_t cache_attention_work_bytes(const cache_shape & c, int64_t n_seq, int64_t n_rows, int64_t width) {      // (rows of any type)
-    return std::max(std::max<int64_t>(16, work_bytes<float>(c, n_seq, n_rows, width)),
-                    std::max(work_bytes<_Float16>(c, n_seq, n_rows, width), work_bytes<__bf16>(c, n_seq, n_rows, width)));
+    return std::max({work_bytes<float>(c, n_seq, n_rows, width), work_bytes<_Float16>(c, n_seq, n_rows, width), work_bytes<__bf16>(c, n_seq, n_rows, width)});
 }
 
 hipError_t launch_cache_attention(const cache_shape & c, int type, const cache_attn_args & a, hipStream_t s) {

@@ -586,6 +586,34 @@ def test_same_pages_in_two_sequences(jlib):
         assert torch.equal(a, check(p, q, [0, 1, 2, 3], [4000] * 3, table, "f32"))
 
 
+def test_one_work_space_for_calls_of_many_shapes(jlib):
+    """One work space, used by one call after another and for other things between: nothing in it matters to the next call."""
+    rng = np.random.default_rng(17)
+    calls, first = [], []
+    for kind, kvh, group, hd, lens, rows in (("f16", 2, 4, 128, [5000, 40, 1300], 1), ("f32", 4, 1, 64, [2500, 900], 200), ("bf16", 1, 8, 96, [3000, 3000], 40),
+                                             ("bf16", 1, 1, 32, [20000], 3), ("f16", 8, 1, 64, rng.integers(1, 3000, 70).tolist(), 2)):
+        p, table = filled(jlib, rng, kvh * group, kvh, hd, 64, lens)
+        start = (np.arange(len(lens) + 1) * rows).tolist()
+        calls.append((p, queries(rng, start[-1], kvh * group * hd, kind), start, lens, table, kind))
+    size = max(jlib.lib().jepa_amd_cache_work_bytes(C.byref(p.s), len(lens), q.shape[0], table.shape[1]) for p, q, _s, lens, table, _k in calls)
+    work = torch.zeros(size, dtype=torch.uint8, device="cuda")
+    for again in range(4):
+        for i, (p, q, start, lens, table, kind) in enumerate(calls):
+            if again == 1:
+                work.random_(0, 256)
+            if again == 2:
+                work.view(torch.int32)[:16384].random_(-2 ** 31, 2 ** 31 - 1)
+                work[7::8] = 0
+            out = torch.full_like(q, float("nan"))
+            torch.cuda.synchronize()
+            p.attend(q, ints(start), ints(lens), ints(table), kind, 1, out=out, work=work)
+            torch.cuda.synchronize()
+            if again == 0:
+                check(p, q, start, lens, table, kind)
+                first.append(out)
+            assert torch.equal(out, first[i]), (again, i)
+
+
 # ------------------------------------------------------------------------------------------------ together
 class Program:
     """The calls as a step-by-step program makes them, on one stream, its lengths and tables on the device throughout."""
