@@ -168,7 +168,9 @@ __device__ __forceinline__ float wave_max(float x) {      // (of values that are
 template <typename X>
 __device__ __forceinline__ X wave_add(X x) { return __builtin_bit_cast(X, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wave_scan(x)), 63)); }
 
-// Unit x of the call, for column tiles of C. Every thread gets it, in scalar registers; false past the last.
+// Unit x of the call, for column tiles of C. Every thread gets it, in scalar registers; false past the last. Sequences whose rows overlap
+// may have more units than the launch has workgroups: then nothing is computed, for a tile that only some of its pieces come to would
+// leave its counter in `work` short.
 // Up to 64 sequences each wave finds it by itself, a sequence a lane, and weighs a few piece lengths against each other; more are
 // dealt to the workgroup's threads.
 template <int C, int SLOTS>
@@ -202,26 +204,30 @@ __device__ __forceinline__ bool find_unit(const cache_attn_args & a, uint32_t x,
         const uint32_t pieces = (uint32_t) pieces_of(v, inv), n = tiles * pieces, parts = pieces > 1 ? tiles * pieces : 0u;
         const uint32_t upto = wave_scan(n), parts_upto = wave_scan(parts);
         const uint64_t mine = __ballot(x >= upto - n && x < upto);
-        if (!mine) return false;
+        if (!mine || (uint32_t) __builtin_amdgcn_readlane((int) upto, 63) > a.units) return false;
         const int i = __builtin_ctzll(mine);
         auto of = [&](uint32_t y) { return (uint32_t) __builtin_amdgcn_readlane((int) y, i); };
         set(u, {(int32_t) of((uint32_t) v.row0), (int32_t) of((uint32_t) v.rows), (int32_t) of((uint32_t) v.len)}, i, of(tiles), of(pieces),
             x - of(upto - n), of(parts_upto - parts));
         return true;
     }
-    __shared__ float keys4[NT / 64];
+    __shared__ float keys4[NT / 64], tiles4[NT / 64];
     __shared__ uint32_t sums[2][NT / 64];
     __shared__ struct { seq_view v; int seq; uint32_t tiles, pieces, at, part; } found;
     const int per = (a.n_seq + NT - 1) / NT, i0 = min(tid * per, a.n_seq), i1 = min(i0 + per, a.n_seq);
-    float keys = 0.0f;
+    float keys = 0.0f, all_tiles = 0.0f;
     for (int i = i0; i < i1; i++) {
         const seq_view v = view_of(a, i);
-        keys += (float) tiles_of<C>(v, group) * (float) v.len;
+        const float tiles = (float) tiles_of<C>(v, group);
+        keys += tiles * (float) v.len;
+        all_tiles += tiles;
     }
     keys = wave_add(keys);
-    if (lane == 0) keys4[wv] = keys;
+    all_tiles = wave_add(all_tiles);
+    if (lane == 0) { keys4[wv] = keys; tiles4[wv] = all_tiles; }
     if (tid == 0) found.seq = -1;
     __syncthreads();
+    if ((tiles4[0] + tiles4[1]) + (tiles4[2] + tiles4[3]) > 0x1p24f) return false;      // (more than any launch's; the sums below are 32 bits)
     const float inv = piece_inv<C>(((keys4[0] + keys4[1]) + (keys4[2] + keys4[3])) * (float) a.n_kv_head, MOST_UNITS * SLOTS);
     uint32_t mine = 0, parts = 0;
     for (int i = i0; i < i1; i++) {
@@ -233,6 +239,7 @@ __device__ __forceinline__ bool find_unit(const cache_attn_args & a, uint32_t x,
     uint32_t before = wave_scan(mine), parts_before = wave_scan(parts);
     if (lane == 63) { sums[0][wv] = before; sums[1][wv] = parts_before; }
     __syncthreads();
+    if (sums[0][0] + sums[0][1] + sums[0][2] + sums[0][3] > a.units) return false;
     for (int w = 0; w < wv; w++) { before += sums[0][w]; parts_before += sums[1][w]; }
     before -= mine;
     parts_before -= parts;
@@ -887,6 +894,7 @@ hipError_t attend(const cache_shape & c, const cache_attn_args & a, hipStream_t 
     void * p[] = {&args};
     const int64_t tiles = tiles_bound(c, C, a.n_seq, a.n_rows), parts = parts_bound<T>(c, C, a.n_seq, a.n_rows, a.width);
     args.parts = parts;
+    args.units = (uint32_t) (tiles + parts);
     const int64_t blocks = (tiles + parts) * c.n_kv_head;
     if (blocks >= 1 << 24) return hipErrorInvalidConfiguration;      // threads of a launch are below 2^32
     return hipLaunchKernel(kernel, dim3((unsigned) blocks), dim3(NT), p, 0, s);

@@ -155,6 +155,7 @@ struct cache_attn_args {
     float scale = 0;
     float * work = nullptr;
     int64_t parts = 0;      // set by the launcher: partial results that `work` holds
+    uint32_t units = 0;     // and its workgroups for each K/V head
 };
 int64_t cache_attention_work_bytes(const cache_shape & c, int64_t n_seq, int64_t n_rows, int64_t width);
 hipError_t launch_cache_attention(const cache_shape & c, int type, const cache_attn_args & a, hipStream_t s);

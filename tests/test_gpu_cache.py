@@ -546,6 +546,27 @@ def test_attention_row_starts_that_overlap(jlib):
             assert (out[12:] == 7).all() and not torch.isnan(out).any()
 
 
+@pytest.mark.parametrize("n_seq,kind", [(8, "f16"), (8, "f32"), (70, "f16"), (70, "bf16")])
+def test_row_starts_that_overlap_leave_the_work_space_usable(jlib, n_seq, kind):
+    """Overlapping rows ask for more pieces than the call launches; the next call in the same work space comes out as in a new one."""
+    rng = np.random.default_rng(23)
+    lens = rng.integers(1500, 2500, n_seq).tolist()
+    p, table = filled(jlib, rng, 2, 1, 64, 64, lens)
+    rows = 2 * n_seq
+    q = queries(rng, rows, 128, kind)
+    work = torch.zeros(jlib.lib().jepa_amd_cache_work_bytes(C.byref(p.s), n_seq, rows, table.shape[1]), dtype=torch.uint8, device="cuda")
+    start = list(range(0, rows + 1, 2))
+    want = check(p, q, start, lens, table, kind)
+    out = torch.empty_like(q)
+    for bad in ([rows * (i % 2) for i in range(n_seq + 1)], [max(rows - 3 * i, 0) if i % 2 else 0 for i in range(n_seq + 1)]):
+        p.attend(q, ints(bad), ints(lens), ints(table), kind, 1, out=out, work=work)
+        torch.cuda.synchronize()
+        out.fill_(float("nan"))
+        p.attend(q, ints(start), ints(lens), ints(table), kind, 1, out=out, work=work)
+        torch.cuda.synchronize()
+        assert torch.equal(out.double(), want)
+
+
 def test_attention_many_sequences(jlib):
     rng = np.random.default_rng(11)
     lens = rng.integers(0, 60, 1500).tolist()
