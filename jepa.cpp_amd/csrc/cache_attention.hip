@@ -864,12 +864,20 @@ __global__ __launch_bounds__(NT, groups_of<T>(HD, prompt<T>::columns)) void k_ca
     if (last_to_arrive(a, u, kvh)) join_pieces<T>(a, u, kvh, part);
 }
 
-// Column tiles: 16 (the four waves split the keys) where a sequence of the call has few columns on average, else the prompts'.
-// Measured, us of a call of 16 sequences of 1500 tokens, 8 K/V heads of 128, 16 against the prompts' tiles: 96 columns bf16 37 / 41, f16
-// 37 / 57, f32 45 / 54; 128 columns 46 / 46, 46 / 57, 57 / 57; 192 columns 66 / 62, 66 / 71, 82 / 86; 256 columns 85 / 63, 85 / 85,
-// 106 / 116; 512 columns 160 / 79, 160 / 122, 198 / 164.
+// Column tiles: 16 (the four waves split the keys) or the prompts'. A prompt's workgroup does more for each key that it stages, so
+// it is the faster one where sequences have many columns, and with fewer where the call's columns over all K/V heads (its heads of
+// rows) fill the chip, less what its last tiles leave empty; else 16 columns are, split into fewer pieces. Measured, us of a call,
+// 16 columns / prompts', rows of 8 K/V heads of 128:
+//   1 sequence of 16000 tokens: 256 columns bf16 56 / 98, f16 57 / 107, f32 70 / 89; 1024 columns 181 / 109, 181 / 164, 231 / 209;
+//   16 of 1500 (128 columns are 16k heads of rows): 128 columns 42 / 47, 43 / 47, 54 / 57; 256 columns 80 / 65, 80 / 88, 101 / 88;
+//   64 of 700 (64 columns are 33k): 32 columns 30 / 33, 30 / 39, 37 / 46; 64 columns 53 / 40, 52 / 43, 63 / 53; 96 columns 74 / 43,
+//   73 / 64, 91 / 86; 256 of 500: 16 columns 55 / 97, 55 / 66, 64 / 89; 32 columns 94 / 99, 94 / 78, 110 / 107;
+//   8 of 1032 to 2064 with 258 columns (33k, 20 % of five tiles empty), 16 K/V heads of 64, f32: 78 / 89.
 template <typename T> int columns_of(const cache_shape & c, int64_t n_seq, int64_t n_rows) {
-    return n_rows * (c.n_head / c.n_kv_head) <= (prompt<T>::scaled ? 128 : 256) * n_seq ? 16 : prompt<T>::columns;
+    constexpr int64_t C = prompt<T>::columns, full = prompt<T>::scaled ? 16000 : 32000, least = 24, many = prompt<T>::scaled ? 256 : 768;
+    const int64_t columns = n_rows * (c.n_head / c.n_kv_head), of_tiles = std::max<int64_t>(n_seq, 1) * C, with_empty = (columns + of_tiles - 1) / of_tiles * of_tiles;
+    const bool prompts = columns > many * n_seq || (columns > least * n_seq && (double) n_rows * c.n_head * columns > (double) full * with_empty);
+    return prompts ? (int) C : 16;
 }
 
 // bounds on the column tiles of all sequences, and on the pieces that the ones split into several have

@@ -405,6 +405,28 @@ def test_attention_prompt(jlib, kind, rows, length, kvh, group, hd):
 
 
 @pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("rows,length,kvh,group,hd,block", [(800, 5000, 1, 1, 64, 1), (790, 3100, 2, 1, 96, 0), (400, 7000, 1, 2, 32, 1), (270, 9000, 1, 3, 128, 90)])
+def test_attention_prompt_in_pieces(jlib, kind, rows, length, kvh, group, hd, block):
+    """Few tiles of a prompt's columns over many keys: its pieces are joined."""
+    rng = np.random.default_rng(24)
+    p, table = filled(jlib, rng, kvh * group, kvh, hd, 64, [length, 70])
+    start = [0, rows, rows + 1]
+    check(p, queries(rng, rows + 1, kvh * group * hd, kind), start, [length, 70], table, kind, block)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("kvh,group", [(16, 4), (4, 16)])
+def test_attention_many_short_prompts(jlib, kind, kvh, group):
+    """Sequences of few columns each that fill the chip together, some of one row or none."""
+    rng = np.random.default_rng(25)
+    lens = rng.integers(1, 260, 70).tolist()
+    rows = [min(n, int(r)) for n, r in zip(lens, rng.integers(0, 30, 70))]
+    start = [0] + np.cumsum(rows).tolist()
+    p, table = filled(jlib, rng, kvh * group, kvh, 32, 32, lens)
+    check(p, queries(rng, start[-1], kvh * group * 32, kind), start, lens, table, kind, 1)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
 def test_attention_long(jlib, kind):
     """Long sequences beside short ones: the keys of one row are split over many workgroups and joined."""
     rng = np.random.default_rng(3)
