@@ -357,16 +357,21 @@ __device__ __forceinline__ void join_pieces(const cache_attn_args & a, const uni
 
 // The column's query row to f16: scaled by a power of two to a largest value in [1, 2), one term or two; c: what a product of it with a
 // key is multiplied by to be an exponent of 2 (never negative: the row carries the scale's sign)
-template <typename T, int HD, int TERMS>
-__device__ __forceinline__ void load_query(const cache_attn_args & a, const seq_view & sv, int kvh, int group, int32_t col, int g, half8_t (*q)[TERMS], float & c) {
-    constexpr int NB = HD / 32;
-    typedef T vec __attribute__((ext_vector_type(8)));
+template <typename T> struct vec8 { typedef T t __attribute__((ext_vector_type(8))); };
+template <typename T, int HD>
+__device__ __forceinline__ void fetch_query(const cache_attn_args & a, const seq_view & sv, int kvh, int group, int32_t col, int g, typename vec8<T>::t * y) {
     const T * p = (const T *) a.q + (sv.row0 + (int64_t) ((uint32_t) col / (uint32_t) group)) * a.ldq + ((int64_t) kvh * group + (uint32_t) col % (uint32_t) group) * HD + g * 8;
+#pragma unroll
+    for (int b = 0; b < HD / 32; b++) y[b] = *(const typename vec8<T>::t *) (p + b * 32);
+}
+template <typename T, int HD, int TERMS>
+__device__ __forceinline__ void turn_query(const cache_attn_args & a, const typename vec8<T>::t * y, half8_t (*q)[TERMS], float & c) {
+    constexpr int NB = HD / 32;
     float8_t x[NB];
     float top = 0.0f;
 #pragma unroll
     for (int b = 0; b < NB; b++) {
-        x[b] = __builtin_convertvector(*(const vec *) (p + b * 32), float8_t);
+        x[b] = __builtin_convertvector(y[b], float8_t);
         for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(x[b][j]));
     }
     const uint32_t ex = __float_as_uint(col_max(top)) >> 23;
@@ -479,6 +484,10 @@ __global__ __launch_bounds__(NT, groups_of<T>(HD, 16)) void k_cache_attention(ca
     auto load_pages = [&](int32_t key) { return table[min(key / 16 + (lane & 3), last_strip) >> page_shift]; };
     uint32_t kn[4][NB], vn[4][NB], sn[4], bad_n = 0;      // the tile's codes and scales, in flight
     int pages = k0 < kend ? load_pages(k0) : 0;            // page numbers of the next one, in lanes 0 to 3
+    const int32_t col = min(col0 + l15, n_cols - 1), lim = visible(col);
+    typename vec8<T>::t y[NB];      // the query row, fetched while the first page numbers are
+    fetch_query<T, HD>(a, sv, kvh, group, col, g, y);
+    __builtin_amdgcn_sched_barrier(0);
     // a strip as a buffer resource (no bytes past the end of this wave's keys: such loads give 0 without a memory access)
     auto strip_of = [&](int32_t key, int pages, int t, uint32_t & bad) {
         const int strip = min(key / 16 + t, last_strip);
@@ -511,10 +520,9 @@ __global__ __launch_bounds__(NT, groups_of<T>(HD, 16)) void k_cache_attention(ca
         load_k();
         pages = pages_after;
     }
-    const int32_t col = min(col0 + l15, n_cols - 1), lim = visible(col);
     float c;
     half8_t q[NB][TERMS];
-    load_query<T, HD, TERMS>(a, sv, kvh, group, col, g, q, c);
+    turn_query<T, HD, TERMS>(a, y, q, c);
     float4_t o[ND];
     float mu = -INFINITY, l = 0.0f;      // mu: -inf before the first key
     for (int d = 0; d < ND; d++) o[d] = float4_t{0, 0, 0, 0};
@@ -727,7 +735,11 @@ __global__ __launch_bounds__(NT, groups_of<T>(HD, prompt<T>::columns)) void k_ca
     half8_t q[CT][NB][TERMS];
     int32_t lim[CT];
 #pragma unroll
-    for (int ct = 0; ct < CT; ct++) load_query<T, HD, TERMS>(a, sv, kvh, group, min(col0 + ct * 16 + l15, n_cols - 1), g, q[ct], c[ct]);
+    for (int ct = 0; ct < CT; ct++) {
+        typename vec8<T>::t y[NB];
+        fetch_query<T, HD>(a, sv, kvh, group, min(col0 + ct * 16 + l15, n_cols - 1), g, y);
+        turn_query<T, HD, TERMS>(a, y, q[ct], c[ct]);
+    }
 #pragma unroll
     for (int ct = 0; ct < CT; ct++) lim[ct] = visible(min(col0 + ct * 16 + l15, n_cols - 1));
     float4_t o[CT][ND];
