@@ -11,17 +11,22 @@
 //   - q is scaled by a power of two to a largest value in [1, 2) (exact) and taken as one f16 (f16 and bf16 rows: below
 //     2^-14 of the row's largest value they lose bits, 2^-25 of it at most) or as the sum of two (f32 rows: 22 bits);
 //   - dv goes into the weights: P'_jb = p_j dv_jb in f32, rounded to one f16 (16-bit rows: half a step of f16, 2^-11
-//     relative at most, as the output's own rounding is or finer, and averaged over the keys) or the sum of two (f32 rows). V itself then holds no NaN whatever a
-//     masked token contains. mu is the running maximum of the scores plus the exponent of the tile's largest dv, less 6, and moves
-//     when a tile passes it by more than 2^8: so P' is below 2^14, f16's range, however small or large the values are.
+//     relative at most, as the output's own rounding is or finer, and averaged over the keys) or the sum of two (f32 rows). V
+//     itself then holds no NaN whatever a masked token contains. mu is the running maximum of the scores plus the exponent of the
+//     tile's largest dv, less 6, and moves when a tile passes it by more than 2^8: so P' is below 2^14, f16's range, however small or
+//     large the values are.
 // Scores, maxima, sums and accumulators are f32.
 //
-// Layout. A wave owns 16 CT columns and sweeps its keys in tiles of 64 (4 strips), by itself: no barrier in the loop. K
-// codes go from memory to the registers of the MFMA's A operand (the strip's layout is the operand's); V codes and scales go
-// through the wave's own LDS, because V^T needs 16 keys of one dimension in a lane: ds_read_b64_tr_b4 turns 16 x 16
-// nibbles around. The next tile's loads (and the page numbers of the one after) are in flight while a tile is computed.
-// The four waves of a workgroup share one tile of columns and split its keys (KW 4, few columns: joined in LDS at the end), or
-// have a tile of columns each (KW 1, prompts: the K/V they share comes from the CU's cache).
+// Few columns (k_cache_attention). The four waves of a workgroup share 16 columns and split the keys, a wave sweeping its tiles of 64
+// (4 strips) by itself: no barrier in the loop, the waves' sums are joined in LDS at the end. K codes go from memory to the registers
+// of the MFMA's A operand (the strip's layout is the operand's); V codes and scales go through the wave's own LDS, because V^T needs
+// 16 keys of one dimension in a lane: ds_read_b64_tr_b4 turns 16 x 16 nibbles around. The next tile's loads (and the page numbers of
+// the one after) are in flight while a tile is computed. Measured: 64 requests of 200 to 8000 tokens, f16, 32 heads over 8 of
+// 128, 63.4 us (259 MB, 4.1 TB/s; a large copy reaches 5.1); 2 contexts of 90000 to 131000 tokens, bf16, 64 heads over 8, 60.8 us (253 MB,
+// 4.15 TB/s). About 8 us of a call are its start (find_unit, the query, the first tile's way from memory, one after the other) and 2 its
+// end, then memory bounds it, with the VALU at 55 % (unpacking codes, scales, softmax). With several tiles of columns a sequence
+// the VALU bounds it: 8 sequences of 258 f32 rows, 77 us, 76 % of its time.
+// Many columns (k_cache_prompt): see there.
 //
 // Work. A unit is (sequence, tile of columns, piece of its keys, K/V head). The piece length is the same for all sequences
 // of a call and chosen on the device from the sum of their lengths, so that long sequences are split and short ones are not and
@@ -640,9 +645,11 @@ __global__ __launch_bounds__(NT, groups_of<T>(HD, 16)) void k_cache_attention(ca
 // ds_read_b64_tr_b16 turns around. The next tile's codes are in flight meanwhile.
 // For bf16 rows the scales go in with the codes (K and V rounded to f16, 2^-11 relative, against bf16's half step of 2^-8): no
 // work per score is left but the softmax, and two column tiles a wave with two LDS buffers (one barrier a tile, two
-// workgroups a CU) are best: 17.6k prompt rows of 32 x 128 take 0.84 ms, one column tile 1.04.
+// workgroups a CU) are best: 17.6k prompt rows of 32 x 128 take 0.81 ms, one column tile 1.04.
 // f16 and f32 rows keep codes exact and scales in 32 bits as above, twice the work per score; what hides its latencies best is four
-// workgroups a CU, of one column tile a wave and one buffer: 2000 f16 rows over 16000 tokens take 0.97 ms, two column tiles 1.14.
+// workgroups a CU, of one column tile a wave and one buffer: 2000 f16 rows over 16000 tokens take 0.96 ms, two column tiles 1.14.
+// Rates: 860 TFLOP/s for bf16 (three quarters of an 8192^3 product's 1130; the LDS reads of K and V take as many cycles as the MFMAs)
+// and 510 for f16 (32 heads over 4: the VALU, 63 % of the time, 12 instructions for each MFMA, most of them scales).
 template <typename T> struct prompt {
     static constexpr bool scaled = std::is_same<T, __bf16>::value;
     static constexpr int tiles = scaled ? 2 : 1, bufs = scaled ? 2 : 1, columns = 64 * tiles;

@@ -4,9 +4,10 @@
 // The pages that sequence i takes are entries [P(i-1), P(i)) behind the ring's head, P the inclusive sum of the pages
 // needed; it is admitted while P(i) fits the free count. Everything is a prefix sum over the sequences and then
 // independent work per page and per row, so one workgroup of 16 waves does it: sums in registers and LDS. What it costs is
-// latency, one global load after another (256 sequences of one token: 5 us), so the thread of a sequence also writes its
-// rows' slots where every sequence has a few; else pages and rows are dealt to all threads by a binary search in the sums, and
-// from PLAN_ROWS rows on to a second launch, which finds from what the first one wrote which page a row is in.
+// latency, one global load after another (256 sequences of one token 5 us; 238k rows of prompts 4.5 and 4.8 us), so the
+// thread of a sequence also writes its rows' slots where every sequence has a few; else pages and rows are dealt to all
+// threads by a binary search in the sums, and from PLAN_ROWS rows on to a second launch, which finds from what the first
+// one wrote which page a row is in.
 #include "cache_dev.h"
 #include "common.h"
 #include "kernels.h"
