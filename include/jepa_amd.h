@@ -190,7 +190,8 @@ int64_t jepa_amd_cache_page_bytes(const jepa_amd_cache_shape * shape);
 /* One step's bookkeeping for n_seq sequences (up to 4096), n_rows packed rows and tables of table_width pages (2^30 tokens at most).
  *   len [n_seq]          tokens that each sequence has in the cache
  *   n_new [n_seq]        tokens that come to it in this step; below zero, that many are dropped from its end
- *   table [n_seq][table_width]   in and out: pages for the new tokens are written in, dropped pages' entries set to -1
+ *   table [n_seq][table_width]   in and out: pages for the new tokens are written in, dropped pages' entries set to -1 (a page
+ *                        that several rows of the table name is given back by each that drops it: let one of them drop it)
  *   ring [n_pages], free_in [2]  the free pages: free_in[1] of them from ring[free_in[0]] on, around the end. Pages are
  *                        taken at the front in sequence order; dropped pages are put behind the last, in sequence and table
  *                        order, and not taken again in the same step. A caller starts with ring = 0 .. n_pages - 1 and (0, n_pages).
@@ -222,8 +223,9 @@ int jepa_amd_cache_read(int device, const jepa_amd_cache_shape * shape, const vo
  * q and out hold rows of n_head * head_dim values of `type`; keys and values enter as they are held, sums and the softmax
  * are f32, and f32 rows are computed to f32 accuracy. Tokens whose page is not one of the cache's are not read; a row that
  * reads nothing comes out zero; rows behind the last sequence (row_start[n_seq] on) are left as they are.
- * `work` is jepa_amd_cache_work_bytes() bytes of device memory (16-byte aligned) with nothing kept in it between calls: calls
- * that may overlap on the device (on two streams, in two graphs) need one each. */
+ * row_start ascends; a call whose rows overlap writes some of them or none.
+ * `work` is jepa_amd_cache_work_bytes() bytes of device memory (16-byte aligned) with nothing kept in it between calls; what
+ * the largest step needs does for smaller ones. Calls that may overlap on the device (on two streams, in two graphs) need one each. */
 int64_t jepa_amd_cache_work_bytes(const jepa_amd_cache_shape * shape, int64_t n_seq, int64_t n_rows, int64_t table_width);
 int jepa_amd_cache_attention(int device, const jepa_amd_cache_shape * shape, const void * cache, int type, const void * q, int64_t q_stride,
                              int64_t n_seq, int64_t n_rows, const int32_t * row_start, const int32_t * kv_len, const int32_t * table,

@@ -892,11 +892,20 @@ __global__ __launch_bounds__(NT, groups_of<T>(HD, prompt<T>::columns)) void k_ca
 //   64 of 700 (64 columns are 33k): 32 columns 30 / 33, 30 / 39, 37 / 46; 64 columns 53 / 40, 52 / 43, 63 / 53; 96 columns 74 / 43,
 //   73 / 64, 91 / 86; 256 of 500: 16 columns 55 / 97, 55 / 66, 64 / 89; 32 columns 94 / 99, 94 / 78, 110 / 107;
 //   8 of 1032 to 2064 with 258 columns (33k, 20 % of five tiles empty), 16 K/V heads of 64, f32: 78 / 89.
+template <typename T> struct column_rule {
+    static constexpr int64_t C = prompt<T>::columns, full = prompt<T>::scaled ? 16000 : 32000, least = 24, many = prompt<T>::scaled ? 256 : 768;
+};
 template <typename T> int columns_of(const cache_shape & c, int64_t n_seq, int64_t n_rows) {
-    constexpr int64_t C = prompt<T>::columns, full = prompt<T>::scaled ? 16000 : 32000, least = 24, many = prompt<T>::scaled ? 256 : 768;
-    const int64_t columns = n_rows * (c.n_head / c.n_kv_head), of_tiles = std::max<int64_t>(n_seq, 1) * C, with_empty = (columns + of_tiles - 1) / of_tiles * of_tiles;
-    const bool prompts = columns > many * n_seq || (columns > least * n_seq && (double) n_rows * c.n_head * columns > (double) full * with_empty);
-    return prompts ? (int) C : 16;
+    typedef column_rule<T> R;
+    const int64_t columns = n_rows * (c.n_head / c.n_kv_head), of_tiles = std::max<int64_t>(n_seq, 1) * R::C, with_empty = (columns + of_tiles - 1) / of_tiles * of_tiles;
+    const bool prompts = columns > R::many * n_seq || (columns > R::least * n_seq && (double) n_rows * c.n_head * columns > (double) R::full * with_empty);
+    return prompts ? (int) R::C : 16;
+}
+// whether columns_of can be the prompts' for this many rows or fewer, of any number of sequences
+template <typename T> bool prompts_within(const cache_shape & c, int64_t n_rows) {
+    typedef column_rule<T> R;
+    const int64_t columns = n_rows * (c.n_head / c.n_kv_head);
+    return columns > R::many || (columns > R::least && n_rows * c.n_head > R::full);
 }
 
 // bounds on the column tiles of all sequences, and on the pieces that the ones split into several have
@@ -910,9 +919,10 @@ template <typename T> int64_t parts_bound(const cache_shape & c, int C, int64_t 
     static_assert(1.5f * MOST_UNITS * 1024 + 4096 <= COUNTERS, "a counter for each part: units and a round-up to K/V heads, of which there are 4096 at most");
     return std::min(tiles_bound(c, C, n_seq, n_rows) * most, (units + c.n_kv_head - 1) / c.n_kv_head);
 }
+// (what any call of no more rows, sequences and pages needs: a program asks once, for its largest step)
 template <typename T> int64_t work_bytes(const cache_shape & c, int64_t n_seq, int64_t n_rows, int64_t width) {
-    const int C = columns_of<T>(c, n_seq, n_rows);
-    return COUNTERS * 8 + parts_bound<T>(c, C, n_seq, n_rows, width) * c.n_kv_head * C * (c.hd + 2) * 4;
+    auto bytes = [&](int C) { return parts_bound<T>(c, C, n_seq, n_rows, width) * c.n_kv_head * C * (c.hd + 2) * 4; };
+    return COUNTERS * 8 + std::max(bytes(16), prompts_within<T>(c, n_rows) ? bytes(prompt<T>::columns) : 0);
 }
 
 template <typename T, int HD, int C>

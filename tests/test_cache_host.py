@@ -111,3 +111,17 @@ def test_work_space_too_small_is_named():
     L.jepa_error_reset()
     assert L.jepa_amd_cache_attention(0, _shape(), P, 0, P, 512, 2, 3, P, P, P, 4, 0.125, 1, P, 512, P, need - 1, None) == -1
     assert str(need) in _lib.error_text()
+
+
+@pytest.mark.parametrize("heads,kvh,hd,page", [(1, 1, 128, 64), (32, 8, 128, 64), (40, 8, 96, 32), (16, 16, 64, 16), (64, 1, 32, 256)])
+def test_work_space_for_the_largest_step_does_for_smaller_ones(heads, kvh, hd, page):
+    """The bytes never fall where one of the sizes grows: a program asks once."""
+    s = _shape(n_head=heads, n_kv_head=kvh, head_dim=hd, page_size=page)
+    need = lambda *a: _lib.lib().jepa_amd_cache_work_bytes(s, *a)  # noqa: E731
+    for n_seq in (1, 2, 7, 64, 300):
+        for width in (1, 4, 16, 100, 2000):
+            rows = sorted({1, 2, 5, 24, 25, 63, 64, 65, 100, 192, 193, 256, 257, 500, 768, 769, 800, 1000, 1001, 2000, 4000, 20000, 32001, 100000})
+            got = [need(n_seq, r, width) for r in rows]
+            assert got == sorted(got), (n_seq, width, list(zip(rows, got)))
+            for r, b in zip(rows, got):
+                assert b >= need(max(1, n_seq // 2), r, width) and b >= need(n_seq, r, max(1, width // 2)), (n_seq, r, width)
