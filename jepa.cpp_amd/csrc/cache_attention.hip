@@ -647,9 +647,11 @@ __global__ __launch_bounds__(NT, groups_of<T>(HD, 16)) void k_cache_attention(ca
 // work per score is left but the softmax, and two column tiles a wave with two LDS buffers (one barrier a tile, two
 // workgroups a CU) are best: 17.6k prompt rows of 32 x 128 take 0.81 ms, one column tile 1.04.
 // f16 and f32 rows keep codes exact and scales in 32 bits as above, twice the work per score; what hides its latencies best is four
-// workgroups a CU, of one column tile a wave and one buffer: 2000 f16 rows over 16000 tokens take 0.96 ms, two column tiles 1.14.
+// workgroups a CU, of one column tile a wave and one buffer: 2000 f16 rows over 16000 tokens take 0.95 ms, two column tiles 1.14.
+// Rows of both are padded by 32 bytes: of 16, 32 and 48 for either this has the fewest bank conflicts (f16 954 us; 16 and 32 971, 32 and 48
+// 966, 48 and 32 970).
 // Rates: 860 TFLOP/s for bf16 (three quarters of an 8192^3 product's 1130; the LDS reads of K and V take as many cycles as the MFMAs)
-// and 510 for f16 (32 heads over 4: the VALU, 63 % of the time, 12 instructions for each MFMA, most of them scales).
+// and 515 for f16 (32 heads over 4: the LDS and the VALU, each 60 % of the time, the latter 12 instructions for each MFMA, most of them scales).
 template <typename T> struct prompt {
     static constexpr bool scaled = std::is_same<T, __bf16>::value;
     static constexpr int tiles = scaled ? 2 : 1, bufs = scaled ? 2 : 1, columns = 64 * tiles;
@@ -658,7 +660,7 @@ template <typename T, int HD>
 __global__ __launch_bounds__(NT, groups_of<T>(HD, prompt<T>::columns)) void k_cache_prompt(cache_attn_args a) {
     constexpr bool SCALED = prompt<T>::scaled;
     constexpr int CT = prompt<T>::tiles, BUFS = prompt<T>::bufs, NB = HD / 32, ND = HD / 16, TERMS = sizeof(T) == 4 ? 2 : 1, WC = 16 * CT, C = 4 * WC;
-    constexpr int KS = 2 * HD + 16, VS = 2 * HD + 32, SCALES = TILE * (KS + VS), BUF = SCALES + (SCALED ? 0 : 8 * HD);
+    constexpr int KS = 2 * HD + 32, VS = 2 * HD + 32, SCALES = TILE * (KS + VS), BUF = SCALES + (SCALED ? 0 : 8 * HD);
     __shared__ __attribute__((aligned(16))) unsigned char lds[BUFS * BUF];
     __shared__ uint32_t tile_dmax[BUFS][4], tile_bad[BUFS][4];
     unit u;
@@ -682,7 +684,7 @@ __global__ __launch_bounds__(NT, groups_of<T>(HD, prompt<T>::columns)) void k_ca
     auto load_page = [&](int32_t key) { return table[min(key / 16 + wv, last_strip) >> page_shift]; };
     uint32_t kx[NB], vx[NB], sx[SCALED ? NB + 2 : 1], bad = 0;
     int32_t page_n = k0 < kend ? load_page(k0) : 0;
-    const int vb0 = (lane & 3) * NB >> 2, vb1 = ((lane & 3) * NB + NB - 1) >> 2;      // blocks of the lane's first and last V word
+    const int vb0 = g * NB >> 2, vb1 = (g * NB + NB - 1) >> 2;      // blocks of the lane's first and last V word
     auto load = [&](int32_t key) {
         const int strip = min(key / 16 + wv, last_strip);
         int64_t page = __builtin_amdgcn_readfirstlane(page_n);
@@ -690,12 +692,12 @@ __global__ __launch_bounds__(NT, groups_of<T>(HD, prompt<T>::columns)) void k_ca
         if (bad) page = 0;
         const brsrc s = make_brsrc(a.cache + ((page * a.n_kv_head + kvh) * strips_of_page + (strip & (strips_of_page - 1))) * (18 * HD), key < kend ? 18 * HD : 0);
         load_words<NB>(kx, s, lane * (4 * NB), 0);
-        load_words<NB>(vx, s, lane * (4 * NB), 8 * HD);
+        load_words<NB>(vx, s, l15 * (16 * NB) + g * (4 * NB), 8 * HD);
         if constexpr (SCALED) {
 #pragma unroll
             for (int b = 0; b < NB; b++) sx[b] = __builtin_amdgcn_raw_buffer_load_b16(s, cache_k_scale(l15, b, HD), 0, 0);
-            sx[NB] = __builtin_amdgcn_raw_buffer_load_b16(s, cache_v_scale(lane >> 2, vb0, HD), 0, 0);
-            sx[NB + 1] = NB == 3 ? (uint32_t) __builtin_amdgcn_raw_buffer_load_b16(s, cache_v_scale(lane >> 2, vb1, HD), 0, 0) : sx[NB];
+            sx[NB] = __builtin_amdgcn_raw_buffer_load_b16(s, cache_v_scale(l15, vb0, HD), 0, 0);
+            sx[NB + 1] = NB == 3 ? (uint32_t) __builtin_amdgcn_raw_buffer_load_b16(s, cache_v_scale(l15, vb1, HD), 0, 0) : sx[NB];
         } else {
             load_words<1>(sx, s, 16 * HD + lane * 4, 0);      // (0 past the strip's scales, from lane HD / 2 on)
         }
@@ -709,20 +711,20 @@ __global__ __launch_bounds__(NT, groups_of<T>(HD, prompt<T>::columns)) void k_ca
     };
     auto stage = [&](int32_t key, int buf) {      // the strip that load(key) brought
         unsigned char * const l = lds + buf * BUF;
-        const bool k_ok = key + wv * 16 + l15 < kend && !bad, v_ok = key + wv * 16 + (lane >> 2) < kend && !bad;
+        const bool ok = key + wv * 16 + l15 < kend && !bad;
 #pragma unroll
         for (int b = 0; b < NB; b++) {
             half8_t x = codes8(kx[b], k1024);
-            if constexpr (SCALED) x = scale2(x, k_ok ? sx[b] : 0u);
+            if constexpr (SCALED) x = scale2(x, ok ? sx[b] : 0u);
             *(half8_t *) (l + (wv * 16 + l15) * KS + b * 64 + g * 16) = x;
         }
 #pragma unroll
         for (int b = 0; b < NB; b++) {
-            const int w = (lane & 3) * NB + b;
+            const int w = g * NB + b;
             half8_t x = codes8(vx[b], k1024);
             x = half8_t{x[0], x[2], x[4], x[6], x[1], x[3], x[5], x[7]};      // dims in order
-            if constexpr (SCALED) x = scale2(x, !v_ok ? 0u : w >> 2 == vb0 ? sx[NB] : sx[NB + 1]);
-            *(half8_t *) (l + TILE * KS + (wv * 16 + (lane >> 2)) * VS + w * 16) = x;
+            if constexpr (SCALED) x = scale2(x, !ok ? 0u : w >> 2 == vb0 ? sx[NB] : sx[NB + 1]);
+            *(half8_t *) (l + TILE * KS + (wv * 16 + l15) * VS + w * 16) = x;
         }
         uint32_t dmax = 0;
         if constexpr (!SCALED) {
