@@ -6,15 +6,17 @@
 // column in a lane (16x16x32 f16 MFMA, 16 keys x 16 columns), so the softmax is lane work and P^T feeds the second product,
 // O^T += V^T P^T, from its registers.
 //
-// Numerics. 4-bit codes are exact in f16, so both products run on codes and every scale is applied in 32 bits:
-//   - the MFMA's depth (32) is one q4_0 block: its sum times dk, in f32, added over the blocks of a head;
+// Numerics. 4-bit codes are exact in f16:
+//   - the first product runs on K's codes: the MFMA's depth (32) is one q4_0 block, whose sum is multiplied by dk in f32 and added over
+//     the blocks of a head;
 //   - q is scaled by a power of two to a largest value in [1, 2) (exact) and taken as one f16 (f16 and bf16 rows: below
 //     2^-14 of the row's largest value they lose bits, 2^-25 of it at most) or as the sum of two (f32 rows: 22 bits);
-//   - dv goes into the weights: P'_jb = p_j dv_jb in f32, rounded to one f16 (16-bit rows: half a step of f16, 2^-11
-//     relative at most, as the output's own rounding is or finer, and averaged over the keys) or the sum of two (f32 rows). V
-//     itself then holds no NaN whatever a masked token contains. mu is the running maximum of the scores plus the exponent of the
-//     tile's largest dv, less 6, and moves when a tile passes it by more than 2^8: so P' is below 2^14, f16's range, however small or
-//     large the values are.
+//   - a value dv (cv - 8) has 15 bits at most and is the sum of two f16, exactly (the second one's last bit is dv's, 2^-24 or more);
+//   - weights are rounded to one f16 (16-bit rows: half a step of f16, 2^-11 relative at most, as the output's own rounding is or finer,
+//     and averaged over the keys) or to the sum of two (f32 rows; the product of both second terms, 2^-22, is left out). mu is the running
+//     maximum of the scores less 10, and moves when a tile passes it by more than 2^15: so the largest weight is between 2^10 and 2^15, and
+//     f16's smallest step is 2^-34 of it or less. Nothing of V takes part in that: a token that a row must not read cannot change
+//     the row, and the blocks of a head may differ in size.
 // Scores, maxima, sums and accumulators are f32.
 //
 // Few columns (k_cache_attention). The four waves of a workgroup share 16 columns and split the keys, a wave sweeping its tiles of 64
@@ -94,16 +96,6 @@ __device__ __forceinline__ float col_sum(float x) {
     x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
     r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
-__device__ __forceinline__ uint32_t wave_umax(uint32_t x) {
-    x = max(x, (uint32_t) __builtin_amdgcn_update_dpp(0, (int) x, 0xb1, 0xf, 0xf, false));       // quad_perm 1 0 3 2
-    x = max(x, (uint32_t) __builtin_amdgcn_update_dpp(0, (int) x, 0x4e, 0xf, 0xf, false));       // quad_perm 2 3 0 1
-    x = max(x, (uint32_t) __builtin_amdgcn_update_dpp(0, (int) x, 0x141, 0xf, 0xf, false));      // row_half_mirror
-    x = max(x, (uint32_t) __builtin_amdgcn_update_dpp(0, (int) x, 0x140, 0xf, 0xf, false));      // row_mirror
-    auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
-    x = max((uint32_t) r[0], (uint32_t) r[1]);
-    r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
-    return (uint32_t) __builtin_amdgcn_readfirstlane((int) max((uint32_t) r[0], (uint32_t) r[1]));
 }
 // N words per lane of a buffer
 template <int N>
@@ -395,7 +387,7 @@ __device__ __forceinline__ void turn_query(const cache_attn_args & a, const type
 
 // One column's scores of a tile, s[t][r] of key + 16 t + r, to weights; its maximum, sum and accumulators follow
 template <bool MASKED, int ND>
-__device__ __forceinline__ void softmax_step(float4_t * s, int32_t key, int32_t lim, uint32_t hidden, float c, float dexp, float & mu, float & l, float4_t * o) {
+__device__ __forceinline__ void softmax_step(float4_t * s, int32_t key, int32_t lim, uint32_t hidden, float c, float & mu, float & l, float4_t * o) {
     if constexpr (MASKED) {
 #pragma unroll
         for (int t = 0; t < 4; t++)
@@ -408,10 +400,10 @@ __device__ __forceinline__ void softmax_step(float4_t * s, int32_t key, int32_t 
     for (int t = 0; t < 4; t++)
 #pragma unroll
         for (int r = 0; r < 4; r++) top = fmaxf(top, s[t][r]);
-    const float want = col_max(top) * c + dexp;
-    const bool move = want - mu > 14.0f;
+    const float want = col_max(top) * c;
+    const bool move = want - mu > 15.0f;
     if (__any(move)) {
-        const float to = move ? want - 6.0f : mu;
+        const float to = move ? want - 10.0f : mu;
         const float f = move ? __builtin_amdgcn_exp2f(mu - to) : 1.0f;
         mu = to;
         l *= f;
@@ -433,17 +425,26 @@ __device__ __forceinline__ void softmax_step(float4_t * s, int32_t key, int32_t 
     l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 
-// The B operand of the product with V, 32 keys of strips 2 h and 2 h + 1: weights times the keys' scales of one block (4 of them at d + t *
-// stride for strip t). The fmas are one v_fma_mix each, from and to f16.
+// The B operand of the product with V, 32 keys of strips 2 h and 2 h + 1: weights as one f16 or two
 template <int TERMS>
-__device__ __forceinline__ void weights_times_scales(const float4_t * s, int h, const unsigned char * d, int stride, half8_t * p) {
-    const half4_t d0 = *(const half4_t *) (d + 2 * h * stride), d1 = *(const half4_t *) (d + (2 * h + 1) * stride);
+__device__ __forceinline__ void turn_weights(const float4_t * s, int h, half8_t * p) {
 #pragma unroll
     for (int r = 0; r < 8; r++) {
-        const float w = s[2 * h + (r >> 2)][r & 3], e = (float) (r < 4 ? d0[r & 3] : d1[r & 3]);
-        p[0][r] = (_Float16) __builtin_fmaf(w, e, 0.0f);
-        if constexpr (TERMS == 2) p[1][r] = (_Float16) __builtin_fmaf(w, e, -(float) p[0][r]);
+        const float w = s[2 * h + (r >> 2)][r & 3];
+        p[0][r] = (_Float16) w;
+        if constexpr (TERMS == 2) p[1][r] = (_Float16) (w - (float) p[0][r]);
     }
+}
+
+// O^T += V^T P^T of 16 dimensions and 32 keys, from V's codes and the scales of the same keys (4 at d, 4 at d + stride)
+template <int TERMS>
+__device__ __forceinline__ float4_t add_values(half8_t codes, const unsigned char * d, int stride, const half8_t * p, float4_t o) {
+    const half8_t scales = __builtin_shufflevector(*(const half4_t *) d, *(const half4_t *) (d + stride), 0, 1, 2, 3, 4, 5, 6, 7);
+    const half8_t v = codes * scales, rest = __builtin_elementwise_fma(codes, scales, -v);
+    o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[0], o, 0, 0, 0);
+    o = __builtin_amdgcn_mfma_f32_16x16x32_f16(rest, p[0], o, 0, 0, 0);
+    if constexpr (TERMS == 2) o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[1], o, 0, 0, 0);
+    return o;
 }
 
 // 16 dimensions x 32 keys of V as the A operand, from rows of f16 VS bytes apart: lane i of 16 names row i / 4, its 4 values i % 4
@@ -538,7 +539,6 @@ __global__ __launch_bounds__(NT, groups_of<T>(HD, 16)) void k_cache_attention(ca
     auto tile = [&](auto masked) {
         constexpr bool MASKED = decltype(masked)::value;
         const uint32_t bad = bad_n;
-        uint32_t dmax = 0;
         wave_order();
 #pragma unroll
         for (int t = 0; t < 4; t++) {
@@ -550,7 +550,6 @@ __global__ __launch_bounds__(NT, groups_of<T>(HD, 16)) void k_cache_attention(ca
                 else if (key + 1 >= kend) sc &= 0xffffu;
             }
             if (lane < HD / 2) *(uint32_t *) (scales + t * 2 * HD + lane * 4) = sc;
-            if (lane >= HD / 4) dmax = max(dmax, max(sc & 0x7fffu, sc >> 16 & 0x7fffu));
 #pragma unroll
             for (int b = 0; b < NB; b++) {
                 const int w = (lane & 3) * NB + b;
@@ -560,7 +559,6 @@ __global__ __launch_bounds__(NT, groups_of<T>(HD, 16)) void k_cache_attention(ca
         // in the order of their use: a wait for one load is a wait for all before it
         const int pages_after = load_pages(k0 + 2 * STEP);
         load_v(k0 + STEP, pages);
-        const float dexp = (float) ((int) (wave_umax(dmax) >> 10) - 14);      // every |dv| of the tile is below 2^dexp
         wave_order();
 
         // scores
@@ -581,23 +579,20 @@ __global__ __launch_bounds__(NT, groups_of<T>(HD, 16)) void k_cache_attention(ca
         }
         load_k();
         pages = pages_after;
-        softmax_step<MASKED, ND>(s, k0 + g * 4, lim, bad, c, dexp, mu, l, o);
-        // O^T += V^T P'^T, block by block of the head
+        softmax_step<MASKED, ND>(s, k0 + g * 4, lim, bad, c, mu, l, o);
+        half8_t p[2][TERMS];
+#pragma unroll
+        for (int h = 0; h < 2; h++) turn_weights<TERMS>(s, h, p[h]);
+        // O^T += V^T P^T, block by block of the head
 #pragma unroll
         for (int b = 0; b < NB; b++) {
-            half8_t p[2][TERMS];
-#pragma unroll
-            for (int h = 0; h < 2; h++) weights_times_scales<TERMS>(s, h, scales + HD + g * (8 * NB) + b * 8, 2 * HD, p[h]);
 #pragma unroll
             for (int dd = 0; dd < 2; dd++) {
                 const int d = 2 * b + dd;
                 const int2_t w = __builtin_amdgcn_ds_read_tr4_b64_v2i32((__attribute__((address_space(3))) int2_t *) (mine + d * 528 + tr_at));
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const half8_t vc = codes8((uint32_t) w[h], k1024);
-#pragma unroll
-                    for (int k = 0; k < TERMS; k++) o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vc, p[h][k], o[d], 0, 0, 0);
-                }
+                for (int h = 0; h < 2; h++)
+                    o[d] = add_values<TERMS>(codes8((uint32_t) w[h], k1024), scales + HD + g * (8 * NB) + b * 8 + 2 * h * (2 * HD), 2 * HD, p[h], o[d]);
             }
             __builtin_amdgcn_sched_barrier(0x100);
         }
@@ -662,7 +657,7 @@ __global__ __launch_bounds__(NT, groups_of<T>(HD, prompt<T>::columns)) void k_ca
     constexpr int CT = prompt<T>::tiles, BUFS = prompt<T>::bufs, NB = HD / 32, ND = HD / 16, TERMS = sizeof(T) == 4 ? 2 : 1, WC = 16 * CT, C = 4 * WC;
     constexpr int KS = 2 * HD + 32, VS = 2 * HD + 32, SCALES = TILE * (KS + VS), BUF = SCALES + (SCALED ? 0 : 8 * HD);
     __shared__ __attribute__((aligned(16))) unsigned char lds[BUFS * BUF];
-    __shared__ uint32_t tile_dmax[BUFS][4], tile_bad[BUFS][4];
+    __shared__ uint32_t tile_bad[BUFS][4];
     unit u;
     const int kvh = (int) (blockIdx.x % (unsigned) a.n_kv_head);
     if (!find_unit<C, slots_of<T>(HD, C)>(a, blockIdx.x / (unsigned) a.n_kv_head, u)) return;
@@ -726,18 +721,13 @@ __global__ __launch_bounds__(NT, groups_of<T>(HD, prompt<T>::columns)) void k_ca
             if constexpr (SCALED) x = scale2(x, !ok ? 0u : w >> 2 == vb0 ? sx[NB] : sx[NB + 1]);
             *(half8_t *) (l + TILE * KS + (wv * 16 + l15) * VS + w * 16) = x;
         }
-        uint32_t dmax = 0;
         if constexpr (!SCALED) {
             const int d = lane % (HD / 4);
             const int32_t at = key + wv * 16 + d / (2 * NB) * 4 + (d & 1) * 2;
             const uint32_t sc = at >= kend || bad ? 0u : at + 1 >= kend ? sx[0] & 0xffffu : sx[0];
             if (lane < HD / 2) *(uint32_t *) (l + SCALES + wv * 2 * HD + lane * 4) = sc;
-            dmax = wave_umax(lane >= HD / 4 ? max(sc & 0x7fffu, sc >> 16 & 0x7fffu) : 0u);
         }
-        if (lane == 0) {
-            tile_dmax[buf][wv] = dmax;
-            tile_bad[buf][wv] = bad;
-        }
+        if (lane == 0) tile_bad[buf][wv] = bad;
     };
 
     float c[CT];
@@ -767,8 +757,6 @@ __global__ __launch_bounds__(NT, groups_of<T>(HD, prompt<T>::columns)) void k_ca
         const unsigned char * const m = lds + buf * BUF, * const scales = m + SCALES;
         uint32_t hidden = 0;
         if constexpr (MASKED) hidden = tile_bad[buf][0] | tile_bad[buf][1] << 1 | tile_bad[buf][2] << 2 | tile_bad[buf][3] << 3;
-        float dexp = 0.0f;
-        if constexpr (!SCALED) dexp = (float) ((int) (max(max(tile_dmax[buf][0], tile_dmax[buf][1]), max(tile_dmax[buf][2], tile_dmax[buf][3])) >> 10) - 14);
         float4_t s[CT][4];
 #pragma unroll
         for (int t = 0; t < 4; t++) {
@@ -794,47 +782,24 @@ __global__ __launch_bounds__(NT, groups_of<T>(HD, prompt<T>::columns)) void k_ca
             __builtin_amdgcn_sched_barrier(0x100);
         }
 #pragma unroll
-        for (int ct = 0; ct < CT; ct++) softmax_step<MASKED, ND>(s[ct], k0 + g * 4, lim[ct], hidden, c[ct], dexp, mu[ct], l[ct], o[ct]);
-        if constexpr (SCALED) {
-            half8_t p[CT][2];
+        for (int ct = 0; ct < CT; ct++) softmax_step<MASKED, ND>(s[ct], k0 + g * 4, lim[ct], hidden, c[ct], mu[ct], l[ct], o[ct]);
+        half8_t p[CT][2][TERMS];
 #pragma unroll
-            for (int ct = 0; ct < CT; ct++)
+        for (int ct = 0; ct < CT; ct++)
 #pragma unroll
-                for (int h = 0; h < 2; h++)
+            for (int h = 0; h < 2; h++) turn_weights<TERMS>(s[ct], h, p[ct][h]);
 #pragma unroll
-                    for (int r = 0; r < 8; r++) p[ct][h][r] = (_Float16) s[ct][2 * h + (r >> 2)][r & 3];
+        for (int d = 0; d < ND; d++) {
 #pragma unroll
-            for (int d = 0; d < ND; d++) {
+            for (int h = 0; h < 2; h++) {
+                const half8_t v = read_v<VS>(m + tr_at + d * 32, h);
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const half8_t v = read_v<VS>(m + tr_at + d * 32, h);
-#pragma unroll
-                    for (int ct = 0; ct < CT; ct++) o[ct][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[ct][h], o[ct][d], 0, 0, 0);
+                for (int ct = 0; ct < CT; ct++) {
+                    if constexpr (SCALED) o[ct][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[ct][h][0], o[ct][d], 0, 0, 0);
+                    else o[ct][d] = add_values<TERMS>(v, scales + HD + g * (8 * NB) + (d >> 1) * 8 + 2 * h * (2 * HD), 2 * HD, p[ct][h], o[ct][d]);
                 }
-                if (d & 1) __builtin_amdgcn_sched_barrier(0x100);
             }
-        } else {
-#pragma unroll
-            for (int b = 0; b < NB; b++) {
-                half8_t p[CT][2][TERMS];
-#pragma unroll
-                for (int h = 0; h < 2; h++)
-#pragma unroll
-                    for (int ct = 0; ct < CT; ct++) weights_times_scales<TERMS>(s[ct], h, scales + HD + g * (8 * NB) + b * 8, 2 * HD, p[ct][h]);
-#pragma unroll
-                for (int dd = 0; dd < 2; dd++) {
-                    const int d = 2 * b + dd;
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const half8_t v = read_v<VS>(m + tr_at + d * 32, h);
-#pragma unroll
-                        for (int ct = 0; ct < CT; ct++)
-#pragma unroll
-                            for (int k = 0; k < TERMS; k++) o[ct][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[ct][h][k], o[ct][d], 0, 0, 0);
-                    }
-                }
-                __builtin_amdgcn_sched_barrier(0x100);
-            }
+            if (d & 1) __builtin_amdgcn_sched_barrier(0x100);
         }
     };
     if (k0 < kend) {
