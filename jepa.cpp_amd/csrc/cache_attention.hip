@@ -16,7 +16,9 @@
 //     and averaged over the keys) or to the sum of two (f32 rows; the product of both second terms, 2^-22, is left out). mu is the running
 //     maximum of the scores less 10, and moves when a tile passes it by more than 2^15: so the largest weight is between 2^10 and 2^15, and
 //     f16's smallest step is 2^-34 of it or less. Nothing of V takes part in that: a token that a row must not read cannot change
-//     the row, and the blocks of a head may differ in size.
+//     the row, and the blocks of a head may differ in size;
+//   - the sum of the weights is that of the rounded ones, by the same instructions (a row of ones beside V^T): the result is a mean
+//     of the values, never past the largest, which f16 might not hold.
 // Scores, maxima, sums and accumulators are f32.
 //
 // Few columns (k_cache_attention). The four waves of a workgroup share 16 columns and split the keys, a wave sweeping its tiles of 64
@@ -84,18 +86,12 @@ __device__ __forceinline__ half8_t codes8(uint32_t w, uint32_t k1024) {
     return half8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// f over the four lanes l, l ^ 16, l ^ 32, l ^ 48 (the lanes of one column), the same bits in each
+// the largest over the four lanes l, l ^ 16, l ^ 32, l ^ 48 (the lanes of one column)
 __device__ __forceinline__ float col_max(float x) {
     auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
     r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float col_sum(float x) {
-    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
-    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 // N words per lane of a buffer
 template <int N>
@@ -385,9 +381,10 @@ __device__ __forceinline__ void turn_query(const cache_attn_args & a, const type
     }
 }
 
-// One column's scores of a tile, s[t][r] of key + 16 t + r, to weights; its maximum, sum and accumulators follow
+// One column's scores of a tile, s[t][r] of key + 16 t + r, to weights; its maximum and accumulators (of ND tiles of dimensions, and the
+// weights' sum behind them) follow
 template <bool MASKED, int ND>
-__device__ __forceinline__ void softmax_step(float4_t * s, int32_t key, int32_t lim, uint32_t hidden, float c, float & mu, float & l, float4_t * o) {
+__device__ __forceinline__ void softmax_step(float4_t * s, int32_t key, int32_t lim, uint32_t hidden, float c, float & mu, float4_t * o) {
     if constexpr (MASKED) {
 #pragma unroll
         for (int t = 0; t < 4; t++)
@@ -406,34 +403,32 @@ __device__ __forceinline__ void softmax_step(float4_t * s, int32_t key, int32_t 
         const float to = move ? want - 10.0f : mu;
         const float f = move ? __builtin_amdgcn_exp2f(mu - to) : 1.0f;
         mu = to;
-        l *= f;
 #pragma unroll
-        for (int d = 0; d < ND; d++) o[d] *= f;
+        for (int d = 0; d <= ND; d++) o[d] *= f;
     }
     const float m = mu == -INFINITY ? 0.0f : mu;
-    float4_t sum = {0, 0, 0, 0};
 #pragma unroll
-    for (int t = 0; t < 4; t++) {
+    for (int t = 0; t < 4; t++)
 #pragma unroll
         for (int r = 0; r < 4; r++) {
             const float x = s[t][r];
             const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x, c, -m));
             s[t][r] = MASKED && x == -INFINITY ? 0.0f : p;
         }
-        sum += s[t];
-    }
-    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 
-// The B operand of the product with V, 32 keys of strips 2 h and 2 h + 1: weights as one f16 or two
+// The B operand of the product with V, 32 keys of strips 2 h and 2 h + 1: weights as one f16 or two. Their sum goes to every element of l.
 template <int TERMS>
-__device__ __forceinline__ void turn_weights(const float4_t * s, int h, half8_t * p) {
+__device__ __forceinline__ void turn_weights(const float4_t * s, int h, half8_t * p, float4_t & l) {
+    const half8_t ones = {1, 1, 1, 1, 1, 1, 1, 1};
 #pragma unroll
     for (int r = 0; r < 8; r++) {
         const float w = s[2 * h + (r >> 2)][r & 3];
         p[0][r] = (_Float16) w;
         if constexpr (TERMS == 2) p[1][r] = (_Float16) (w - (float) p[0][r]);
     }
+#pragma unroll
+    for (int k = 0; k < TERMS; k++) l = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, p[k], l, 0, 0, 0);
 }
 
 // O^T += V^T P^T of 16 dimensions and 32 keys, from V's codes and the scales of the same keys (4 at d, 4 at d + stride)
@@ -529,9 +524,9 @@ __global__ __launch_bounds__(NT, groups_of<T>(HD, 16)) void k_cache_attention(ca
     float c;
     half8_t q[NB][TERMS];
     turn_query<T, HD, TERMS>(a, y, q, c);
-    float4_t o[ND];
-    float mu = -INFINITY, l = 0.0f;      // mu: -inf before the first key
-    for (int d = 0; d < ND; d++) o[d] = float4_t{0, 0, 0, 0};
+    float4_t o[ND + 1];      // the last: the weights' sum, four times
+    float mu = -INFINITY;     // (before the first key)
+    for (int d = 0; d <= ND; d++) o[d] = float4_t{0, 0, 0, 0};
 
     uint32_t k1024 = 0x64006400u;
     asm volatile("" : "+v"(k1024));
@@ -579,10 +574,10 @@ __global__ __launch_bounds__(NT, groups_of<T>(HD, 16)) void k_cache_attention(ca
         }
         load_k();
         pages = pages_after;
-        softmax_step<MASKED, ND>(s, k0 + g * 4, lim, bad, c, mu, l, o);
+        softmax_step<MASKED, ND>(s, k0 + g * 4, lim, bad, c, mu, o);
         half8_t p[2][TERMS];
 #pragma unroll
-        for (int h = 0; h < 2; h++) turn_weights<TERMS>(s, h, p[h]);
+        for (int h = 0; h < 2; h++) turn_weights<TERMS>(s, h, p[h], o[ND]);
         // O^T += V^T P^T, block by block of the head
 #pragma unroll
         for (int b = 0; b < NB; b++) {
@@ -599,7 +594,6 @@ __global__ __launch_bounds__(NT, groups_of<T>(HD, 16)) void k_cache_attention(ca
     };
     for (; k0 + TILE <= min(lim_lo, kend) && bad_n == 0; k0 += STEP) tile(std::false_type{});
     for (; k0 < kend; k0 += STEP) tile(std::true_type{});
-    l = col_sum(l);
 
     const parts_view<HD, C> part(a, u.part, kvh);
     auto out_at = [&](int32_t col) { return (T *) a.out + (sv.row0 + (int64_t) ((uint32_t) col / (uint32_t) group)) * a.ldo + ((int64_t) kvh * group + (uint32_t) col % (uint32_t) group) * HD; };
@@ -608,7 +602,7 @@ __global__ __launch_bounds__(NT, groups_of<T>(HD, 16)) void k_cache_attention(ca
     __syncthreads();      // the loop's LDS is read out
     if (g == 0) {
         stat[(wv * C + l15) * 2] = mu;
-        stat[(wv * C + l15) * 2 + 1] = l;
+        stat[(wv * C + l15) * 2 + 1] = o[ND][0];
     }
 #pragma unroll
     for (int d = 0; d < ND; d++) *(float4_t *) (sum + (wv * C + l15) * (HD + 4) + d * 16 + g * 4) = o[d];
@@ -741,13 +735,12 @@ __global__ __launch_bounds__(NT, groups_of<T>(HD, prompt<T>::columns)) void k_ca
     }
 #pragma unroll
     for (int ct = 0; ct < CT; ct++) lim[ct] = visible(min(col0 + ct * 16 + l15, n_cols - 1));
-    float4_t o[CT][ND];
-    float mu[CT], l[CT];
+    float4_t o[CT][ND + 1];
+    float mu[CT];
 #pragma unroll
     for (int ct = 0; ct < CT; ct++) {
         mu[ct] = -INFINITY;
-        l[ct] = 0.0f;
-        for (int d = 0; d < ND; d++) o[ct][d] = float4_t{0, 0, 0, 0};
+        for (int d = 0; d <= ND; d++) o[ct][d] = float4_t{0, 0, 0, 0};
     }
 
     int buf = 0;
@@ -782,12 +775,12 @@ __global__ __launch_bounds__(NT, groups_of<T>(HD, prompt<T>::columns)) void k_ca
             __builtin_amdgcn_sched_barrier(0x100);
         }
 #pragma unroll
-        for (int ct = 0; ct < CT; ct++) softmax_step<MASKED, ND>(s[ct], k0 + g * 4, lim[ct], hidden, c[ct], mu[ct], l[ct], o[ct]);
+        for (int ct = 0; ct < CT; ct++) softmax_step<MASKED, ND>(s[ct], k0 + g * 4, lim[ct], hidden, c[ct], mu[ct], o[ct]);
         half8_t p[CT][2][TERMS];
 #pragma unroll
         for (int ct = 0; ct < CT; ct++)
 #pragma unroll
-            for (int h = 0; h < 2; h++) turn_weights<TERMS>(s[ct], h, p[ct][h]);
+            for (int h = 0; h < 2; h++) turn_weights<TERMS>(s[ct], h, p[ct][h], o[ct][ND]);
 #pragma unroll
         for (int d = 0; d < ND; d++) {
 #pragma unroll
@@ -826,14 +819,12 @@ __global__ __launch_bounds__(NT, groups_of<T>(HD, prompt<T>::columns)) void k_ca
     for (; k0 + TILE <= min(lim_lo, kend) && no_bad(); k0 += TILE) step(std::false_type{});
     for (; k0 < kend; k0 += TILE) step(std::true_type{});
 
-#pragma unroll
-    for (int ct = 0; ct < CT; ct++) l[ct] = col_sum(l[ct]);
     if (u.pieces == 1) {
 #pragma unroll
         for (int ct = 0; ct < CT; ct++) {
             const int32_t col = col0 + ct * 16 + l15;
             if (col >= n_cols) continue;
-            const float inv = l[ct] == 0.0f ? 0.0f : 1.0f / l[ct];
+            const float l = o[ct][ND][0], inv = l == 0.0f ? 0.0f : 1.0f / l;
             T * p = (T *) a.out + (sv.row0 + (int64_t) ((uint32_t) col / (uint32_t) group)) * a.ldo + ((int64_t) kvh * group + (uint32_t) col % (uint32_t) group) * HD;
             for (int d = 0; d < ND; d++) store4(p + d * 16 + g * 4, o[ct][d] * inv);
         }
@@ -844,7 +835,7 @@ __global__ __launch_bounds__(NT, groups_of<T>(HD, prompt<T>::columns)) void k_ca
     for (int ct = 0; ct < CT; ct++) {
         const int32_t at = wv * WC + ct * 16 + l15;
         if (first + at >= n_cols) continue;
-        if (g == 0) part.put_stat(u.piece, at, mu[ct], l[ct]);
+        if (g == 0) part.put_stat(u.piece, at, mu[ct], o[ct][ND][0]);
         for (int d = 0; d < ND; d++) part.put(u.piece, at, d * 16 + g * 4, o[ct][d]);
     }
     if (last_to_arrive(a, u, kvh)) join_pieces<T>(a, u, kvh, part);

@@ -125,3 +125,22 @@ def test_values_that_grow_along_the_sequence(jlib, rows, kvh, group, hd, kind):
     for f in (grow, grow.flip(0), some):
         s.set(s.k, s.v * f)
         s.check(q, kind)
+
+
+@pytest.mark.parametrize("rows", [1, 1000])
+def test_means_of_the_largest_f16_stay_finite(jlib, rows):
+    """Every value +-65504: a mean of them is that, whatever the weights round to. One token of 64 has the largest weight,
+    and the others' common one takes 64 places between two powers of two."""
+    n = 1000
+    s = Sequence(jlib, 5, n, 1, 1, 64)
+    k, v = torch.zeros(n, 64, device="cuda"), torch.full((n, 64), 1e6, device="cuda")
+    k[7::64, 0] = -8.0      # a q4_0 block of its largest value and zeros: exact
+    v[:, 32:] = -1e6      # (a q4_0 block reaches its largest magnitude on one side only)
+    s.set(k, v)
+    q = torch.zeros(rows, 64, dtype=torch.float16, device="cuda")
+    q[:, 0] = -1.0
+    want = torch.tensor([65504.0] * 32 + [-65504.0] * 32, device="cuda")
+    for i in range(64):
+        got = s.p.attend(q, base.ints([0, rows]), base.ints([n]), base.ints(s.table), "f16", 0, np.log(2.0) / 8 * (1 + i / 64))
+        torch.cuda.synchronize()
+        assert ((got.float() - want).abs() <= 32).all(), i      # (a step of f16 there)
