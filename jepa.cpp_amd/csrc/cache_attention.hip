@@ -9,8 +9,8 @@
 // Numerics. 4-bit codes are exact in f16:
 //   - the first product runs on K's codes: the MFMA's depth (32) is one q4_0 block, whose sum is multiplied by dk in f32 and added over
 //     the blocks of a head;
-//   - q is scaled by a power of two to a largest value in [1, 2) (exact) and taken as one f16 (f16 and bf16 rows: below
-//     2^-14 of the row's largest value they lose bits, 2^-25 of it at most) or as the sum of two (f32 rows: 22 bits);
+//   - q is scaled by a power of two (exact) to a largest value in [2^14, 2^15), so that f16's subnormals begin at 2^-28 of it, and taken as
+//     one f16 (f16 and bf16 rows: as they are, to 2^-39 of the row's largest value) or as the sum of two (f32 rows: 22 bits, to the same);
 //   - a value dv (cv - 8) has 15 bits at most and is the sum of two f16, exactly (the second one's last bit is dv's, 2^-24 or more);
 //   - weights are rounded to one f16 (16-bit rows: half a step of f16, 2^-11 relative at most, as the output's own rounding is or finer,
 //     and averaged over the keys) or to the sum of two (f32 rows; the product of both second terms, 2^-22, is left out). mu is the running
@@ -348,8 +348,8 @@ __device__ __forceinline__ void join_pieces(const cache_attn_args & a, const uni
     }
 }
 
-// The column's query row to f16: scaled by a power of two to a largest value in [1, 2), one term or two; c: what a product of it with a
-// key is multiplied by to be an exponent of 2 (never negative: the row carries the scale's sign)
+// The column's query row to f16: scaled by a power of two to a largest value in [2^14, 2^15), one term or two; c: what a product of it with
+// a key is multiplied by to be an exponent of 2 (never negative: the row carries the scale's sign)
 template <typename T> struct vec8 { typedef T t __attribute__((ext_vector_type(8))); };
 template <typename T, int HD>
 __device__ __forceinline__ void fetch_query(const cache_attn_args & a, const seq_view & sv, int kvh, int group, int32_t col, int g, typename vec8<T>::t * y) {
@@ -367,11 +367,9 @@ __device__ __forceinline__ void turn_query(const cache_attn_args & a, const type
         x[b] = __builtin_convertvector(y[b], float8_t);
         for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(x[b][j]));
     }
-    const uint32_t ex = __float_as_uint(col_max(top)) >> 23;
-    float f = ex < 254 ? __uint_as_float((254 - ex) << 23) : 0x1p-127f;
-    c = fabsf(a.scale) * LOG2E * (ex ? __uint_as_float(ex << 23) : 0x1p-127f);
-    if (ex == 0) f = 0x1p127f;                  // (below f32's normal range: 2^127 will do)
-    if (ex == 255) f = __builtin_nanf("");      // an infinity in the row: all of it NaN
+    const uint32_t of_top = __float_as_uint(col_max(top)) >> 23, ex = max(of_top, 15u);      // (a row below 2^-112 is scaled by 2^126)
+    float f = of_top == 255 ? __builtin_nanf("") : __uint_as_float((268 - ex) << 23);      // an infinity in the row: all of it NaN
+    c = fabsf(a.scale) * LOG2E * __uint_as_float((ex - 14) << 23);
     if (a.scale < 0.0f) f = -f;
 #pragma unroll
     for (int b = 0; b < NB; b++) {

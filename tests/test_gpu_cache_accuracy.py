@@ -144,3 +144,35 @@ def test_means_of_the_largest_f16_stay_finite(jlib, rows):
         got = s.p.attend(q, base.ints([0, rows]), base.ints([n]), base.ints(s.table), "f16", 0, np.log(2.0) / 8 * (1 + i / 64))
         torch.cuda.synchronize()
         assert ((got.float() - want).abs() <= 32).all(), i      # (a step of f16 there)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows,kvh,group,hd", SHAPES)
+def test_queries_with_one_large_element(jlib, rows, kvh, group, hd, kind):
+    """An element of the query 2^13 to 2^19 times the others' size, which meets keys that are 0 there: the others decide the scores, and
+    count with their own bits.
+
+    Tolerance: one score is a sum of products of exact keys and a query held to 2^-22 of each element (16-bit rows: exactly) or half of
+    f16's smallest step where the row's largest element is 2^14, 2^-39 of that: off by Q = scale sum_n |k_n| (2^-22 |q_n| + 2^-39 |q|max) and the 32-bit
+    sums' (head_dim / 8 + 8) 2^-22 of S1 = max_j scale sum_n |q_n| |k_jn|, on both sides of the fraction; the rest as above."""
+    s = Sequence(jlib, rows + hd + 3, rows, kvh, group, hd)
+    s.k[:, ::hd] = 0.0
+    s.set(s.k, s.v)
+    s.k, s.v = s.p.read(s.slot)
+    assert (s.k[:, ::hd] == 0).all()
+    for large in (2.0 ** 9, 2.0 ** 13, 2.0 ** 15 - 16):
+        q = base.queries(s.rng, rows, s.width, kind, 0.06)
+        q[:, ::hd] = large
+        got = s.run(q, kind).double()
+        hidden = torch.triu(torch.ones(rows, rows, dtype=torch.bool, device="cuda"), 1)
+        for h in range(kvh * group):
+            at = slice(h // group * hd, (h // group + 1) * hd)
+            x, k, v = q[:, h * hd:(h + 1) * hd].double(), s.k[:, at].double(), s.v[:, at].double()
+            w = torch.softmax((x @ k.T.contiguous() * s.scale).masked_fill(hidden, float("-inf")), -1)
+            y, A, N = w @ v, w @ v.abs(), (~hidden).double() @ v.abs()
+            S1 = s.scale * (x.abs() @ k.abs().T.contiguous()).amax(-1, keepdim=True)
+            Q = 2.0 ** -22 * S1 + 2.0 ** -39 * large * s.scale * k.abs().sum(-1).max()
+            f = 2.0 ** -20 + 2 * (Q + (hd / 8 + 8) * 2.0 ** -22 * S1) + (2.0 ** -11 if kind != "f32" else 0.0) + (2.0 ** -11 * (1 + 2 * S1) if kind == "bf16" else 0.0)
+            tol = torch.finfo(base.TYPES[kind][0]).eps / 2 * y.abs() * (1 + f) + f * A + 2.0 ** -35 * N + (2.0 ** -25 if kind == "f16" else 1e-38)
+            off = (got[:, h] - y).abs()
+            assert (off <= tol).all(), f"{large}: off by {(off / tol).max().item():.3g} of the tolerance"
