@@ -57,7 +57,7 @@ __device__ __forceinline__ uint16_t quantize8(float8 x, int lane, uint32_t code[
     // quad_perm 1 0 3 2, then 2 3 0 1: of equal magnitudes the lower lane's is the first
     join((uint32_t) __builtin_amdgcn_update_dpp(0, (int) most, 0xb1, 0xf, 0xf, true), (uint32_t) __builtin_amdgcn_update_dpp(0, (int) from, 0xb1, 0xf, 0xf, true), lane & 1);
     join((uint32_t) __builtin_amdgcn_update_dpp(0, (int) most, 0x4e, 0xf, 0xf, true), (uint32_t) __builtin_amdgcn_update_dpp(0, (int) from, 0x4e, 0xf, 0xf, true), lane & 2);
-    const float d = __uint_as_float(most | (from & 0x80000000u)) / -8.0f;
+    const float d = __uint_as_float(most | (most ? from & 0x80000000u : 0u)) / -8.0f;      // (zeros of either sign: the format's -0)
     const float id = d != 0.0f ? 1.0f / d : 0.0f;
 #pragma unroll
     for (int j = 0; j < 8; j++) code[j] = (uint32_t) __builtin_amdgcn_fmed3f(x[j] * id + 8.5f, 0.0f, 15.0f);      // (an overflowing id: in range all the same)
