@@ -350,12 +350,15 @@ __device__ __forceinline__ void join_pieces(const cache_attn_args & a, const uni
 
 // The column's query row to f16: scaled by a power of two to a largest value in [2^14, 2^15), one term or two; c: what a product of it with
 // a key is multiplied by to be an exponent of 2 (never negative: the row carries the scale's sign)
-template <typename T> struct vec8 { typedef T t __attribute__((ext_vector_type(8))); };
+template <typename T> struct vec8 {
+    typedef T t __attribute__((ext_vector_type(8)));
+    typedef t at16 __attribute__((aligned(16)));      // rows lie at whole 16 bytes, f32's 8 values too
+};
 template <typename T, int HD>
 __device__ __forceinline__ void fetch_query(const cache_attn_args & a, const seq_view & sv, int kvh, int group, int32_t col, int g, typename vec8<T>::t * y) {
     const T * p = (const T *) a.q + (sv.row0 + (int64_t) ((uint32_t) col / (uint32_t) group)) * a.ldq + ((int64_t) kvh * group + (uint32_t) col % (uint32_t) group) * HD + g * 8;
 #pragma unroll
-    for (int b = 0; b < HD / 32; b++) y[b] = *(const typename vec8<T>::t *) (p + b * 32);
+    for (int b = 0; b < HD / 32; b++) y[b] = *(const typename vec8<T>::at16 *) (p + b * 32);
 }
 template <typename T, int HD, int TERMS>
 __device__ __forceinline__ void turn_query(const cache_attn_args & a, const typename vec8<T>::t * y, half8_t (*q)[TERMS], float & c) {

@@ -24,13 +24,15 @@ template <> struct vec8<float> { typedef float8 t; };
 template <> struct vec8<_Float16> { typedef half8 t; };
 template <> struct vec8<__bf16> { typedef bhalf8 t; };
 
+template <typename T> struct at16 { typedef typename vec8<T>::t t __attribute__((aligned(16))); };      // (rows lie at whole 16 bytes, f32's 8 values too)
+
 template <typename T>
 __device__ __forceinline__ float8 load8(const T * p) {
-    return __builtin_convertvector(*(const typename vec8<T>::t *) p, float8);
+    return __builtin_convertvector(*(const typename at16<T>::t *) p, float8);
 }
 template <typename T>
 __device__ __forceinline__ void store8(T * p, float8 x) {
-    *(typename vec8<T>::t *) p = __builtin_convertvector(x, typename vec8<T>::t);
+    *(typename at16<T>::t *) p = __builtin_convertvector(x, typename vec8<T>::t);
 }
 
 __device__ __forceinline__ uint16_t f2h(float f) {

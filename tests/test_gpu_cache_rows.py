@@ -62,3 +62,44 @@ def test_bytes_are_the_quantizers(jlib, hd, kvh, page, kind):
         raw = raw.cpu().numpy()
         np.testing.assert_array_equal(d.reshape(-1), raw[:, 0] | (raw[:, 1].astype(np.uint16) << 8), err_msg=name + " scales")
         np.testing.assert_array_equal(c.reshape(-1, 32), np.concatenate([raw[:, 2:] & 15, raw[:, 2:] >> 4], 1), err_msg=name + " codes")
+
+
+@pytest.mark.parametrize("kind", list(base.TYPES))
+@pytest.mark.parametrize("rows", [3, 400])
+@pytest.mark.parametrize("hd,kvh,group", [(64, 2, 2), (96, 1, 3), (128, 1, 1), (32, 3, 1)])
+def test_rows_at_odd_multiples_of_16_bytes(jlib, hd, kvh, group, rows, kind):
+    """Start and stride of every row array 16 bytes past a multiple of 32: the same as from rows side by side."""
+    dtype, code = base.TYPES[kind]
+    step = 16 // torch.empty(0, dtype=dtype).element_size()      # elements of 16 bytes
+    rng = np.random.default_rng(rows + hd)
+
+    def apart(x):
+        wide = torch.full((x.shape[0], (x.shape[1] // (2 * step) + 1) * 2 * step + 3 * step), 7.0, dtype=dtype, device="cuda")
+        out = wide[:, step:step + x.shape[1]]
+        assert out.data_ptr() % 32 == 16 and out.stride(0) * out.element_size() % 32 == 16
+        out.copy_(x)
+        return out, wide
+
+    p = base.Pool(jlib, kvh * group, kvh, hd, 16, rows // 16 + 1)
+    k, v = (base.queries(rng, rows, kvh * hd, kind) for _ in range(2))
+    slot = torch.arange(rows, device="cuda")
+    p.store(k, v, slot, kind)
+    want = p.read(slot, kind)
+    p.cache.fill_(0xff)
+    (ka, _), (va, _) = apart(k), apart(v)
+    torch.cuda.synchronize()
+    p.store(ka, va, slot, kind)
+    (kr, kw), (vr, vw) = apart(torch.zeros_like(k)), apart(torch.zeros_like(v))
+    torch.cuda.synchronize()
+    base.ok(jlib, jlib.lib().jepa_amd_cache_read(0, base.C.byref(p.s), p.cache.data_ptr(), slot.data_ptr(), rows, code, kr.data_ptr(), kr.stride(0), vr.data_ptr(),
+                                                 vr.stride(0), None))
+    torch.cuda.synchronize()
+    q = base.queries(rng, rows, kvh * group * hd, kind)
+    (qa, _), (oa, ow) = apart(q), apart(torch.zeros_like(q))
+    table = base.ints(np.arange(rows // 16 + 1)[None])
+    out = p.attend(q, base.ints([0, rows]), base.ints([rows]), table, kind)
+    p.attend(qa, base.ints([0, rows]), base.ints([rows]), table, kind, out=oa)
+    torch.cuda.synchronize()
+    for got, wide, exact in ((kr, kw, want[0]), (vr, vw, want[1]), (oa, ow, out)):
+        assert torch.equal(got, exact) and not torch.isnan(got).any()
+        assert (wide[:, :step] == 7).all() and (wide[:, step + got.shape[1]:] == 7).all()
