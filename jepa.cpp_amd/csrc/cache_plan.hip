@@ -18,16 +18,15 @@ constexpr int NT = 1024;
 constexpr int64_t PLAN_ROWS = 4 * NT;      // rows whose pages and slots the first kernel writes itself
 constexpr uint32_t FEW = 4;                // rows of a sequence that its own thread writes
 
-__device__ __forceinline__ uint32_t add_sat(uint32_t a, uint32_t b) { return __builtin_elementwise_add_sat(a, b); }
 // sums over the lanes up to this one, held at 2^32 - 1: within rows of 16 lanes, then across rows
 __device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
 #define DPP(ctrl, rows) (uint32_t) __builtin_amdgcn_update_dpp(0, (int) x, ctrl, rows, 0xf, true)
-    x = add_sat(x, DPP(0x111, 0xf));      // row_shr 1, 2, 4, 8
-    x = add_sat(x, DPP(0x112, 0xf));
-    x = add_sat(x, DPP(0x114, 0xf));
-    x = add_sat(x, DPP(0x118, 0xf));
-    x = add_sat(x, DPP(0x142, 0xa));      // row_bcast 15, 31
-    x = add_sat(x, DPP(0x143, 0xc));
+    x = cache_add_sat(x, DPP(0x111, 0xf));      // row_shr 1, 2, 4, 8
+    x = cache_add_sat(x, DPP(0x112, 0xf));
+    x = cache_add_sat(x, DPP(0x114, 0xf));
+    x = cache_add_sat(x, DPP(0x118, 0xf));
+    x = cache_add_sat(x, DPP(0x142, 0xa));      // row_bcast 15, 31
+    x = cache_add_sat(x, DPP(0x143, 0xc));
 #undef DPP
     return x;
 }
@@ -80,9 +79,9 @@ __global__ __launch_bounds__(NT) void k_cache_plan(cache_plan_args a, bool rows_
             uint32_t before = total[k], all = total[k];
             for (int w = 0; w < NT / 64; w++) {
                 if (w == wv) before = all;
-                all = add_sat(all, wsum[k][w]);
+                all = cache_add_sat(all, wsum[k][w]);
             }
-            sum[k] = add_sat(before, sum[k]);
+            sum[k] = cache_add_sat(before, sum[k]);
             total[k] = all;
         }
         if (i < a.n_seq) {
