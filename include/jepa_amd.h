@@ -175,7 +175,9 @@ int jepa_amd_copy(int device, const float * src_dev, float * dst_dev, int64_t n,
  * The calls queue their work on `stream` (a hipStream_t of `device`; NULL: the null stream), allocate nothing, do not wait
  * and can be captured into a HIP graph. All pointers but `shape` are device pointers. Rows are packed one after the other,
  * sequence by sequence, each row its heads one after the other; types are 0 f32, 1 f16, 30 bf16; strides are in elements;
- * row pointers and strides are multiples of 16 bytes. Outputs must not overlap inputs or each other unless stated. */
+ * row pointers and strides are multiples of 16 bytes. Outputs must not overlap inputs or each other unless stated. A call of _store, _read or
+ * _attention has fewer than 2^27 heads of rows (n_rows times n_kv_head, for _attention n_head), one of _attention less than about 2^24 of
+ * n_rows * n_head / 16 + n_seq * n_kv_head; larger ones are refused. */
 typedef struct {
     int32_t n_head;      /* query heads, a multiple of n_kv_head; head h reads K/V head h / (n_head / n_kv_head) */
     int32_t n_kv_head;

@@ -157,6 +157,12 @@ extern "C" int jepa_amd_cache_attention(int device, const jepa_amd_cache_shape *
         jepa_log("jepa: %s: scale %g, causal block %lld\n", who, (double) scale, (long long) causal_block);
         return -1;
     }
+    const int64_t blocks = cache_attention_blocks(c, type, n_seq, n_rows, table_width);
+    if (n_rows && n_seq && blocks >= 1 << 24) {      // (threads of a launch are below 2^32)
+        jepa_log("jepa: %s: %lld rows of %d heads in %lld sequences over %d K/V heads: %lld workgroups in one call (below 2^24)\n", who, (long long) n_rows, c.n_head,
+                 (long long) n_seq, c.n_kv_head, (long long) blocks);
+        return -1;
+    }
     const int64_t need = cache_attention_work_bytes(c, n_seq, n_rows, table_width);
     if (n_rows && n_seq && (!all(who, {row_start, kv_len, table, work}))) return -1;
     if (n_rows && n_seq && ((uintptr_t) work % 16 || work_bytes < need)) {

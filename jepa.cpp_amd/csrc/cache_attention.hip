@@ -884,6 +884,11 @@ template <typename T> int64_t work_bytes(const cache_shape & c, int64_t n_seq, i
     return COUNTERS * 8 + std::max(bytes(16), prompts_within<T>(c, n_rows) ? bytes(prompt<T>::columns) : 0);
 }
 
+template <typename T> int64_t blocks_of(const cache_shape & c, int64_t n_seq, int64_t n_rows, int64_t width) {
+    const int C = columns_of<T>(c, n_seq, n_rows);
+    return (tiles_bound(c, C, n_seq, n_rows) + parts_bound<T>(c, C, n_seq, n_rows, width)) * c.n_kv_head;
+}
+
 template <typename T, int HD, int C>
 hipError_t attend(const cache_shape & c, const cache_attn_args & a, hipStream_t s, const void * kernel) {
     cache_attn_args args = a;
@@ -891,9 +896,7 @@ hipError_t attend(const cache_shape & c, const cache_attn_args & a, hipStream_t 
     const int64_t tiles = tiles_bound(c, C, a.n_seq, a.n_rows), parts = parts_bound<T>(c, C, a.n_seq, a.n_rows, a.width);
     args.parts = parts;
     args.units = (uint32_t) (tiles + parts);
-    const int64_t blocks = (tiles + parts) * c.n_kv_head;
-    if (blocks >= 1 << 24) return hipErrorInvalidConfiguration;      // threads of a launch are below 2^32
-    return hipLaunchKernel(kernel, dim3((unsigned) blocks), dim3(NT), p, 0, s);
+    return hipLaunchKernel(kernel, dim3((unsigned) ((tiles + parts) * c.n_kv_head)), dim3(NT), p, 0, s);
 }
 
 template <typename T, int HD>
@@ -911,6 +914,10 @@ hipError_t by_head(const cache_shape & c, const cache_attn_args & a, hipStream_t
 
 int64_t cache_attention_work_bytes(const cache_shape & c, int64_t n_seq, int64_t n_rows, int64_t width) {      // (rows of any type)
     return std::max({work_bytes<float>(c, n_seq, n_rows, width), work_bytes<_Float16>(c, n_seq, n_rows, width), work_bytes<__bf16>(c, n_seq, n_rows, width)});
+}
+
+int64_t cache_attention_blocks(const cache_shape & c, int type, int64_t n_seq, int64_t n_rows, int64_t width) {
+    return type == T_F32 ? blocks_of<float>(c, n_seq, n_rows, width) : type == T_F16 ? blocks_of<_Float16>(c, n_seq, n_rows, width) : blocks_of<__bf16>(c, n_seq, n_rows, width);
 }
 
 hipError_t launch_cache_attention(const cache_shape & c, int type, const cache_attn_args & a, hipStream_t s) {

@@ -158,6 +158,7 @@ struct cache_attn_args {
     uint32_t units = 0;     // and its workgroups for each K/V head
 };
 int64_t cache_attention_work_bytes(const cache_shape & c, int64_t n_seq, int64_t n_rows, int64_t width);
+int64_t cache_attention_blocks(const cache_shape & c, int type, int64_t n_seq, int64_t n_rows, int64_t width);      // workgroups of the launch (256 threads)
 hipError_t launch_cache_attention(const cache_shape & c, int type, const cache_attn_args & a, hipStream_t s);
 
 // weight expansion at load: raw ggml blocks (device) -> dev_linear operand arrays (int8: q4_0 rows
