@@ -175,9 +175,9 @@ int jepa_amd_copy(int device, const float * src_dev, float * dst_dev, int64_t n,
  * The calls queue their work on `stream` (a hipStream_t of `device`; NULL: the null stream), allocate nothing, do not wait
  * and can be captured into a HIP graph. All pointers but `shape` are device pointers. Rows are packed one after the other,
  * sequence by sequence, each row its heads one after the other; types are 0 f32, 1 f16, 30 bf16; strides are in elements;
- * row pointers and strides are multiples of 16 bytes. Outputs must not overlap inputs or each other unless stated. A call of _store, _read or
- * _attention has fewer than 2^27 heads of rows (n_rows times n_kv_head, for _attention n_head), one of _attention less than about 2^24 of
- * n_rows * n_head / 16 + n_seq * n_kv_head; larger ones are refused. */
+ * row pointers and strides are multiples of 16 bytes. Outputs must not overlap inputs or each other unless stated. A call of
+ * _store, _read or _attention has fewer than 2^27 heads of rows (n_rows times n_kv_head, for _attention n_head), and for
+ * _attention n_rows * n_head / 16 + n_seq * n_kv_head stays below 2^24 - 2^13; much larger ones are refused. */
 typedef struct {
     int32_t n_head;      /* query heads, a multiple of n_kv_head; head h reads K/V head h / (n_head / n_kv_head) */
     int32_t n_kv_head;
@@ -203,14 +203,17 @@ int64_t jepa_amd_cache_page_bytes(const jepa_amd_cache_shape * shape);
  *   slot [n_rows]        the cache slot of each row, page * page_size + place; -1 for a row of a refused sequence and behind the last
  *   refused [n_seq]      1 where the step could not be done for a sequence: its lengths do not fit a table row, its rows end
  *                        past n_rows, or the free pages end before it (then every later one that needs a page is refused
- *                        too). It keeps its len and pages. */
+ *                        too). It keeps its len and pages. Its rows keep their places: what _attention gives them is not the step's.
+ * Entries of the ring, and of a table row within its len, are to be pages of the cache. They are not checked: other numbers
+ * are handed on as they are (to the table, or to the ring where they are dropped) and refuse nothing; tokens on them have slot
+ * -1, are not stored and not read. */
 int jepa_amd_cache_plan(int device, const jepa_amd_cache_shape * shape, int64_t n_seq, int64_t n_rows, const int32_t * len,
                         const int32_t * n_new, int32_t * table, int64_t table_width, int32_t * ring, const int32_t * free_in,
                         int32_t * free_out, int32_t * kv_len, int32_t * row_start, int64_t * slot, int32_t * refused, void * stream);
 
 /* Keys and values of n_rows rows ([n_kv_head * head_dim], k_stride / v_stride apart) quantized into their slots, ggml's
- * q4_0 bit for bit (as jepa_amd_quantize_rows). Rows whose slot is negative or past the cache are skipped; no slot may be given
- * twice. Values beyond +-65504 are held there; a head of a row with a NaN or an infinity in its K or V is stored as K NaN and V
+ * q4_0 scales and codes bit for bit (as jepa_amd_quantize_rows makes them of the rows in f32). Rows whose slot is negative or
+ * past the cache are skipped; no slot may be given twice. Values beyond +-65504 are held there; a head of a row with a NaN or an infinity in its K or V is stored as K NaN and V
  * zero, so that a query which reads the token comes out NaN. */
 int jepa_amd_cache_store(int device, const jepa_amd_cache_shape * shape, void * cache, int type, const void * k, int64_t k_stride,
                          const void * v, int64_t v_stride, int64_t n_rows, const int64_t * slot, void * stream);
@@ -222,9 +225,14 @@ int jepa_amd_cache_read(int device, const jepa_amd_cache_shape * shape, const vo
 /* out = softmax(scale * q K^T) V for each row and head over its sequence's cached tokens. Row j of the r rows of a sequence of
  * kv_len tokens stands at position kv_len - r + j, so the step's own tokens are stored first. causal_block 0: every row reads
  * all kv_len tokens; 1: those up to its own position; T: those of its own and earlier blocks of T positions (frames).
- * q and out hold rows of n_head * head_dim values of `type`; keys and values enter as they are held, sums and the softmax
- * are f32, and f32 rows are computed to f32 accuracy. Tokens whose page is not one of the cache's are not read; a row that
- * reads nothing comes out zero; rows behind the last sequence (row_start[n_seq] on) are left as they are.
+ * q and out hold rows of n_head * head_dim values of `type`; scores, sums and the softmax are f32. Keys and values enter as they
+ * are held, with one exception: in a call with many rows of a sequence, bf16 rows take them rounded to f16 (2^-11 relative, an
+ * eighth of bf16's half step). Weights are rounded to 2^-11 of themselves for f16 and bf16 rows, to 2^-22 for f32 rows, and to
+ * 2^-35 of the row's largest; queries to 2^-22 (f32 rows) and to 2^-39 of the row's largest element: f32 rows are computed to f32
+ * accuracy. Keys and values that a row does not read do not change it; the sizes and lengths of the call's sequences may
+ * change its last bits (they decide how its keys are split and joined), and equal calls give equal bits.
+ * Tokens whose page is not one of the cache's are not read; a row that reads nothing comes out zero; rows behind the last
+ * sequence (row_start[n_seq] on) are left as they are.
  * row_start ascends; a call whose rows overlap writes some of them or none.
  * `work` is jepa_amd_cache_work_bytes() bytes of device memory (16-byte aligned) with nothing kept in it between calls; what
  * the largest step needs does for smaller ones. Calls that may overlap on the device (on two streams, in two graphs) need one each. */

@@ -11,7 +11,9 @@
 //     the blocks of a head;
 //   - q is scaled by a power of two (exact) to a largest value in [2^14, 2^15), so that f16's subnormals begin at 2^-28 of it, and taken as
 //     one f16 (f16 and bf16 rows: as they are, to 2^-39 of the row's largest value) or as the sum of two (f32 rows: 22 bits, to the same);
-//   - a value dv (cv - 8) has 15 bits at most and is the sum of two f16, exactly (the second one's last bit is dv's, 2^-24 or more);
+//   - a value dv (cv - 8) has 15 bits at most and is the sum of two f16, exactly (the second one's last bit is dv's, 2^-24 or more). That is half
+//     as many MFMAs again as one f16 and, for 2000 f16 rows over 16000 tokens, 8 % of the time of scaled weights on V's codes; but a weight times a
+//     scale needs a range that follows V, and then values of other tokens and blocks take its bits;
 //   - weights are rounded to one f16 (16-bit rows: half a step of f16, 2^-11 relative at most, as the output's own rounding is or finer,
 //     and averaged over the keys) or to the sum of two (f32 rows; the product of both second terms, 2^-22, is left out). mu is the running
 //     maximum of the scores less 10, and moves when a tile passes it by more than 2^15: so the largest weight is between 2^10 and 2^15, and
@@ -26,10 +28,10 @@
 // of the MFMA's A operand (the strip's layout is the operand's); V codes and scales go through the wave's own LDS, because V^T needs
 // 16 keys of one dimension in a lane: ds_read_b64_tr_b4 turns 16 x 16 nibbles around. The next tile's loads (and the page numbers of
 // the one after) are in flight while a tile is computed. Measured: 64 requests of 200 to 8000 tokens, f16, 32 heads over 8 of
-// 128, 63.4 us (259 MB, 4.1 TB/s; a large copy reaches 5.1); 2 contexts of 90000 to 131000 tokens, bf16, 64 heads over 8, 60.8 us (253 MB,
-// 4.15 TB/s). About 8 us of a call are its start (find_unit, the query, the first tile's way from memory, one after the other) and 2 its
-// end, then memory bounds it, with the VALU at 55 % (unpacking codes, scales, softmax). With several tiles of columns a sequence
-// the VALU bounds it: 8 sequences of 258 f32 rows, 77 us, 76 % of its time.
+// 128, 65.5 us (259 MB, 3.95 TB/s; a large copy reaches 5.2); 2 contexts of 90000 to 131000 tokens, bf16, 64 heads over 8, 62.3 us (253 MB,
+// 4.05 TB/s). About 8 us of a call are its start (find_unit, the query, the first tile's way from memory, one after the other) and 2 its
+// end, then memory bounds it, with the VALU at 57 % (unpacking codes, scales, softmax). With several tiles of columns a sequence
+// the VALU bounds it: 8 sequences of 258 f32 rows, 78.5 us, 76 % of its time.
 // Many columns (k_cache_prompt): see there.
 //
 // Work. A unit is (sequence, tile of columns, piece of its keys, K/V head). The piece length is the same for all sequences
@@ -69,6 +71,7 @@ constexpr int piece_min(int c) { return c == 16 ? PIECE : 2 * PIECE; }      // m
 template <typename T> constexpr int groups_of(int hd, int c) { return c == 128 ? 2 : c == 64 ? (sizeof(T) == 4 && hd == 128 ? 3 : 4) : hd > 64 ? 3 : 4; }
 template <typename T> constexpr int slots_of(int hd, int c) { return 256 * groups_of<T>(hd, c); }
 // What a unit costs beside its keys, in keys; and how many units a call is split into at most, in slots
+// (24 requests of 5 f16 rows, two column tiles each: 37.5 us, with 384 keys 42.1, with 1536 37.5; single tokens and frames do not change)
 constexpr float UNIT_KEYS = 768.0f;
 constexpr float MOST_UNITS = 1.9f;
 
@@ -186,7 +189,9 @@ __device__ __forceinline__ bool find_unit(const cache_attn_args & a, uint32_t x,
         float inv = 0.0f, least = INFINITY;
 #pragma unroll
         for (int i = 0; i < 3; i++) {
-            // so many units for each slot: the time of all, and of the longest while the last round is not full
+            // so many units for each slot: the time of all, and of the longest while the last round is not full. A little less than one: the
+            // rounding of pieces may not then add a second round (24 requests of 5 f16 rows 37.5 us, without it 41.8). Only the last would do
+            // for ragged single tokens, but takes 71 us instead of 62 for two long contexts.
             constexpr float SHARE[3] = {1.0f, 0.93f, MOST_UNITS};
             const float x1 = piece_inv<C>(keys, SHARE[i] * SLOTS), n = pieces_of(v, x1);
             const float units = wave_add((float) tiles * n) * heads, rounds = units * (1.0f / SLOTS);
@@ -635,13 +640,14 @@ __global__ __launch_bounds__(NT, groups_of<T>(HD, 16)) void k_cache_attention(ca
 // ds_read_b64_tr_b16 turns around. The next tile's codes are in flight meanwhile.
 // For bf16 rows the scales go in with the codes (K and V rounded to f16, 2^-11 relative, against bf16's half step of 2^-8): no
 // work per score is left but the softmax, and two column tiles a wave with two LDS buffers (one barrier a tile, two
-// workgroups a CU) are best: 17.6k prompt rows of 32 x 128 take 0.81 ms, one column tile 1.04.
-// f16 and f32 rows keep codes exact and scales in 32 bits as above, twice the work per score; what hides its latencies best is four
-// workgroups a CU, of one column tile a wave and one buffer: 2000 f16 rows over 16000 tokens take 0.95 ms, two column tiles 1.14.
-// Rows of both are padded by 32 bytes: of 16, 32 and 48 for either this has the fewest bank conflicts (f16 954 us; 16 and 32 971, 32 and 48
-// 966, 48 and 32 970).
-// Rates: 860 TFLOP/s for bf16 (three quarters of an 8192^3 product's 1130; the LDS reads of K and V take as many cycles as the MFMAs)
-// and 515 for f16 (32 heads over 4: the LDS and the VALU, each 60 % of the time, the latter 12 instructions for each MFMA, most of them scales).
+// workgroups a CU) are best: 17.6k prompt rows of 32 x 128 take 0.80 ms, one column tile took 1.04 (then 0.81).
+// f16 and f32 rows keep codes in LDS and the arithmetic above, K's scales in 32 bits and V as two f16, more than twice the work per score; what
+// hides its latencies best is four workgroups a CU, of one column tile a wave and one buffer: 2000 f16 rows over 16000 tokens take 1.03 ms,
+// two column tiles 1.12, with two buffers 1.14.
+// Rows of both are padded by 32 bytes: of 16, 32 and 48 for either this has the fewest bank conflicts (f16, with scaled weights, 954 us; 16 and
+// 32 971, 32 and 48 966, 48 and 32 970).
+// Rates: 865 TFLOP/s for bf16 (three quarters of an 8192^3 product's 1130; the LDS reads of K and V take as many cycles as the MFMAs)
+// and 475 for f16 (32 heads over 4: the VALU 63 % of the time, 8 instructions for each MFMA, most of them scales, the LDS 55 %, the MFMAs 30 %).
 template <typename T> struct prompt {
     static constexpr bool scaled = std::is_same<T, __bf16>::value;
     static constexpr int tiles = scaled ? 2 : 1, bufs = scaled ? 2 : 1, columns = 64 * tiles;
@@ -846,11 +852,18 @@ __global__ __launch_bounds__(NT, groups_of<T>(HD, prompt<T>::columns)) void k_ca
 // it is the faster one where sequences have many columns, and with fewer where the call's columns over all K/V heads (its heads of
 // rows) fill the chip, less what its last tiles leave empty; else 16 columns are, split into fewer pieces. Measured, us of a call,
 // 16 columns / prompts', rows of 8 K/V heads of 128:
-//   1 sequence of 16000 tokens: 256 columns bf16 56 / 98, f16 57 / 107, f32 70 / 89; 1024 columns 181 / 109, 181 / 164, 231 / 209;
-//   16 of 1500 (128 columns are 16k heads of rows): 128 columns 42 / 47, 43 / 47, 54 / 57; 256 columns 80 / 65, 80 / 88, 101 / 88;
-//   64 of 700 (64 columns are 33k): 32 columns 30 / 33, 30 / 39, 37 / 46; 64 columns 53 / 40, 52 / 43, 63 / 53; 96 columns 74 / 43,
-//   73 / 64, 91 / 86; 256 of 500: 16 columns 55 / 97, 55 / 66, 64 / 89; 32 columns 94 / 99, 94 / 78, 110 / 107;
-//   8 of 1032 to 2064 with 258 columns (33k, 20 % of five tiles empty), 16 K/V heads of 64, f32: 78 / 89.
+//   1 sequence of 16000 tokens: 256 columns bf16 65 / 99, f16 58 / 106, f32 68 / 86; 1024 columns 190 / 102, 189 / 163, 224 / 204;
+//   16 of 1500 (128 columns are 16k heads of rows): 128 columns 49 / 55, 48 / 51, 57 / 58; 256 columns 89 / 65, 89 / 91, 105 / 94;
+//   64 of 700 (64 columns are 33k): 32 columns 30 / 32, 30 / 38, 34 / 44; 64 columns 51 / 39, 51 / 42, 59 / 50; 96 columns 76 / 45,
+//   76 / 62, 88 / 80; 256 of 500: 16 columns 55 / 92, 55 / 63, 60 / 86; 32 columns 92 / 94, 92 / 77, 104 / 102;
+// and of 16 K/V heads of 64:
+//   1 of 16000: 256 columns 63 / 52, 63 / 63, 73 / 74; 1024 columns 219 / 124, 219 / 190, 262 / 239;
+//   16 of 1500: 128 columns 54 / 44, 54 / 58, 62 / 68; 258 columns 109 / 67, 110 / 118, 128 / 146;
+//   64 of 700: 32 columns 36 / 40, 36 / 34, 40 / 40; 64 columns 62 / 45, 62 / 42, 70 / 52;
+//   8 of 1806 (33k, 20 % of five tiles empty): 258 columns 69 / 60, 70 / 72, 80 / 89.
+// The rule knows neither the width nor the number of keys. Of these it takes the slower kernel for 1 of 16000 with 256 columns of width 64 in bf16
+// (by 24 %), 16 of 1500 with 128 columns in bf16 (14 %), in f16 and f32 of width 64 (7, 9 %) and with 258 there (7, 15 %), 64 of 700 with 32
+// f16 columns of width 64 (8 %); two more are within 3 %.
 template <typename T> struct column_rule {
     static constexpr int64_t C = prompt<T>::columns, full = prompt<T>::scaled ? 16000 : 32000, least = 24, many = prompt<T>::scaled ? 256 : 768;
 };

@@ -8,8 +8,8 @@
 //
 // Memory-bound: 32k bf16 rows of 8 x 128 are stored in 44 us (4.0 TB/s; the VALU is busy 70 % of it) and read in 26 (6.6 TB/s, the
 // codes come from the last-level cache after a store). One thread takes 8 values of K and V (a 32-bit word of codes each), four threads a block (its maximum
-// by two shuffles). A workgroup has up to 16 consecutive rows of one head: of a prompt that is a whole strip, which leaves its
-// L2 as whole lines (rows of all heads in a workgroup spread a strip over the L2s of all XCDs).
+// by two shuffles). A workgroup has 16 to 64 consecutive rows of one head (256 threads, 4 to 16 a row): of a prompt whole strips, which leave
+// their L2 as whole lines (rows of all heads in a workgroup spread a strip over the L2s of all XCDs).
 #include "cache_dev.h"
 #include "common.h"
 #include "kernels.h"
