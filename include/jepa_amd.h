@@ -213,8 +213,8 @@ int jepa_amd_cache_plan(int device, const jepa_amd_cache_shape * shape, int64_t 
 
 /* Keys and values of n_rows rows ([n_kv_head * head_dim], k_stride / v_stride apart) quantized into their slots, ggml's
  * q4_0 scales and codes bit for bit (as jepa_amd_quantize_rows makes them of the rows in f32). Rows whose slot is negative or
- * past the cache are skipped; no slot may be given twice. Values beyond +-65504 are held there; a head of a row with a NaN or an infinity in its K or V is stored as K NaN and V
- * zero, so that a query which reads the token comes out NaN. */
+ * past the cache are skipped; no slot may be given twice. Values beyond +-65504 are held there; a head of a row with a NaN or an
+ * infinity in its K or V is stored as K NaN and V zero, so that a query which reads the token comes out NaN. */
 int jepa_amd_cache_store(int device, const jepa_amd_cache_shape * shape, void * cache, int type, const void * k, int64_t k_stride,
                          const void * v, int64_t v_stride, int64_t n_rows, const int64_t * slot, void * stream);
 

@@ -9,7 +9,9 @@ N_n = sum_j |v_jn|:
   a weight                    16-bit rows: one f16, half a step 2^-11 relative. f32 rows: two f16, 2^-22, and the product of both low terms
                               that is left out, 2^-11 2^-11; with the 32-bit exponential and sums 2^-20 in all.
                               The largest is brought to 2^10 or more, so half of f16's smallest step, 2^-25, is 2^-35 of the largest, which is at
-                              most their sum: 2^-35 N_n for both
+                              most their sum: 2^-35 N_n for both. (The sum that divides is of the same rounded weights, so a weight's error
+                              counts with v_jn - out_n instead of v_jn: at most A_n + |out_n| in all, and about A_n where the errors of many
+                              keys have no common sign. A_n is asked for.)
   scores                      head_dim products of a query held to 2^-22 and an exact key in 32 bits, times a scale: off by at most
                               (head_dim / 8 + 8) 2^-22 S, S = max_j scale |q|max |k_j|_1, on both sides of the fraction (e^x ~ 1 + x): twice that,
                               times A_n. The queries here are small, so that this is not what decides.
