@@ -242,6 +242,85 @@ int jepa_amd_cache_attention(int device, const jepa_amd_cache_shape * shape, con
                              int64_t table_width, float scale, int64_t causal_block, void * out, int64_t out_stride, void * work,
                              int64_t work_bytes, void * stream);
 
+/* ---- rotary positions of several axes, and the cache with them -----------------------------------------
+ * Frames step by (time, row, column), text by one position or the same on every axis. A head's first dims[0] elements belong to axis 0, the
+ * next dims[1] to axis 1 and so on; the rest of it does not turn. Element j of a section of width w turns by the angle
+ * A_j = pos[axis] * scale[axis] * theta^(-2 f / w), x'_j = x_j cos A_j -+ x_p sin A_j, p being its partner (minus for the first of a pair):
+ *     form 0   pairs (2i, 2i + 1), f = j mod w / 2: a pair's elements turn by different angles (V-JEPA 2; reference src/rope3d.cpp:9-134, "tiled")
+ *     form 1   pairs (2i, 2i + 1), f = i (V-JEPA 2.1, "interleaved"; the scales are its interpolation)
+ *     form 2   pairs (i, i + w / 2), f = i
+ *     form 3   pairs (i, i + W / 2) of all W = dims[0] + dims[1] + ... elements that turn, f = i with W for w; pair i belongs to the axis whose
+ *              dims[axis] / 2 pairs it falls into
+ * Angles are made in 64 bits, their cosines and sines rounded to f32, and so are the two products and their sum. Positions are int32, of either sign. */
+typedef struct {
+    int32_t head_dim;    /* 8 to 256, whole 8 */
+    int32_t form;
+    int32_t n_axes;      /* 1 to 4 */
+    int32_t dims[4];     /* even; form 2: whole 16; form 3: whole 16 together */
+    double  theta;       /* above 0 */
+    double  scale[4];
+} jepa_amd_rope_axes;
+
+/* n_rows rows of n_head heads at positions pos [n_rows][n_axes] (device, int32), types, strides and pointers as for the cache's calls below. backward 0:
+ * rotated; else the gradient with respect to x of the rotated rows' gradient (the transposed map). out may be x with the same stride. Up to 4096
+ * heads, n_rows * n_head below 2^26. Queued on `stream`; allocates nothing, does not wait, can be captured into a HIP graph. */
+int jepa_amd_rope_rows(int device, const jepa_amd_rope_axes * rope, int type, const void * x, int64_t x_stride, int64_t n_rows, int n_head,
+                       const int32_t * pos, int backward, void * out, int64_t out_stride, void * stream);
+
+/* jepa_amd_cache_store of keys that are rotated on the way, and queries rotated into q_out (which may be q, with the same stride; q NULL: keys and values
+ * alone), in one launch. The rotated key is quantized from f32. Rows whose slot is negative or past the cache are not stored; their queries are rotated all
+ * the same. n_rows * n_head stays below 2^26. */
+int jepa_amd_cache_append(int device, const jepa_amd_cache_shape * shape, const jepa_amd_rope_axes * rope, void * cache, int type, const void * q,
+                          int64_t q_stride, const void * k, int64_t k_stride, const void * v, int64_t v_stride, int64_t n_rows, const int32_t * pos,
+                          const int64_t * slot, void * q_out, int64_t q_out_stride, void * stream);
+
+/* ---- attention over pages that each row selects ----------------------------------------------------------
+ * For long contexts: each row reads the n_select pages of its sequence that a cheap score finds best, not all. A step is, after _plan and for each layer,
+ *     jepa_amd_cache_append (or _store)       the rows into their slots
+ *     jepa_amd_cache_digest                   the digests of the pages that they went to
+ *     jepa_amd_cache_select                   which pages each row reads
+ *     jepa_amd_cache_attention_selected       attention over these
+ * What is said of the cache's calls holds for these too: device pointers, the caller's stream, no allocation, nothing kept, row_start / kv_len / table as
+ * jepa_amd_cache_plan gives them. Their workgroups (below) stay under 2^24 in a call; larger ones are refused.
+ *
+ * A page's digest is, for each K/V head, the largest and the smallest value of each dimension of K over the page's tokens, as 8-bit codes with one f32 scale (s / 127,
+ * s the largest magnitude; codes are rounded to nearest; a digest whose s is below 2^-100 is zeros): 2 * head_dim + 16 bytes. Tokens stored as NaN are left out. */
+
+/* Bytes of one page's digests (all K/V heads), or -1. The caller keeps n_pages times this (16-byte aligned) beside each layer's cache; it need not be cleared. */
+int64_t jepa_amd_cache_digest_bytes(const jepa_amd_cache_shape * shape);
+
+/* The digests of the pages that the step's rows (those of row_start) lie in, from all their tokens up to kv_len. A page's digest is otherwise kept, so it
+ * still holds after tokens were dropped from the page, if not as tightly. Pages that are none of the cache's are passed over. */
+int jepa_amd_cache_digest(int device, const jepa_amd_cache_shape * shape, const void * cache, int64_t n_seq, int64_t n_rows, const int32_t * row_start,
+                          const int32_t * kv_len, const int32_t * table, int64_t table_width, void * digest, void * stream);
+
+/* The values that the digests of n pages (device, int32) stand for: bounds [n][n_kv_head][2][head_dim] f32 (16-byte aligned), largest first; zeros for a page
+ * that is none of the cache's. n * n_kv_head below 2^25. */
+int jepa_amd_cache_digest_read(int device, const jepa_amd_cache_shape * shape, const void * digest, const int32_t * page, int64_t n, float * bounds, void * stream);
+
+/* selected [n_rows][n_kv_head][n_select]: for each row and K/V head the pages (places in its sequence's table row) that it is to read, ascending, -1 behind the
+ * last. Of the pages that the row sees (causal_block as for jepa_amd_cache_attention) the first n_first and the last n_last (1 or more) are always taken, the
+ * others by score, the highest first and of equal ones the lower page; all of them where there are n_select or fewer (1 to 256). A page's score is the sum, over the
+ * query heads of the K/V head, of the largest value that the product of the head's query with a key within the page's bounds could have (for a scale above 0). Of the
+ * queries it takes the sums over those heads of their positive and of their negative elements, in 8 bits each: whole-number products, so that the choice is the same
+ * however a call is split. A row with a NaN or an infinity in these queries scores zero everywhere; pages that are none of the cache's come last. Rows of no
+ * sequence are left as they are. `work` is jepa_amd_cache_select_work_bytes() bytes (16-byte aligned, may be NULL where that is 0) under the same terms as
+ * jepa_amd_cache_attention's. */
+int64_t jepa_amd_cache_select_work_bytes(const jepa_amd_cache_shape * shape, int64_t n_seq, int64_t n_rows, int64_t table_width, int64_t n_select);
+int jepa_amd_cache_select(int device, const jepa_amd_cache_shape * shape, const void * digest, int type, const void * q, int64_t q_stride, int64_t n_seq,
+                          int64_t n_rows, const int32_t * row_start, const int32_t * kv_len, const int32_t * table, int64_t table_width,
+                          int64_t causal_block, int64_t n_first, int64_t n_last, int64_t n_select, int32_t * selected, void * work, int64_t work_bytes,
+                          void * stream);
+
+/* jepa_amd_cache_attention over the pages `selected` [n_rows][n_kv_head][n_select] of each row and K/V head, with its accuracy (keys and values always as
+ * they are held). Entries may come in any order; negative ones, pages past what the row sees and pages that are none of the cache's are passed over, tokens that it
+ * does not see are not read, and a page named twice counts twice. `work` as for jepa_amd_cache_select. */
+int64_t jepa_amd_cache_selected_work_bytes(const jepa_amd_cache_shape * shape, int64_t n_rows, int64_t n_select);
+int jepa_amd_cache_attention_selected(int device, const jepa_amd_cache_shape * shape, const void * cache, int type, const void * q, int64_t q_stride,
+                                      int64_t n_seq, int64_t n_rows, const int32_t * row_start, const int32_t * kv_len, const int32_t * table,
+                                      int64_t table_width, const int32_t * selected, int64_t n_select, float scale, int64_t causal_block, void * out,
+                                      int64_t out_stride, void * work, int64_t work_bytes, void * stream);
+
 /* Force the MFMA GEMM onto workgroup tile `index` for later launches whose n_out it divides; -1
  * restores the automatic choice. Process-wide (tests and tuning). Tiles (weight rows x tokens):
  * 0: 256x128, 1: 192x128, 2: 128x128, 3: 128x128 (other wave shape), 4: 64x128, 5: 128x64, 6: 256x64,

@@ -1,11 +1,13 @@
-// cache_api.cpp - the 4-bit paged key/value cache's entry points of include/jepa_amd.h: argument checks, then one or two
+// cache_api.cpp - entry points of include/jepa_amd.h for rotary positions and the 4-bit paged key/value cache: argument checks, then one or two
 // launches on the caller's stream. Nothing is allocated and nothing waits, so the calls can be captured into a graph.
 #include "../../include/jepa_amd.h"
 #include "cache_dev.h"
 #include "kernels.h"
 #include "model.h"
 
+#include <algorithm>
 #include <cmath>
+#include <iterator>
 
 namespace {
 
@@ -49,6 +51,50 @@ bool rows_ok(const char * who, const char * what, int type, const void * p, int6
     return true;
 }
 
+// the description of a rotation, checked; frequencies in more than 64 bits, each rounded once
+bool rope_of(const char * who, const jepa_amd_rope_axes * r, rope_map & m) {
+    if (!r) { jepa_log("jepa: %s: no rotation\n", who); return false; }
+    bool ok = r->head_dim >= 8 && r->head_dim <= 256 && r->head_dim % 8 == 0 && r->form >= 0 && r->form <= 3 && r->n_axes >= 1 && r->n_axes <= 4 &&
+              std::isfinite(r->theta) && r->theta > 0.0;
+    int rot = 0;
+    for (int a = 0; ok && a < r->n_axes; a++) {
+        ok = r->dims[a] >= 2 && r->dims[a] <= 256 && r->dims[a] % (r->form == 2 ? 16 : 2) == 0 && std::isfinite(r->scale[a]);
+        rot += r->dims[a];
+    }
+    if (!ok || rot > r->head_dim || (r->form == 3 && rot % 16)) {
+        jepa_log("jepa: %s: rotation of form %d over %d axes of heads of %d not supported (forms 0 to 3; 1 to 4 axes of an even number of dims each, of whole 16 "
+                 "in form 2, whole 16 together in form 3, no more than the head; heads of 8 to 256, whole 8; theta above 0, scales finite)\n",
+                 who, r->form, r->n_axes, r->head_dim);
+        return false;
+    }
+    m.form = r->form; m.hd = r->head_dim; m.rot = rot; m.n_axes = r->n_axes;
+    const bool halves = r->form >= 2;
+    std::fill(std::begin(m.rev), std::end(m.rev), 0.0);
+    std::fill(std::begin(m.axis), std::end(m.axis), (uint8_t) 0);
+    std::fill(std::begin(m.delta), std::end(m.delta), (int16_t) 0);
+    const long double two_pi = 6.283185307179586476925286766559L;
+    auto step_of = [&](int width) { return powl((long double) r->theta, -2.0L / width); };
+    auto put = [&](int e, int axis, long double f) { m.rev[e] = (double) (f * r->scale[axis] / two_pi); m.axis[e] = (uint8_t) axis; };
+    long double f = 1.0L, step = r->form == 3 ? step_of(rot) : 0.0L;
+    for (int a = 0, at = 0; a < r->n_axes; at += r->dims[a++]) {
+        const int w = r->dims[a], h = w / 2;
+        if (r->form != 3) { f = 1.0L; step = step_of(w); }
+        for (int i = 0; i < h; i++, f *= step) {
+            if (r->form == 0) { put(at + i, a, f); put(at + i + h, a, f); }      // the frequencies run twice through the section, across its pairs
+            if (r->form == 1) { put(at + 2 * i, a, f); put(at + 2 * i + 1, a, f); }
+            if (r->form == 2) { put(at + i, a, f); put(at + i + h, a, f); }
+            if (r->form == 3) { put(at / 2 + i, a, f); put(at / 2 + i + rot / 2, a, f); }
+        }
+        for (int i = 0; r->form == 2 && i < w / 8; i++) m.delta[at / 8 + i] = (int16_t) (i < w / 16 ? h : -h);
+    }
+    for (int i = 0; r->form == 3 && i < rot / 8; i++) m.delta[i] = (int16_t) (i < rot / 16 ? rot / 2 : -(rot / 2));
+    int leads = 0;
+    std::fill(std::begin(m.lead), std::end(m.lead), (uint8_t) 0);
+    for (int i = 0; i < m.hd / 8; i++)
+        if (!halves || m.delta[i] >= 0) m.lead[leads++] = (uint8_t) i;
+    return true;
+}
+
 // heads of rows that one launch takes (its threads are below 2^32, 16 of them for a head of a row, or 64 for one of a few rows)
 bool grid_ok(const char * who, int64_t n) {
     if (n < (int64_t) 1 << 27) return true;
@@ -66,6 +112,32 @@ bool all(const char * who, std::initializer_list<const void *> ps) {
     for (const void * p : ps)
         if (!p) { jepa_log("jepa: %s: a pointer is NULL\n", who); return false; }
     return true;
+}
+
+bool digest_ok(const char * who, const void * digest) {
+    if (digest && (uintptr_t) digest % 16 == 0) return true;
+    jepa_log("jepa: %s: the digests must be 16-byte aligned device memory\n", who);
+    return false;
+}
+
+bool take_ok(const char * who, int64_t first, int64_t last, int64_t take) {
+    if (take >= 1 && take <= CACHE_MOST_SELECTED && first >= 0 && first <= take && last >= 0 && last <= take - first) return true;
+    jepa_log("jepa: %s: %lld pages of a row, %lld first and %lld last ones among them, not supported (1 to %d pages)\n", who, (long long) take, (long long) first,
+             (long long) last, CACHE_MOST_SELECTED);
+    return false;
+}
+
+// (threads of a launch are below 2^32)
+bool blocks_ok(const char * who, int64_t blocks) {
+    if (blocks < 1 << 24) return true;
+    jepa_log("jepa: %s: %lld workgroups in one call (below 2^24)\n", who, (long long) blocks);
+    return false;
+}
+
+bool work_ok(const char * who, const void * work, int64_t bytes, int64_t need) {
+    if (need == 0 || (work && (uintptr_t) work % 16 == 0 && bytes >= need)) return true;
+    jepa_log("jepa: %s: %lld bytes of work space, %lld needed (16-byte aligned)\n", who, (long long) bytes, (long long) need);
+    return false;
 }
 
 // `f` with `device` current, which it is no longer afterwards if it was not before
@@ -174,4 +246,139 @@ extern "C" int jepa_amd_cache_attention(int device, const jepa_amd_cache_shape *
     a.block = cache_block_of(causal_block); a.row_start = row_start; a.kv_len = kv_len; a.table = table; a.n_seq = (int) n_seq; a.width = (int) table_width;
     a.n_head = c.n_head; a.n_kv_head = c.n_kv_head; a.page_size = c.page_size; a.scale = scale; a.work = (float *) work;
     return on_device(who, device, [&] { return n_rows && n_seq ? launch_cache_attention(c, type, a, (hipStream_t) stream) : hipSuccess; });
+}
+
+extern "C" int jepa_amd_rope_rows(int device, const jepa_amd_rope_axes * rope, int type, const void * x, int64_t x_stride, int64_t n_rows, int n_head,
+                                  const int32_t * pos, int backward, void * out, int64_t out_stride, void * stream) {
+    const char * who = "jepa_amd_rope_rows";
+    rope_map m;
+    if (!rope_of(who, rope, m)) return -1;
+    if (n_head < 1 || n_head > 4096 || n_rows < 0 || n_rows * n_head >= (int64_t) 1 << 26 || n_rows >= I31) {
+        jepa_log("jepa: %s: %lld rows of %d heads not supported (up to 4096 heads, below 2^26 heads of rows)\n", who, (long long) n_rows, n_head);
+        return -1;
+    }
+    const int64_t width = (int64_t) n_head * m.hd;
+    if (!rows_ok(who, "x", type, x, x_stride, width, n_rows) || !rows_ok(who, "out", type, out, out_stride, width, n_rows) || (n_rows && !all(who, {pos}))) return -1;
+    if (x == out && x_stride != out_stride) { jepa_log("jepa: %s: rows in place must keep their stride\n", who); return -1; }
+    rope_args a;
+    a.x = x; a.out = out; a.ldx = x_stride; a.ldo = out_stride; a.n_rows = n_rows; a.pos = pos; a.n_head = n_head; a.hd = m.hd; a.back = backward != 0;
+    return on_device(who, device, [&] { return n_rows ? launch_rope_axes(a, m, type, (hipStream_t) stream) : hipSuccess; });
+}
+
+extern "C" int jepa_amd_cache_append(int device, const jepa_amd_cache_shape * shape, const jepa_amd_rope_axes * rope, void * cache, int type, const void * q,
+                                     int64_t q_stride, const void * k, int64_t k_stride, const void * v, int64_t v_stride, int64_t n_rows, const int32_t * pos,
+                                     const int64_t * slot, void * q_out, int64_t q_out_stride, void * stream) {
+    const char * who = "jepa_amd_cache_append";
+    cache_shape c;
+    rope_map m;
+    if (!shape_of(who, shape, c) || !sizes_ok(who, c, 0, n_rows, 1) || !rope_of(who, rope, m)) return -1;
+    if (m.hd != c.hd) { jepa_log("jepa: %s: a rotation of heads of %d for a cache of %d\n", who, m.hd, c.hd); return -1; }
+    const int64_t width = (int64_t) c.n_kv_head * c.hd, q_width = (int64_t) c.n_head * c.hd;
+    if (!cache_ok(who, cache) || !rows_ok(who, "k", type, k, k_stride, width, n_rows) || !rows_ok(who, "v", type, v, v_stride, width, n_rows) ||
+        (q && (!rows_ok(who, "q", type, q, q_stride, q_width, n_rows) || !rows_ok(who, "q_out", type, q_out, q_out_stride, q_width, n_rows))) ||
+        (n_rows && !all(who, {pos, slot})))
+        return -1;
+    if (n_rows * c.n_head >= (int64_t) 1 << 26) { jepa_log("jepa: %s: %lld heads of rows in one call (below 2^26)\n", who, (long long) (n_rows * c.n_head)); return -1; }
+    if (q && q == q_out && q_stride != q_out_stride) { jepa_log("jepa: %s: rows in place must keep their stride\n", who); return -1; }
+    append_args a;
+    a.cache = (unsigned char *) cache; a.k = k; a.v = v; a.ldk = k_stride; a.ldv = v_stride; a.n_rows = n_rows; a.n_slots = c.n_pages * c.page_size; a.pos = pos;
+    a.slots = slot; a.n_kv_head = c.n_kv_head; a.page_shift = __builtin_ctz((unsigned) c.page_size);
+    rope_args r;
+    r.x = q; r.out = q_out; r.ldx = q_stride; r.ldo = q_out_stride; r.n_rows = n_rows; r.pos = pos; r.n_head = c.n_head; r.hd = c.hd;
+    return on_device(who, device, [&] { return n_rows ? launch_cache_append(a, r, m, type, (hipStream_t) stream) : hipSuccess; });
+}
+
+extern "C" int64_t jepa_amd_cache_digest_bytes(const jepa_amd_cache_shape * shape) {
+    cache_shape c;
+    if (!shape_of("jepa_amd_cache_digest_bytes", shape, c)) return -1;
+    return c.n_kv_head * cache_digest_bytes(c.hd);
+}
+
+extern "C" int jepa_amd_cache_digest(int device, const jepa_amd_cache_shape * shape, const void * cache, int64_t n_seq, int64_t n_rows, const int32_t * row_start,
+                                     const int32_t * kv_len, const int32_t * table, int64_t table_width, void * digest, void * stream) {
+    const char * who = "jepa_amd_cache_digest";
+    cache_shape c;
+    if (!shape_of(who, shape, c) || !sizes_ok(who, c, n_seq, n_rows, table_width) || !cache_ok(who, cache) || !digest_ok(who, digest)) return -1;
+    const bool some = n_seq && n_rows;
+    if (some && (!all(who, {row_start, kv_len, table}) || !blocks_ok(who, cache_digest_blocks(c, n_seq, n_rows)))) return -1;
+    cache_digest_args a;
+    a.cache = (const unsigned char *) cache; a.digest = (unsigned char *) digest; a.row_start = row_start; a.kv_len = kv_len; a.table = table; a.n_rows = n_rows;
+    a.n_pages = c.n_pages; a.n_seq = (int) n_seq; a.width = (int) table_width; a.n_kv_head = c.n_kv_head; a.page_size = c.page_size;
+    return on_device(who, device, [&] { return some ? launch_cache_digest(a, c.hd, (hipStream_t) stream) : hipSuccess; });
+}
+
+extern "C" int jepa_amd_cache_digest_read(int device, const jepa_amd_cache_shape * shape, const void * digest, const int32_t * page, int64_t n, float * bounds, void * stream) {
+    const char * who = "jepa_amd_cache_digest_read";
+    cache_shape c;
+    if (!shape_of(who, shape, c) || !digest_ok(who, digest)) return -1;
+    if (n < 0 || n >= I31 || n * c.n_kv_head >= 1 << 25) { jepa_log("jepa: %s: %lld pages of %d heads in one call (below 2^25 heads)\n", who, (long long) n, c.n_kv_head); return -1; }
+    if (n && (!all(who, {page, bounds}))) return -1;
+    if ((uintptr_t) bounds % 16) { jepa_log("jepa: %s: the bounds must be 16-byte aligned\n", who); return -1; }
+    return on_device(who, device, [&] {
+        return n ? launch_cache_digest_read((const unsigned char *) digest, page, n, c.n_pages, c.n_kv_head, c.hd, bounds, (hipStream_t) stream) : hipSuccess;
+    });
+}
+
+extern "C" int64_t jepa_amd_cache_select_work_bytes(const jepa_amd_cache_shape * shape, int64_t n_seq, int64_t n_rows, int64_t table_width, int64_t n_select) {
+    const char * who = "jepa_amd_cache_select_work_bytes";
+    cache_shape c;
+    if (!shape_of(who, shape, c) || !sizes_ok(who, c, n_seq, n_rows, table_width) || !take_ok(who, 0, 0, n_select)) return -1;
+    return cache_select_work_bytes(c, n_rows, table_width, (int) n_select);
+}
+
+extern "C" int jepa_amd_cache_select(int device, const jepa_amd_cache_shape * shape, const void * digest, int type, const void * q, int64_t q_stride, int64_t n_seq,
+                                     int64_t n_rows, const int32_t * row_start, const int32_t * kv_len, const int32_t * table, int64_t table_width,
+                                     int64_t causal_block, int64_t n_first, int64_t n_last, int64_t n_select, int32_t * selected, void * work, int64_t work_bytes,
+                                     void * stream) {
+    const char * who = "jepa_amd_cache_select";
+    cache_shape c;
+    if (!shape_of(who, shape, c) || !sizes_ok(who, c, n_seq, n_rows, table_width) || !digest_ok(who, digest) ||
+        !rows_ok(who, "q", type, q, q_stride, (int64_t) c.n_head * c.hd, n_rows) || !grid_ok(who, n_rows * c.n_head) || !take_ok(who, n_first, n_last, n_select))
+        return -1;
+    if (causal_block < 0 || n_last < 1) {
+        jepa_log("jepa: %s: causal block %lld, %lld last pages (1 or more: the page that a row ends in is one)\n", who, (long long) causal_block, (long long) n_last);
+        return -1;
+    }
+    const bool some = n_seq && n_rows;
+    if (some && (!all(who, {row_start, kv_len, table, selected}) || !blocks_ok(who, cache_select_blocks(c, n_seq, n_rows, table_width)) ||
+                 !work_ok(who, work, work_bytes, cache_select_work_bytes(c, n_rows, table_width, (int) n_select))))
+        return -1;
+    cache_select_args a;
+    a.digest = (const unsigned char *) digest; a.q = q; a.selected = selected; a.ldq = q_stride; a.n_rows = n_rows; a.n_pages = c.n_pages; a.row_start = row_start;
+    a.kv_len = kv_len; a.table = table; a.n_seq = (int) n_seq; a.width = (int) table_width; a.n_head = c.n_head; a.n_kv_head = c.n_kv_head; a.page_size = c.page_size;
+    a.block = cache_block_of(causal_block); a.first = (int) n_first; a.last = (int) n_last; a.take = (int) n_select; a.work = (float *) work;
+    return on_device(who, device, [&] { return some ? launch_cache_select(c, type, a, (hipStream_t) stream) : hipSuccess; });
+}
+
+extern "C" int64_t jepa_amd_cache_selected_work_bytes(const jepa_amd_cache_shape * shape, int64_t n_rows, int64_t n_select) {
+    const char * who = "jepa_amd_cache_selected_work_bytes";
+    cache_shape c;
+    if (!shape_of(who, shape, c) || !sizes_ok(who, c, 0, n_rows, 1) || !take_ok(who, 0, 0, n_select)) return -1;
+    return cache_selected_work_bytes(c, n_rows, (int) n_select);
+}
+
+extern "C" int jepa_amd_cache_attention_selected(int device, const jepa_amd_cache_shape * shape, const void * cache, int type, const void * q, int64_t q_stride,
+                                                 int64_t n_seq, int64_t n_rows, const int32_t * row_start, const int32_t * kv_len, const int32_t * table,
+                                                 int64_t table_width, const int32_t * selected, int64_t n_select, float scale, int64_t causal_block, void * out,
+                                                 int64_t out_stride, void * work, int64_t work_bytes, void * stream) {
+    const char * who = "jepa_amd_cache_attention_selected";
+    cache_shape c;
+    if (!shape_of(who, shape, c) || !sizes_ok(who, c, n_seq, n_rows, table_width)) return -1;
+    const int64_t width = (int64_t) c.n_head * c.hd;
+    if (!cache_ok(who, cache) || !rows_ok(who, "q", type, q, q_stride, width, n_rows) || !rows_ok(who, "out", type, out, out_stride, width, n_rows) ||
+        !grid_ok(who, n_rows * c.n_head) || !take_ok(who, 0, 0, n_select))
+        return -1;
+    if (!std::isfinite(scale) || causal_block < 0) {
+        jepa_log("jepa: %s: scale %g, causal block %lld\n", who, (double) scale, (long long) causal_block);
+        return -1;
+    }
+    const bool some = n_seq && n_rows;
+    if (some && (!all(who, {row_start, kv_len, table, selected}) || !blocks_ok(who, cache_selected_blocks(c, n_rows, (int) n_select)) ||
+                 !work_ok(who, work, work_bytes, cache_selected_work_bytes(c, n_rows, (int) n_select))))
+        return -1;
+    cache_selected_args a;
+    a.cache = (const unsigned char *) cache; a.q = q; a.out = out; a.ldq = q_stride; a.ldo = out_stride; a.n_rows = n_rows; a.n_pages = c.n_pages;
+    a.row_start = row_start; a.kv_len = kv_len; a.table = table; a.selected = selected; a.n_seq = (int) n_seq; a.width = (int) table_width; a.n_head = c.n_head;
+    a.n_kv_head = c.n_kv_head; a.page_size = c.page_size; a.block = cache_block_of(causal_block); a.take = (int) n_select; a.scale = scale; a.work = (float *) work;
+    return on_device(who, device, [&] { return some ? launch_cache_selected(c, type, a, (hipStream_t) stream) : hipSuccess; });
 }

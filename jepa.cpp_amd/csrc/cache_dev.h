@@ -22,6 +22,7 @@
 
 constexpr int CACHE_STRIP = 16;              // tokens of a strip
 constexpr int CACHE_MAX_SEQ = 4096;          // sequences of one step (the planner's LDS)
+constexpr int CACHE_MOST_SELECTED = 256;     // pages that a row selects
 
 CACHE_HD int64_t cache_strip_bytes(int hd) { return 18 * (int64_t) hd; }
 CACHE_HD int64_t cache_page_bytes(int n_kv_head, int page_size, int hd) { return (int64_t) n_kv_head * (page_size / CACHE_STRIP) * cache_strip_bytes(hd); }
@@ -55,6 +56,9 @@ CACHE_HD cache_seq_step cache_step_of(int32_t have, int32_t come, int32_t width,
     s.len = s.bad ? (int32_t) (have < 0 ? 0 : have > cap ? cap : have) : (int32_t) keep;
     return s;
 }
+// A page's digest for one head: hd largest values of K as signed codes, hd smallest, their f32 scale and 12 bytes of zeros
+CACHE_HD int64_t cache_digest_bytes(int hd) { return 2 * (int64_t) hd + 16; }
+
 CACHE_HD uint32_t cache_add_sat(uint32_t a, uint32_t b) { return a + b < a ? 0xffffffffu : a + b; }
 // first index of the ascending ends[n] that is greater than x (n if none)
 CACHE_HD int cache_find(const uint32_t * ends, int n, uint32_t x) {

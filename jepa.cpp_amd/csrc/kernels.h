@@ -161,6 +161,80 @@ int64_t cache_attention_work_bytes(const cache_shape & c, int64_t n_seq, int64_t
 int64_t cache_attention_blocks(const cache_shape & c, int type, int64_t n_seq, int64_t n_rows, int64_t width);      // workgroups of the launch (256 threads)
 hipError_t launch_cache_attention(const cache_shape & c, int type, const cache_attn_args & a, hipStream_t s);
 
+// Rotary positions of several axes (rope_dev.h). Element e of a head turns by rev[e] revolutions a position of axis[e]; rot of the hd
+// elements do. form 0, 1: with its neighbour; 2, 3: elements of a chunk of 8 with those `delta` further (positive in the first half
+// of a section, negative in the second, 0 where they do not turn); lead: the chunks that are no second halves, in order.
+struct rope_map {
+    int form = 0, hd = 0, rot = 0, n_axes = 0;
+    double rev[256];
+    uint8_t axis[256], lead[32];
+    int16_t delta[32];
+};
+struct rope_args {
+    const void * x = nullptr;
+    void * out = nullptr;
+    int64_t ldx = 0, ldo = 0, n_rows = 0;
+    const int32_t * pos = nullptr;
+    int n_head = 0, hd = 0, back = 0;
+    int units = 0, rows_per = 0, heads_per = 0, head_blocks = 0;      // set by the launcher
+};
+hipError_t launch_rope_axes(const rope_args & a, const rope_map & m, int type, hipStream_t s);
+// rows of keys rotated and quantized into their slots with their values, rows of queries (q.x may be null) rotated
+struct append_args {
+    unsigned char * cache = nullptr;
+    const void * k = nullptr, * v = nullptr;
+    int64_t ldk = 0, ldv = 0, n_rows = 0, n_slots = 0;
+    const int32_t * pos = nullptr;
+    const int64_t * slots = nullptr;
+    int n_kv_head = 0, page_shift = 0;
+    int heads_per = 0, head_blocks = 0;      // set by the launcher
+    unsigned kv_blocks = 0;
+};
+hipError_t launch_cache_append(const append_args & a, const rope_args & q, const rope_map & m, int type, hipStream_t s);
+
+// Digests of pages: [n_pages][n_kv_head][cache_digest_bytes(hd)]. The pages that n_rows packed rows went to are made anew.
+struct cache_digest_args {
+    const unsigned char * cache = nullptr;
+    unsigned char * digest = nullptr;
+    const int32_t * row_start = nullptr, * kv_len = nullptr, * table = nullptr;
+    int64_t n_rows = 0, n_pages = 0;
+    int n_seq = 0, width = 0, n_kv_head = 0, page_size = 0;
+    int rows_per = 0;      // set by the launcher
+};
+int64_t cache_digest_blocks(const cache_shape & c, int64_t n_seq, int64_t n_rows);      // workgroups of the launch (256 threads)
+hipError_t launch_cache_digest(const cache_digest_args & a, int hd, hipStream_t s);
+hipError_t launch_cache_digest_read(const unsigned char * digest, const int32_t * page, int64_t n, int64_t n_pages, int n_kv_head, int hd, float * bounds, hipStream_t s);
+// the pages that each row and K/V head selects; `work` holds cache_select_work_bytes
+struct cache_select_args {
+    const unsigned char * digest = nullptr;
+    const void * q = nullptr;
+    int32_t * selected = nullptr;
+    int64_t ldq = 0, n_rows = 0, n_pages = 0;
+    const int32_t * row_start = nullptr, * kv_len = nullptr, * table = nullptr;
+    int n_seq = 0, width = 0, n_head = 0, n_kv_head = 0, page_size = 0, block = 0, first = 0, last = 0, take = 0;
+    float * work = nullptr;
+    int pieces = 0, piece = 0;      // set by the launcher
+};
+int64_t cache_select_work_bytes(const cache_shape & c, int64_t n_rows, int64_t width, int take);
+int64_t cache_select_blocks(const cache_shape & c, int64_t n_seq, int64_t n_rows, int64_t width);
+hipError_t launch_cache_select(const cache_shape & c, int type, const cache_select_args & a, hipStream_t s);
+// attention of packed rows over selected pages; `work` holds cache_selected_work_bytes
+struct cache_selected_args {
+    const unsigned char * cache = nullptr;
+    const void * q = nullptr;
+    void * out = nullptr;
+    int64_t ldq = 0, ldo = 0, n_rows = 0, n_pages = 0;
+    const int32_t * row_start = nullptr, * kv_len = nullptr, * table = nullptr, * selected = nullptr;
+    int n_seq = 0, width = 0, n_head = 0, n_kv_head = 0, page_size = 0, block = 0, take = 0;
+    float scale = 0;
+    float * work = nullptr;
+    int64_t parts = 0;                            // set by the launcher
+    int tiles = 0, pieces = 0, piece_tiles = 0;
+};
+int64_t cache_selected_work_bytes(const cache_shape & c, int64_t n_rows, int take);
+int64_t cache_selected_blocks(const cache_shape & c, int64_t n_rows, int take);      // workgroups of the launch (256 threads)
+hipError_t launch_cache_selected(const cache_shape & c, int type, const cache_selected_args & a, hipStream_t s);
+
 // weight expansion at load: raw ggml blocks (device) -> dev_linear operand arrays (int8: q4_0 rows
 // go to the int8 layout of q8_0 whatever their length, for a linear whose parts mix the two)
 void launch_repack(int gtype, const void * raw, int64_t n_out, int64_t n_in, void * w, void * wd,

@@ -43,6 +43,19 @@ class CacheShape(C.Structure):
     _fields_ = [("n_head", C.c_int32), ("n_kv_head", C.c_int32), ("head_dim", C.c_int32), ("page_size", C.c_int32), ("n_pages", C.c_int64)]
 
 
+class RopeAxes(C.Structure):
+    """Rotary positions of several axes (jepa_amd_rope_axes)."""
+    _fields_ = [("head_dim", C.c_int32), ("form", C.c_int32), ("n_axes", C.c_int32), ("dims", C.c_int32 * 4), ("theta", C.c_double), ("scale", C.c_double * 4)]
+
+    @classmethod
+    def of(cls, head_dim, form, dims, theta=10000.0, scale=None):
+        """Sections of `dims` elements, one for each axis, whose positions are multiplied by `scale` (1 where it is not given)."""
+        scale = [1.0] * len(dims) if scale is None else list(scale)
+        if not 1 <= len(dims) <= 4 or len(scale) != len(dims):
+            raise ValueError(f"{len(dims)} axes and {len(scale)} scales: 1 to 4 of both")
+        return cls(head_dim, form, len(dims), (C.c_int32 * 4)(*dims), theta, (C.c_double * 4)(*scale))
+
+
 _lib = None
 
 
@@ -134,6 +147,16 @@ def lib() -> C.CDLL:
         "jepa_amd_cache_read": (C.c_int, [C.c_int, C.POINTER(CacheShape), vp, vp, i64, C.c_int, vp, i64, vp, i64, vp]),
         "jepa_amd_cache_attention": (C.c_int, [C.c_int, C.POINTER(CacheShape), vp, C.c_int, vp, i64, i64, i64, vp, vp, vp, i64, C.c_float, i64,
                                                vp, i64, vp, i64, vp]),
+        "jepa_amd_rope_rows": (C.c_int, [C.c_int, C.POINTER(RopeAxes), C.c_int, vp, i64, i64, C.c_int, vp, C.c_int, vp, i64, vp]),
+        "jepa_amd_cache_append": (C.c_int, [C.c_int, C.POINTER(CacheShape), C.POINTER(RopeAxes), vp, C.c_int, vp, i64, vp, i64, vp, i64, i64, vp, vp, vp, i64, vp]),
+        "jepa_amd_cache_digest_bytes": (i64, [C.POINTER(CacheShape)]),
+        "jepa_amd_cache_digest": (C.c_int, [C.c_int, C.POINTER(CacheShape), vp, i64, i64, vp, vp, vp, i64, vp, vp]),
+        "jepa_amd_cache_digest_read": (C.c_int, [C.c_int, C.POINTER(CacheShape), vp, vp, i64, vp, vp]),
+        "jepa_amd_cache_select_work_bytes": (i64, [C.POINTER(CacheShape), i64, i64, i64, i64]),
+        "jepa_amd_cache_select": (C.c_int, [C.c_int, C.POINTER(CacheShape), vp, C.c_int, vp, i64, i64, i64, vp, vp, vp, i64, i64, i64, i64, i64, vp, vp, i64, vp]),
+        "jepa_amd_cache_selected_work_bytes": (i64, [C.POINTER(CacheShape), i64, i64]),
+        "jepa_amd_cache_attention_selected": (C.c_int, [C.c_int, C.POINTER(CacheShape), vp, C.c_int, vp, i64, i64, i64, vp, vp, vp, i64, vp, i64, C.c_float, i64,
+                                                        vp, i64, vp, i64, vp]),
         "jepa_amd_mfma_probe": (C.c_int, [C.c_int, vp, vp, vp]),
         "jepa_amd_copy": (C.c_int, [C.c_int, vp, vp, i64, C.c_int, C.POINTER(C.c_double)]),
         "jepa_amd_gemm_step_probe": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int, C.POINTER(C.c_double)]),
