@@ -304,7 +304,7 @@ extern "C" int jepa_amd_cache_digest(int device, const jepa_amd_cache_shape * sh
     cache_digest_args a;
     a.cache = (const unsigned char *) cache; a.digest = (unsigned char *) digest; a.row_start = row_start; a.kv_len = kv_len; a.table = table; a.n_rows = n_rows;
     a.n_pages = c.n_pages; a.n_seq = (int) n_seq; a.width = (int) table_width; a.n_kv_head = c.n_kv_head; a.page_size = c.page_size;
-    return on_device(who, device, [&] { return some ? launch_cache_digest(a, c.hd, (hipStream_t) stream) : hipSuccess; });
+    return on_device(who, device, [&] { return some ? launch_cache_digest(c, a, (hipStream_t) stream) : hipSuccess; });
 }
 
 extern "C" int jepa_amd_cache_digest_read(int device, const jepa_amd_cache_shape * shape, const void * digest, const int32_t * page, int64_t n, float * bounds, void * stream) {

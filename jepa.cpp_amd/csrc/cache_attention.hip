@@ -74,20 +74,6 @@ template <int C> __device__ __forceinline__ float piece_inv(float keys, float un
     return __builtin_amdgcn_rcpf(fmaxf(keys * (1.0f / units), (float) piece_min(C)));
 }
 
-// sums over the lanes up to this one, and over all of them, in the VALU: within rows of 16 lanes, then across rows
-template <typename X>
-__device__ __forceinline__ X wave_scan(X x) {
-    static_assert(sizeof(X) == 4, "one register");
-#define DPP(ctrl, rows) __builtin_bit_cast(X, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), ctrl, rows, 0xf, true))
-    x += DPP(0x111, 0xf);      // row_shr 1, 2, 4, 8
-    x += DPP(0x112, 0xf);
-    x += DPP(0x114, 0xf);
-    x += DPP(0x118, 0xf);
-    x += DPP(0x142, 0xa);      // row_bcast 15, 31
-    x += DPP(0x143, 0xc);
-#undef DPP
-    return x;
-}
 __device__ __forceinline__ float wave_max(float x) {      // (of values that are not negative)
 #define DPP(ctrl, rows) __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), ctrl, rows, 0xf, true))
     x = fmaxf(x, DPP(0x111, 0xf));
@@ -99,9 +85,6 @@ __device__ __forceinline__ float wave_max(float x) {      // (of values that are
 #undef DPP
     return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
 }
-template <typename X>
-__device__ __forceinline__ X wave_add(X x) { return __builtin_bit_cast(X, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wave_scan(x)), 63)); }
-
 // Unit x of the call, for column tiles of C. Every thread gets it, in scalar registers; false past the last. Sequences whose rows overlap
 // may have more units than the launch has workgroups: then nothing is computed, for a tile that only some of its pieces come to would
 // leave its counter in `work` short.

@@ -78,18 +78,48 @@ __device__ __forceinline__ seq_view view_of(const int32_t * row_start, const int
 template <typename A> __device__ __forceinline__ seq_view view_of(const A & a, int i) { return view_of(a.row_start, a.kv_len, a.n_rows, a.width, a.page_size, i); }
 
 __device__ __forceinline__ int32_t uniform(int32_t x) { return __builtin_amdgcn_readfirstlane(x); }
-// the sequence of packed row r, for the whole wave: two rounds of loads at most (CACHE_MAX_SEQ is 64 x 64); -1: none. In bounds whatever the array holds.
-__device__ __forceinline__ int seq_of_row(const int32_t * row_start, int n_seq, int32_t r) {
+// sums over the lanes up to this one, and over all of them, in the VALU: within rows of 16 lanes, then across rows
+template <typename X>
+__device__ __forceinline__ X wave_scan(X x) {
+    static_assert(sizeof(X) == 4, "one register");
+#define DPP(ctrl, rows) __builtin_bit_cast(X, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), ctrl, rows, 0xf, true))
+    x += DPP(0x111, 0xf);      // row_shr 1, 2, 4, 8
+    x += DPP(0x112, 0xf);
+    x += DPP(0x114, 0xf);
+    x += DPP(0x118, 0xf);
+    x += DPP(0x142, 0xa);      // row_bcast 15, 31
+    x += DPP(0x143, 0xc);
+#undef DPP
+    return x;
+}
+template <typename X>
+__device__ __forceinline__ X wave_add(X x) { return __builtin_bit_cast(X, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wave_scan(x)), 63)); }
+
+// The sequence of packed row r and its view, for the whole wave; false: none. A call of up to 64 sequences takes one round of loads, a sequence a lane, more take
+// two to find it and one for its view. In bounds whatever the arrays hold.
+template <typename A>
+__device__ __forceinline__ bool place_of(const A & a, int32_t r, int & seq, seq_view & v) {
     static_assert(CACHE_MAX_SEQ <= 64 * 64, "a sequence a lane, or 64");
-    const int lane = (int) threadIdx.x & 63, step = (n_seq + 63) >> 6;
-    const int32_t * ends = row_start + 1;
-    int at = (int) __popcll(__ballot(ends[min((lane + 1) * step, n_seq) - 1] <= r)) * step;
-    if (at >= n_seq) return -1;
-    if (step > 1) {
-        const int i = at + lane;
-        at += (int) __popcll(__ballot(lane < step && i < n_seq && ends[min(i, n_seq - 1)] <= r));
+    const int lane = (int) threadIdx.x & 63;
+    if (a.n_seq <= 64) {
+        const int i = min(lane, a.n_seq - 1);
+        const seq_view mine = view_of(a, i);
+        const uint64_t has = __ballot(lane < a.n_seq && r >= mine.row0 && r < mine.row0 + mine.rows);
+        if (!has) return false;
+        seq = __builtin_ctzll(has);
+        v = {__builtin_amdgcn_readlane(mine.row0, seq), __builtin_amdgcn_readlane(mine.rows, seq), __builtin_amdgcn_readlane(mine.len, seq)};
+        return true;
     }
-    return at < n_seq && row_start[at] <= r ? uniform(at) : -1;
+    const int step = (a.n_seq + 63) >> 6;
+    const int32_t * ends = a.row_start + 1;
+    int at = (int) __popcll(__ballot(ends[min((lane + 1) * step, a.n_seq) - 1] <= r)) * step;
+    if (at >= a.n_seq) return false;
+    const int i = at + lane;
+    at += (int) __popcll(__ballot(lane < step && i < a.n_seq && ends[min(i, a.n_seq - 1)] <= r));
+    if (at >= a.n_seq) return false;
+    seq = uniform(at);
+    v = view_of(a, seq);
+    return r >= v.row0 && r < v.row0 + v.rows;
 }
 
 template <typename T>

@@ -3,8 +3,9 @@
 //   hi_n = max_t k_tn, lo_n = min_t k_tn over the page's tokens t (none that is NaN), s = max_n max(|hi_n|, |lo_n|)
 //   codes rint(hi_n * fl(127 / s)), rint(lo_n * fl(127 / s)), scale fl(s / 127); all zero where s is below 2^-100
 //
-// A wave has one page and K/V head. Its lanes read K's codes as the attention does (lane 16 g + token: dims 32 b + 8 g .. + 7 of
-// every block b), multiply them by the token's scale (f32, exact: 4 bits times 11), keep the largest and smallest over the strips and join the 16 tokens' lanes.
+// A wave has one K/V head of the pages that some rows lie in, mostly one. A lane takes 8 dimensions (a word of codes) of a few tokens of each strip, so that
+// most of the largest and smallest are found in its registers and the few lanes of the same dimensions are joined by DPP. AHEAD strips, up to four of a page, are
+// in flight (all four for pages of one strip were 35 us for 41000 tokens of 8 x 128, one is 21).
 #include "cache_attn_dev.h"
 #include "common.h"
 
@@ -14,85 +15,93 @@ namespace {
 
 constexpr float LEAST = 0x1p-100f;
 
-template <int HD>
+#define DPP(x, ctrl) __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), ctrl, 0xf, 0xf, true))
+// the largest over aligned groups of N lanes: pairs, quads, mirrored halves of 16, mirrored 16
+template <int N>
+__device__ __forceinline__ float max_of(float x) {
+    x = fmaxf(x, DPP(x, 0xb1));
+    x = fmaxf(x, DPP(x, 0x4e));
+    if constexpr (N >= 8) x = fmaxf(x, DPP(x, 0x141));
+    if constexpr (N >= 16) x = fmaxf(x, DPP(x, 0x140));
+    return x;
+}
+#undef DPP
+
+template <int HD, int AHEAD>
 __global__ __launch_bounds__(NT) void k_cache_digest(cache_digest_args a) {
-    constexpr int NB = HD / 32, WORDS = 2 * HD / 4;      // of codes
-    __shared__ __attribute__((aligned(16))) float box[4][2 * HD];
-    const int tid = (int) threadIdx.x, lane = tid & 63, l15 = lane & 15, g = lane >> 4, wv = uniform(tid >> 6), kvh = (int) (blockIdx.x % (unsigned) a.n_kv_head);
-    const int64_t r0 = (int64_t) (blockIdx.x / (unsigned) a.n_kv_head) * a.rows_per, r1 = min(r0 + a.rows_per, a.n_rows);
+    // lanes of the same dimensions, tokens of each: 64 lanes are 4 NB words of codes (of 8 dimensions) times TL (48 of 64 for three blocks)
+    constexpr int NB = HD / 32, TL = HD == 32 ? 16 : HD == 64 ? 8 : 4, TOKENS = 16 / TL;
+    const int lane = (int) threadIdx.x & 63, tl = lane % TL, word = min(lane / TL, 4 * NB - 1), g = word / NB, b = word % NB;
+    const int64_t unit = (int64_t) blockIdx.x * 4 + uniform((int) threadIdx.x >> 6);
+    const int kvh = (int) (unit % a.n_kv_head);
+    const int64_t r0 = unit / a.n_kv_head * a.rows_per, r1 = min(r0 + a.rows_per, a.n_rows);
     const int page_shift = __builtin_ctz((unsigned) a.page_size), strips_of_page = a.page_size / 16;
-    int at = 0;      // pages of the workgroup so far, dealt to its waves
+    uint32_t k1024 = 0x64006400u;
+    asm volatile("" : "+v"(k1024));
     for (int64_t r = r0; r < r1;) {
-        const int i = seq_of_row(a.row_start, a.n_seq, (int32_t) r);
-        if (i < 0) {      // before the first sequence, or behind the last
+        int i;
+        seq_view v;
+        if (!place_of(a, (int32_t) r, i, v)) {      // before the first sequence, or behind the last
             if (r >= a.row_start[0]) break;
             r = min((int64_t) a.row_start[0], r1);
             continue;
         }
-        const seq_view v = view_of(a, i);
         const int64_t end = min(r1, (int64_t) v.row0 + v.rows);
-        if (end <= r) { r++; continue; }      // (row_start that does not ascend)
         // the pages that begin within these rows, and the sequence's first
         const int64_t pos = (int64_t) v.len - v.rows + (r - v.row0), pos_end = pos + (end - r);
         auto page_from = [&](int64_t t) { return (int32_t) (((t < 0 ? 0 : t) + a.page_size - 1) >> page_shift); };      // the first one that begins at t or later
         const int32_t p0 = r == v.row0 ? (int32_t) ((pos < 0 ? 0 : pos) >> page_shift) : page_from(pos), p1 = page_from(pos_end);
         for (int32_t p = p0; p < p1; p++) {
-            if ((at++ & 3) != wv) continue;
             const int64_t page = uniform(a.table[(int64_t) i * a.width + p]);
             if (page < 0 || page >= a.n_pages) continue;
             const int tokens = min(a.page_size, v.len - (p << page_shift));
-            float hi[NB * 8], lo[NB * 8];
+            const unsigned char * strips = a.cache + (page * a.n_kv_head + kvh) * strips_of_page * (18 * HD);
+            float hi[8], lo[8];
 #pragma unroll
-            for (int j = 0; j < NB * 8; j++) { hi[j] = -INFINITY; lo[j] = INFINITY; }
-            uint32_t k1024 = 0x64006400u;
-            asm volatile("" : "+v"(k1024));
-            for (int t = 0; t * 16 < tokens; t++) {
-                const brsrc s = make_brsrc(a.cache + ((page * a.n_kv_head + kvh) * strips_of_page + t) * (18 * HD), 18 * HD);
-                uint32_t w[NB];
-                load_words<NB>(w, s, lane * (4 * NB), 0);
+            for (int j = 0; j < 8; j++) { hi[j] = -INFINITY; lo[j] = INFINITY; }
+            for (int t0 = 0; t0 * 16 < tokens; t0 += AHEAD) {
+                uint32_t w[AHEAD][TOKENS], d[AHEAD][(TOKENS + 1) / 2];
 #pragma unroll
-                for (int b = 0; b < NB; b++) {
-                    const uint32_t d = __builtin_amdgcn_raw_buffer_load_b16(s, cache_k_scale(l15, b, HD), 0, 0);
-                    const float scale = t * 16 + l15 < tokens ? (float) __builtin_bit_cast(_Float16, (uint16_t) d) : __builtin_nanf("");      // (no number: not counted)
-                    const half8_t c = codes8(w[b], k1024);
+                for (int t = 0; t < AHEAD; t++) {
+                    const brsrc s = make_brsrc(strips + (t0 + t) * (18 * HD), (t0 + t) * 16 < tokens ? 18 * HD : 0);
 #pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        const float x = (float) c[j] * scale;
-                        hi[b * 8 + j] = fmaxf(hi[b * 8 + j], x);
-                        lo[b * 8 + j] = fminf(lo[b * 8 + j], x);
+                    for (int k = 0; k < TOKENS; k++) w[t][k] = __builtin_amdgcn_raw_buffer_load_b32(s, cache_k_word(tl * TOKENS + k, g, b, HD), 0, 0);
+                    if constexpr (TOKENS == 1) d[t][0] = __builtin_amdgcn_raw_buffer_load_b16(s, cache_k_scale(tl, b, HD), 0, 0);
+                    else load_words<TOKENS / 2>(d[t], s, cache_k_scale(tl * TOKENS, b, HD), 0);      // (of consecutive tokens of four)
+                }
+#pragma unroll
+                for (int t = 0; t < AHEAD; t++) {
+#pragma unroll
+                    for (int k = 0; k < TOKENS; k++) {
+                        const uint16_t bits = (uint16_t) (d[t][k / 2] >> (16 * (k & 1)));
+                        const float scale = (t0 + t) * 16 + tl * TOKENS + k < tokens ? (float) __builtin_bit_cast(_Float16, bits) : __builtin_nanf("");      // (no number: not counted)
+                        const half8_t c = codes8(w[t][k], k1024);
+#pragma unroll
+                        for (int j = 0; j < 8; j++) {
+                            const float x = (float) c[j] * scale;
+                            hi[j] = fmaxf(hi[j], x);
+                            lo[j] = fminf(lo[j], x);
+                        }
                     }
                 }
             }
             float top = 0.0f;
 #pragma unroll
-            for (int j = 0; j < NB * 8; j++) {
-                const float h = row_max16(hi[j]), l = -row_max16(-lo[j]);
+            for (int j = 0; j < 8; j++) {
+                const float h = max_of<TL>(hi[j]), l = -max_of<TL>(-lo[j]);
                 hi[j] = h == -INFINITY ? 0.0f : h;
                 lo[j] = l == INFINITY ? 0.0f : l;
                 top = fmaxf(top, fmaxf(fabsf(hi[j]), fabsf(lo[j])));
             }
-            top = col_max(top);
+            top = col_max(row_max16(top));
             const float inv = top >= LEAST ? 127.0f / top : 0.0f, scale = top >= LEAST ? top / 127.0f : 0.0f;
-            if (l15 == 0) {
-#pragma unroll
-                for (int b = 0; b < NB; b++)
-#pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        box[wv][b * 32 + g * 8 + j] = hi[b * 8 + j];
-                        box[wv][HD + b * 32 + g * 8 + j] = lo[b * 8 + j];
-                    }
-            }
-            wave_order();
+            // the first lane of the same dimensions writes the largest, the second the smallest
             unsigned char * out = a.digest + (page * a.n_kv_head + kvh) * cache_digest_bytes(HD);
-            if (lane < WORDS) {
-                const float4_t x = *(const float4_t *) &box[wv][lane * 4];
-                uint32_t word = 0;
+            word2_t codes = {0, 0};
 #pragma unroll
-                for (int j = 0; j < 4; j++) word |= ((uint32_t) (int) rintf(x[j] * inv) & 255u) << (8 * j);
-                *(uint32_t *) (out + lane * 4) = word;
-            }
+            for (int j = 0; j < 8; j++) codes[j / 4] |= ((uint32_t) (int) rintf((tl == 0 ? hi[j] : lo[j]) * inv) & 255u) << (8 * (j & 3));
+            if (tl < 2 && lane < 4 * NB * TL) *(word2_t *) (out + tl * HD + 32 * b + 8 * g) = codes;
             if (lane < 4) *(uint32_t *) (out + 2 * HD + lane * 4) = lane == 0 ? __float_as_uint(scale) : 0u;
-            wave_order();
         }
         r = end;
     }
@@ -100,25 +109,23 @@ __global__ __launch_bounds__(NT) void k_cache_digest(cache_digest_args a) {
 
 // the bounds [n][n_kv_head][2][HD] of pages; zeros for a page that is none
 __global__ __launch_bounds__(NT) void k_cache_digest_read(const unsigned char * digest, const int32_t * pages, int64_t n, int64_t n_pages, int n_kv_head, int hd, float * bounds) {
-    const int64_t words = n * n_kv_head * (hd / 2), at = (int64_t) blockIdx.x * NT + threadIdx.x;
-    if (at >= words) return;
-    const int64_t of = at / (hd / 2);      // (page, head)
-    const int w = (int) (at % (hd / 2));
-    const int64_t page = pages[of / n_kv_head];
+    const uint32_t words = (uint32_t) hd / 2, at = blockIdx.x * NT + threadIdx.x, of = at / words, w = at % words, i = of / (uint32_t) n_kv_head;      // (words of a page and head)
+    if (i >= n) return;
+    const int64_t page = pages[i];
     float4_t x = {0, 0, 0, 0};
     if (page >= 0 && page < n_pages) {
-        const unsigned char * d = digest + (page * n_kv_head + of % n_kv_head) * cache_digest_bytes(hd);
+        const unsigned char * d = digest + (page * n_kv_head + of % (uint32_t) n_kv_head) * cache_digest_bytes(hd);
         const int32_t word = *(const int32_t *) (d + w * 4);
         const float scale = *(const float *) (d + 2 * hd);
 #pragma unroll
         for (int j = 0; j < 4; j++) x[j] = (float) (word << (24 - 8 * j) >> 24) * scale;
     }
-    *(float4_t *) (bounds + at * 4) = x;
+    *(float4_t *) (bounds + (int64_t) at * 4) = x;
 }
 
 }  // namespace
 
-// A workgroup has some consecutive rows: one where sequences get a row or so each, up to a page of a prompt's
+// A wave has some consecutive rows: one where sequences get a row or so each, up to a page of a prompt's
 static int rows_per_of(int page_size, int64_t n_seq, int64_t n_rows) {
     int n = 1;
     while (n < page_size && 2 * n * n_seq <= n_rows) n *= 2;
@@ -126,14 +133,16 @@ static int rows_per_of(int page_size, int64_t n_seq, int64_t n_rows) {
 }
 int64_t cache_digest_blocks(const cache_shape & c, int64_t n_seq, int64_t n_rows) {
     const int n = rows_per_of(c.page_size, n_seq, n_rows);
-    return (n_rows + n - 1) / n * c.n_kv_head;
+    return ((n_rows + n - 1) / n * c.n_kv_head + 3) / 4;
 }
-hipError_t launch_cache_digest(const cache_digest_args & a, int hd, hipStream_t s) {
+hipError_t launch_cache_digest(const cache_shape & c, const cache_digest_args & a, hipStream_t s) {
     cache_digest_args args = a;
     args.rows_per = rows_per_of(a.page_size, a.n_seq, a.n_rows);
     void * p[] = {&args};
-    const void * k = hd == 32 ? (const void *) k_cache_digest<32> : hd == 64 ? (const void *) k_cache_digest<64> : hd == 96 ? (const void *) k_cache_digest<96> : (const void *) k_cache_digest<128>;
-    return hipLaunchKernel(k, dim3((unsigned) ((a.n_rows + args.rows_per - 1) / args.rows_per * a.n_kv_head)), dim3(NT), p, 0, s);
+#define OF(HD) (c.page_size == 16 ? (const void *) k_cache_digest<HD, 1> : c.page_size == 32 ? (const void *) k_cache_digest<HD, 2> : (const void *) k_cache_digest<HD, 4>)
+    const void * k = c.hd == 32 ? OF(32) : c.hd == 64 ? OF(64) : c.hd == 96 ? OF(96) : OF(128);
+#undef OF
+    return hipLaunchKernel(k, dim3((unsigned) cache_digest_blocks(c, a.n_seq, a.n_rows)), dim3(NT), p, 0, s);
 }
 
 hipError_t launch_cache_digest_read(const unsigned char * digest, const int32_t * page, int64_t n, int64_t n_pages, int n_kv_head, int hd, float * bounds, hipStream_t s) {

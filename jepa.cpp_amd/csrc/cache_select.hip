@@ -8,10 +8,13 @@
 // (16x16x64 i8, 16 pages x 16 rows) and as an f32, so a score has one rounding and the selection does not depend on how the pages
 // are dealt out. Ties go to the lower page.
 //
-// A workgroup has a K/V head and a tile of 16 consecutive packed rows, or one row where rows are few (then, if the table is long, a piece of
-// its pages; the last piece to arrive joins the pieces' candidates). It goes through the pages in chunks: its waves score 16 pages each, then
-// take rows: what passes a row's threshold is put behind its candidates, in the pages' order, and when they might not take the
-// next chunk's the best are kept. The best n of some hundred keys are found bit by bit, the keys in registers, a ballot for each 64.
+//   few rows (k_select_row)    a workgroup has a row and K/V head, or a piece of its pages where the table is long (the last piece to arrive takes the
+//                              best of all pieces' best). Its waves score 64 pages at a time, the loads of four matrix tiles in flight. The best of up to
+//                              CAP keys: histograms of 256 bins between the smallest and the largest key narrow the range of the last one that is
+//                              taken, 8 bits at a time and mostly twice; ballots and a scan put the taken ones behind each other in their order.
+//   many rows (k_select_rows)  a workgroup of 16 waves has a K/V head and 16 consecutive rows, which share the digests that it reads. Each wave scores 16 pages of
+//                              a chunk for all rows and then takes one row: its keys stay in registers, the bits of the last one that is taken are found one
+//                              by one with a ballot for each 64 keys.
 #include "cache_attn_dev.h"
 #include "common.h"
 
@@ -23,31 +26,102 @@ typedef int int4_t __attribute__((ext_vector_type(4)));
 
 constexpr int MOST = CACHE_MOST_SELECTED;
 constexpr float LEAST = 0x1p-100f;
-constexpr int ROWS = 16;                                                   // of a tile
-constexpr int chunk_of(int rt) { return rt == 1 ? 1024 : 128; }             // pages scored before rows are taken
+constexpr int ROWS = 16;                      // of k_select_rows' tile, its waves
+constexpr int CHUNK = 16 * ROWS;              // pages that it scores before rows are taken
+constexpr int CAP = 2048, PER = CAP / NT;     // keys that k_select_row takes the best of, those of a thread
+constexpr int PIECE = 512;                    // pages of a piece, at least
 constexpr int MOST_PIECES = 64;
-constexpr int SPLIT_UNITS = 2048;                                           // pieces of all rows and K/V heads of a call together
+constexpr int SPLIT_UNITS = 2048;             // pieces of all rows and K/V heads of a call together
 
-// f32 -> a number in the same order; 0 and 1 are none's
+// f32 -> a number in the same order; smaller ones than KEY_LOWEST, -infinity's, are no score's
 __device__ __forceinline__ uint32_t key_of(float x) {
     const uint32_t u = __float_as_uint(x + 0.0f);
     return u ^ ((uint32_t) ((int32_t) u >> 31) | 0x80000000u);
 }
-constexpr uint32_t KEY_LOWEST = 0x007fffffu;      // -infinity's
+constexpr uint32_t KEY_LOWEST = 0x007fffffu;
 
-// The `keep` largest of n candidates (E 64 at most), ties to the first, left at the front in their order; by one wave. Returns how many are left,
-// and a threshold that a later candidate has to pass.
-template <int E>
-__device__ __forceinline__ int keep_best(uint32_t * keys, uint32_t * pages, int n, int keep, uint32_t & pass) {
-    const int lane = (int) threadIdx.x & 63;
-    if (n <= keep) return n;
-    uint32_t k[E], p[E];
-    uint32_t most = 0, least = 0xffffffffu;
+// in all lanes' joined halves: x + x of the lane 16 and 32 further
+__device__ __forceinline__ double sum_groups(double x) {
+    uint64_t u = __builtin_bit_cast(uint64_t, x);
+    auto lo = __builtin_amdgcn_permlane16_swap((uint32_t) u, (uint32_t) u, false, false);
+    auto hi = __builtin_amdgcn_permlane16_swap((uint32_t) (u >> 32), (uint32_t) (u >> 32), false, false);
+    x = __builtin_bit_cast(double, (uint64_t) hi[0] << 32 | lo[0]) + __builtin_bit_cast(double, (uint64_t) hi[1] << 32 | lo[1]);
+    u = __builtin_bit_cast(uint64_t, x);
+    lo = __builtin_amdgcn_permlane32_swap((uint32_t) u, (uint32_t) u, false, false);
+    hi = __builtin_amdgcn_permlane32_swap((uint32_t) (u >> 32), (uint32_t) (u >> 32), false, false);
+    return __builtin_bit_cast(double, (uint64_t) hi[0] << 32 | lo[0]) + __builtin_bit_cast(double, (uint64_t) hi[1] << 32 | lo[1]);
+}
+
+// The codes of P and N of a row's queries at q (group heads) to out [2 HD], by a wave: 16 lanes have the dimensions, four groups of them the heads in turn
+template <typename T, int HD>
+__device__ __forceinline__ void query_codes(const T * q, int group, unsigned char * out) {
+    constexpr int DIMS = HD / 16, WORDS = DIMS * sizeof(T) / 4;
+    struct values { T x[DIMS]; };
+    struct words { uint32_t w[WORDS]; };
+    const int lane = (int) threadIdx.x & 63, d0 = (lane & 15) * DIMS;
+    double pos[DIMS] = {}, neg[DIMS] = {};
+    bool odd = false;
+#pragma unroll 2
+    for (int h = lane >> 4; h < group; h += 4) {
+        words w;
 #pragma unroll
-    for (int e = 0; e < E; e++) {
-        const bool has = e * 64 + lane < n;
-        k[e] = has ? keys[e * 64 + lane] : 0u;
-        p[e] = has ? pages[e * 64 + lane] : 0u;
+        for (int i = 0; i < WORDS; i++) w.w[i] = ((const uint32_t *) (q + (int64_t) h * HD + d0))[i];
+        const values y = __builtin_bit_cast(values, w);
+#pragma unroll
+        for (int d = 0; d < DIMS; d++) {
+            const float x = (float) y.x[d];
+            odd |= !(fabsf(x) < INFINITY);
+            pos[d] += (double) fmaxf(x, 0.0f);
+            neg[d] += (double) fminf(x, 0.0f);
+        }
+    }
+    float p[DIMS], n[DIMS], top = 0.0f;
+#pragma unroll
+    for (int d = 0; d < DIMS; d++) {
+        p[d] = (float) sum_groups(pos[d]);
+        n[d] = (float) sum_groups(neg[d]);
+        top = fmaxf(top, fmaxf(p[d], -n[d]));
+    }
+    top = row_max16(top);
+    if (__any(odd)) top = INFINITY;
+    const float inv = top >= LEAST && top < INFINITY ? 127.0f / top : 0.0f;
+    if (lane < 16) {
+#pragma unroll
+        for (int d = 0; d < DIMS; d++) {
+            out[d0 + d] = (unsigned char) (signed char) (inv == 0.0f ? 0 : (int) rintf(p[d] * inv));
+            out[HD + d0 + d] = (unsigned char) (signed char) (inv == 0.0f ? 0 : (int) rintf(n[d] * inv));
+        }
+    }
+}
+
+// pages that the row sees
+__device__ __forceinline__ int see_of(const cache_select_args & a, const seq_view & v, int64_t row, int page_shift) {
+    return (cache_visible(v.len - v.rows + (int32_t) (row - v.row0), v.len, a.block) + a.page_size - 1) >> page_shift;
+}
+
+// Place i of a row's list: the first pages, those found (n, in `found`), the last ones, -1; or all that the row sees
+__device__ __forceinline__ int32_t entry(const cache_select_args & a, int i, int see, const uint32_t * found, int n) {
+    if (see <= a.take) return i < see ? i : -1;
+    return i < a.first ? i : i < a.first + n ? (int32_t) found[i - a.first] : i < a.first + n + a.last ? see - a.last + (i - a.first - n) : -1;
+}
+
+// ---------------------------------------------------------------------------------------------- a row a workgroup
+struct row_lds {
+    uint32_t keys[CAP], pages[CAP], hist[256];
+    int32_t count[2][PER * 4];
+    uint32_t range[2][4];
+};
+
+// The `keep` largest of n keys (CAP at most), ties to the first, left at the front in their order; by the workgroup. Returns how many are left.
+__device__ __forceinline__ int best_of(row_lds & l, int n, int keep) {
+    if (n <= keep) return n;
+    const int tid = (int) threadIdx.x, lane = tid & 63, wv = uniform(tid >> 6);
+    uint32_t k[PER], p[PER], most = 0, least = 0xffffffffu;
+#pragma unroll
+    for (int e = 0; e < PER; e++) {
+        const bool has = e * NT + tid < n;
+        k[e] = has ? l.keys[e * NT + tid] : 0u;      // (0 is nobody's)
+        p[e] = has ? l.pages[e * NT + tid] : 0u;
         most = max(most, k[e]);
         if (has) least = min(least, k[e]);
     }
@@ -56,52 +130,72 @@ __device__ __forceinline__ int keep_best(uint32_t * keys, uint32_t * pages, int 
     JOIN(0x111, 0xf); JOIN(0x112, 0xf); JOIN(0x114, 0xf); JOIN(0x118, 0xf); JOIN(0x142, 0xa); JOIN(0x143, 0xc);
 #undef JOIN
 #undef DPP
-    most = (uint32_t) __builtin_amdgcn_readlane((int) most, 63);
-    least = (uint32_t) __builtin_amdgcn_readlane((int) least, 63);
-    auto count = [&](uint32_t c) {
-        int s = 0;
+    if (lane == 63) { l.range[0][wv] = most; l.range[1][wv] = least; }
+    l.hist[tid] = 0;
+    __syncthreads();
+    most = max(max(l.range[0][0], l.range[0][1]), max(l.range[0][2], l.range[0][3]));
+    least = min(min(l.range[1][0], l.range[1][1]), min(l.range[1][2], l.range[1][3]));
+    // the last one taken lies in [least, most], `need` of those are taken
+    int need = keep;
+    for (;;) {
+        const int shift = most == least ? 0 : max(0, 24 - __builtin_clz(most - least));
 #pragma unroll
-        for (int e = 0; e < E; e++) s += (int) __popcll(__ballot(k[e] >= c));
-        return s;
-    };
-    // the largest t that `keep` or more pass, from the bits that all have on
-    uint32_t t = least;
-    if (most != least) {
-        int bit = 31 - __builtin_clz(most ^ least);
-        t = most & ~(((2u << bit) - 1));
-        for (; bit >= 0; bit--) {
-            const uint32_t c = t | 1u << bit;
-            const int s = count(c);
-            if (s >= keep) t = c;
-            if (s == keep) break;
-        }
+        for (int e = 0; e < PER; e++)
+            if (k[e] >= least && k[e] <= most) atomicAdd(&l.hist[(k[e] - least) >> shift], 1u);
+        __syncthreads();
+        // every wave: four bins a lane, from the last
+        const int b0 = 255 - lane * 4;
+        int c[4], all = 0;
+#pragma unroll
+        for (int j = 0; j < 4; j++) all += c[j] = (int) l.hist[b0 - j];
+        const int upto = wave_scan(all);
+        const int at = __builtin_ctzll(__ballot(upto >= need));      // (some lane's: all of the range's are need or more)
+        int above = upto - all, bin = b0;
+#pragma unroll
+        for (int j = 0; j < 3; j++)
+            if (bin == b0 - j && above + c[j] < need) { above += c[j]; bin--; }
+        const int in = bin == b0 ? c[0] : bin == b0 - 1 ? c[1] : bin == b0 - 2 ? c[2] : c[3];
+        const int take = need - __builtin_amdgcn_readlane(above, at), has = __builtin_amdgcn_readlane(in, at);
+        const uint32_t from = least + ((uint32_t) __builtin_amdgcn_readlane(bin, at) << shift);
+        need = take;
+        least = from;
+        most = most - from < 1u << shift ? most : from + ((1u << shift) - 1);
+        if (take == has || shift == 0) break;
+        __syncthreads();
+        l.hist[tid] = 0;
+        __syncthreads();
     }
-    int above = 0;      // more than t: all of them; t itself: the first ones
+    // more than `most`: all; in the range: the first `need`. A group is 64 consecutive keys, of a wave
+    uint64_t eq[PER], gt[PER];
 #pragma unroll
-    for (int e = 0; e < E; e++) above += (int) __popcll(__ballot(k[e] > t));
-    int ties = keep - above, at = 0;
-    if (ties < 0) ties = 0;
-    wave_order();
-    const uint64_t before = (1ull << lane) - 1;
+    for (int e = 0; e < PER; e++) {
+        eq[e] = __ballot(k[e] >= least && k[e] <= most);
+        gt[e] = __ballot(k[e] > most);
+        if (lane == 0) { l.count[0][e * 4 + wv] = (int) __popcll(eq[e]); l.count[1][e * 4 + wv] = (int) __popcll(gt[e]); }
+    }
+    __syncthreads();
+    static_assert(PER * 4 <= 64, "a group a lane");
+    const int mine_eq = lane < PER * 4 ? l.count[0][min(lane, PER * 4 - 1)] : 0, mine_gt = lane < PER * 4 ? l.count[1][min(lane, PER * 4 - 1)] : 0;
+    const int eq_before = wave_scan(mine_eq) - mine_eq, ties = min(max(need - eq_before, 0), mine_eq);
+    const int upto = wave_scan(mine_gt + ties), before = upto - mine_gt - ties;
+    const uint64_t below = (1ull << lane) - 1;
 #pragma unroll
-    for (int e = 0; e < E; e++) {
-        const uint64_t eq = __ballot(k[e] == t && e * 64 + lane < n);
-        const bool mine = k[e] > t || ((eq >> lane & 1) && (int) __popcll(eq & before) < ties);
+    for (int e = 0; e < PER; e++) {
+        const int of = e * 4 + wv, t = __builtin_amdgcn_readlane(ties, of), at = __builtin_amdgcn_readlane(before, of);
+        const bool mine = (gt[e] >> lane & 1) || ((eq[e] >> lane & 1) && (int) __popcll(eq[e] & below) < t);
         const uint64_t in = __ballot(mine);
         if (mine) {
-            const int i = at + (int) __popcll(in & before);
-            keys[i] = k[e];
-            pages[i] = p[e];
+            const int i = at + (int) __popcll(in & below);
+            l.keys[i] = k[e];
+            l.pages[i] = p[e];
         }
-        at += (int) __popcll(in);
-        ties -= min(ties, (int) __popcll(eq));
     }
-    wave_order();
-    pass = t;
-    return at;
+    __syncthreads();
+    return __builtin_amdgcn_readlane(upto, 63);
 }
 
-// `work`: a counter for each (row, K/V head) of several pieces, SPLIT_UNITS of them, then [row][K/V head][piece] candidates: their number, keys [take], pages [take]
+// `work`: a counter for each (row, K/V head) of several pieces, SPLIT_UNITS of them, then [row][K/V head][piece] what they found: their number, keys [take],
+// pages [take]
 struct pieces_view {
     static constexpr int SC1 = 16;
     const brsrc r;
@@ -112,197 +206,282 @@ struct pieces_view {
     __device__ uint32_t get(int piece, int word) const { return __builtin_amdgcn_raw_buffer_load_b32(r, piece * bytes + word * 4, 0, SC1); }
 };
 
-template <typename T, int HD, int RT>
-__global__ __launch_bounds__(NT) void k_cache_select(cache_select_args a) {
-    constexpr int CH = chunk_of(RT), QS = 2 * HD + 16, SS = CH + 4, E = (CH + MOST) / 64, DIMS = HD / 16;
-    __shared__ __attribute__((aligned(16))) unsigned char codes[ROWS * QS];
-    __shared__ __attribute__((aligned(16))) int32_t dots[RT * SS];
-    __shared__ float scales[CH];
-    extern __shared__ __attribute__((aligned(16))) uint32_t lists[];      // keys [RT][cap], pages [RT][cap]
+template <typename T, int HD>
+__global__ __launch_bounds__(NT) void k_select_row(cache_select_args a) {
+    constexpr int NK = 2 * HD / 64, CHUNK1 = CAP - MOST;
+    __shared__ __attribute__((aligned(16))) unsigned char codes[4][2 * HD];
+    __shared__ row_lds l;
     const int tid = (int) threadIdx.x, lane = tid & 63, l15 = lane & 15, g = lane >> 4, wv = uniform(tid >> 6);
     const int group = a.n_head / a.n_kv_head, kvh = (int) (blockIdx.x % (unsigned) a.n_kv_head);
     const unsigned at_block = blockIdx.x / (unsigned) a.n_kv_head;
-    const int piece = RT == 1 ? (int) (at_block % (unsigned) a.pieces) : 0;
-    const int64_t t0 = (int64_t) (RT == 1 ? at_block / (unsigned) a.pieces : at_block) * RT, t1 = min(t0 + RT, a.n_rows);
-    const int page_shift = __builtin_ctz((unsigned) a.page_size), cap = CH + a.take;
-    uint32_t * const keys = lists, * const pages = lists + RT * cap;
+    const int piece = (int) (at_block % (unsigned) a.pieces);
+    const int64_t row = at_block / (unsigned) a.pieces;
+    const int page_shift = __builtin_ctz((unsigned) a.page_size);
+    int seq;
+    seq_view v;
+    if (!place_of(a, (int32_t) row, seq, v)) return;
+    const int see = see_of(a, v, row, page_shift), keep = a.take - a.first - a.last;
+    int32_t * const out = a.selected + (row * a.n_kv_head + kvh) * a.take;
+    if (see <= a.take || keep == 0) {      // nothing to choose
+        if (piece == 0 && tid < a.take) out[tid] = entry(a, tid, see, nullptr, 0);
+        return;
+    }
+    const int p0 = a.first + piece * a.piece, p1 = min(see - a.last, p0 + a.piece);
+    int n = 0;
+    if (p0 < p1) {
+        const int32_t * table = a.table + (int64_t) seq * a.width;
+        // a lane's page of 64: the one whose score the matrix tiles will leave in it (tile l15 / 4, its page 4 g + l15 % 4)
+        const int mine = (l15 >> 2) * 16 + g * 4 + (l15 & 3);
+        auto load_page = [&](int p) { return table[min(p + mine, p1 - 1)]; };
+        int32_t next = load_page(p0 + wv * 64);
+        query_codes<T, HD>((const T *) a.q + row * a.ldq + (int64_t) kvh * group * HD, group, codes[wv]);
+        wave_order();
+        int4_t b[NK];
+#pragma unroll
+        for (int k = 0; k < NK; k++) b[k] = *(const int4_t *) (codes[wv] + k * 64 + g * 16);      // (every column is the row)
+        for (int c0 = p0; c0 < p1; c0 += CHUNK1) {
+            const int c1 = min(c0 + CHUNK1, p1);
+            for (int s0 = c0 + wv * 64; s0 < c1; s0 += NT) {
+                const bool bad = next < 0 || next >= a.n_pages;
+                const int32_t page = bad ? 0 : next;
+                const unsigned char * const heads = a.digest + (int64_t) kvh * cache_digest_bytes(HD);
+                const int64_t per = a.n_kv_head * cache_digest_bytes(HD);
+                int4_t y[4][NK];
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+                    const int32_t of = __builtin_amdgcn_ds_bpermute(((l15 >> 2) * 16 + t * 4 + (l15 & 3)) * 4, page);      // the lane of the tile's page l15
+                    const unsigned char * d = heads + of * per + g * 16;
+#pragma unroll
+                    for (int k = 0; k < NK; k++) y[t][k] = *(const int4_t *) (d + k * 64);
+                }
+                const float scale = *(const float *) (heads + page * per + 2 * HD);
+                next = load_page(s0 + NT < c1 ? s0 + NT : c0 + CHUNK1 + wv * 64);
+                int dot = 0;
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+                    int4_t x = {0, 0, 0, 0};
+#pragma unroll
+                    for (int k = 0; k < NK; k++) x = __builtin_amdgcn_mfma_i32_16x16x64_i8(y[t][k], b[k], x, 0, 0, 0);
+                    const int r = l15 & 3, of = r == 0 ? x[0] : r == 1 ? x[1] : r == 2 ? x[2] : x[3];
+                    if (l15 >> 2 == t) dot = of;
+                }
+                const int p = s0 + mine;
+                if (p < c1) {
+                    l.keys[n + p - c0] = bad ? KEY_LOWEST : key_of((float) dot * scale);
+                    l.pages[n + p - c0] = (uint32_t) p;
+                }
+            }
+            __syncthreads();
+            n = best_of(l, n + c1 - c0, keep);
+        }
+    }
+    if (a.pieces > 1) {
+        const int64_t unit = row * a.n_kv_head + kvh;
+        const pieces_view w(a, unit);
+        if (tid == 0) w.put(piece, 0, (uint32_t) n);
+        if (tid < n) {
+            w.put(piece, 4 + tid, l.keys[tid]);
+            w.put(piece, 4 + a.take + tid, l.pages[tid]);
+        }
+        if (!last_to_arrive(a.work, unit, a.pieces)) return;
+        static_assert(MOST_PIECES <= 64 && MOST <= NT, "a piece a lane, a page a thread");
+        const int has = lane < a.pieces ? min((int) w.get(lane, 0), a.take) : 0, upto = wave_scan(has);
+        n = 0;
+        for (int k = 0, base = 0; k < a.pieces;) {      // as many pieces as fit behind what is kept
+            int m = n;
+            for (; k < a.pieces; k++) {
+                const int to = __builtin_amdgcn_readlane(upto, k), from = k ? __builtin_amdgcn_readlane(upto, k - 1) : 0;
+                if (n + to - base > CAP) break;
+                if (tid < to - from) {
+                    l.keys[m + tid] = w.get(k, 4 + tid);
+                    l.pages[m + tid] = w.get(k, 4 + a.take + tid);
+                }
+                m += to - from;
+            }
+            base = k ? __builtin_amdgcn_readlane(upto, k - 1) : 0;
+            __syncthreads();
+            n = best_of(l, m, keep);
+        }
+    }
+    if (tid < a.take) out[tid] = entry(a, tid, see, l.pages, n);
+}
 
+// ---------------------------------------------------------------------------------------------- a row a wave
+// The `keep` largest of the keys in E registers of the lanes (0: none), ties to the first, put into keys and pages in their order; by a wave. Returns how
+// many, and what a later key has to pass.
+template <int E>
+__device__ __forceinline__ int keep_best(const uint32_t * k, const uint32_t * p, int keep, uint32_t * keys, uint32_t * pages, uint32_t & pass) {
+    const int lane = (int) threadIdx.x & 63;
+    uint32_t most = 0, least = 0xffffffffu;
+    int n = 0;
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        most = max(most, k[e]);
+        least = min(least, k[e] - 1);      // (0 becomes the largest)
+        n += (int) __popcll(__ballot(k[e] != 0));
+    }
+    uint32_t t = 0;
+    if (n > keep) {
+#define DPP(x, ctrl, rows) (uint32_t) __builtin_amdgcn_update_dpp((int) x, (int) x, ctrl, rows, 0xf, false)
+#define JOIN(ctrl, rows) most = max(most, DPP(most, ctrl, rows)); least = min(least, DPP(least, ctrl, rows))
+        JOIN(0x111, 0xf); JOIN(0x112, 0xf); JOIN(0x114, 0xf); JOIN(0x118, 0xf); JOIN(0x142, 0xa); JOIN(0x143, 0xc);
+#undef JOIN
+#undef DPP
+        most = (uint32_t) __builtin_amdgcn_readlane((int) most, 63);
+        least = (uint32_t) __builtin_amdgcn_readlane((int) least, 63) + 1;
+        // the largest t that `keep` or more reach, from the bits that all have on
+        t = least;
+        if (most != least) {
+            int bit = 31 - __builtin_clz(most ^ least);
+            t = most & ~((2u << bit) - 1);
+            for (; bit >= 0; bit--) {
+                const uint32_t c = t | 1u << bit;
+                int s = 0;
+#pragma unroll
+                for (int e = 0; e < E; e++) s += (int) __popcll(__ballot(k[e] >= c));
+                if (s >= keep) t = c;
+                if (s == keep) break;
+            }
+        }
+    }
+    int ties = keep, at = 0;      // more than t: all of them; t itself: the first ones
+#pragma unroll
+    for (int e = 0; e < E; e++) ties -= (int) __popcll(__ballot(k[e] > t));
+    const uint64_t before = (1ull << lane) - 1;
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        const uint64_t eq = __ballot(k[e] == t && t != 0);
+        const bool mine = k[e] > t || ((eq >> lane & 1) && (int) __popcll(eq & before) < ties);
+        const uint64_t in = __ballot(mine);
+        if (mine) {
+            const int i = at + (int) __popcll(in & before);
+            keys[i] = k[e];
+            pages[i] = p[e];
+        }
+        at += (int) __popcll(in);
+        ties -= min(ties, (int) __popcll(eq));
+    }
+    pass = t;
+    return at;
+}
+
+template <typename T, int HD>
+__global__ __launch_bounds__(64 * ROWS) void k_select_rows(cache_select_args a) {
+    constexpr int NK = 2 * HD / 64, QS = 2 * HD + 16, SS = CHUNK + 4, CE = CHUNK / 64, KE = MOST / 64;
+    __shared__ __attribute__((aligned(16))) unsigned char codes[ROWS * QS];
+    __shared__ __attribute__((aligned(16))) int32_t dots[ROWS * SS];
+    __shared__ float scales[CHUNK];
+    extern __shared__ __attribute__((aligned(16))) uint32_t lists[];      // what rows keep: keys [ROWS][take], pages [ROWS][take]
+    const int lane = (int) threadIdx.x & 63, l15 = lane & 15, g = lane >> 4, wv = uniform((int) threadIdx.x >> 6);
+    const int group = a.n_head / a.n_kv_head, kvh = (int) (blockIdx.x % (unsigned) a.n_kv_head), page_shift = __builtin_ctz((unsigned) a.page_size);
+    const int64_t t0 = (int64_t) (blockIdx.x / (unsigned) a.n_kv_head) * ROWS, t1 = min(t0 + ROWS, a.n_rows);
+    const int keep = a.take - a.first - a.last;
+    uint32_t * const keys = lists + wv * a.take, * const pages = lists + (ROWS + wv) * a.take;
     for (int64_t r0 = t0; r0 < t1;) {      // the sequences of the tile's rows
-        const int seq = seq_of_row(a.row_start, a.n_seq, (int32_t) r0);
-        if (seq < 0) {
+        int seq;
+        seq_view v;
+        if (!place_of(a, (int32_t) r0, seq, v)) {
             if (r0 >= a.row_start[0]) break;
             r0 = min((int64_t) a.row_start[0], t1);
             continue;
         }
-        const seq_view v = view_of(a, seq);
-        const int64_t r1 = min(t1, (int64_t) v.row0 + v.rows);
-        if (r1 <= r0) { r0++; continue; }
-        const int rows = (int) (r1 - r0);
-        auto see_of = [&](int row) {      // pages that a row of these sees
-            return (cache_visible(v.len - v.rows + (int32_t) (r0 - v.row0) + row, v.len, a.block) + a.page_size - 1) >> page_shift;
-        };
-        const int see_all = see_of(rows - 1);      // (the last row sees the most)
-        // pages that are scored: neither a first nor a last one of the last row
-        const int p0 = RT == 1 ? a.first + piece * a.piece : a.first, p1 = RT == 1 ? min(see_all - a.last, p0 + a.piece) : see_all - a.last;
-        const bool choose = see_all > a.take && a.take > a.first + a.last;
-        if (RT == 1 && !choose && piece != 0) return;
-        int n[RT == 1 ? 1 : ROWS / 4] = {};            // candidates of this wave's rows, and what a key has to pass
-        uint32_t pass[RT == 1 ? 1 : ROWS / 4] = {};
-        if (choose && p0 < p1) {
-            // queries: 16 threads a row
-            __syncthreads();
-            {
-                const int row = min(tid >> 4, rows - 1), d0 = (tid & 15) * DIMS;
-                constexpr int WORDS = DIMS * sizeof(T) / 4;
-                struct values { T x[DIMS]; };
-                struct words { uint32_t w[WORDS]; };
-                const T * q = (const T *) a.q + (r0 + row) * a.ldq + (int64_t) kvh * group * HD + d0;
-                double pos[DIMS] = {}, neg[DIMS] = {};
-                bool odd = false;
-                for (int h = 0; h < group; h++) {
-                    words w;
-#pragma unroll
-                    for (int i = 0; i < WORDS; i++) w.w[i] = ((const uint32_t *) (q + (int64_t) h * HD))[i];
-                    const values y = __builtin_bit_cast(values, w);
-#pragma unroll
-                    for (int d = 0; d < DIMS; d++) {
-                        const float x = (float) y.x[d];
-                        odd |= !(fabsf(x) < INFINITY);
-                        pos[d] += (double) fmaxf(x, 0.0f);
-                        neg[d] += (double) fminf(x, 0.0f);
-                    }
-                }
-                float top = 0.0f;
-#pragma unroll
-                for (int d = 0; d < DIMS; d++) top = fmaxf(top, fmaxf((float) pos[d], -(float) neg[d]));
-                if (odd) top = INFINITY;
-                top = row_max16(top);
-                const float inv = top >= LEAST && top < INFINITY ? 127.0f / top : 0.0f;
-                unsigned char * const c = codes + (tid >> 4) * QS + d0;
-#pragma unroll
-                for (int d = 0; d < DIMS; d++) {
-                    c[d] = (unsigned char) (signed char) (inv == 0.0f ? 0 : (int) rintf((float) pos[d] * inv));
-                    c[HD + d] = (unsigned char) (signed char) (inv == 0.0f ? 0 : (int) rintf((float) neg[d] * inv));
-                }
-            }
-            __syncthreads();
-            int4_t b[2 * HD / 64];
-#pragma unroll
-            for (int k = 0; k < 2 * HD / 64; k++) b[k] = *(const int4_t *) (codes + l15 * QS + k * 64 + g * 16);
+        const int64_t r1 = min(t1, (int64_t) v.row0 + v.rows), row = min(r0 + wv, r1 - 1);
+        const bool has = r0 + wv < r1;
+        const int see = see_of(a, v, row, page_shift), see_all = see_of(a, v, r1 - 1, page_shift);      // (the last row sees the most)
+        int n = 0;
+        if (see_all > a.take && keep > 0) {
+            const int p0 = a.first, p1 = see_all - a.last, end = see > a.take && has ? see - a.last : 0;
             const int32_t * table = a.table + (int64_t) seq * a.width;
-            for (int c0 = p0; c0 < p1; c0 += CH) {
-                const int c1 = min(c0 + CH, p1);
-                for (int s0 = c0 + wv * 16; s0 < c1; s0 += 64) {
-                    int64_t page = table[min(s0 + l15, c1 - 1)];
-                    const bool bad = page < 0 || page >= a.n_pages;
-                    if (bad) page = 0;
-                    const unsigned char * d = a.digest + (page * a.n_kv_head + kvh) * cache_digest_bytes(HD);
-                    int4_t x = {0, 0, 0, 0};
-                    int4_t y[2 * HD / 64];
+            bool bad = false;
+            int4_t y[NK];
+            float scale = 0.0f;
+            auto load_page = [&](int c0) { return table[min(c0 + wv * 16 + l15, p1 - 1)]; };
+            auto load = [&](int32_t page) {
+                bad = page < 0 || page >= a.n_pages;
+                const unsigned char * d = a.digest + ((bad ? 0 : (int64_t) page) * a.n_kv_head + kvh) * cache_digest_bytes(HD);
 #pragma unroll
-                    for (int k = 0; k < 2 * HD / 64; k++) y[k] = *(const int4_t *) (d + k * 64 + g * 16);
-                    if (g == 0) scales[s0 - c0 + l15] = bad ? -1.0f : *(const float *) (d + 2 * HD);
+                for (int k = 0; k < NK; k++) y[k] = *(const int4_t *) (d + k * 64 + g * 16);
+                scale = *(const float *) (d + 2 * HD);
+            };
+            const int32_t first_page = load_page(p0);
+            int32_t next = load_page(p0 + CHUNK);
+            query_codes<T, HD>((const T *) a.q + row * a.ldq + (int64_t) kvh * group * HD, group, codes + wv * QS);
+            load(first_page);
+            __syncthreads();
+            int4_t b[NK];
 #pragma unroll
-                    for (int k = 0; k < 2 * HD / 64; k++) x = __builtin_amdgcn_mfma_i32_16x16x64_i8(y[k], b[k], x, 0, 0, 0);
-                    if (l15 < RT) *(int4_t *) (dots + l15 * SS + (s0 - c0) + g * 4) = x;
+            for (int k = 0; k < NK; k++) b[k] = *(const int4_t *) (codes + l15 * QS + k * 64 + g * 16);
+            uint32_t pass = 0;
+            for (int c0 = p0; c0 < p1; c0 += CHUNK) {
+                int4_t x = {0, 0, 0, 0};
+#pragma unroll
+                for (int k = 0; k < NK; k++) x = __builtin_amdgcn_mfma_i32_16x16x64_i8(y[k], b[k], x, 0, 0, 0);
+                *(int4_t *) (dots + l15 * SS + wv * 16 + g * 4) = x;
+                if (g == 0) scales[wv * 16 + l15] = bad ? -1.0f : scale;
+                if (c0 + CHUNK < p1) {
+                    load(next);
+                    next = load_page(c0 + 2 * CHUNK);
                 }
                 __syncthreads();
-                // rows
+                // this wave's row: the chunk's keys behind the ones it kept
+                const int m = min(CHUNK, end - c0);
+                uint32_t k[KE + CE], p[KE + CE];
+                bool some = false;
 #pragma unroll
-                for (int i = 0; i < (RT == 1 ? 1 : ROWS / 4); i++) {
-                    const int row = RT == 1 ? 0 : i * 4 + wv;
-                    if (row >= rows || (RT == 1 && wv != 0)) continue;
-                    const int see = see_of(row);
-                    if (see <= a.take) continue;
-                    const int end = min(c1, see - a.last), keep = a.take - a.first - a.last;
-                    for (int s = c0; s < end; s += 64) {
-                        const int p = s + lane;
-                        const float scale = scales[p - c0];
-                        uint32_t key = scale < 0.0f ? KEY_LOWEST : key_of((float) dots[row * SS + p - c0] * scale);
-                        const bool in = p < end && key > pass[i];
-                        const uint64_t all = __ballot(in);
-                        if (in) {
-                            const int to = n[i] + (int) __popcll(all & ((1ull << lane) - 1));
-                            keys[row * cap + to] = key;
-                            pages[row * cap + to] = (uint32_t) p;
-                        }
-                        n[i] += (int) __popcll(all);
+                for (int e = 0; e < CE; e++) {
+                    const int i = e * 64 + lane;
+                    const float f = scales[i];
+                    const uint32_t key = f < 0.0f ? KEY_LOWEST : key_of((float) dots[wv * SS + i] * f);
+                    k[KE + e] = i < m && key > pass ? key : 0u;
+                    p[KE + e] = (uint32_t) (c0 + i);
+                    some |= k[KE + e] != 0;
+                }
+                if (n == 0) {
+                    n = keep_best<CE>(k + KE, p + KE, keep, keys, pages, pass);
+                } else if (__any(some)) {
+#pragma unroll
+                    for (int e = 0; e < KE; e++) {
+                        const int i = e * 64 + lane;
+                        k[e] = i < n ? keys[i] : 0u;
+                        p[e] = i < n ? pages[i] : 0u;
                     }
                     wave_order();
-                    if (n[i] > keep) n[i] = keep_best<E>(keys + row * cap, pages + row * cap, n[i], keep, pass[i]);
+                    n = keep_best<KE + CE>(k, p, keep, keys, pages, pass);
                 }
-                if (c0 + CH < p1) __syncthreads();
+                wave_order();
+                if (c0 + CHUNK < p1) __syncthreads();
             }
         }
-        // what was found, between the first and the last pages
-        auto write = [&](int row, const uint32_t * found, int n) {
-            int32_t * out = a.selected + ((r0 + row) * a.n_kv_head + kvh) * a.take;
-            const int see = see_of(row);
-            const bool all = see <= a.take;
-            for (int i = lane; i < a.take; i += 64) {
-                int32_t p;
-                if (all) p = i < see ? i : -1;
-                else p = i < a.first ? i : i < a.first + n ? (int32_t) found[i - a.first] : i < a.first + n + a.last ? see - a.last + (i - a.first - n) : -1;
-                out[i] = p;
-            }
-        };
-        if constexpr (RT == 1) {
-            if (a.pieces > 1 && choose) {
-                const int64_t unit = r0 * a.n_kv_head + kvh;
-                const pieces_view w(a, unit);
-                if (wv == 0) {
-                    if (lane == 0) w.put(piece, 0, (uint32_t) n[0]);
-                    for (int i = lane; i < n[0]; i += 64) {
-                        w.put(piece, 4 + i, keys[i]);
-                        w.put(piece, 4 + a.take + i, pages[i]);
-                    }
-                }
-                if (!last_to_arrive(a.work, unit, a.pieces)) return;
-                if (wv != 0) return;
-                int m = 0;
-                uint32_t over = 0;
-                const int keep = a.take - a.first - a.last;
-                for (int k = 0; k < a.pieces; k++) {
-                    const int has = min((int) w.get(k, 0), a.take);
-                    for (int i = lane; i < has; i += 64) {
-                        keys[m + i] = w.get(k, 4 + i);
-                        pages[m + i] = w.get(k, 4 + a.take + i);
-                    }
-                    m += uniform(has);
-                    wave_order();
-                    if (m + a.take > cap || k + 1 == a.pieces) m = keep_best<E>(keys, pages, m, keep, over);
-                }
-                n[0] = m;
-            }
-            if (wv == 0) write(0, pages, n[0]);
-            return;
-        } else {
-#pragma unroll
-            for (int i = 0; i < ROWS / 4; i++)
-                if (i * 4 + wv < rows) write(i * 4 + wv, pages + (i * 4 + wv) * cap, n[i]);
-            __syncthreads();
-            r0 = r1;
+        if (has) {
+            int32_t * out = a.selected + (row * a.n_kv_head + kvh) * a.take;
+            for (int i = lane; i < a.take; i += 64) out[i] = entry(a, i, see, pages, n);
         }
+        __syncthreads();
+        r0 = r1;
     }
 }
 
 // Tiles of 16 rows where they fill the chip and sequences have rows for them; else a row a workgroup, and pieces of its pages where a table is long
-int rows_of(const cache_shape & c, int64_t n_seq, int64_t n_rows) { return n_rows >= 4 * n_seq && n_rows * c.n_kv_head >= 256 * ROWS ? ROWS : 1; }
+bool tiles_of(const cache_shape & c, int64_t n_seq, int64_t n_rows) { return n_rows >= 4 * n_seq && n_rows * c.n_kv_head >= 256 * ROWS; }
 int pieces_of(const cache_shape & c, int64_t n_seq, int64_t n_rows, int64_t width) {
-    if (rows_of(c, n_seq, n_rows) != 1) return 1;
-    return (int) std::clamp<int64_t>(std::min((width + chunk_of(1) - 1) / chunk_of(1), SPLIT_UNITS / (n_rows * c.n_kv_head)), 1, MOST_PIECES);
+    if (tiles_of(c, n_seq, n_rows)) return 1;
+    return (int) std::clamp<int64_t>(std::min((width + PIECE - 1) / PIECE, SPLIT_UNITS / (n_rows * c.n_kv_head)), 1, MOST_PIECES);
+}
+
+int64_t blocks_of(const cache_shape & c, int64_t n_seq, int64_t n_rows, int64_t width) {
+    const int rows = tiles_of(c, n_seq, n_rows) ? ROWS : 1;
+    return (n_rows + rows - 1) / rows * pieces_of(c, n_seq, n_rows, width) * c.n_kv_head;
 }
 
 template <typename T, int HD>
 hipError_t select(const cache_shape & c, const cache_select_args & a, hipStream_t s) {
     cache_select_args args = a;
     void * p[] = {&args};
-    const int rt = rows_of(c, a.n_seq, a.n_rows);
+    const bool tiles = tiles_of(c, a.n_seq, a.n_rows);
     args.pieces = pieces_of(c, a.n_seq, a.n_rows, a.width);
     args.piece = (a.width + args.pieces - 1) / args.pieces;
-    const unsigned lds = (unsigned) (2 * rt * (chunk_of(rt) + a.take) * 4);
-    return hipLaunchKernel(rt == 1 ? (const void *) k_cache_select<T, HD, 1> : (const void *) k_cache_select<T, HD, ROWS>,
-                           dim3((unsigned) cache_select_blocks(c, a.n_seq, a.n_rows, a.width)), dim3(NT), p, lds, s);
+    return hipLaunchKernel(tiles ? (const void *) k_select_rows<T, HD> : (const void *) k_select_row<T, HD>, dim3((unsigned) blocks_of(c, a.n_seq, a.n_rows, a.width)),
+                           dim3(tiles ? 64 * ROWS : NT), p, tiles ? (unsigned) (2 * ROWS * a.take * 4) : 0, s);
 }
 
 template <typename T>
@@ -312,14 +491,14 @@ hipError_t by_head(const cache_shape & c, const cache_select_args & a, hipStream
 
 }  // namespace
 
+// workgroups of 256 threads that the launch's are worth
 int64_t cache_select_blocks(const cache_shape & c, int64_t n_seq, int64_t n_rows, int64_t width) {
-    const int rt = rows_of(c, n_seq, n_rows);
-    return (n_rows + rt - 1) / rt * pieces_of(c, n_seq, n_rows, width) * c.n_kv_head;
+    return blocks_of(c, n_seq, n_rows, width) * (tiles_of(c, n_seq, n_rows) ? 64 * ROWS / NT : 1);
 }
 
 // What any call of no more rows, pages and pages taken needs
 int64_t cache_select_work_bytes(const cache_shape & c, int64_t n_rows, int64_t width, int take) {
-    const int64_t most = (width + chunk_of(1) - 1) / chunk_of(1);
+    const int64_t most = std::min<int64_t>((width + PIECE - 1) / PIECE, MOST_PIECES);
     return most > 1 ? SPLIT_UNITS * 8 + std::min<int64_t>(n_rows * c.n_kv_head * most, SPLIT_UNITS) * (8 * (int64_t) take + 16) : 0;
 }
 

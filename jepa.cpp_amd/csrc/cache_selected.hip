@@ -40,9 +40,9 @@ __global__ __launch_bounds__(NT, groups_of<T>(HD)) void k_cache_selected(cache_s
     const int64_t row = unit / a.tiles;
     if (row >= a.n_rows) return;      // (WHOLE: of a wave; no barrier follows)
     const int col0 = (int) (unit % a.tiles) * C;
-    const int seq = seq_of_row(a.row_start, a.n_seq, (int32_t) row);
-    if (seq < 0) return;
-    const seq_view v = view_of(a, seq);
+    int seq;
+    seq_view v;
+    if (!place_of(a, (int32_t) row, seq, v)) return;
     const int32_t lim = cache_visible(v.len - v.rows + (int32_t) (row - v.row0), v.len, a.block);
     const int col = min(col0 + l15, group - 1);
     typename vec8<T>::t y[NB];

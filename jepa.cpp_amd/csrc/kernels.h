@@ -202,7 +202,7 @@ struct cache_digest_args {
     int rows_per = 0;      // set by the launcher
 };
 int64_t cache_digest_blocks(const cache_shape & c, int64_t n_seq, int64_t n_rows);      // workgroups of the launch (256 threads)
-hipError_t launch_cache_digest(const cache_digest_args & a, int hd, hipStream_t s);
+hipError_t launch_cache_digest(const cache_shape & c, const cache_digest_args & a, hipStream_t s);
 hipError_t launch_cache_digest_read(const unsigned char * digest, const int32_t * page, int64_t n, int64_t n_pages, int n_kv_head, int hd, float * bounds, hipStream_t s);
 // the pages that each row and K/V head selects; `work` holds cache_select_work_bytes
 struct cache_select_args {

@@ -110,7 +110,7 @@ TABLES = [dict(shape=None), dict(shape=shape(head_dim=80)), dict(n_seq=-1), dict
 
 
 @pytest.mark.parametrize("kw", TABLES + [dict(cache=None), dict(cache=P + 8), dict(digest=None), dict(digest=P + 4),
-                                         dict(shape=shape(n_head=4096, n_kv_head=4096), n_seq=4096, n_rows=8191)])
+                                         dict(shape=shape(n_head=4096, n_kv_head=4096), n_seq=4096, n_rows=1 << 24)])
 def test_digest_refuses(kw):
     refused(digest, "jepa_amd_cache_digest", **kw)
 
