@@ -26,9 +26,10 @@ typedef int int4_t __attribute__((ext_vector_type(4)));
 
 constexpr int MOST = CACHE_MOST_SELECTED;
 constexpr float LEAST = 0x1p-100f;
-constexpr int ROWS = 16;                      // of k_select_rows' tile, its waves
-constexpr int CHUNK = 16 * ROWS;              // pages that it scores before rows are taken
-constexpr int CAP = 2048, PER = CAP / NT;     // keys that k_select_row takes the best of, those of a thread
+constexpr int WAVES = 8;                      // of a workgroup
+constexpr int ROWS = 16;                      // of k_select_rows' tile
+constexpr int CHUNK = 256;                    // pages that it scores before rows are taken
+constexpr int CAP = 2048;                     // keys that k_select_row takes the best of at once
 constexpr int PIECE = 512;                    // pages of a piece, at least
 constexpr int MOST_PIECES = 64;
 constexpr int SPLIT_UNITS = 2048;             // pieces of all rows and K/V heads of a call together
@@ -38,61 +39,78 @@ __device__ __forceinline__ uint32_t key_of(float x) {
     const uint32_t u = __float_as_uint(x + 0.0f);
     return u ^ ((uint32_t) ((int32_t) u >> 31) | 0x80000000u);
 }
+__device__ __forceinline__ float score_of(uint32_t key) { return __uint_as_float(key ^ (~(uint32_t) ((int32_t) key >> 31) | 0x80000000u)); }
 constexpr uint32_t KEY_LOWEST = 0x007fffffu;
 
-// in all lanes' joined halves: x + x of the lane 16 and 32 further
-__device__ __forceinline__ double sum_groups(double x) {
-    uint64_t u = __builtin_bit_cast(uint64_t, x);
-    auto lo = __builtin_amdgcn_permlane16_swap((uint32_t) u, (uint32_t) u, false, false);
-    auto hi = __builtin_amdgcn_permlane16_swap((uint32_t) (u >> 32), (uint32_t) (u >> 32), false, false);
-    x = __builtin_bit_cast(double, (uint64_t) hi[0] << 32 | lo[0]) + __builtin_bit_cast(double, (uint64_t) hi[1] << 32 | lo[1]);
-    u = __builtin_bit_cast(uint64_t, x);
-    lo = __builtin_amdgcn_permlane32_swap((uint32_t) u, (uint32_t) u, false, false);
-    hi = __builtin_amdgcn_permlane32_swap((uint32_t) (u >> 32), (uint32_t) (u >> 32), false, false);
+// x of this lane and the one 32 (16) further, added
+template <int BY>
+__device__ __forceinline__ double add_across(double x) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    auto swap = [](uint32_t w) {
+        if constexpr (BY == 32) return __builtin_amdgcn_permlane32_swap(w, w, false, false);
+        else return __builtin_amdgcn_permlane16_swap(w, w, false, false);
+    };
+    const auto lo = swap((uint32_t) u), hi = swap((uint32_t) (u >> 32));
     return __builtin_bit_cast(double, (uint64_t) hi[0] << 32 | lo[0]) + __builtin_bit_cast(double, (uint64_t) hi[1] << 32 | lo[1]);
 }
 
-// The codes of P and N of a row's queries at q (group heads) to out [2 HD], by a wave: 16 lanes have the dimensions, four groups of them the heads in turn
+// The codes of P and N of a row's queries at q (group heads) to out [2 HD], by a wave: a lane has two dimensions, of all heads or of every second or fourth.
+// Some heads are fetched ahead: loads come back in their order, and the digests' are to be on their way behind them.
 template <typename T, int HD>
-__device__ __forceinline__ void query_codes(const T * q, int group, unsigned char * out) {
-    constexpr int DIMS = HD / 16, WORDS = DIMS * sizeof(T) / 4;
-    struct values { T x[DIMS]; };
+struct row_queries {
+    static constexpr int LANES = HD / 2, EACH = HD == 96 ? 1 : 64 / LANES, WORDS = 2 * sizeof(T) / 4, AHEAD = 8 / EACH / WORDS;
+    struct values { T x[2]; };
     struct words { uint32_t w[WORDS]; };
-    const int lane = (int) threadIdx.x & 63, d0 = (lane & 15) * DIMS;
-    double pos[DIMS] = {}, neg[DIMS] = {};
-    bool odd = false;
-#pragma unroll 2
-    for (int h = lane >> 4; h < group; h += 4) {
-        words w;
+    words w[AHEAD];
+    __device__ __forceinline__ static int first() { return EACH == 1 ? 0 : ((int) threadIdx.x & 63) / LANES; }
+    __device__ __forceinline__ static int dim() { return min(((int) threadIdx.x & 63) % (EACH == 1 ? 64 : LANES), LANES - 1) * 2; }
+    __device__ __forceinline__ static words load(const T * q, int h) {
+        words x;
+        const uint32_t * at = (const uint32_t *) (q + (int64_t) h * HD + dim());
 #pragma unroll
-        for (int i = 0; i < WORDS; i++) w.w[i] = ((const uint32_t *) (q + (int64_t) h * HD + d0))[i];
-        const values y = __builtin_bit_cast(values, w);
+        for (int i = 0; i < WORDS; i++) x.w[i] = at[i];
+        return x;
+    }
+    __device__ __forceinline__ void fetch(const T * q, int group) {
 #pragma unroll
-        for (int d = 0; d < DIMS; d++) {
-            const float x = (float) y.x[d];
-            odd |= !(fabsf(x) < INFINITY);
-            pos[d] += (double) fmaxf(x, 0.0f);
-            neg[d] += (double) fminf(x, 0.0f);
+        for (int i = 0; i < AHEAD; i++) w[i] = load(q, min(first() + EACH * i, group - 1));
+    }
+    __device__ __forceinline__ void codes(const T * q, int group, unsigned char * out) const {
+        double pos[2] = {}, neg[2] = {};
+        bool odd = false;
+        auto add = [&](const words & from) {
+            const values y = __builtin_bit_cast(values, from);
+#pragma unroll
+            for (int d = 0; d < 2; d++) {
+                const float x = (float) y.x[d];
+                odd |= !(fabsf(x) < INFINITY);
+                pos[d] += (double) fmaxf(x, 0.0f);
+                neg[d] += (double) fminf(x, 0.0f);
+            }
+        };
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++)
+            if (first() + EACH * i < group) add(w[i]);
+        for (int h = first() + EACH * AHEAD; h < group; h += EACH) add(load(q, h));
+        float p[2], n[2], top = 0.0f;
+#pragma unroll
+        for (int d = 0; d < 2; d++) {
+            if constexpr (EACH >= 2) { pos[d] = add_across<32>(pos[d]); neg[d] = add_across<32>(neg[d]); }
+            if constexpr (EACH >= 4) { pos[d] = add_across<16>(pos[d]); neg[d] = add_across<16>(neg[d]); }
+            p[d] = (float) pos[d];
+            n[d] = (float) neg[d];
+            top = fmaxf(top, fmaxf(p[d], -n[d]));
+        }
+        top = col_max(row_max16(top));
+        if (__any(odd)) top = INFINITY;
+        const float inv = top >= LEAST && top < INFINITY ? 127.0f / top : 0.0f;
+        auto code = [&](float x) { return inv == 0.0f ? 0u : (uint32_t) (int) rintf(x * inv) & 255u; };
+        if (((int) threadIdx.x & 63) < LANES) {
+            *(uint16_t *) (out + dim()) = (uint16_t) (code(p[0]) | code(p[1]) << 8);
+            *(uint16_t *) (out + HD + dim()) = (uint16_t) (code(n[0]) | code(n[1]) << 8);
         }
     }
-    float p[DIMS], n[DIMS], top = 0.0f;
-#pragma unroll
-    for (int d = 0; d < DIMS; d++) {
-        p[d] = (float) sum_groups(pos[d]);
-        n[d] = (float) sum_groups(neg[d]);
-        top = fmaxf(top, fmaxf(p[d], -n[d]));
-    }
-    top = row_max16(top);
-    if (__any(odd)) top = INFINITY;
-    const float inv = top >= LEAST && top < INFINITY ? 127.0f / top : 0.0f;
-    if (lane < 16) {
-#pragma unroll
-        for (int d = 0; d < DIMS; d++) {
-            out[d0 + d] = (unsigned char) (signed char) (inv == 0.0f ? 0 : (int) rintf(p[d] * inv));
-            out[HD + d0 + d] = (unsigned char) (signed char) (inv == 0.0f ? 0 : (int) rintf(n[d] * inv));
-        }
-    }
-}
+};
 
 // pages that the row sees
 __device__ __forceinline__ int see_of(const cache_select_args & a, const seq_view & v, int64_t row, int page_shift) {
@@ -108,80 +126,94 @@ __device__ __forceinline__ int32_t entry(const cache_select_args & a, int i, int
 // ---------------------------------------------------------------------------------------------- a row a workgroup
 struct row_lds {
     uint32_t keys[CAP], pages[CAP], hist[256];
-    int32_t count[2][PER * 4];
-    uint32_t range[2][4];
+    int32_t count[2][CAP / 64];
+    uint32_t range[2][WAVES];
 };
 
-// The `keep` largest of n keys (CAP at most), ties to the first, left at the front in their order; by the workgroup. Returns how many are left.
-__device__ __forceinline__ int best_of(row_lds & l, int n, int keep) {
-    if (n <= keep) return n;
-    const int tid = (int) threadIdx.x, lane = tid & 63, wv = uniform(tid >> 6);
-    uint32_t k[PER], p[PER], most = 0, least = 0xffffffffu;
+// The `keep` largest of 64 WAVES PER keys in registers (key e 64 WAVES + thread in k[e]; 0: none), ties to the first, to the front of l.keys and l.pages in their
+// order; by the workgroup. Returns how many.
+template <int PER>
+__device__ __forceinline__ int best_of(row_lds & l, const uint32_t * k, const uint32_t * p, int keep) {
+    const int lane = (int) threadIdx.x & 63, tid = (int) threadIdx.x, wv = uniform(tid >> 6);
+    auto clear = [&] { if (tid < 256) l.hist[tid] = 0; };
+    // the smallest and largest key, and how many there are
+    uint32_t most = 0, least = 0xffffffffu;
+    int n = 0;
 #pragma unroll
     for (int e = 0; e < PER; e++) {
-        const bool has = e * NT + tid < n;
-        k[e] = has ? l.keys[e * NT + tid] : 0u;      // (0 is nobody's)
-        p[e] = has ? l.pages[e * NT + tid] : 0u;
         most = max(most, k[e]);
-        if (has) least = min(least, k[e]);
+        least = min(least, k[e] - 1);      // (0 becomes the largest)
+        n += (int) __popcll(__ballot(k[e] != 0));
     }
 #define DPP(x, ctrl, rows) (uint32_t) __builtin_amdgcn_update_dpp((int) x, (int) x, ctrl, rows, 0xf, false)
 #define JOIN(ctrl, rows) most = max(most, DPP(most, ctrl, rows)); least = min(least, DPP(least, ctrl, rows))
     JOIN(0x111, 0xf); JOIN(0x112, 0xf); JOIN(0x114, 0xf); JOIN(0x118, 0xf); JOIN(0x142, 0xa); JOIN(0x143, 0xc);
 #undef JOIN
 #undef DPP
-    if (lane == 63) { l.range[0][wv] = most; l.range[1][wv] = least; }
-    l.hist[tid] = 0;
+    most = (uint32_t) __builtin_amdgcn_readlane((int) most, 63);
+    least = (uint32_t) __builtin_amdgcn_readlane((int) least, 63);
+    clear();
+    if (lane == 0) { l.range[0][wv] = most; l.range[1][wv] = least; l.count[0][wv] = n; }
     __syncthreads();
-    most = max(max(l.range[0][0], l.range[0][1]), max(l.range[0][2], l.range[0][3]));
-    least = min(min(l.range[1][0], l.range[1][1]), min(l.range[1][2], l.range[1][3]));
+    n = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; w++) {
+        most = max(most, l.range[0][w]);
+        least = min(least, l.range[1][w]);
+        n += l.count[0][w];
+    }
+    least++;
     // the last one taken lies in [least, most], `need` of those are taken
     int need = keep;
-    for (;;) {
-        const int shift = most == least ? 0 : max(0, 24 - __builtin_clz(most - least));
+    if (n <= keep) {      // all of them
+        need = n;
+    } else {
+        for (;;) {
+            const int shift = most == least ? 0 : max(0, 24 - __builtin_clz(most - least));
 #pragma unroll
-        for (int e = 0; e < PER; e++)
-            if (k[e] >= least && k[e] <= most) atomicAdd(&l.hist[(k[e] - least) >> shift], 1u);
-        __syncthreads();
-        // every wave: four bins a lane, from the last
-        const int b0 = 255 - lane * 4;
-        int c[4], all = 0;
+            for (int e = 0; e < PER; e++)
+                if (k[e] >= least && k[e] <= most) atomicAdd(&l.hist[(k[e] - least) >> shift], 1u);
+            __syncthreads();
+            // every wave: four bins a lane, from the last
+            const int b0 = 255 - lane * 4;
+            int c[4], all = 0;
 #pragma unroll
-        for (int j = 0; j < 4; j++) all += c[j] = (int) l.hist[b0 - j];
-        const int upto = wave_scan(all);
-        const int at = __builtin_ctzll(__ballot(upto >= need));      // (some lane's: all of the range's are need or more)
-        int above = upto - all, bin = b0;
+            for (int j = 0; j < 4; j++) all += c[j] = (int) l.hist[b0 - j];
+            const int upto = wave_scan(all);
+            const int at = __builtin_ctzll(__ballot(upto >= need));      // (some lane's: all of the range's are need or more)
+            int above = upto - all, bin = b0;
 #pragma unroll
-        for (int j = 0; j < 3; j++)
-            if (bin == b0 - j && above + c[j] < need) { above += c[j]; bin--; }
-        const int in = bin == b0 ? c[0] : bin == b0 - 1 ? c[1] : bin == b0 - 2 ? c[2] : c[3];
-        const int take = need - __builtin_amdgcn_readlane(above, at), has = __builtin_amdgcn_readlane(in, at);
-        const uint32_t from = least + ((uint32_t) __builtin_amdgcn_readlane(bin, at) << shift);
-        need = take;
-        least = from;
-        most = most - from < 1u << shift ? most : from + ((1u << shift) - 1);
-        if (take == has || shift == 0) break;
-        __syncthreads();
-        l.hist[tid] = 0;
-        __syncthreads();
+            for (int j = 0; j < 3; j++)
+                if (bin == b0 - j && above + c[j] < need) { above += c[j]; bin--; }
+            const int in = bin == b0 ? c[0] : bin == b0 - 1 ? c[1] : bin == b0 - 2 ? c[2] : c[3];
+            need -= __builtin_amdgcn_readlane(above, at);
+            const uint32_t from = least + ((uint32_t) __builtin_amdgcn_readlane(bin, at) << shift);
+            least = from;
+            most = most - from < 1u << shift ? most : from + ((1u << shift) - 1);
+            if (need == __builtin_amdgcn_readlane(in, at) || shift == 0) break;
+            __syncthreads();
+            clear();
+            __syncthreads();
+        }
     }
     // more than `most`: all; in the range: the first `need`. A group is 64 consecutive keys, of a wave
     uint64_t eq[PER], gt[PER];
+    __syncthreads();      // (l.count has been read)
 #pragma unroll
     for (int e = 0; e < PER; e++) {
         eq[e] = __ballot(k[e] >= least && k[e] <= most);
         gt[e] = __ballot(k[e] > most);
-        if (lane == 0) { l.count[0][e * 4 + wv] = (int) __popcll(eq[e]); l.count[1][e * 4 + wv] = (int) __popcll(gt[e]); }
+        if (lane == 0) { l.count[0][e * WAVES + wv] = (int) __popcll(eq[e]); l.count[1][e * WAVES + wv] = (int) __popcll(gt[e]); }
     }
     __syncthreads();
-    static_assert(PER * 4 <= 64, "a group a lane");
-    const int mine_eq = lane < PER * 4 ? l.count[0][min(lane, PER * 4 - 1)] : 0, mine_gt = lane < PER * 4 ? l.count[1][min(lane, PER * 4 - 1)] : 0;
+    static_assert(PER * WAVES <= 64, "a group a lane");
+    const int of = min(lane, PER * WAVES - 1), mine_eq = lane < PER * WAVES ? l.count[0][of] : 0, mine_gt = lane < PER * WAVES ? l.count[1][of] : 0;
     const int eq_before = wave_scan(mine_eq) - mine_eq, ties = min(max(need - eq_before, 0), mine_eq);
     const int upto = wave_scan(mine_gt + ties), before = upto - mine_gt - ties;
     const uint64_t below = (1ull << lane) - 1;
 #pragma unroll
     for (int e = 0; e < PER; e++) {
-        const int of = e * 4 + wv, t = __builtin_amdgcn_readlane(ties, of), at = __builtin_amdgcn_readlane(before, of);
+        const int t = __builtin_amdgcn_readlane(ties, e * WAVES + wv), at = __builtin_amdgcn_readlane(before, e * WAVES + wv);
         const bool mine = (gt[e] >> lane & 1) || ((eq[e] >> lane & 1) && (int) __popcll(eq[e] & below) < t);
         const uint64_t in = __ballot(mine);
         if (mine) {
@@ -194,22 +226,38 @@ __device__ __forceinline__ int best_of(row_lds & l, int n, int keep) {
     return __builtin_amdgcn_readlane(upto, 63);
 }
 
-// `work`: a counter for each (row, K/V head) of several pieces, SPLIT_UNITS of them, then [row][K/V head][piece] what they found: their number, keys [take],
-// pages [take]
+// the same of n keys that `of` gives by their number, those of a thread before all threads are past this
+template <int PER, typename OF>
+__device__ __forceinline__ int best_from(row_lds & l, int keep, OF of) {
+    uint32_t k[PER], p[PER];
+#pragma unroll
+    for (int e = 0; e < PER; e++) of(e * 64 * WAVES + (int) threadIdx.x, k[e], p[e]);
+    return best_of<PER>(l, k, p, keep);
+}
+template <typename OF>
+__device__ __forceinline__ int best(row_lds & l, int n, int keep, OF of) {
+    static_assert(CAP == 4 * 64 * WAVES, "up to four keys a thread");
+    return n <= 64 * WAVES ? best_from<1>(l, keep, of) : n <= 2 * 64 * WAVES ? best_from<2>(l, keep, of) : best_from<4>(l, keep, of);
+}
+
+// `work`: a counter for each (row, K/V head) of several pieces, SPLIT_UNITS of them, then [row][K/V head][piece] what they found: keys [take] (0 behind the
+// last), pages [take]
 struct pieces_view {
     static constexpr int SC1 = 16;
     const brsrc r;
     const uint32_t bytes;
     __device__ pieces_view(const cache_select_args & a, int64_t unit)
-        : r(make_brsrc((unsigned char *) a.work + SPLIT_UNITS * 8 + unit * a.pieces * (8 * a.take + 16), (int64_t) a.pieces * (8 * a.take + 16))), bytes(8 * a.take + 16) {}
-    __device__ void put(int piece, int word, uint32_t x) const { __builtin_amdgcn_raw_buffer_store_b32(x, r, piece * bytes + word * 4, 0, SC1); }
-    __device__ uint32_t get(int piece, int word) const { return __builtin_amdgcn_raw_buffer_load_b32(r, piece * bytes + word * 4, 0, SC1); }
+        : r(make_brsrc((unsigned char *) a.work + SPLIT_UNITS * 8 + unit * a.pieces * (8 * a.take), (int64_t) a.pieces * (8 * a.take))), bytes(8 * a.take) {}
+    __device__ void put(int piece, int i, uint32_t key, uint32_t page) const {
+        __builtin_amdgcn_raw_buffer_store_b64(word2_t{key, page}, r, piece * bytes + i * 8, 0, SC1);
+    }
+    __device__ word2_t get(int piece, int i) const { return __builtin_amdgcn_raw_buffer_load_b64(r, piece * bytes + i * 8, 0, SC1); }
 };
 
 template <typename T, int HD>
-__global__ __launch_bounds__(NT) void k_select_row(cache_select_args a) {
-    constexpr int NK = 2 * HD / 64, CHUNK1 = CAP - MOST;
-    __shared__ __attribute__((aligned(16))) unsigned char codes[4][2 * HD];
+__global__ __launch_bounds__(64 * WAVES, 4) void k_select_row(cache_select_args a) {
+    constexpr int NK = 2 * HD / 64, THREADS = 64 * WAVES, AT_ONCE = (CAP - MOST) / THREADS * THREADS;
+    __shared__ __attribute__((aligned(16))) unsigned char codes[2 * HD];
     __shared__ row_lds l;
     const int tid = (int) threadIdx.x, lane = tid & 63, l15 = lane & 15, g = lane >> 4, wv = uniform(tid >> 6);
     const int group = a.n_head / a.n_kv_head, kvh = (int) (blockIdx.x % (unsigned) a.n_kv_head);
@@ -232,30 +280,38 @@ __global__ __launch_bounds__(NT) void k_select_row(cache_select_args a) {
         const int32_t * table = a.table + (int64_t) seq * a.width;
         // a lane's page of 64: the one whose score the matrix tiles will leave in it (tile l15 / 4, its page 4 g + l15 % 4)
         const int mine = (l15 >> 2) * 16 + g * 4 + (l15 & 3);
+        const unsigned char * const heads = a.digest + (int64_t) kvh * cache_digest_bytes(HD);
+        const int64_t per = a.n_kv_head * cache_digest_bytes(HD);
+        int4_t y[4][NK];
+        float scale;
+        bool bad;
         auto load_page = [&](int p) { return table[min(p + mine, p1 - 1)]; };
-        int32_t next = load_page(p0 + wv * 64);
-        query_codes<T, HD>((const T *) a.q + row * a.ldq + (int64_t) kvh * group * HD, group, codes[wv]);
-        wave_order();
+        auto load = [&](int32_t next) {
+            bad = next < 0 || next >= a.n_pages;
+            const int32_t page = bad ? 0 : next;
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                const int32_t of = __builtin_amdgcn_ds_bpermute(((l15 >> 2) * 16 + t * 4 + (l15 & 3)) * 4, page);      // the lane of the tile's page l15
+                const unsigned char * d = heads + of * per + g * 16;
+#pragma unroll
+                for (int k = 0; k < NK; k++) y[t][k] = *(const int4_t *) (d + k * 64);
+            }
+            scale = *(const float *) (heads + page * per + 2 * HD);
+        };
+        const int32_t first_page = load_page(p0 + wv * 64);
+        int32_t next = load_page(p0 + wv * 64 + THREADS);
+        const T * q = (const T *) a.q + row * a.ldq + (int64_t) kvh * group * HD;
+        row_queries<T, HD> queries;
+        if (wv == 0) queries.fetch(q, group);
+        load(first_page);      // (on their way while the queries' codes are made)
+        if (wv == 0) queries.codes(q, group, codes);
+        __syncthreads();
         int4_t b[NK];
 #pragma unroll
-        for (int k = 0; k < NK; k++) b[k] = *(const int4_t *) (codes[wv] + k * 64 + g * 16);      // (every column is the row)
-        for (int c0 = p0; c0 < p1; c0 += CHUNK1) {
-            const int c1 = min(c0 + CHUNK1, p1);
-            for (int s0 = c0 + wv * 64; s0 < c1; s0 += NT) {
-                const bool bad = next < 0 || next >= a.n_pages;
-                const int32_t page = bad ? 0 : next;
-                const unsigned char * const heads = a.digest + (int64_t) kvh * cache_digest_bytes(HD);
-                const int64_t per = a.n_kv_head * cache_digest_bytes(HD);
-                int4_t y[4][NK];
-#pragma unroll
-                for (int t = 0; t < 4; t++) {
-                    const int32_t of = __builtin_amdgcn_ds_bpermute(((l15 >> 2) * 16 + t * 4 + (l15 & 3)) * 4, page);      // the lane of the tile's page l15
-                    const unsigned char * d = heads + of * per + g * 16;
-#pragma unroll
-                    for (int k = 0; k < NK; k++) y[t][k] = *(const int4_t *) (d + k * 64);
-                }
-                const float scale = *(const float *) (heads + page * per + 2 * HD);
-                next = load_page(s0 + NT < c1 ? s0 + NT : c0 + CHUNK1 + wv * 64);
+        for (int k = 0; k < NK; k++) b[k] = *(const int4_t *) (codes + k * 64 + g * 16);      // (every column is the row)
+        for (int c0 = p0; c0 < p1; c0 += AT_ONCE) {
+            const int c1 = min(c0 + AT_ONCE, p1);
+            for (int s0 = c0 + wv * 64; s0 < c1; s0 += THREADS) {
                 int dot = 0;
 #pragma unroll
                 for (int t = 0; t < 4; t++) {
@@ -270,40 +326,51 @@ __global__ __launch_bounds__(NT) void k_select_row(cache_select_args a) {
                     l.keys[n + p - c0] = bad ? KEY_LOWEST : key_of((float) dot * scale);
                     l.pages[n + p - c0] = (uint32_t) p;
                 }
+                if (s0 + THREADS < p1) {      // (the next chunk's begin behind this one's: chunks are whole THREADS)
+                    load(next);
+                    next = load_page(s0 + 2 * THREADS);
+                }
             }
+            const int all = n + c1 - c0;
             __syncthreads();
-            n = best_of(l, n + c1 - c0, keep);
+            if (all > keep) {
+                auto of = [&](int i, uint32_t & key, uint32_t & page) {
+                    key = i < all ? l.keys[i] : 0u;
+                    page = i < all ? l.pages[i] : 0u;
+                };
+                n = best(l, all, keep, of);
+            } else {
+                n = all;
+            }
         }
     }
     if (a.pieces > 1) {
         const int64_t unit = row * a.n_kv_head + kvh;
         const pieces_view w(a, unit);
-        if (tid == 0) w.put(piece, 0, (uint32_t) n);
-        if (tid < n) {
-            w.put(piece, 4 + tid, l.keys[tid]);
-            w.put(piece, 4 + a.take + tid, l.pages[tid]);
-        }
+        static_assert(MOST <= THREADS, "a page a thread");
+        if (tid < keep) w.put(piece, tid, tid < n ? l.keys[tid] : 0u, tid < n ? l.pages[tid] : 0u);
         if (!last_to_arrive(a.work, unit, a.pieces)) return;
-        static_assert(MOST_PIECES <= 64 && MOST <= NT, "a piece a lane, a page a thread");
-        const int has = lane < a.pieces ? min((int) w.get(lane, 0), a.take) : 0, upto = wave_scan(has);
+        // all pieces' in their order, as many pieces at once as fit behind what is kept
         n = 0;
-        for (int k = 0, base = 0; k < a.pieces;) {      // as many pieces as fit behind what is kept
-            int m = n;
-            for (; k < a.pieces; k++) {
-                const int to = __builtin_amdgcn_readlane(upto, k), from = k ? __builtin_amdgcn_readlane(upto, k - 1) : 0;
-                if (n + to - base > CAP) break;
-                if (tid < to - from) {
-                    l.keys[m + tid] = w.get(k, 4 + tid);
-                    l.pages[m + tid] = w.get(k, 4 + a.take + tid);
+        for (int k0 = 0; k0 < a.pieces;) {
+            const int pieces = min((CAP - n) / keep, a.pieces - k0), all = n + pieces * keep;
+            auto of = [&](int i, uint32_t & key, uint32_t & page) {
+                key = page = 0;
+                if (i < n) {
+                    key = l.keys[i];
+                    page = l.pages[i];
+                } else if (i < all) {
+                    const word2_t x = w.get(k0 + (i - n) / keep, (i - n) % keep);
+                    key = x[0];
+                    page = x[1];
                 }
-                m += to - from;
-            }
-            base = k ? __builtin_amdgcn_readlane(upto, k - 1) : 0;
-            __syncthreads();
-            n = best_of(l, m, keep);
+            };
+            n = best(l, all, keep, of);
+            k0 += pieces;
         }
     }
-    if (tid < a.take) out[tid] = entry(a, tid, see, l.pages, n);
+    if (wv == 0)
+        for (int i = lane; i < a.take; i += 64) out[i] = entry(a, i, see, l.pages, n);
 }
 
 // ---------------------------------------------------------------------------------------------- a row a wave
@@ -329,20 +396,29 @@ __device__ __forceinline__ int keep_best(const uint32_t * k, const uint32_t * p,
 #undef DPP
         most = (uint32_t) __builtin_amdgcn_readlane((int) most, 63);
         least = (uint32_t) __builtin_amdgcn_readlane((int) least, 63) + 1;
-        // the largest t that `keep` or more reach, from the bits that all have on
-        t = least;
-        if (most != least) {
-            int bit = 31 - __builtin_clz(most ^ least);
-            t = most & ~((2u << bit) - 1);
-            for (; bit >= 0; bit--) {
-                const uint32_t c = t | 1u << bit;
-                int s = 0;
-#pragma unroll
-                for (int e = 0; e < E; e++) s += (int) __popcll(__ballot(k[e] >= c));
-                if (s >= keep) t = c;
-                if (s == keep) break;
+        // t: one that `keep` or more reach, and of these as many as differ from it fewer. Between lo, which is one, and hi, which fewer reach, by where a
+        // straight line through their counts (over the scores) has keep, or by half the keys where that did not halve their range: mostly five steps, 64 at most
+        uint32_t lo = least, hi = most + 1, was = 0;
+        int at_lo = n, at_hi = 0;
+        while (hi - lo > 1) {
+            const uint32_t range = hi - lo;
+            uint32_t c = lo + range / 2;
+            if (range <= was / 2 || !was) {
+                const float x = score_of(lo), part = ((float) (at_lo - keep) + 0.5f) * __builtin_amdgcn_rcpf((float) (at_lo - at_hi));
+                const float line = __builtin_fmaf(score_of(hi) - x, part, x);
+                if (fabsf(line) < INFINITY) c = min(max((uint32_t) __builtin_amdgcn_readfirstlane((int) key_of(line)), lo + 1), hi - 1);
+                was = range;
+            } else {
+                was = 0;
             }
+            int s = 0;
+#pragma unroll
+            for (int e = 0; e < E; e++) s += (int) __popcll(__ballot(k[e] >= c));
+            if (s >= keep) { lo = c; at_lo = s; }
+            else { hi = c; at_hi = s; }
+            if (s == keep) break;
         }
+        t = lo;
     }
     int ties = keep, at = 0;      // more than t: all of them; t itself: the first ones
 #pragma unroll
@@ -366,8 +442,8 @@ __device__ __forceinline__ int keep_best(const uint32_t * k, const uint32_t * p,
 }
 
 template <typename T, int HD>
-__global__ __launch_bounds__(64 * ROWS) void k_select_rows(cache_select_args a) {
-    constexpr int NK = 2 * HD / 64, QS = 2 * HD + 16, SS = CHUNK + 4, CE = CHUNK / 64, KE = MOST / 64;
+__global__ __launch_bounds__(64 * WAVES, 4) void k_select_rows(cache_select_args a) {
+    constexpr int NK = 2 * HD / 64, QS = 2 * HD + 16, SS = CHUNK + 4, CE = CHUNK / 64, KE = MOST / 64, EACH = ROWS / WAVES, TILES = CHUNK / (16 * WAVES);
     __shared__ __attribute__((aligned(16))) unsigned char codes[ROWS * QS];
     __shared__ __attribute__((aligned(16))) int32_t dots[ROWS * SS];
     __shared__ float scales[CHUNK];
@@ -376,7 +452,6 @@ __global__ __launch_bounds__(64 * ROWS) void k_select_rows(cache_select_args a) 
     const int group = a.n_head / a.n_kv_head, kvh = (int) (blockIdx.x % (unsigned) a.n_kv_head), page_shift = __builtin_ctz((unsigned) a.page_size);
     const int64_t t0 = (int64_t) (blockIdx.x / (unsigned) a.n_kv_head) * ROWS, t1 = min(t0 + ROWS, a.n_rows);
     const int keep = a.take - a.first - a.last;
-    uint32_t * const keys = lists + wv * a.take, * const pages = lists + (ROWS + wv) * a.take;
     for (int64_t r0 = t0; r0 < t1;) {      // the sequences of the tile's rows
         int seq;
         seq_view v;
@@ -385,76 +460,96 @@ __global__ __launch_bounds__(64 * ROWS) void k_select_rows(cache_select_args a) 
             r0 = min((int64_t) a.row_start[0], t1);
             continue;
         }
-        const int64_t r1 = min(t1, (int64_t) v.row0 + v.rows), row = min(r0 + wv, r1 - 1);
-        const bool has = r0 + wv < r1;
-        const int see = see_of(a, v, row, page_shift), see_all = see_of(a, v, r1 - 1, page_shift);      // (the last row sees the most)
-        int n = 0;
+        const int64_t r1 = min(t1, (int64_t) v.row0 + v.rows);
+        const int rows = (int) (r1 - r0), see_all = see_of(a, v, r1 - 1, page_shift);      // (the last row sees the most)
+        int n[EACH] = {};
         if (see_all > a.take && keep > 0) {
-            const int p0 = a.first, p1 = see_all - a.last, end = see > a.take && has ? see - a.last : 0;
+            const int p0 = a.first, p1 = see_all - a.last;
             const int32_t * table = a.table + (int64_t) seq * a.width;
-            bool bad = false;
-            int4_t y[NK];
-            float scale = 0.0f;
-            auto load_page = [&](int c0) { return table[min(c0 + wv * 16 + l15, p1 - 1)]; };
-            auto load = [&](int32_t page) {
-                bad = page < 0 || page >= a.n_pages;
-                const unsigned char * d = a.digest + ((bad ? 0 : (int64_t) page) * a.n_kv_head + kvh) * cache_digest_bytes(HD);
+            int4_t y[TILES][NK];
+            float scale[TILES];
+            int32_t next[TILES];
+            auto load_pages = [&](int c0) {
 #pragma unroll
-                for (int k = 0; k < NK; k++) y[k] = *(const int4_t *) (d + k * 64 + g * 16);
-                scale = *(const float *) (d + 2 * HD);
+                for (int i = 0; i < TILES; i++) next[i] = table[min(c0 + (wv * TILES + i) * 16 + l15, p1 - 1)];
             };
-            const int32_t first_page = load_page(p0);
-            int32_t next = load_page(p0 + CHUNK);
-            query_codes<T, HD>((const T *) a.q + row * a.ldq + (int64_t) kvh * group * HD, group, codes + wv * QS);
-            load(first_page);
+            auto load = [&] {
+#pragma unroll
+                for (int i = 0; i < TILES; i++) {
+                    const bool bad = next[i] < 0 || next[i] >= a.n_pages;
+                    const unsigned char * d = a.digest + ((bad ? 0 : (int64_t) next[i]) * a.n_kv_head + kvh) * cache_digest_bytes(HD);
+#pragma unroll
+                    for (int k = 0; k < NK; k++) y[i][k] = *(const int4_t *) (d + k * 64 + g * 16);
+                    scale[i] = bad ? -1.0f : *(const float *) (d + 2 * HD);
+                }
+            };
+            load_pages(p0);
+            auto q_of = [&](int i) { return (const T *) a.q + min(r0 + wv * EACH + i, r1 - 1) * a.ldq + (int64_t) kvh * group * HD; };
+            row_queries<T, HD> queries[EACH];
+#pragma unroll
+            for (int i = 0; i < EACH; i++) queries[i].fetch(q_of(i), group);
+            load();      // (on their way while the queries' codes are made)
+            load_pages(p0 + CHUNK);
+#pragma unroll
+            for (int i = 0; i < EACH; i++) queries[i].codes(q_of(i), group, codes + (wv * EACH + i) * QS);
             __syncthreads();
-            int4_t b[NK];
-#pragma unroll
-            for (int k = 0; k < NK; k++) b[k] = *(const int4_t *) (codes + l15 * QS + k * 64 + g * 16);
-            uint32_t pass = 0;
+            uint32_t pass[EACH] = {};
             for (int c0 = p0; c0 < p1; c0 += CHUNK) {
-                int4_t x = {0, 0, 0, 0};
 #pragma unroll
-                for (int k = 0; k < NK; k++) x = __builtin_amdgcn_mfma_i32_16x16x64_i8(y[k], b[k], x, 0, 0, 0);
-                *(int4_t *) (dots + l15 * SS + wv * 16 + g * 4) = x;
-                if (g == 0) scales[wv * 16 + l15] = bad ? -1.0f : scale;
+                for (int i = 0; i < TILES; i++) {
+                    int4_t x = {0, 0, 0, 0};
+#pragma unroll
+                    for (int k = 0; k < NK; k++)
+                        x = __builtin_amdgcn_mfma_i32_16x16x64_i8(y[i][k], *(const int4_t *) (codes + l15 * QS + k * 64 + g * 16), x, 0, 0, 0);
+                    *(int4_t *) (dots + l15 * SS + (wv * TILES + i) * 16 + g * 4) = x;
+                    if (g == 0) scales[(wv * TILES + i) * 16 + l15] = scale[i];
+                }
                 if (c0 + CHUNK < p1) {
-                    load(next);
-                    next = load_page(c0 + 2 * CHUNK);
+                    load();
+                    load_pages(c0 + 2 * CHUNK);
                 }
                 __syncthreads();
-                // this wave's row: the chunk's keys behind the ones it kept
-                const int m = min(CHUNK, end - c0);
-                uint32_t k[KE + CE], p[KE + CE];
-                bool some = false;
+                // this wave's rows: the chunk's keys behind the ones they kept
 #pragma unroll
-                for (int e = 0; e < CE; e++) {
-                    const int i = e * 64 + lane;
-                    const float f = scales[i];
-                    const uint32_t key = f < 0.0f ? KEY_LOWEST : key_of((float) dots[wv * SS + i] * f);
-                    k[KE + e] = i < m && key > pass ? key : 0u;
-                    p[KE + e] = (uint32_t) (c0 + i);
-                    some |= k[KE + e] != 0;
-                }
-                if (n == 0) {
-                    n = keep_best<CE>(k + KE, p + KE, keep, keys, pages, pass);
-                } else if (__any(some)) {
+                for (int i = 0; i < EACH; i++) {
+                    const int at = wv * EACH + i, see = see_of(a, v, r0 + at, page_shift), m = at < rows && see > a.take ? min(CHUNK, see - a.last - c0) : 0;
+                    if (m <= 0) continue;
+                    uint32_t * const keys = lists + at * a.take, * const pages = lists + (ROWS + at) * a.take;
+                    uint32_t k[KE + CE], p[KE + CE];
+                    bool some = false;
 #pragma unroll
-                    for (int e = 0; e < KE; e++) {
-                        const int i = e * 64 + lane;
-                        k[e] = i < n ? keys[i] : 0u;
-                        p[e] = i < n ? pages[i] : 0u;
+                    for (int e = 0; e < CE; e++) {
+                        const int j = e * 64 + lane;
+                        const float f = scales[j];
+                        const uint32_t key = f < 0.0f ? KEY_LOWEST : key_of((float) dots[at * SS + j] * f);
+                        k[KE + e] = j < m && key > pass[i] ? key : 0u;
+                        p[KE + e] = (uint32_t) (c0 + j);
+                        some |= k[KE + e] != 0;
+                    }
+                    if (n[i] == 0) {
+                        n[i] = keep_best<CE>(k + KE, p + KE, keep, keys, pages, pass[i]);
+                    } else if (__any(some)) {
+#pragma unroll
+                        for (int e = 0; e < KE; e++) {
+                            const int j = e * 64 + lane;
+                            k[e] = j < n[i] ? keys[j] : 0u;
+                            p[e] = j < n[i] ? pages[j] : 0u;
+                        }
+                        wave_order();
+                        n[i] = keep_best<KE + CE>(k, p, keep, keys, pages, pass[i]);
                     }
                     wave_order();
-                    n = keep_best<KE + CE>(k, p, keep, keys, pages, pass);
                 }
-                wave_order();
                 if (c0 + CHUNK < p1) __syncthreads();
             }
         }
-        if (has) {
-            int32_t * out = a.selected + (row * a.n_kv_head + kvh) * a.take;
-            for (int i = lane; i < a.take; i += 64) out[i] = entry(a, i, see, pages, n);
+#pragma unroll
+        for (int i = 0; i < EACH; i++) {
+            const int at = wv * EACH + i;
+            if (at >= rows) continue;
+            const int see = see_of(a, v, r0 + at, page_shift);
+            int32_t * out = a.selected + ((r0 + at) * a.n_kv_head + kvh) * a.take;
+            for (int j = lane; j < a.take; j += 64) out[j] = entry(a, j, see, lists + (ROWS + at) * a.take, n[i]);
         }
         __syncthreads();
         r0 = r1;
@@ -481,7 +576,7 @@ hipError_t select(const cache_shape & c, const cache_select_args & a, hipStream_
     args.pieces = pieces_of(c, a.n_seq, a.n_rows, a.width);
     args.piece = (a.width + args.pieces - 1) / args.pieces;
     return hipLaunchKernel(tiles ? (const void *) k_select_rows<T, HD> : (const void *) k_select_row<T, HD>, dim3((unsigned) blocks_of(c, a.n_seq, a.n_rows, a.width)),
-                           dim3(tiles ? 64 * ROWS : NT), p, tiles ? (unsigned) (2 * ROWS * a.take * 4) : 0, s);
+                           dim3(64 * WAVES), p, tiles ? (unsigned) (2 * ROWS * a.take * 4) : 0, s);
 }
 
 template <typename T>
@@ -493,13 +588,13 @@ hipError_t by_head(const cache_shape & c, const cache_select_args & a, hipStream
 
 // workgroups of 256 threads that the launch's are worth
 int64_t cache_select_blocks(const cache_shape & c, int64_t n_seq, int64_t n_rows, int64_t width) {
-    return blocks_of(c, n_seq, n_rows, width) * (tiles_of(c, n_seq, n_rows) ? 64 * ROWS / NT : 1);
+    return blocks_of(c, n_seq, n_rows, width) * (64 * WAVES / NT);
 }
 
 // What any call of no more rows, pages and pages taken needs
 int64_t cache_select_work_bytes(const cache_shape & c, int64_t n_rows, int64_t width, int take) {
     const int64_t most = std::min<int64_t>((width + PIECE - 1) / PIECE, MOST_PIECES);
-    return most > 1 ? SPLIT_UNITS * 8 + std::min<int64_t>(n_rows * c.n_kv_head * most, SPLIT_UNITS) * (8 * (int64_t) take + 16) : 0;
+    return most > 1 ? SPLIT_UNITS * 8 + std::min<int64_t>(n_rows * c.n_kv_head * most, SPLIT_UNITS) * 8 * (int64_t) take : 0;
 }
 
 hipError_t launch_cache_select(const cache_shape & c, int type, const cache_select_args & a, hipStream_t s) {
