@@ -34,6 +34,14 @@ __device__ __forceinline__ half8_t codes8(uint32_t w, uint32_t k1024) {
     return half8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
+// The codes of a word in the order of its elements as f16 subnormals, without less 8: c 2^-24, elements 2, 3, 6 and 7 sixteen times that. The matrix
+// instruction takes subnormals as they are, and half the work of codes8 goes where the other operand can hold the factors and the sum the offset.
+__device__ __forceinline__ half8_t raw8(uint32_t w) {
+    const uint32_t u = w >> 8;
+    const word4_t x = {w & 0x000f000fu, w & 0x00f000f0u, u & 0x000f000fu, u & 0x00f000f0u};
+    return __builtin_bit_cast(half8_t, x);
+}
+
 // the largest over the four lanes l, l ^ 16, l ^ 32, l ^ 48 (the lanes of one column)
 __device__ __forceinline__ float col_max(float x) {
     auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -58,6 +66,12 @@ __device__ __forceinline__ void load_words(uint32_t * x, brsrc r, int at, int of
     if constexpr (N == 2) { const word2_t v = __builtin_amdgcn_raw_buffer_load_b64(r, at, off, 0); x[0] = v[0]; x[1] = v[1]; }
     if constexpr (N == 3) { const word3_t v = __builtin_amdgcn_raw_buffer_load_b96(r, at, off, 0); x[0] = v[0]; x[1] = v[1]; x[2] = v[2]; }
     if constexpr (N == 4) { const word4_t v = __builtin_amdgcn_raw_buffer_load_b128(r, at, off, 0); x[0] = v[0]; x[1] = v[1]; x[2] = v[2]; x[3] = v[3]; }
+}
+__device__ __forceinline__ float col_sum(float x) {      // (the same of sums)
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 __device__ __forceinline__ void wave_order() {      // LDS accesses of the wave's lanes before and after stay in this order
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -301,13 +315,14 @@ __device__ __forceinline__ void turn_weights(const float4_t * s, int h, half8_t 
     for (int k = 0; k < TERMS; k++) l = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, p[k], l, 0, 0, 0);
 }
 
-// O^T += V^T P^T of 16 dimensions and 32 keys, from V's codes and the scales of the same keys (4 at d, 4 at d + stride)
-template <int TERMS>
+// O^T += V^T P^T of 16 dimensions and 32 keys, from V's codes and the scales of the same keys (4 at d, 4 at d + stride); EXACT: values as two f16, else
+// rounded to one
+template <int TERMS, bool EXACT = true>
 __device__ __forceinline__ float4_t add_values(half8_t codes, const unsigned char * d, int stride, const half8_t * p, float4_t o) {
     const half8_t scales = __builtin_shufflevector(*(const half4_t *) d, *(const half4_t *) (d + stride), 0, 1, 2, 3, 4, 5, 6, 7);
-    const half8_t v = codes * scales, rest = __builtin_elementwise_fma(codes, scales, -v);
+    const half8_t v = codes * scales;
     o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[0], o, 0, 0, 0);
-    o = __builtin_amdgcn_mfma_f32_16x16x32_f16(rest, p[0], o, 0, 0, 0);
+    if constexpr (EXACT) o = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_elementwise_fma(codes, scales, -v), p[0], o, 0, 0, 0);
     if constexpr (TERMS == 2) o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[1], o, 0, 0, 0);
     return o;
 }

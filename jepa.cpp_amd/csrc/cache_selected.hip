@@ -29,6 +29,7 @@ template <int HD> constexpr int split_lds() {
 template <typename T, int HD, bool WHOLE>
 __global__ __launch_bounds__(NT, groups_of<T>(HD)) void k_cache_selected(cache_selected_args a) {
     constexpr int NB = HD / 32, ND = HD / 16, TERMS = sizeof(T) == 4 ? 2 : 1, LISTS = WHOLE ? 4 : 1;
+    constexpr bool RAW = TERMS == 1, EXACT = !std::is_same<T, __bf16>::value;
     __shared__ __attribute__((aligned(16))) unsigned char lds[WHOLE ? 4 * wave_lds<HD>() : split_lds<HD>()];
     __shared__ int2_t lists[LISTS][MOST];      // a page of the cache, the token it begins with
     const int tid = (int) threadIdx.x, lane = tid & 63, l15 = lane & 15, g = lane >> 4, wv = uniform(tid >> 6), group = a.n_head / a.n_kv_head;
@@ -114,6 +115,20 @@ __global__ __launch_bounds__(NT, groups_of<T>(HD)) void k_cache_selected(cache_s
     float c;
     half8_t q[NB][TERMS];
     turn_query<T, HD, TERMS>(a.scale, y, q, c);
+    float offset[NB];      // what the product with the raw codes of a block begins with
+    if constexpr (RAW) {
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                if (j & 2) q[b][0][j] *= (_Float16) 0.0625f;
+                sum = __builtin_fmaf((float) q[b][0][j], j & 2 ? 16.0f : 1.0f, sum);
+            }
+            offset[b] = col_sum(sum) * -0x1p-21f;
+        }
+        c *= 0x1p24f;
+    }
     float4_t o[ND + 1];
     float mu = -INFINITY;
     for (int d = 0; d <= ND; d++) o[d] = float4_t{0, 0, 0, 0};
@@ -150,9 +165,10 @@ __global__ __launch_bounds__(NT, groups_of<T>(HD)) void k_cache_selected(cache_s
             const half4_t * dk = (const half4_t *) (scales + t * 2 * HD + g * (8 * NB));
 #pragma unroll
             for (int b = 0; b < NB; b++) {
-                const half8_t kc = codes8(kn[t][b], k1024);
+                const half8_t kc = RAW ? raw8(kn[t][b]) : codes8(kn[t][b], k1024);
                 const half4_t d = dk[b];
-                float4_t x = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc, q[b][0], float4_t{0, 0, 0, 0}, 0, 0, 0);
+                const float z = RAW ? offset[b] : 0.0f;
+                float4_t x = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc, q[b][0], float4_t{z, z, z, z}, 0, 0, 0);
                 if constexpr (TERMS == 2) x = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc, q[b][1], x, 0, 0, 0);
 #pragma unroll
                 for (int r = 0; r < 4; r++) s[t][r] = __builtin_fmaf((float) d[r], x[r], b == 0 ? 0.0f : s[t][r]);
@@ -179,7 +195,7 @@ __global__ __launch_bounds__(NT, groups_of<T>(HD)) void k_cache_selected(cache_s
                 const int2_t w = __builtin_amdgcn_ds_read_tr4_b64_v2i32((__attribute__((address_space(3))) int2_t *) (mine + d * 528 + tr_at));
 #pragma unroll
                 for (int h = 0; h < 2; h++)
-                    o[d] = add_values<TERMS>(codes8((uint32_t) w[h], k1024), scales + HD + g * (8 * NB) + b * 8 + 2 * h * (2 * HD), 2 * HD, p[h], o[d]);
+                    o[d] = add_values<TERMS, EXACT>(codes8((uint32_t) w[h], k1024), scales + HD + g * (8 * NB) + b * 8 + 2 * h * (2 * HD), 2 * HD, p[h], o[d]);
             }
             __builtin_amdgcn_sched_barrier(0x100);
         }

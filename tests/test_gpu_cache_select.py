@@ -4,7 +4,7 @@ together as a program makes them step by step, eager and captured.
 
 Attention's tolerance for one row, head and dimension n, out_n = sum_j p_j v_jn, A_n = sum_j p_j |v_jn| and N_n = sum_j |v_jn| over the tokens that the row reads:
   the output's own rounding   eps_T / 2 |out_n|, and half its smallest step
-  a value                     enters exactly
+  a value                     enters exactly; for bf16 rows rounded to f16, 2^-11 A_n
   a weight                    16-bit rows: 2^-11 relative (half a step of f16); f32 rows 2^-20 with the exponential and the sums. The sum that divides is of the same
                               rounded weights, so that it counts with |v_jn - out_n|: at most A_n + |out_n|. Weights far below the largest (brought to 2^10 or
                               more) lose half of f16's smallest step: 2^-35 N_n
@@ -378,7 +378,7 @@ def definition(c, q, lens, where, chosen, block, scale, kind, table=None):
             f = 2.0 ** -20 + 2 * (hd / 8 + 8) * 2.0 ** -22 * S + (0 if kind == "f32" else 2.0 ** -11)
             sl = slice(h * group, (h + 1) * group)
             out[r, sl] = y
-            tol[r, sl] = eps * y.abs() * (1 + f) + f * (A + y.abs()) + 2.0 ** -35 * N + (2.0 ** -25 if kind == "f16" else 1e-38)
+            tol[r, sl] = eps * y.abs() * (1 + f) + f * (A + y.abs()) + (2.0 ** -11 * A if kind == "bf16" else 0) + 2.0 ** -35 * N + (2.0 ** -25 if kind == "f16" else 1e-38)
     return out, tol
 
 
