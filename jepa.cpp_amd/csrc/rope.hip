@@ -96,12 +96,15 @@ __global__ __launch_bounds__(256) void k_cache_append(append_args a, rope_args q
     }
 }
 
-// Threads share a row's cosines and sines over as many heads as leave the chip this many threads
-constexpr int64_t ENOUGH = 1 << 18;
+// A thread makes its cosines and sines once for some heads, up to 8, as long as that leaves the chip threads enough. Measured, us: 8192 bf16 rows of 16 heads of 88
+// with 2^16 threads 11.4, 2^17 12.3, 2^18 12.9, 2^19 17.3; 4128 f32 frame rows of 16 + 16 + 16 heads of 64 appended with 2^17 threads for keys 18.4 to 18.6 (2^16 19.2,
+// 2^18 23.8, 2^19 34); 32768 bf16 rows of 32 + 8 + 8 heads of 128 with up to 16 heads a thread 164, 8 151, 4 164, 2 214.
+constexpr int64_t THREADS = 1 << 16, KEY_THREADS = 1 << 17;
+constexpr int MOST_HEADS = 8;
 void share(rope_args & a, const rope_map & m, bool halves) {
     a.units = halves ? m.rot / 16 + (m.hd - m.rot) / 8 : m.hd / 8;
     a.rows_per = 256 / a.units;
-    a.heads_per = (int) std::clamp<int64_t>(a.n_rows * a.units * a.n_head / ENOUGH, 1, std::min(16, a.n_head));
+    a.heads_per = (int) std::clamp<int64_t>(a.n_rows * a.units * a.n_head / THREADS, 1, std::min(MOST_HEADS, a.n_head));
     a.head_blocks = (a.n_head + a.heads_per - 1) / a.heads_per;
 }
 int64_t blocks_of(const rope_args & a) { return (a.n_rows + a.rows_per - 1) / a.rows_per * a.head_blocks; }
@@ -117,7 +120,7 @@ hipError_t rope(rope_args a, rope_map m, hipStream_t s) {
 template <typename T, int HD>
 hipError_t append(append_args a, rope_args q, rope_map m, hipStream_t s) {
     const int64_t rows = group<HD>::rows, row_blocks = (a.n_rows + rows - 1) / rows;
-    a.heads_per = (int) std::clamp<int64_t>(row_blocks * a.n_kv_head * 256 / ENOUGH, 1, std::min(16, a.n_kv_head));
+    a.heads_per = (int) std::clamp<int64_t>(row_blocks * a.n_kv_head * 256 / KEY_THREADS, 1, std::min(MOST_HEADS, a.n_kv_head));
     a.head_blocks = (a.n_kv_head + a.heads_per - 1) / a.heads_per;
     a.kv_blocks = (unsigned) (row_blocks * a.head_blocks);
     int64_t q_blocks = 0;
