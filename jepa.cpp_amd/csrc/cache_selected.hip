@@ -247,17 +247,19 @@ __global__ __launch_bounds__(NT, groups_of<T>(HD)) void k_cache_selected(cache_s
     }
 }
 
-// A wave for each unit where there are enough of them to fill the chip's waves; else a workgroup, or as many as fill the chip's workgroups once, if
-// each has a step of its waves to do
+// A wave for each unit where there are two for each SIMD; else a workgroup, or as many as there are CUs, if each has a step of its waves to do. Measured, us of
+// a call with a workgroup / a wave a unit: f16 rows of 32 heads over 8 of 128, 1024 tokens each, 512 units 21.4 / 37.1, 1024 36.2 / 37.7, 1536 49.0 / 52.4,
+// 2048 60.5 / 58.1, 3072 86.7 / 78.1, 4096 110 / 105; bf16 rows of 16 heads of 64, 512 tokens each, 1024 units 14.2 / 15.0, 3072 32.4 / 24.7.
+// Pieces of 240 units into 480 or 720 workgroups 16.2, whole 14.5; of 128 units (2048 tokens each) whole 21.2, 256 workgroups 15.9, 512 15.8, 768 16.0.
+constexpr int64_t WAVE_UNITS = 2048, SLOTS = 256;
 int64_t steps_of(const cache_shape & c, int take) { return ((int64_t) take * c.page_size + 4 * TILE - 1) / (4 * TILE); }
-int64_t slots_of(const cache_shape & c) { return 256 * groups_of<float>(c.hd); }
 struct split { int tiles; bool whole; int pieces, piece_tiles; };
 split split_of(const cache_shape & c, int64_t n_rows, int take) {
     split s;
     s.tiles = (c.n_head / c.n_kv_head + C - 1) / C;
-    const int64_t units = n_rows * s.tiles * c.n_kv_head, slots = slots_of(c), steps = steps_of(c, take);
-    s.whole = units >= 4 * slots;
-    s.pieces = s.whole ? 1 : (int) std::clamp<int64_t>(slots / std::max<int64_t>(units, 1), 1, steps);
+    const int64_t units = n_rows * s.tiles * c.n_kv_head, steps = steps_of(c, take);
+    s.whole = units >= WAVE_UNITS;
+    s.pieces = s.whole ? 1 : (int) std::clamp<int64_t>(SLOTS / std::max<int64_t>(units, 1), 1, steps);
     const int64_t each = (steps + s.pieces - 1) / s.pieces;
     s.piece_tiles = (int) each * 4;
     s.pieces = (int) ((steps + each - 1) / each);
@@ -290,11 +292,11 @@ int64_t cache_selected_blocks(const cache_shape & c, int64_t n_rows, int take) {
     return (f.whole ? (units + 3) / 4 : units * f.pieces) * c.n_kv_head;
 }
 
-// What any call of no more rows and pages needs: pieces are there only while units are half the slots or fewer, and then no more than these together
+// What any call of no more rows and pages needs: of units in several pieces there are half the slots or fewer, and no more pieces than slots
 int64_t cache_selected_work_bytes(const cache_shape & c, int64_t n_rows, int take) {
-    static_assert(256 * 4 <= COUNTERS, "a counter for each unit of several pieces");
+    static_assert(SLOTS <= COUNTERS, "a counter for each unit of several pieces");
     const int64_t units = n_rows * ((c.n_head / c.n_kv_head + C - 1) / C) * c.n_kv_head, steps = steps_of(c, take);
-    return steps > 1 ? COUNTERS * 8 + std::min(units * steps, slots_of(c)) * C * (c.hd + 2) * 4 : 0;
+    return steps > 1 ? COUNTERS * 8 + std::min(units * steps, SLOTS) * C * (c.hd + 2) * 4 : 0;
 }
 
 hipError_t launch_cache_selected(const cache_shape & c, int type, const cache_selected_args & a, hipStream_t s) {
