@@ -15,26 +15,38 @@ namespace {
 
 constexpr float LEAST = 0x1p-100f;
 
-#define DPP(x, ctrl) __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), ctrl, 0xf, 0xf, true))
-// the largest over aligned groups of N lanes: pairs, quads, mirrored halves of 16, mirrored 16
+// The largest over aligned groups of N lanes (pairs, quads, halves of 16 mirrored, 16 mirrored) of eight values that are no NaN, in place. In one block, for
+// the compiler would make each of them canonical first: a DPP operand has to be two instructions old, which the others of the eight see to.
+#define STEP(how)                                                                                                                                                       \
+    asm volatile("s_nop 1\n\tv_max_f32_dpp %0, %0, %0 " how "\n\tv_max_f32_dpp %1, %1, %1 " how "\n\tv_max_f32_dpp %2, %2, %2 " how "\n\tv_max_f32_dpp %3, %3, %3 " how  \
+                 "\n\tv_max_f32_dpp %4, %4, %4 " how "\n\tv_max_f32_dpp %5, %5, %5 " how "\n\tv_max_f32_dpp %6, %6, %6 " how "\n\tv_max_f32_dpp %7, %7, %7 " how "\n\ts_nop 1"  \
+                 : "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3]), "+v"(x[4]), "+v"(x[5]), "+v"(x[6]), "+v"(x[7]))
 template <int N>
-__device__ __forceinline__ float max_of(float x) {
-    x = fmaxf(x, DPP(x, 0xb1));
-    x = fmaxf(x, DPP(x, 0x4e));
-    if constexpr (N >= 8) x = fmaxf(x, DPP(x, 0x141));
-    if constexpr (N >= 16) x = fmaxf(x, DPP(x, 0x140));
-    return x;
+__device__ __forceinline__ void max_of(float * x) {
+    STEP("quad_perm:[1,0,3,2] row_mask:0xf bank_mask:0xf");
+    STEP("quad_perm:[2,3,0,1] row_mask:0xf bank_mask:0xf");
+    if constexpr (N >= 8) STEP("row_half_mirror row_mask:0xf bank_mask:0xf");
+    if constexpr (N >= 16) STEP("row_mirror row_mask:0xf bank_mask:0xf");
 }
-#undef DPP
+#undef STEP
+
+// rint of four values of magnitude 127 at most, as bytes: what an addition of 1.5 * 2^23 leaves in the lowest bits
+__device__ __forceinline__ uint32_t bytes_of(const float * x) {
+    uint32_t u[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) u[j] = __float_as_uint(x[j] + 0x1.8p23f);
+    const uint32_t lo = __builtin_amdgcn_perm(u[1], u[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(u[3], u[2], 0x04000c0cu);
+    return lo | hi;
+}
 
 template <int HD, int AHEAD>
 __global__ __launch_bounds__(NT) void k_cache_digest(cache_digest_args a) {
     // lanes of the same dimensions, tokens of each: 64 lanes are 4 NB words of codes (of 8 dimensions) times TL (48 of 64 for three blocks)
     constexpr int NB = HD / 32, TL = HD == 32 ? 16 : HD == 64 ? 8 : 4, TOKENS = 16 / TL;
     const int lane = (int) threadIdx.x & 63, tl = lane % TL, word = min(lane / TL, 4 * NB - 1), g = word / NB, b = word % NB;
-    const int64_t unit = (int64_t) blockIdx.x * 4 + uniform((int) threadIdx.x >> 6);
-    const int kvh = (int) (unit % a.n_kv_head);
-    const int64_t r0 = unit / a.n_kv_head * a.rows_per, r1 = min(r0 + a.rows_per, a.n_rows);
+    const uint32_t unit = blockIdx.x * 4 + (uint32_t) uniform((int) threadIdx.x >> 6);      // (below 2^26)
+    const int kvh = (int) (unit % (uint32_t) a.n_kv_head);
+    const int64_t r0 = (int64_t) (unit / (uint32_t) a.n_kv_head) * a.rows_per, r1 = min(r0 + a.rows_per, a.n_rows);
     const int page_shift = __builtin_ctz((unsigned) a.page_size), strips_of_page = a.page_size / 16;
     uint32_t k1024 = 0x64006400u;
     asm volatile("" : "+v"(k1024));
@@ -56,9 +68,9 @@ __global__ __launch_bounds__(NT) void k_cache_digest(cache_digest_args a) {
             if (page < 0 || page >= a.n_pages) continue;
             const int tokens = min(a.page_size, v.len - (p << page_shift));
             const unsigned char * strips = a.cache + (page * a.n_kv_head + kvh) * strips_of_page * (18 * HD);
-            float hi[8], lo[8];
+            float hi[8], lo[8];      // the largest value, and the largest of the values' negatives
 #pragma unroll
-            for (int j = 0; j < 8; j++) { hi[j] = -INFINITY; lo[j] = INFINITY; }
+            for (int j = 0; j < 8; j++) hi[j] = lo[j] = -INFINITY;
             for (int t0 = 0; t0 * 16 < tokens; t0 += AHEAD) {
                 uint32_t w[AHEAD][TOKENS], d[AHEAD][(TOKENS + 1) / 2];
 #pragma unroll
@@ -78,28 +90,32 @@ __global__ __launch_bounds__(NT) void k_cache_digest(cache_digest_args a) {
                         const half8_t c = codes8(w[t][k], k1024);
 #pragma unroll
                         for (int j = 0; j < 8; j++) {
-                            const float x = (float) c[j] * scale;
+                            const float x = __builtin_fmaf((float) c[j], scale, 0.0f);      // (takes the f16 as it is)
                             hi[j] = fmaxf(hi[j], x);
-                            lo[j] = fminf(lo[j], x);
+                            lo[j] = fmaxf(lo[j], -x);
                         }
                     }
                 }
             }
+            max_of<TL>(hi);
+            max_of<TL>(lo);
+            if (__any(hi[0] == -INFINITY)) {      // no token of this block of the head is a number
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    if (hi[j] == -INFINITY) hi[j] = lo[j] = 0.0f;
+            }
             float top = 0.0f;
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const float h = max_of<TL>(hi[j]), l = -max_of<TL>(-lo[j]);
-                hi[j] = h == -INFINITY ? 0.0f : h;
-                lo[j] = l == INFINITY ? 0.0f : l;
-                top = fmaxf(top, fmaxf(fabsf(hi[j]), fabsf(lo[j])));
-            }
+            for (int j = 0; j < 8; j++) top = fmaxf(top, fmaxf(fabsf(hi[j]), fabsf(lo[j])));
             top = col_max(row_max16(top));
             const float inv = top >= LEAST ? 127.0f / top : 0.0f, scale = top >= LEAST ? top / 127.0f : 0.0f;
             // the first lane of the same dimensions writes the largest, the second the smallest
             unsigned char * out = a.digest + (page * a.n_kv_head + kvh) * cache_digest_bytes(HD);
-            word2_t codes = {0, 0};
+            float x[8];
+            const float by = tl == 0 ? inv : -inv;
 #pragma unroll
-            for (int j = 0; j < 8; j++) codes[j / 4] |= ((uint32_t) (int) rintf((tl == 0 ? hi[j] : lo[j]) * inv) & 255u) << (8 * (j & 3));
+            for (int j = 0; j < 8; j++) x[j] = (tl == 0 ? hi[j] : lo[j]) * by;
+            const word2_t codes = {bytes_of(x), bytes_of(x + 4)};
             if (tl < 2 && lane < 4 * NB * TL) *(word2_t *) (out + tl * HD + 32 * b + 8 * g) = codes;
             if (lane < 4) *(uint32_t *) (out + 2 * HD + lane * 4) = lane == 0 ? __float_as_uint(scale) : 0u;
         }
