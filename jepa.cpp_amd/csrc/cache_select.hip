@@ -9,16 +9,20 @@
 // are dealt out. Ties go to the lower page.
 //
 //   few rows (k_select_row)    a workgroup has a row and K/V head, or a piece of its pages where the table is long (the last piece to arrive takes the
-//                              best of all pieces' best). Its waves score 64 pages at a time, the loads of four matrix tiles in flight. The best of up to
-//                              CAP keys: histograms of 256 bins between the smallest and the largest key narrow the range of the last one that is
-//                              taken, 8 bits at a time and mostly twice; ballots and a scan put the taken ones behind each other in their order.
-//   many rows (k_select_rows)  a workgroup of 16 waves has a K/V head and 16 consecutive rows, which share the digests that it reads. Each wave scores 16 pages of
-//                              a chunk for all rows and then takes one row: its keys stay in registers, the bits of the last one that is taken are found one
-//                              by one with a ballot for each 64 keys.
+//                              best of all pieces' best). Its waves score 64 pages at a time, the loads of four matrix tiles in flight.
+//   many rows (k_select_rows)  a workgroup has a K/V head and 16 consecutive rows, which share the digests that it reads; scores go from the matrix
+//                              instruction's registers into the search, all rows in step.
+// The best of some keys are found by histograms of 256 bins between the smallest and the largest: they narrow the range of the last one that is taken, 8
+// bits at a time and mostly twice; counts and a scan of them put the taken ones behind each other in their order.
+//
+// Measured: a token of 64 requests of 200 to 8000 tokens in pages of 16, 32 heads over 8 of 128, 15.6 us (35 MB of digests, 2.2 TB/s: 1 us until a row's sequence is known, 2 for
+// page numbers and queries' codes, 2 to 6 for the digests, 2 to 3 for the search); two contexts of 90000 to 131000 tokens in pages of 32, 14.2; 2000 rows over 250 pages of 64,
+// 32 heads over 4, 19.4: 10 us of the VALU's time, 1600 instructions of each wave, in phases that wait for each other.
 #include "cache_attn_dev.h"
 #include "common.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace {
 
@@ -28,7 +32,7 @@ constexpr int MOST = CACHE_MOST_SELECTED;
 constexpr float LEAST = 0x1p-100f;
 constexpr int WAVES = 8;                      // of a workgroup
 constexpr int ROWS = 16;                      // of k_select_rows' tile
-constexpr int CHUNK = 256;                    // pages that it scores before rows are taken
+constexpr int CHUNK = 256;                    // pages that it scores before rows take the best
 constexpr int CAP = 2048;                     // keys that k_select_row takes the best of at once
 constexpr int PIECE = 512;                    // pages of a piece, at least
 constexpr int MOST_PIECES = 64;
@@ -39,7 +43,6 @@ __device__ __forceinline__ uint32_t key_of(float x) {
     const uint32_t u = __float_as_uint(x + 0.0f);
     return u ^ ((uint32_t) ((int32_t) u >> 31) | 0x80000000u);
 }
-__device__ __forceinline__ float score_of(uint32_t key) { return __uint_as_float(key ^ (~(uint32_t) ((int32_t) key >> 31) | 0x80000000u)); }
 constexpr uint32_t KEY_LOWEST = 0x007fffffu;
 
 // x of this lane and the one 32 (16) further, added
@@ -373,85 +376,32 @@ __global__ __launch_bounds__(64 * WAVES, 4) void k_select_row(cache_select_args 
         for (int i = lane; i < a.take; i += 64) out[i] = entry(a, i, see, l.pages, n);
 }
 
-// ---------------------------------------------------------------------------------------------- a row a wave
-// The `keep` largest of the keys in E registers of the lanes (0: none), ties to the first, put into keys and pages in their order; by a wave. Returns how
-// many, and what a later key has to pass.
-template <int E>
-__device__ __forceinline__ int keep_best(const uint32_t * k, const uint32_t * p, int keep, uint32_t * keys, uint32_t * pages, uint32_t & pass) {
-    const int lane = (int) threadIdx.x & 63;
-    uint32_t most = 0, least = 0xffffffffu;
-    int n = 0;
-#pragma unroll
-    for (int e = 0; e < E; e++) {
-        most = max(most, k[e]);
-        least = min(least, k[e] - 1);      // (0 becomes the largest)
-        n += (int) __popcll(__ballot(k[e] != 0));
-    }
-    uint32_t t = 0;
-    if (n > keep) {
-#define DPP(x, ctrl, rows) (uint32_t) __builtin_amdgcn_update_dpp((int) x, (int) x, ctrl, rows, 0xf, false)
-#define JOIN(ctrl, rows) most = max(most, DPP(most, ctrl, rows)); least = min(least, DPP(least, ctrl, rows))
-        JOIN(0x111, 0xf); JOIN(0x112, 0xf); JOIN(0x114, 0xf); JOIN(0x118, 0xf); JOIN(0x142, 0xa); JOIN(0x143, 0xc);
-#undef JOIN
-#undef DPP
-        most = (uint32_t) __builtin_amdgcn_readlane((int) most, 63);
-        least = (uint32_t) __builtin_amdgcn_readlane((int) least, 63) + 1;
-        // t: one that `keep` or more reach, and of these as many as differ from it fewer. Between lo, which is one, and hi, which fewer reach, by where a
-        // straight line through their counts (over the scores) has keep, or by half the keys where that did not halve their range: mostly five steps, 64 at most
-        uint32_t lo = least, hi = most + 1, was = 0;
-        int at_lo = n, at_hi = 0;
-        while (hi - lo > 1) {
-            const uint32_t range = hi - lo;
-            uint32_t c = lo + range / 2;
-            if (range <= was / 2 || !was) {
-                const float x = score_of(lo), part = ((float) (at_lo - keep) + 0.5f) * __builtin_amdgcn_rcpf((float) (at_lo - at_hi));
-                const float line = __builtin_fmaf(score_of(hi) - x, part, x);
-                if (fabsf(line) < INFINITY) c = min(max((uint32_t) __builtin_amdgcn_readfirstlane((int) key_of(line)), lo + 1), hi - 1);
-                was = range;
-            } else {
-                was = 0;
-            }
-            int s = 0;
-#pragma unroll
-            for (int e = 0; e < E; e++) s += (int) __popcll(__ballot(k[e] >= c));
-            if (s >= keep) { lo = c; at_lo = s; }
-            else { hi = c; at_hi = s; }
-            if (s == keep) break;
-        }
-        t = lo;
-    }
-    int ties = keep, at = 0;      // more than t: all of them; t itself: the first ones
-#pragma unroll
-    for (int e = 0; e < E; e++) ties -= (int) __popcll(__ballot(k[e] > t));
-    const uint64_t before = (1ull << lane) - 1;
-#pragma unroll
-    for (int e = 0; e < E; e++) {
-        const uint64_t eq = __ballot(k[e] == t && t != 0);
-        const bool mine = k[e] > t || ((eq >> lane & 1) && (int) __popcll(eq & before) < ties);
-        const uint64_t in = __ballot(mine);
-        if (mine) {
-            const int i = at + (int) __popcll(in & before);
-            keys[i] = k[e];
-            pages[i] = p[e];
-        }
-        at += (int) __popcll(in);
-        ties -= min(ties, (int) __popcll(eq));
-    }
-    pass = t;
-    return at;
-}
+// ---------------------------------------------------------------------------------------------- 16 rows a workgroup
+// Lane l15 of each group of 16 has row l15 of the tile, as the matrix instruction leaves the scores, in every wave: its keys of 16 pages of each tile of scores stay in
+// registers, what belongs to a row as a whole is in all its lanes, and the rows go through the search in step.
+constexpr int TILES = CHUNK / (16 * WAVES);          // tiles of scores of a wave
+constexpr int KEPT_KEYS = MOST / (4 * WAVES);        // keys that a lane takes of those that its row has kept
+constexpr int SLOTS = 4 * WAVES * (1 + TILES);       // groups of keys of one lane, in the keys' order: the kept ones, then each tile's
+constexpr int BINS = 257;                            // of a row, a word between rows
+struct rows_lds {
+    uint32_t hist[ROWS * BINS];                      // (the slots' counts lie here afterwards)
+    __attribute__((aligned(16))) uint32_t edge[3][ROWS][WAVES];
+    __attribute__((aligned(16))) uint32_t found[ROWS][4];
+    __attribute__((aligned(16))) float scales[CHUNK];
+};
+static_assert(SLOTS * ROWS <= ROWS * BINS && SLOTS <= 192, "the counts in the histograms' place, three slots a lane");
 
 template <typename T, int HD>
 __global__ __launch_bounds__(64 * WAVES, 4) void k_select_rows(cache_select_args a) {
-    constexpr int NK = 2 * HD / 64, QS = 2 * HD + 16, SS = CHUNK + 4, CE = CHUNK / 64, KE = MOST / 64, EACH = ROWS / WAVES, TILES = CHUNK / (16 * WAVES);
+    constexpr int NK = 2 * HD / 64, QS = 2 * HD + 16, EACH = ROWS / WAVES, THREADS = 64 * WAVES;
     __shared__ __attribute__((aligned(16))) unsigned char codes[ROWS * QS];
-    __shared__ __attribute__((aligned(16))) int32_t dots[ROWS * SS];
-    __shared__ float scales[CHUNK];
+    __shared__ rows_lds l;
     extern __shared__ __attribute__((aligned(16))) uint32_t lists[];      // what rows keep: keys [ROWS][take], pages [ROWS][take]
-    const int lane = (int) threadIdx.x & 63, l15 = lane & 15, g = lane >> 4, wv = uniform((int) threadIdx.x >> 6);
+    const int tid = (int) threadIdx.x, lane = tid & 63, l15 = lane & 15, g = lane >> 4, wv = uniform(tid >> 6);
     const int group = a.n_head / a.n_kv_head, kvh = (int) (blockIdx.x % (unsigned) a.n_kv_head), page_shift = __builtin_ctz((unsigned) a.page_size);
     const int64_t t0 = (int64_t) (blockIdx.x / (unsigned) a.n_kv_head) * ROWS, t1 = min(t0 + ROWS, a.n_rows);
     const int keep = a.take - a.first - a.last;
+    uint32_t * const keys = lists + l15 * a.take, * const pages = lists + (ROWS + l15) * a.take;
     for (int64_t r0 = t0; r0 < t1;) {      // the sequences of the tile's rows
         int seq;
         seq_view v;
@@ -462,17 +412,23 @@ __global__ __launch_bounds__(64 * WAVES, 4) void k_select_rows(cache_select_args
         }
         const int64_t r1 = min(t1, (int64_t) v.row0 + v.rows);
         const int rows = (int) (r1 - r0), see_all = see_of(a, v, r1 - 1, page_shift);      // (the last row sees the most)
-        int n[EACH] = {};
+        int kept = 0;      // of the lane's row
         if (see_all > a.take && keep > 0) {
-            const int p0 = a.first, p1 = see_all - a.last;
+            const int p0 = a.first, p1 = see_all - a.last, see = see_of(a, v, min(r0 + l15, r1 - 1), page_shift);
+            const int end = l15 < rows && see > a.take ? see - a.last : 0;      // the row's own
             const int32_t * table = a.table + (int64_t) seq * a.width;
-            int4_t y[TILES][NK];
-            float scale[TILES];
             int32_t next[TILES];
             auto load_pages = [&](int c0) {
 #pragma unroll
                 for (int i = 0; i < TILES; i++) next[i] = table[min(c0 + (wv * TILES + i) * 16 + l15, p1 - 1)];
             };
+            load_pages(p0);
+            auto q_of = [&](int i) { return (const T *) a.q + min(r0 + wv * EACH + i, r1 - 1) * a.ldq + (int64_t) kvh * group * HD; };
+            row_queries<T, HD> queries[EACH];
+#pragma unroll
+            for (int i = 0; i < EACH; i++) queries[i].fetch(q_of(i), group);
+            int4_t y[TILES][NK];
+            float scale[TILES];
             auto load = [&] {
 #pragma unroll
                 for (int i = 0; i < TILES; i++) {
@@ -483,81 +439,191 @@ __global__ __launch_bounds__(64 * WAVES, 4) void k_select_rows(cache_select_args
                     scale[i] = bad ? -1.0f : *(const float *) (d + 2 * HD);
                 }
             };
-            load_pages(p0);
-            auto q_of = [&](int i) { return (const T *) a.q + min(r0 + wv * EACH + i, r1 - 1) * a.ldq + (int64_t) kvh * group * HD; };
-            row_queries<T, HD> queries[EACH];
-#pragma unroll
-            for (int i = 0; i < EACH; i++) queries[i].fetch(q_of(i), group);
             load();      // (on their way while the queries' codes are made)
-            load_pages(p0 + CHUNK);
 #pragma unroll
             for (int i = 0; i < EACH; i++) queries[i].codes(q_of(i), group, codes + (wv * EACH + i) * QS);
-            __syncthreads();
-            uint32_t pass[EACH] = {};
-            for (int c0 = p0; c0 < p1; c0 += CHUNK) {
+            uint32_t pass = 0;      // what a key of the row has to be more than
+            // a chunk's pages and, but for the first, those that rows have kept of the ones before
+            auto chunk = [&](int c0, auto first) {
+                constexpr bool FIRST = decltype(first)::value;
+                constexpr int KEPT = FIRST ? 0 : KEPT_KEYS;
+                if constexpr (!FIRST) load();
+                load_pages(c0 + CHUNK);
+                for (int i = tid; i < ROWS * BINS; i += THREADS) l.hist[i] = 0;
+                if (g == 0) {
+#pragma unroll
+                    for (int i = 0; i < TILES; i++) l.scales[(wv * TILES + i) * 16 + l15] = scale[i];
+                }
+                __syncthreads();
+                // keys in their order: KEPT of the row's list, then 4 pages of each tile
+                uint32_t k[KEPT + 4 * TILES], kp[KEPT + 1];
+#pragma unroll
+                for (int j = 0; j < KEPT; j++) {
+                    const int at = (wv * 4 + g) * KEPT + j;
+                    k[j] = at < kept ? keys[at] : 0u;
+                    kp[j] = at < kept ? pages[at] : 0u;
+                }
+                const int base = c0 + wv * TILES * 16 + g * 4;      // + 16 i + r
+                uint32_t most = 0, least = 0xffffffffu;
+                int n = 0;
 #pragma unroll
                 for (int i = 0; i < TILES; i++) {
                     int4_t x = {0, 0, 0, 0};
 #pragma unroll
-                    for (int k = 0; k < NK; k++)
-                        x = __builtin_amdgcn_mfma_i32_16x16x64_i8(y[i][k], *(const int4_t *) (codes + l15 * QS + k * 64 + g * 16), x, 0, 0, 0);
-                    *(int4_t *) (dots + l15 * SS + (wv * TILES + i) * 16 + g * 4) = x;
-                    if (g == 0) scales[(wv * TILES + i) * 16 + l15] = scale[i];
+                    for (int j = 0; j < NK; j++)
+                        x = __builtin_amdgcn_mfma_i32_16x16x64_i8(y[i][j], *(const int4_t *) (codes + l15 * QS + j * 64 + g * 16), x, 0, 0, 0);
+                    const float4_t f = *(const float4_t *) (l.scales + (wv * TILES + i) * 16 + g * 4);
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const uint32_t key = f[r] < 0.0f ? KEY_LOWEST : key_of((float) x[r] * f[r]);
+                        k[KEPT + 4 * i + r] = base + 16 * i + r < end && key > pass ? key : 0u;
+                    }
                 }
-                if (c0 + CHUNK < p1) {
-                    load();
-                    load_pages(c0 + 2 * CHUNK);
+#pragma unroll
+                for (int j = 0; j < KEPT + 4 * TILES; j++) {
+                    most = max(most, k[j]);
+                    least = min(least, k[j] - 1);      // (0 becomes the largest)
+                    n += k[j] != 0;
+                }
+                // the row's: over the four groups, then over the waves
+                auto over_groups = [](uint32_t x, auto f) {
+                    auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+                    x = f((uint32_t) r[0], (uint32_t) r[1]);
+                    r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+                    return f((uint32_t) r[0], (uint32_t) r[1]);
+                };
+                auto larger = [](uint32_t x, uint32_t y) { return max(x, y); };
+                auto smaller = [](uint32_t x, uint32_t y) { return min(x, y); };
+                auto sum = [](uint32_t x, uint32_t y) { return x + y; };
+                auto over_waves = [&](int which, auto f) {
+                    const word4_t x = *(const word4_t *) l.edge[which][l15], z = *(const word4_t *) (l.edge[which][l15] + 4);
+                    return f(f(f(x[0], x[1]), f(x[2], x[3])), f(f(z[0], z[1]), f(z[2], z[3])));
+                };
+                static_assert(WAVES == 8, "two words of four");
+                most = over_groups(most, larger);
+                least = over_groups(least, smaller);
+                n = (int) over_groups((uint32_t) n, sum);
+                if (g == 0) {
+                    l.edge[0][l15][wv] = most;
+                    l.edge[1][l15][wv] = least;
+                    l.edge[2][l15][wv] = (uint32_t) n;
                 }
                 __syncthreads();
-                // this wave's rows: the chunk's keys behind the ones they kept
+                most = over_waves(0, larger);
+                least = over_waves(1, smaller) + 1;
+                n = (int) over_waves(2, sum);
+                // the last one taken lies in [least, most], `need` of those are taken (of no more than `keep` keys: all)
+                int need = min(keep, n);
+                bool done = n <= keep;
+                while (__any(!done)) {      // (the same in every wave)
+                    const int shift = most == least ? 0 : max(0, 24 - __builtin_clz(most - least));
+#pragma unroll
+                    for (int j = 0; j < KEPT + 4 * TILES; j++)
+                        if (!done && k[j] >= least && k[j] <= most) atomicAdd(&l.hist[l15 * BINS + ((k[j] - least) >> shift)], 1u);
+                    __syncthreads();
+#pragma unroll
+                    for (int i = 0; i < EACH; i++) {      // a wave finds its rows' bins: four a lane, from the last
+                        const int row = wv * EACH + i, b0 = row * BINS + 255 - lane * 4;
+                        int c[4], all = 0;
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            all += c[j] = (int) l.hist[b0 - j];
+                            l.hist[b0 - j] = 0;
+                        }
+                        const int want = __builtin_amdgcn_readlane(need, row);
+                        const int upto = wave_scan(all);
+                        const uint64_t reach = __ballot(upto >= want);
+                        if (!reach) continue;      // (a row that is done)
+                        const int at = __builtin_ctzll(reach);
+                        int above = upto - all, bin = 0;
+#pragma unroll
+                        for (int j = 0; j < 3; j++)
+                            if (bin == j && above + c[j] < want) { above += c[j]; bin++; }
+                        const int in = bin == 0 ? c[0] : bin == 1 ? c[1] : bin == 2 ? c[2] : c[3];
+                        if (lane == at) *(word4_t *) l.found[row] = word4_t{(uint32_t) (255 - lane * 4 - bin), (uint32_t) (want - above), (uint32_t) in, 0};
+                    }
+                    __syncthreads();
+                    if (!done) {
+                        const word4_t f = *(const word4_t *) l.found[l15];
+                        least += f[0] << shift;
+                        most = most - least < 1u << shift ? most : least + ((1u << shift) - 1);
+                        need = (int) f[1];
+                        done = f[1] == f[2] || shift == 0;
+                    }
+                }
+                // more than `most`: all; in the range: the first `need`. Counts of every lane's groups of keys (in the range, more << 16), then their sums before each
+                uint32_t * const counts = l.hist;
+                auto place = [&](int s) { return l15 * SLOTS + s; };
+                auto count = [&](int j0, int m) {
+                    uint32_t c = 0;
+#pragma unroll
+                    for (int j = j0; j < j0 + m; j++) c += k[j] > most ? 0x10000u : k[j] >= least && k[j] != 0 ? 1u : 0u;
+                    return c;
+                };
+                if constexpr (!FIRST) counts[place(wv * 4 + g)] = count(0, KEPT);
+                else counts[place(wv * 4 + g)] = 0;
+#pragma unroll
+                for (int i = 0; i < TILES; i++) counts[place(4 * WAVES + (wv * TILES + i) * 4 + g)] = count(KEPT + 4 * i, 4);
+                __syncthreads();
 #pragma unroll
                 for (int i = 0; i < EACH; i++) {
-                    const int at = wv * EACH + i, see = see_of(a, v, r0 + at, page_shift), m = at < rows && see > a.take ? min(CHUNK, see - a.last - c0) : 0;
-                    if (m <= 0) continue;
-                    uint32_t * const keys = lists + at * a.take, * const pages = lists + (ROWS + at) * a.take;
-                    uint32_t k[KE + CE], p[KE + CE];
-                    bool some = false;
+                    uint32_t * const row = counts + (wv * EACH + i) * SLOTS;
+                    uint32_t c[3], all = 0;
 #pragma unroll
-                    for (int e = 0; e < CE; e++) {
-                        const int j = e * 64 + lane;
-                        const float f = scales[j];
-                        const uint32_t key = f < 0.0f ? KEY_LOWEST : key_of((float) dots[at * SS + j] * f);
-                        k[KE + e] = j < m && key > pass[i] ? key : 0u;
-                        p[KE + e] = (uint32_t) (c0 + j);
-                        some |= k[KE + e] != 0;
-                    }
-                    if (n[i] == 0) {
-                        n[i] = keep_best<CE>(k + KE, p + KE, keep, keys, pages, pass[i]);
-                    } else if (__any(some)) {
+                    for (int j = 0; j < 3; j++) all += c[j] = lane * 3 + j < SLOTS ? row[min(lane * 3 + j, SLOTS - 1)] : 0u;
+                    uint32_t before = wave_scan(all) - all;
 #pragma unroll
-                        for (int e = 0; e < KE; e++) {
-                            const int j = e * 64 + lane;
-                            k[e] = j < n[i] ? keys[j] : 0u;
-                            p[e] = j < n[i] ? pages[j] : 0u;
-                        }
-                        wave_order();
-                        n[i] = keep_best<KE + CE>(k, p, keep, keys, pages, pass[i]);
+                    for (int j = 0; j < 3; j++) {
+                        if (lane * 3 + j < SLOTS) row[lane * 3 + j] = before;
+                        before += c[j];
                     }
-                    wave_order();
                 }
-                if (c0 + CHUNK < p1) __syncthreads();
-            }
+                __syncthreads();
+                auto put = [&](int j0, int m, int slot, auto page_of) {
+                    const uint32_t before = counts[place(slot)];
+                    int in = (int) (before & 0xffffu), above = (int) (before >> 16);
+#pragma unroll
+                    for (int j = 0; j < m; j++) {
+                        const uint32_t key = k[j0 + j];
+                        const bool more = key > most, eq = !more && key >= least && key != 0;
+                        if (more || (eq && in < need)) {
+                            keys[above + min(in, need)] = key;
+                            pages[above + min(in, need)] = page_of(j);
+                        }
+                        above += more;
+                        in += eq;
+                    }
+                };
+                if constexpr (!FIRST) put(0, KEPT, wv * 4 + g, [&](int j) { return kp[j]; });
+#pragma unroll
+                for (int i = 0; i < TILES; i++) put(KEPT + 4 * i, 4, 4 * WAVES + (wv * TILES + i) * 4 + g, [&](int r) { return (uint32_t) (base + 16 * i + r); });
+                kept = min(keep, n);
+                if (n > keep) pass = least - 1;
+                __syncthreads();
+            };
+            chunk(p0, std::true_type{});
+            for (int c0 = p0 + CHUNK; c0 < p1; c0 += CHUNK) chunk(c0, std::false_type{});
         }
 #pragma unroll
         for (int i = 0; i < EACH; i++) {
             const int at = wv * EACH + i;
             if (at >= rows) continue;
-            const int see = see_of(a, v, r0 + at, page_shift);
+            const int see = see_of(a, v, r0 + at, page_shift), n = __builtin_amdgcn_readlane(kept, at);
             int32_t * out = a.selected + ((r0 + at) * a.n_kv_head + kvh) * a.take;
-            for (int j = lane; j < a.take; j += 64) out[j] = entry(a, j, see, lists + (ROWS + at) * a.take, n[i]);
+            for (int j = lane; j < a.take; j += 64) out[j] = entry(a, j, see, lists + (ROWS + at) * a.take, n);
         }
         __syncthreads();
         r0 = r1;
     }
 }
 
-// Tiles of 16 rows where they fill the chip and sequences have rows for them; else a row a workgroup, and pieces of its pages where a table is long
-bool tiles_of(const cache_shape & c, int64_t n_seq, int64_t n_rows) { return n_rows >= 4 * n_seq && n_rows * c.n_kv_head >= 256 * ROWS; }
+// A workgroup a row takes time by the rows (some 7 us for 512 rows and K/V heads, after the first), a tile of 16 some 13 us for each sequence that it has rows of, however
+// few there are. So tiles where sequences have four rows or more and the rows are worth it. Measured, us of a call with a row / with tiles, rows times K/V heads in
+// brackets: 1 sequence of 14000 tokens in pages of 64, 128 rows (512) 12.2 / 13.3, 256 (1024) 16.8 / 13.2, 1024 (4096) 53.0 / 14.6; sequences of 200 to 8000
+// in pages of 16: 64 of 1 row (512) 15.6 / 214, of 4 (2048) 38.4 / 65.2, of 8 (4096) 67.4 / 40.5; 16 of 8 (1024) 23.2 / 36.6, of 16 (2048) 35.1 / 22.0.
+bool tiles_of(const cache_shape & c, int64_t n_seq, int64_t n_rows) {
+    return n_rows >= 4 * n_seq && (double) n_rows * c.n_kv_head * n_rows >= 700.0 * (double) (n_rows + ROWS * n_seq);
+}
 int pieces_of(const cache_shape & c, int64_t n_seq, int64_t n_rows, int64_t width) {
     if (tiles_of(c, n_seq, n_rows)) return 1;
     return (int) std::clamp<int64_t>(std::min((width + PIECE - 1) / PIECE, SPLIT_UNITS / (n_rows * c.n_kv_head)), 1, MOST_PIECES);
