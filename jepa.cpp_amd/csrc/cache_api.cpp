@@ -253,7 +253,7 @@ extern "C" int jepa_amd_rope_rows(int device, const jepa_amd_rope_axes * rope, i
     const char * who = "jepa_amd_rope_rows";
     rope_map m;
     if (!rope_of(who, rope, m)) return -1;
-    if (n_head < 1 || n_head > 4096 || n_rows < 0 || n_rows * n_head >= (int64_t) 1 << 26 || n_rows >= I31) {
+    if (n_head < 1 || n_head > 4096 || n_rows < 0 || n_rows >= I31 || n_rows * n_head >= (int64_t) 1 << 26) {
         jepa_log("jepa: %s: %lld rows of %d heads not supported (up to 4096 heads, below 2^26 heads of rows)\n", who, (long long) n_rows, n_head);
         return -1;
     }

@@ -127,8 +127,9 @@ __global__ __launch_bounds__(NT, groups_of<T>(HD)) void k_cache_selected(cache_s
             }
             offset[b] = col_sum(sum) * -0x1p-21f;
         }
-        c *= 0x1p24f;
     }
+    // (held where scores times it stay finite for the largest queries of f32 and bf16: there all weight is on the largest scores, of c as of this)
+    c = RAW ? fminf(c * 0x1p24f, 0x1p100f) : fminf(c, 0x1p76f);
     float4_t o[ND + 1];
     float mu = -INFINITY;
     for (int d = 0; d <= ND; d++) o[d] = float4_t{0, 0, 0, 0};

@@ -250,7 +250,7 @@ SELECT = [
     ("f32", 4, 2, 32, 64, [70000], [1], 0, 0, 1, 256), ("f16", 8, 1, 128, 16, [40000, 17000], [1, 2], 1, 1, 1, 200), ("bf16", 2, 5, 128, 16, [20000], [1], 1, 4, 9, 14),
     ("f16", 1, 1, 64, 16, [9000], [2], 1, 0, 1, 1), ("f32", 16, 2, 64, 16, [900, 1200, 16], [300, 258, 16], 1, 1, 2, 12), ("f16", 4, 8, 128, 64, [16000], [1100], 1, 1, 2, 16),
     ("bf16", 8, 4, 96, 16, [5000, 0, 2100], [600, 0, 400], 7, 0, 1, 256), ("f16", 16, 1, 32, 32, [3000] * 4, [129] * 4, 129, 1, 1, 31), ("f32", 8, 3, 128, 256, [30000], [700], 0, 0, 2, 30),
-    ("f16", 2, 2, 64, 16, [600] * 100, [1] * 100, 1, 1, 1, 8), ("bf16", 64, 1, 32, 16, [2500, 900], [50, 30], 1, 3, 3, 7), ("f32", 2, 1, 64, 16, [50000], [1], 1, 0, 1, 255),
+    ("f16", 2, 2, 64, 16, [600] * 100, [1] * 100, 1, 1, 1, 8), ("bf16", 64, 1, 32, 16, [2500, 900], [50, 30], 1, 3, 3, 7), ("f32", 2, 1, 64, 16, [50000], [1], 1, 0, 1, 255), ("f16", 4, 2, 64, 16, [20000, 4500], [300, 90], 1, 1, 2, 200), ("f32", 8, 1, 32, 16, [9000], [200], 50, 0, 1, 2),
 ]
 
 
@@ -325,6 +325,21 @@ def test_select_row_starts_and_lengths_out_of_range(jlib):
         assert out.shape == q.shape
         c.make_digest(start, lens, 9)
     torch.cuda.synchronize()
+
+
+def test_select_long_tables_of_many_rows(jlib):
+    """More rows than are split into pieces, over more pages than a workgroup takes at once; the sequences name the same pages."""
+    rng = np.random.default_rng(23)
+    c = Cache(jlib, 2, 1, 32, 16, [32000], rng, fill=False)
+    c.table = np.repeat(c.table, 1100, 0)
+    lens = rng.integers(25000, 32001, 1100).tolist()
+    start, where = rows_of(lens, [1] * 1100)
+    q = queries(rng, 1100, 64, "bf16")
+    for levels in (0, 3):
+        random_digests(rng, c, levels)
+        for first, take in ((1, 256), (0, 3)):
+            got = c.select(q, "bf16", start, lens, 1, first, 1, take).cpu().numpy()
+            np.testing.assert_array_equal(got, choose(c, q, lens, where, 1, first, 1, take))
 
 
 def test_select_many_sequences(jlib):
@@ -486,6 +501,39 @@ def test_attention_magnitudes_and_scales(jlib, kind, q_scale, k_scale):
     for scale in (0.125, -0.125, 0.0):
         want, tol = definition(c, q, [900], where, chosen, 1, scale, kind)
         near(c.attend(q, kind, start, [900], ints(chosen), 1, scale), want, tol)
+
+
+@pytest.mark.parametrize("rows", [1, 600])
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_attention_of_the_largest_queries_and_values(jlib, kind, rows):
+    """Queries up to the type's end put all weight on the largest scores, without a NaN; a mean of f16's largest values stays finite."""
+    rng = np.random.default_rng(22)
+    kvh, group, hd, page, n = 2, 2, 64, 16, 640
+    c = Cache(jlib, kvh * group, kvh, hd, page, [n], rng)
+    start, where = rows_of([n], [rows])
+    chosen = lists(rng, c, [n], where, 1, 12)
+    chosen[:, :, 0] = 0
+    for top in (1.0, 0.25, 2.0 ** -9):
+        q = queries(rng, rows, kvh * group * hd, "f32")
+        q = (q / q.abs().max() * (torch.finfo(TYPES[kind][0]).max * top)).to(TYPES[kind][0])
+        want, tol = definition(c, q, [n], where, chosen, 1, hd ** -0.5, kind)
+        got = c.attend(q, kind, [0, rows], [n], ints(chosen), 1, hd ** -0.5)
+        near(got, want, tol)
+        # the tolerance says little here: but where one score is well ahead of the others the output is its value, rounded. Ahead by the scores' own rounding and
+        # by 40 after the scale, so that the others weigh less than 640 e^-40 < 2^-48 together
+        k, v = (x.double() for x in c.read())
+        for r in (0, rows - 1):
+            pg, t = torch.tensor([(c.table[0, p], t) for p in chosen[r][1] if 0 <= p for t in range(min(page, visible(where[r][1], n, 1) - p * page))], device="cuda").T
+            s = k[pg, t, 1] @ q[r, -hd:].double()
+            if len(s) > 1 and s.topk(2).values.diff().abs() < max(s.abs().max().item() * 2.0 ** -9, 40 * hd ** 0.5):
+                continue
+            best = v[pg, t, 1][s.argmax()]
+            assert ((got[r, -hd:].double() - best).abs() <= torch.finfo(TYPES[kind][0]).eps * best.abs() + 1e-7).all()
+    big = torch.full((c.n_pages * page, kvh * hd), 65504.0, device="cuda")
+    k = next(c.read()).reshape(-1, kvh * hd).clone()
+    c.store(k, big, torch.arange(c.n_pages * page, device="cuda"))
+    got = c.attend(queries(rng, rows, kvh * group * hd, kind), kind, [0, rows], [n], ints(chosen), 1, hd ** -0.5).double()
+    assert ((got - 65504).abs() <= 65504 * (torch.finfo(TYPES[kind][0]).eps / 2 + 2.0 ** -20)).all()
 
 
 @pytest.mark.parametrize("kind", list(TYPES))
