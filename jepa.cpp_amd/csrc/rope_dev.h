@@ -2,8 +2,8 @@
 //
 // Element e turns by A_e = pos[axis(e)] rev[e] revolutions (rev: frequency times the axis's scale over 2 pi, made in more than 64 bits on the
 // host). The turn is reduced in 64 bits, where dropping whole revolutions and quarters is exact, so that a position of a million is
-// as good as one of ten; what is left, at most an eighth of a revolution, goes through the Taylor series of sine and cosine (in 64 bits to x^15
-// and x^16: 2e-14 and 1e-15 at pi / 4) and is rounded to f32 once. The rotation itself is two f32 products, each rounded, and their rounded sum:
+// as good as one of ten; what is left, at most an eighth of a revolution, goes through the Taylor series of sine and cosine (in 64 bits, to x^15
+// and x^16: the next terms are 5e-17 and 2e-18 at pi / 4) and is rounded to f32 once. The rotation itself is two f32 products, each rounded, and their rounded sum:
 // a key has the same bits, and so the same 4-bit codes, whichever kernel rotates it.
 #pragma once
 #include "kernels.h"

@@ -572,6 +572,36 @@ def test_attention_strides(jlib):
     assert torch.equal(c.select(q, "f16", start, [300], 1, 0, 1, 3), c.select(q.contiguous(), "f16", start, [300], 1, 0, 1, 3))
 
 
+def test_one_work_space_for_all_calls(jlib):
+    """Selection in pieces, attention over selected pages in pieces and attention over all take turns in one work space, which holds anything at first."""
+    rng = np.random.default_rng(24)
+    L, work = jlib.lib(), None
+    for kvh, n, take in ((1, 40000, 60), (2, 9000, 200), (1, 40000, 60)):
+        c = Cache(jlib, 2 * kvh, kvh, 32, 16, [n], rng)
+        start, where = rows_of([n], [2])
+        q = queries(rng, 2, 64 * kvh, "f16")
+        random_digests(rng, c)
+        if work is None:
+            need = [L.jepa_amd_cache_select_work_bytes(C.byref(c.s), 1, 8, 1 << 16, 256), L.jepa_amd_cache_selected_work_bytes(C.byref(c.s), 8, 256),
+                    L.jepa_amd_cache_work_bytes(C.byref(c.s), 8, 64, 1 << 16)]
+            work = torch.randint(0, 256, (max(need),), dtype=torch.uint8, device="cuda")
+        want_list, outs, dense = choose(c, q, [n], where, 1, 1, 2, take), [], []
+        for _ in range(3):
+            chosen = c.select(q, "f16", start, [n], 1, 1, 2, take, work=work)
+            np.testing.assert_array_equal(chosen.cpu().numpy(), want_list)
+            outs.append(c.attend(q, "f16", start, [n], chosen, 1, 0.2, work=work))
+            t, out = [ints(start), ints([n]), ints(c.table)], torch.empty_like(q)
+            ok(jlib, L.jepa_amd_cache_attention(0, C.byref(c.s), c.mem.data_ptr(), 1, q.data_ptr(), q.stride(0), 1, 2, t[0].data_ptr(), t[1].data_ptr(), t[2].data_ptr(), c.width, 0.2, 1,
+                                                out.data_ptr(), out.stride(0), work.data_ptr(), work.numel(), None))
+            dense.append(out)
+        want, tol = definition(c, q, [n], where, want_list, 1, 0.2, "f16")
+        near(outs[0], want, tol)
+        want, tol = definition(c, q, [n], where, np.tile(np.arange(c.width), (2, kvh, 1)), 1, 0.2, "f16")
+        near(dense[0], want, tol)
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, outs[0]) for x in outs) and all(torch.equal(x, dense[0]) for x in dense)
+
+
 def test_offsets_past_32_bits(jlib):
     """A cache and digests whose far pages lie past 2^32 bytes."""
     hd, kvh, page, n_pages = 128, 8, 256, 16000
