@@ -312,7 +312,7 @@ int jepa_amd_cache_select(int device, const jepa_amd_cache_shape * shape, const 
                           int64_t causal_block, int64_t n_first, int64_t n_last, int64_t n_select, int32_t * selected, void * work, int64_t work_bytes,
                           void * stream);
 
-/* jepa_amd_cache_attention over the pages `selected` [n_rows][n_kv_head][n_select] of each row and K/V head, with its accuracy: keys enter as they are
+/* jepa_amd_cache_attention over the pages `selected` [n_rows][n_kv_head][n_select] of each row and K/V head, with its accuracy (queries of 16-bit rows to 2^-35 of the row's largest element): keys enter as they are
  * held, values too but for bf16 rows, which take them rounded to f16 (2^-11 relative, an eighth of bf16's half step). Entries may come in any order; negative ones, pages past what the row sees and pages that are none of the cache's are passed over, tokens that it
  * does not see are not read, and a page named twice counts twice. `work` as for jepa_amd_cache_select. */
 int64_t jepa_amd_cache_selected_work_bytes(const jepa_amd_cache_shape * shape, int64_t n_rows, int64_t n_select);

@@ -7,8 +7,8 @@
 // most of the largest and smallest are found in its registers and the few lanes of the same dimensions are joined by DPP. AHEAD strips, up to four of a page, are
 // in flight (all four for pages of one strip were 35 us for 41000 tokens of 8 x 128, one was 21).
 //
-// Measured: 41000 prompt tokens of 8 x 128 in pages of 16, 18.2 us: the VALU, 380 instructions for each of 20.9 thousand waves (73 % of its time), a third of them before and
-// behind the tokens; several heads a wave, the next one's loads ahead, took no less. One token of 64 requests in pages of 64, 4.8 us: one chain of loads.
+// Measured: 41000 prompt tokens of 8 x 128 in pages of 16, 18.2 us: the VALU, 380 instructions for each of 20.9 thousand waves (71 % of its time), a third of them before and
+// behind the tokens; several heads or pages a wave took no less (two pages 18.3, four 19.2, two heads 21.6 instead of 21.7 then). One token of 64 requests in pages of 64, 4.8 us: one chain of loads.
 #include "cache_attn_dev.h"
 #include "common.h"
 

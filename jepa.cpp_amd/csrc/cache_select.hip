@@ -17,7 +17,7 @@
 //
 // Measured: a token of 64 requests of 200 to 8000 tokens in pages of 16, 32 heads over 8 of 128, 15.6 us (35 MB of digests, 2.2 TB/s: 1 us until a row's sequence is known, 2 for
 // page numbers and queries' codes, 2 to 6 for the digests, 2 to 3 for the search); two contexts of 90000 to 131000 tokens in pages of 32, 14.2; 2000 rows over 250 pages of 64,
-// 32 heads over 4, 19.4: 10 us of the VALU's time, 1600 instructions of each wave, in phases that wait for each other.
+// 32 heads over 4, 19.4: 9.4 us of the VALU's time, 1450 instructions of each wave, in phases that wait for each other.
 #include "cache_attn_dev.h"
 #include "common.h"
 

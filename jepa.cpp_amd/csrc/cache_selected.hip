@@ -12,9 +12,9 @@
 //   many rows (WHOLE)   a wave has a row and K/V head by itself and writes its result from its registers
 //   few rows            the four waves of a workgroup have 64 keys each in turn and join in LDS; fewer still: several workgroups a row, the
 //                       last of which joins their sums
-// Measured, 32 heads over 4 or 8 of 128: 2000 bf16 rows over 16 pages of 64 each 140 us (1.18 GB from the L2s, 8.4 TB/s; the VALU 78 % of its time, 480 instructions and 16
-// exponentials a tile of 64 keys; half of the 16 columns are empty with 8 heads), f16 172, f32 207; 64 f16 requests, 64 pages of 16 each, 19.8 us (72 MB, 3.7 TB/s: 6 us until
-// the first tile, a chain of sequence, list, page numbers and codes, and the join); one f32 token over 32 pages of 16, 16 heads of 64, 8.1 us, that chain.
+// Measured, 32 heads over 4 or 8 of 128: 2000 bf16 rows over 16 pages of 64 each 140 us (1.18 GB from the L2s, 8.4 TB/s; the VALU 76 % of its time, 510 instructions a
+// tile of 64 keys; half of the 16 columns are empty with 8 heads), f16 172, f32 207; 64 f16 requests, 64 pages of 16 each, 19.8 us (72 MB, 3.7 TB/s; 5.1 between the first
+// tile, 3.4 us after the start by the chain of sequence, list, page numbers and codes, and the tail of 4); one f32 token over 32 pages of 16, 16 heads of 64, 8.1 us, that chain.
 #include "cache_attn_dev.h"
 #include "common.h"
 
@@ -25,7 +25,7 @@ namespace {
 
 constexpr int C = 16;                     // columns
 constexpr int MOST = CACHE_MOST_SELECTED;
-template <typename T> constexpr int groups_of(int hd) { return hd > 64 ? 3 : 4; }      // workgroups of a CU
+constexpr int groups_of(int hd) { return hd > 64 ? 3 : 4; }      // workgroups of a CU
 
 template <int HD> constexpr int split_lds() {
     const int loop = 4 * wave_lds<HD>(), join = 4 * C * (HD + 4) * 4 + 4 * C * 8;
@@ -33,7 +33,7 @@ template <int HD> constexpr int split_lds() {
 }
 
 template <typename T, int HD, bool WHOLE>
-__global__ __launch_bounds__(NT, groups_of<T>(HD)) void k_cache_selected(cache_selected_args a) {
+__global__ __launch_bounds__(NT, groups_of(HD)) void k_cache_selected(cache_selected_args a) {
     constexpr int NB = HD / 32, ND = HD / 16, TERMS = sizeof(T) == 4 ? 2 : 1, LISTS = WHOLE ? 4 : 1;
     constexpr bool RAW = TERMS == 1, EXACT = !std::is_same<T, __bf16>::value;
     __shared__ __attribute__((aligned(16))) unsigned char lds[WHOLE ? 4 * wave_lds<HD>() : split_lds<HD>()];
