@@ -258,7 +258,7 @@ typedef struct {
     int32_t n_axes;      /* 1 to 4 */
     int32_t dims[4];     /* even; form 2: whole 16; form 3: whole 16 together */
     double  theta;       /* above 0 */
-    double  scale[4];
+    double  scale[4];    /* every angle of a position is finite, or the call is refused */
 } jepa_amd_rope_axes;
 
 /* n_rows rows of n_head heads at positions pos [n_rows][n_axes] (device, int32), types, strides and pointers as for the cache's calls below. backward 0:
@@ -312,8 +312,9 @@ int jepa_amd_cache_select(int device, const jepa_amd_cache_shape * shape, const 
                           int64_t causal_block, int64_t n_first, int64_t n_last, int64_t n_select, int32_t * selected, void * work, int64_t work_bytes,
                           void * stream);
 
-/* jepa_amd_cache_attention over the pages `selected` [n_rows][n_kv_head][n_select] of each row and K/V head, with its accuracy (queries of 16-bit rows to 2^-35 of the row's largest element): keys enter as they are
- * held, values too but for bf16 rows, which take them rounded to f16 (2^-11 relative, an eighth of bf16's half step). Entries may come in any order; negative ones, pages past what the row sees and pages that are none of the cache's are passed over, tokens that it
+/* jepa_amd_cache_attention over the pages `selected` [n_rows][n_kv_head][n_select] of each row and K/V head, with its accuracy (queries of 16-bit rows to 2^-35
+ * of the row's largest element): keys enter as they are held, values too but for bf16 rows, which take them rounded to f16 (2^-11 relative, an eighth of bf16's
+ * half step). Entries may come in any order; negative ones, pages past what the row sees and pages that are none of the cache's are passed over, tokens that it
  * does not see are not read, and a page named twice counts twice. `work` as for jepa_amd_cache_select. */
 int64_t jepa_amd_cache_selected_work_bytes(const jepa_amd_cache_shape * shape, int64_t n_rows, int64_t n_select);
 int jepa_amd_cache_attention_selected(int device, const jepa_amd_cache_shape * shape, const void * cache, int type, const void * q, int64_t q_stride,

@@ -88,6 +88,11 @@ bool rope_of(const char * who, const jepa_amd_rope_axes * r, rope_map & m) {
         for (int i = 0; r->form == 2 && i < w / 8; i++) m.delta[at / 8 + i] = (int16_t) (i < w / 16 ? h : -h);
     }
     for (int i = 0; r->form == 3 && i < rot / 8; i++) m.delta[i] = (int16_t) (i < rot / 16 ? rot / 2 : -(rot / 2));
+    for (int e = 0; e < rot; e++)
+        if (!(std::fabs(m.rev[e]) <= 0x1p990)) {      // (times a position of 32 bits, still finite)
+            jepa_log("jepa: %s: theta %g, axis %d scaled by %g: angles past 64 bits\n", who, r->theta, m.axis[e], r->scale[m.axis[e]]);
+            return false;
+        }
     int leads = 0;
     std::fill(std::begin(m.lead), std::end(m.lead), (uint8_t) 0);
     for (int i = 0; i < m.hd / 8; i++)

@@ -256,7 +256,7 @@ __global__ __launch_bounds__(NT, groups_of(HD)) void k_cache_selected(cache_sele
 
 // A wave for each unit where there are two for each SIMD; else a workgroup, or as many as there are CUs, if each has a step of its waves to do. Measured, us of
 // a call with a workgroup / a wave a unit: f16 rows of 32 heads over 8 of 128, 1024 tokens each, 512 units 21.4 / 37.1, 1024 36.2 / 37.7, 1536 49.0 / 52.4,
-// 2048 60.5 / 58.1, 3072 86.7 / 78.1, 4096 110 / 105; bf16 rows of 16 heads of 64, 512 tokens each, 1024 units 14.2 / 15.0, 3072 32.4 / 24.7.
+// 2048 60.5 / 58.1, 4096 110 / 105; bf16 rows of 16 heads of 64, 512 tokens each, 1024 units 14.2 / 15.0 (and at three times as many 32.4 / 24.7).
 // Pieces of 240 units into 480 or 720 workgroups 16.2, whole 14.5; of 128 units (2048 tokens each) whole 21.2, 256 workgroups 15.9, 512 15.8, 768 16.0.
 constexpr int64_t WAVE_UNITS = 2048, SLOTS = 256;
 int64_t steps_of(const cache_shape & c, int take) { return ((int64_t) take * c.page_size + 4 * TILE - 1) / (4 * TILE); }

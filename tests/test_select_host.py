@@ -78,6 +78,14 @@ def test_rotations_refused(kw):
     refused(append, "jepa_amd_cache_append", rope=axes(**kw))
 
 
+@pytest.mark.parametrize("form, dims", [(0, (20, 20, 20)), (1, (20, 20, 20)), (2, (16, 16)), (3, (20, 20, 24))])
+def test_angles_past_64_bits_refused(form, dims):
+    # theta^(-2 f / w) of 1e-320 passes 1e288 = 2^957 in the higher of these widths, the scale takes it past 2^990
+    refused(rope, "jepa_amd_rope_rows", rope=axes(form=form, dims=dims, theta=1e-320, scale=(1e40,) * len(dims)))
+    refused(append, "jepa_amd_cache_append", rope=axes(form=form, dims=dims, theta=5e-324, scale=(1e200,) * len(dims)))
+    refused(rope, "jepa_amd_rope_rows", rope=axes(form=form, dims=dims, scale=(1e299,) * len(dims)))
+
+
 @pytest.mark.parametrize("n", [-1, 0, 5])
 def test_number_of_axes_refused(n):
     r = _lib.RopeAxes.of(64, 1, (20, 20, 20))
