@@ -62,11 +62,11 @@ template <int HD> struct group { static constexpr int work = HD / 8, size = HD =
 template <int HD>
 __device__ __forceinline__ void store_head(unsigned char * __restrict__ cache, float8 xk, float8 xv, int64_t slot, int lane, int t, int head, int n_kv_head, int page_shift,
                                            int64_t n_slots) {
-    constexpr int GS = group<HD>::size;
+    constexpr int GS = group<HD>::size, GW = group<HD>::work;
     uint32_t ck[8], cv[8];
     bool fk, fv;
     uint16_t dk = quantize8(xk, lane, ck, fk), dv = quantize8(xv, lane, cv, fv);
-    const uint64_t odd = __ballot(!(fk && fv)) >> (lane & ~(GS - 1));
+    const uint64_t odd = __ballot((GW == GS || t < GW) && !(fk && fv)) >> (lane & ~(GS - 1));      // (lanes without work may hold anything)
     if (slot < 0 || slot >= n_slots) return;
     if (odd & ((1ull << GS) - 1)) {
         dk = 0x7e00; dv = 0;

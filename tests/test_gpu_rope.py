@@ -264,3 +264,32 @@ def test_append_no_rows(jlib):
                                               None, 0, None))
     torch.cuda.synchronize()
     assert (c.mem == 0x5a).all()
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("form,hd,dims,partner", [(0, 96, (30, 34, 32), 1), (1, 96, (30, 34, 32), 1), (2, 96, (16, 64), 8), (3, 96, (90, 6), 48), (2, 64, (16, 32), 8), (3, 32, (10, 6), 8)])
+def test_append_rows_do_not_touch_each_other(jlib, form, hd, dims, partner, kind):
+    """A NaN or an infinity in the first row's first elements, in the partners they turn with or in its values, stored or not: its own head is stored as none, every
+    other row as if it stood alone (heads of 96 leave lanes of a row without work)."""
+    rng = np.random.default_rng(hd * 4 + form)
+    axes = jlib.RopeAxes.of(hd, form, dims, 1e4)
+    rows, kvh, page = 37, 3, 16
+    given_k, given_v = given(rng, rows, kvh, hd, kind), given(rng, rows, kvh, hd, kind)
+    pos = torch.tensor(rng.integers(0, 1000, (rows, len(dims))), dtype=torch.int32, device="cuda")
+    for of_v, at, bad in ((False, 0, "nan"), (False, partner, "inf"), (True, 5, "-inf"), (True, 0, "nan")):
+        for stored in (True, False):
+            k, v = given_k.clone(), given_v.clone()
+            (v if of_v else k)[0, hd + at] = float(bad)      # of head 1
+            slot = torch.arange(rows, device="cuda")
+            if not stored:
+                slot[0] = -1
+            a, b = (Cache(jlib, kvh, kvh, hd, page, 3) for _ in range(2))
+            a.append(axes, None, k, v, pos, slot, kind)
+            b.store(rotate(jlib, axes, k.float(), pos, "f32"), v.float(), slot, "f32")
+            got_k, got_v = (torch.zeros(rows, kvh * hd, device="cuda") for _ in range(2))
+            ok(jlib, jlib.lib().jepa_amd_cache_read(0, C.byref(a.s), a.mem.data_ptr(), slot.data_ptr(), rows, 0, got_k.data_ptr(), got_k.stride(0), got_v.data_ptr(),
+                                                    got_v.stride(0), None))
+            odd = torch.isnan(got_k).reshape(rows, kvh, hd)
+            assert not odd[1:].any(), f"{int(odd[1:].any(-1).sum())} heads of other rows, {at} of {'v' if of_v else 'k'} {bad}, stored {stored}"
+            assert odd[0, 1].all() == stored and not odd[0, ::2].any()
+            assert torch.equal(a.mem, b.mem)
