@@ -313,9 +313,10 @@ int jepa_amd_cache_select(int device, const jepa_amd_cache_shape * shape, const 
                           void * stream);
 
 /* jepa_amd_cache_attention over the pages `selected` [n_rows][n_kv_head][n_select] of each row and K/V head, with its accuracy (queries of 16-bit rows to 2^-35
- * of the row's largest element): keys enter as they are held, values too but for bf16 rows, which take them rounded to f16 (2^-11 relative, an eighth of bf16's
- * half step). Entries may come in any order; negative ones, pages past what the row sees and pages that are none of the cache's are passed over, tokens that it
- * does not see are not read, and a page named twice counts twice. `work` as for jepa_amd_cache_select. */
+ * of the row's largest element): keys and values enter as they are held, with one exception: in a call of many rows (2048 rows times K/V heads and more, or
+ * fewer where a K/V head has more than 16 heads), bf16 rows take values rounded to f16 (2^-11 relative, an eighth of bf16's half step). Entries may come in
+ * any order; negative ones, pages past what the row sees and pages that are none of the cache's are passed over, tokens that it does not see are not read, and a
+ * page named twice counts twice. `work` as for jepa_amd_cache_select. */
 int64_t jepa_amd_cache_selected_work_bytes(const jepa_amd_cache_shape * shape, int64_t n_rows, int64_t n_select);
 int jepa_amd_cache_attention_selected(int device, const jepa_amd_cache_shape * shape, const void * cache, int type, const void * q, int64_t q_stride,
                                       int64_t n_seq, int64_t n_rows, const int32_t * row_start, const int32_t * kv_len, const int32_t * table,

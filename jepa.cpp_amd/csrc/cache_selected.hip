@@ -1,9 +1,10 @@
 // cache_selected.hip - attention of packed rows over pages that each row and K/V head selects from the 4-bit paged cache.
 //
 // The arithmetic is k_cache_attention's (scales in f32, weights of one f16 or two, V as two f16) but for two things: 16-bit rows take K's codes as f16 subnormals
-// without their offset, which the sum begins with instead (raw8: 64 instructions of a tile's 650 less), and bf16 rows take V rounded to one f16 (64 more). f32 rows take
-// them as there, for the offset costs the sum two bits. f16 weights of two terms were measured: 14 % slower for many rows, 10 % for few, for an
-// error of 2.1e-4 instead of 2.6e-4, of which 2.0e-4 is the output's own rounding.
+// without their offset, which the sum begins with instead (raw8: 64 instructions of a tile's 650 less), and many bf16 rows take V rounded to one f16, as there (64 more). f32
+// rows take K as there, for the offset costs the sum two bits. Few bf16 rows keep V's bits, for 2 to 5 % of their time (a call, V as one f16 / as two: one token over 512 of
+// 16 heads of 64 6.9 / 7.0 us, 30 requests of 32 heads over 8 of 128 over 1024 tokens each 12.8 / 13.5, 64 of them 19.4 / 20.4). f16 weights of two terms were measured: 14 %
+// slower for many rows, 10 % for few, for an error of 2.1e-4 instead of 2.6e-4, of which 2.0e-4 is the output's own rounding.
 // A row's columns are the heads that share a K/V head, its keys the tokens of its own pages, so nothing is shared between rows but the caches that hold
 // the pages: with the K/V head in the workgroup's low bits an XCD's L2 sees one head of the cache (or a few).
 //
@@ -35,7 +36,7 @@ template <int HD> constexpr int split_lds() {
 template <typename T, int HD, bool WHOLE>
 __global__ __launch_bounds__(NT, groups_of(HD)) void k_cache_selected(cache_selected_args a) {
     constexpr int NB = HD / 32, ND = HD / 16, TERMS = sizeof(T) == 4 ? 2 : 1, LISTS = WHOLE ? 4 : 1;
-    constexpr bool RAW = TERMS == 1, EXACT = !std::is_same<T, __bf16>::value;
+    constexpr bool RAW = TERMS == 1, EXACT = !(WHOLE && std::is_same<T, __bf16>::value);
     __shared__ __attribute__((aligned(16))) unsigned char lds[WHOLE ? 4 * wave_lds<HD>() : split_lds<HD>()];
     __shared__ int2_t lists[LISTS][MOST];      // a page of the cache, the token it begins with
     const int tid = (int) threadIdx.x, lane = tid & 63, l15 = lane & 15, g = lane >> 4, wv = uniform(tid >> 6), group = a.n_head / a.n_kv_head;
@@ -256,7 +257,8 @@ __global__ __launch_bounds__(NT, groups_of(HD)) void k_cache_selected(cache_sele
 
 // A wave for each unit where there are two for each SIMD; else a workgroup, or as many as there are CUs, if each has a step of its waves to do. Measured, us of
 // a call with a workgroup / a wave a unit: f16 rows of 32 heads over 8 of 128, 1024 tokens each, 512 units 21.4 / 37.1, 1024 36.2 / 37.7, 1536 49.0 / 52.4,
-// 2048 60.5 / 58.1, 4096 110 / 105; bf16 rows of 16 heads of 64, 512 tokens each, 1024 units 14.2 / 15.0 (and at three times as many 32.4 / 24.7).
+// 2048 60.5 / 58.1, 4096 110 / 105; bf16 rows of 16 heads of 64, 512 tokens each (a workgroup with V as two f16, a wave as one), 512 units 9.7 / 13.9, 1024 14.3 / 14.3,
+// 1536 19.7 / 18.2, 2040 24.2 / 18.9.
 // Pieces of 240 units into 480 or 720 workgroups 16.2, whole 14.5; of 128 units (2048 tokens each) whole 21.2, 256 workgroups 15.9, 512 15.8, 768 16.0.
 constexpr int64_t WAVE_UNITS = 2048, SLOTS = 256;
 int64_t steps_of(const cache_shape & c, int take) { return ((int64_t) take * c.page_size + 4 * TILE - 1) / (4 * TILE); }

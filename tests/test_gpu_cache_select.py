@@ -750,3 +750,22 @@ def test_step_captured_and_replayed(jlib):
         for prog in progs:
             prog.verify(new)
     graphs.clear()
+
+
+@pytest.mark.parametrize("hd,page,take", [(64, 16, 4), (128, 64, 1), (96, 32, 9), (32, 16, 200)])
+def test_attention_of_few_bf16_rows_takes_values_as_they_are(jlib, hd, page, take):
+    """Keys of zeros, so that all weights are the same power of two, and values that nearly cancel in pairs. What is left off: the output's rounding, half a step of
+    bf16 (2^-8 relative), and the sum of `tokens` exact products in 32 bits with the weights' sum, its reciprocal and the product, (tokens + 4) 2^-24 of the sum of magnitudes."""
+    rng = np.random.default_rng(33)
+    n = take * page
+    c = Cache(jlib, 2, 1, hd, page, [n], rng, fill=False)
+    v = torch.tensor(rng.standard_normal((n // 2, 1, hd)).astype(np.float32), device="cuda")
+    v = torch.cat([v, -v * (1 + 2.0 ** -9)], 1).reshape(n, hd)      # (a scale some steps of f16 further)
+    slot = torch.tensor(c.table[0].astype(np.int64)[:, None] * page + np.arange(page), device="cuda").flatten()
+    c.store(torch.zeros(n, hd, device="cuda"), v, slot)
+    q = queries(rng, 1, 2 * hd, "bf16")
+    got = c.attend(q, "bf16", [0, 1], [n], ints(np.arange(take)[None, None]), 1, hd ** -0.5).double().reshape(2, hd)
+    held = list(c.read())[1].double()[torch.tensor(c.table[0].astype(np.int64), device="cuda"), :, 0].reshape(n, hd)
+    want, A = held.mean(0), held.abs().mean(0)
+    tol = want.abs() * 2.0 ** -8 + (n + 4) * 2.0 ** -24 * A * (1 + 2.0 ** -8) + 1e-38
+    assert ((got - want).abs() <= tol).all(), ((got - want).abs() / tol).max()
