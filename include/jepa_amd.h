@@ -303,7 +303,8 @@ int jepa_amd_cache_digest_read(int device, const jepa_amd_cache_shape * shape, c
  * others by score, the highest first and of equal ones the lower page; all of them where there are n_select or fewer (1 to 256). A page's score is the sum, over the
  * query heads of the K/V head, of the largest value that the product of the head's query with a key within the page's bounds could have (for a scale above 0). Of the
  * queries it takes the sums over those heads of their positive and of their negative elements, in 8 bits each: whole-number products, so that the choice is the same
- * however a call is split. A row with a NaN or an infinity in these queries scores zero everywhere; pages that are none of the cache's come last. Rows of no
+ * however a call is split. A row and K/V head score zero everywhere, so that the lowest pages are taken, where these queries have a NaN or an infinity, where one of
+ * the sums passes f32's largest value, and where the largest of them is below 2^-100. Pages that are none of the cache's come last. Rows of no
  * sequence are left as they are. `work` is jepa_amd_cache_select_work_bytes() bytes (16-byte aligned, may be NULL where that is 0) under the same terms as
  * jepa_amd_cache_attention's. */
 int64_t jepa_amd_cache_select_work_bytes(const jepa_amd_cache_shape * shape, int64_t n_seq, int64_t n_rows, int64_t table_width, int64_t n_select);

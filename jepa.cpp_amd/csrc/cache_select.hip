@@ -4,7 +4,7 @@
 //   score(page) = scale(page) * sum_n (P_n hi_n + N_n lo_n): the sum over those heads of the largest product that a key in the page's box could have
 //
 // The sums P and N are made in 64 bits, rounded to f32 and held as 8-bit codes with one factor for all 2 hd of them, which the order of the
-// scores does not depend on. The dot product is of whole numbers, at most 2 * 128 * 127^2 < 2^24: it is exact in the matrix instruction
+// scores does not depend on (codes of zeros where a query is no number, a sum passes f32's end or all are below 2^-100). The dot product is of whole numbers, at most 2 * 128 * 127^2 < 2^24: it is exact in the matrix instruction
 // (16x16x64 i8, 16 pages x 16 rows) and as an f32, so a score has one rounding and the selection does not depend on how the pages
 // are dealt out. Ties go to the lower page.
 //

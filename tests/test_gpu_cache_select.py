@@ -769,3 +769,28 @@ def test_attention_of_few_bf16_rows_takes_values_as_they_are(jlib, hd, page, tak
     want, A = held.mean(0), held.abs().mean(0)
     tol = want.abs() * 2.0 ** -8 + (n + 4) * 2.0 ** -24 * A * (1 + 2.0 ** -8) + 1e-38
     assert ((got - want).abs() <= tol).all(), ((got - want).abs() / tol).max()
+
+
+@pytest.mark.parametrize("rows", [1, 600])
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_select_sums_past_the_ends_of_f32(jlib, kind, rows):
+    """Finite queries whose sum over the heads passes f32's largest value, and ones whose sums are all below 2^-100, score zero everywhere: the lowest pages. At
+    either end, just inside, they are ranked as any others."""
+    rng = np.random.default_rng(32)
+    kvh, group, hd, page, take, n = 8, 2, 64, 16, 10, 3000
+    c = Cache(jlib, kvh * group, kvh, hd, page, [n], rng, fill=False)
+    random_digests(rng, c)
+    start, where = rows_of([n], [rows])
+    base = (rng.integers(-64, 65, (rows, kvh, group, hd)) / 64.0).astype(np.float32)
+    base[..., 3] = 1.0      # its sum over the heads: 2
+    zero = [*range(take - 1)]
+    for power, ranked in ((126, True), (127, False), (-101, True), (-102, False)):
+        q = torch.tensor(base * np.float32(2.0) ** power, device="cuda").reshape(rows, -1).to(TYPES[kind][0])
+        assert torch.isfinite(q).all()
+        got = c.select(q, kind, start, [n], 1, 0, 1, take).cpu().numpy()
+        last = np.array([-(-visible(p, n, 1) // page) - 1 for _, p in where])
+        if ranked:
+            plain = torch.tensor(base, device="cuda").reshape(rows, -1).to(TYPES[kind][0])
+            np.testing.assert_array_equal(got, choose(c, plain, [n], where, 1, 0, 1, take))
+        else:
+            assert (got[..., :-1] == zero).all() and (got[..., -1] == last[:, None]).all()
