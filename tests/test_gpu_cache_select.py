@@ -794,3 +794,70 @@ def test_select_sums_past_the_ends_of_f32(jlib, kind, rows):
             np.testing.assert_array_equal(got, choose(c, plain, [n], where, 1, 0, 1, take))
         else:
             assert (got[..., :-1] == zero).all() and (got[..., -1] == last[:, None]).all()
+
+
+# ------------------------------------------------------------------------------------------------ steps of one prompt and many single tokens
+@pytest.mark.parametrize("kind,hd,page,at", [("f16", 64, 16, 0), ("bf16", 128, 64, 30), ("f32", 32, 16, 63)])
+def test_a_prompt_among_single_tokens(jlib, kind, hd, page, at):
+    """A piece of a prompt and 63 single tokens in one call, a few sequences that get none among them: tiles of 16 rows that are 16 sequences', and of both kinds."""
+    rng = np.random.default_rng(hd + at)
+    kvh, group, take = 8, 2, 9
+    lens = rng.integers(12 * page, 40 * page, 68).tolist()
+    new = [1] * 68
+    lens[at], new[at] = 60 * page + 5, 300
+    for i in (5, 40, 41, 66):
+        new[i] = 0
+    c = Cache(jlib, kvh * group, kvh, hd, page, lens, rng)
+    start, where = rows_of(lens, new)
+    c.make_digest(start, [0] * 68, start[-1])
+    assert not c.digest.any()
+    random_digests(rng, c)
+    others = c.digest.clone()
+    c.make_digest(start, lens, start[-1])
+    keys = next(c.read()).cpu().numpy()
+    touched = [(i, p) for i, (m, r) in enumerate(zip(lens, new)) for p in range((m - r) // page, -(-m // page)) if r]
+    pages = [c.table[i, p] for i, p in touched]
+    codes, scales, _ = digests(c, pages)
+    for n, (i, p) in enumerate(touched):
+        for h in range(kvh):
+            want, s = box(keys[pages[n], :min(page, lens[i] - p * page), h])
+            np.testing.assert_array_equal(codes[n, h], want)
+            assert scales[n, h] == s
+    others[pages] = c.digest[pages]
+    assert torch.equal(c.digest, others)
+    q = queries(rng, start[-1], kvh * group * hd, kind)
+    got = c.select(q, kind, start, lens, 1, 1, 2, take)
+    np.testing.assert_array_equal(got.cpu().numpy(), choose(c, q, lens, where, 1, 1, 2, take))
+    out = c.attend(q, kind, start, lens, got, 1, hd ** -0.5)
+    some = [r for r, (i, _) in enumerate(where) if i != at] + list(range(start[at], start[at + 1], 50))
+    want, tol = definition(c, q[some], lens, [where[r] for r in some], got[some].tolist(), 1, hd ** -0.5, kind)
+    near(out[some], want, tol)
+
+
+@pytest.mark.parametrize("kvh,group,rows", [(2, 5, 1), (8, 3, 400)])
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_select_against_the_sum_over_heads(jlib, kind, kvh, group, rows):
+    """The score as it is defined, head by head and dimension by dimension: the sum of max(q hi, q lo). Queries of small whole numbers whose positive and
+    negative sums over the heads reach 127 are their own codes, so that both are the same whole number times the page's scale, rounded once."""
+    rng = np.random.default_rng(31)
+    hd, page, take, n = 96, 16, 12, 3000
+    c = Cache(jlib, kvh * group, kvh, hd, page, [n], rng, fill=False)
+    random_digests(rng, c)
+    start, where = rows_of([n], [rows])
+    x = rng.integers(-20, 21, (rows, kvh, group, hd))
+    sums = np.where(x[:, :, 1:, 7] > 0, x[:, :, 1:, 7], 0).sum(-1)
+    x[:, :, 0, 7] = 127 - sums      # dimension 7's positive sum: 127, which no other one's of `group` values passes
+    x[:, :, 1:, 7] = np.maximum(x[:, :, 1:, 7], 0)
+    assert np.abs(x).max() <= 127 and np.maximum(x, 0).sum(2).max() == 127 and np.minimum(x, 0).sum(2).min() >= -127
+    q = torch.tensor(x.reshape(rows, -1).astype(np.float32), device="cuda").to(TYPES[kind][0])
+    got = c.select(q, kind, start, [n], 1, 1, 1, take).cpu().numpy()
+    d = c.digest.cpu().numpy()[c.table[0]]
+    codes, scale = d[..., :2 * hd].view(np.int8).astype(np.int64), d[..., 2 * hd:2 * hd + 4].copy().view(np.float32)[..., 0]
+    for r in range(0, rows, 13):
+        see = -(-visible(where[r][1], n, 1) // page)
+        for h in range(kvh):
+            hi, lo = codes[1:see - 1, h, :hd], codes[1:see - 1, h, hd:]
+            whole = sum(np.maximum(x[r, h, j] * hi, x[r, h, j] * lo).sum(-1) for j in range(group))
+            score = (whole.astype(np.float64) * scale[1:see - 1, h].astype(np.float64)).astype(np.float32)      # (24 by 24 bits: exact in 64, rounded once)
+            best = 1 + np.sort(np.argsort(-score, kind="stable")[:take - 2])
+            np.testing.assert_array_equal(got[r, h], np.concatenate([[0], best, [see - 1]]))
