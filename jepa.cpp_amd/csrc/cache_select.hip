@@ -4,9 +4,9 @@
 //   score(page) = scale(page) * sum_n (P_n hi_n + N_n lo_n): the sum over those heads of the largest product that a key in the page's box could have
 //
 // The sums P and N are made in 64 bits, rounded to f32 and held as 8-bit codes with one factor for all 2 hd of them, which the order of the
-// scores does not depend on (codes of zeros where a query is no number, a sum passes f32's end or all are below 2^-100). The dot product is of whole numbers, at most 2 * 128 * 127^2 < 2^24: it is exact in the matrix instruction
-// (16x16x64 i8, 16 pages x 16 rows) and as an f32, so a score has one rounding and the selection does not depend on how the pages
-// are dealt out. Ties go to the lower page.
+// scores does not depend on (codes of zeros where a query is no number, a sum passes f32's end or all are below 2^-100). The dot product is of whole
+// numbers, at most 2 * 128 * 127^2 < 2^24: it is exact in the matrix instruction (16x16x64 i8, 16 pages x 16 rows) and as an f32, so a score has one rounding and
+// the selection does not depend on how the pages are dealt out. Ties go to the lower page.
 //
 //   few rows (k_select_row)    a workgroup has a row and K/V head, or a piece of its pages where the table is long (the last piece to arrive takes the
 //                              best of all pieces' best). Its waves score 64 pages at a time, the loads of four matrix tiles in flight.
@@ -15,8 +15,8 @@
 // The best of some keys are found by histograms of 256 bins between the smallest and the largest: they narrow the range of the last one that is taken, 8
 // bits at a time and mostly twice; counts and a scan of them put the taken ones behind each other in their order.
 //
-// Measured: a token of 64 requests of 200 to 8000 tokens in pages of 16, 32 heads over 8 of 128, 15.6 us (35 MB of digests, 2.2 TB/s: 1 us until a row's sequence is known, 2 for
-// page numbers and queries' codes, 2 to 6 for the digests, 2 to 3 for the search); two contexts of 90000 to 131000 tokens in pages of 32, 14.2; 2000 rows over 250 pages of 64,
+// Measured: a token of 64 requests of 200 to 8000 tokens in pages of 16, 32 heads over 8 of 128, 15.6 us (35 MB of digests, 2.2 TB/s; of a workgroup, medians: 0.9 us until
+// its row's sequence is known, 4.7 for page numbers and queries' codes, 2 to 10 as the loads of others go before, 1.4 for the digests, 3.5 for scores and search); two contexts of 90000 to 131000 tokens in pages of 32, 14.2; 2000 rows over 250 pages of 64,
 // 32 heads over 4, 19.4: 9.4 us of the VALU's time, 1450 instructions of each wave, in phases that wait for each other.
 #include "cache_attn_dev.h"
 #include "common.h"
@@ -621,6 +621,8 @@ __global__ __launch_bounds__(64 * WAVES, 4) void k_select_rows(cache_select_args
 // few there are. So tiles where sequences have four rows or more and the rows are worth it. Measured, us of a call with a row / with tiles, rows times K/V heads in
 // brackets: 1 sequence of 14000 tokens in pages of 64, 128 rows (512) 12.2 / 13.3, 256 (1024) 16.8 / 13.2, 1024 (4096) 53.0 / 14.6; sequences of 200 to 8000
 // in pages of 16: 64 of 1 row (512) 15.6 / 214, of 4 (2048) 38.4 / 65.2, of 8 (4096) 67.4 / 40.5; 16 of 8 (1024) 23.2 / 36.6, of 16 (2048) 35.1 / 22.0.
+// These are sequences of equal rows; the rule knows only what the call is sized for. Single tokens beside a prompt, or in a captured call with room for one, come into tiles of
+// up to 16 sequences: a token of 63 requests 14.8 us, in a call of 2000 rows 190, beside a prompt of 1000 rows (28.6 by itself) 195.
 bool tiles_of(const cache_shape & c, int64_t n_seq, int64_t n_rows) {
     return n_rows >= 4 * n_seq && (double) n_rows * c.n_kv_head * n_rows >= 700.0 * (double) (n_rows + ROWS * n_seq);
 }

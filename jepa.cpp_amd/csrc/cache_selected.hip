@@ -258,7 +258,8 @@ __global__ __launch_bounds__(NT, groups_of(HD)) void k_cache_selected(cache_sele
 // A wave for each unit where there are two for each SIMD; else a workgroup, or as many as there are CUs, if each has a step of its waves to do. Measured, us of
 // a call with a workgroup / a wave a unit: f16 rows of 32 heads over 8 of 128, 1024 tokens each, 512 units 21.4 / 37.1, 1024 36.2 / 37.7, 1536 49.0 / 52.4,
 // 2048 60.5 / 58.1, 4096 110 / 105; bf16 rows of 16 heads of 64, 512 tokens each (a workgroup with V as two f16, a wave as one), 512 units 9.7 / 13.9, 1024 14.3 / 14.3,
-// 1536 19.7 / 18.2, 2040 24.2 / 18.9.
+// 1536 19.7 / 18.2, 2040 24.2 / 18.9. The rows are those that the call is sized for: a token of 63 f16 requests, 32 heads over 8 of 128, 1024 tokens each, 20.3, in a call of
+// 2000 rows 35.9.
 // Pieces of 240 units into 480 or 720 workgroups 16.2, whole 14.5; of 128 units (2048 tokens each) whole 21.2, 256 workgroups 15.9, 512 15.8, 768 16.0.
 constexpr int64_t WAVE_UNITS = 2048, SLOTS = 256;
 int64_t steps_of(const cache_shape & c, int take) { return ((int64_t) take * c.page_size + 4 * TILE - 1) / (4 * TILE); }

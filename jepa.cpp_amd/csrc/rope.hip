@@ -4,7 +4,8 @@
 // Both are bound by memory once there are rows enough: a value is read and written once, and the 64-bit operations of a cosine and sine (some 35) are
 // shared by the heads that one thread goes through, four of them in flight. Measured: the gradient of 8192 bf16 rows of 16 heads of 88 11.4 us
 // (46 MB, 4.1 TB/s; a large copy reaches 5.05), 4128 f32 frame rows of 16 + 16 + 16 heads of 64 appended 18.4 us (73 MB, 4.0 TB/s, the VALU busy 35 % of it), 32768 bf16 rows of
-// 32 + 8 + 8 heads of 128 151 us (709 MB, 4.7 TB/s), 64 f16 rows of 40 heads of 128 5.0 us (a launch and a chain of three loads and the cosines).
+// 32 + 8 + 8 heads of 128 151 us (709 MB, 4.7 TB/s), 64 f16 rows of 40 heads of 128 5.0 us (a launch and a chain of three loads and the cosines),
+// 64 rows of 32 + 8 + 8 heads of 128, one token of 64 requests, appended 4.4 us, one row of 16 + 16 + 16 heads of 64 4.2 (calls of a captured graph; the same chain).
 #include "common.h"
 #include "rope_dev.h"
 
